@@ -1,0 +1,175 @@
+// row_values.cuh — eight neighbouring values of a row: loads, stores and conversion of bf16, fp16 and fp32, the 8-bit form in
+// which activations are kept between the forward and the backward pass, and sums over the threads of a row.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <cstring>
+
+namespace bshmem {
+namespace rows {
+
+// ---- conversion ---------------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float(float v) { return v; }
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+
+// Eight values as they lie in memory: one 16-byte word of a 2-byte type, two of fp32.
+template <typename T> struct alignas(16) Raw8 {
+  static constexpr int kWords = sizeof(T) / 2;
+  T v[8];
+  __device__ __forceinline__ void set(int i, uint4 w) { memcpy(reinterpret_cast<char*>(v) + 16 * i, &w, 16); }
+  __device__ __forceinline__ uint4 get(int i) const {
+    uint4 w;
+    memcpy(&w, reinterpret_cast<const char*>(v) + 16 * i, 16);
+    return w;
+  }
+};
+
+template <typename T> __device__ __forceinline__ void unpack(const Raw8<T>& r, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = to_float<T>(r.v[i]);
+}
+template <typename T> __device__ __forceinline__ Raw8<T> pack(const float (&v)[8]) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.v[i] = from_float<T>(v[i]);
+  return r;
+}
+
+// Columns col .. col + 7 of the row at `row`, zeros from column n on.  kVec: the row is 16-byte aligned and n % 8 == 0.
+template <bool kVec, typename T> __device__ __forceinline__ Raw8<T> load8(const T* row, int col, int n) {
+  Raw8<T> r;
+  if constexpr (kVec) {
+#pragma unroll
+    for (int i = 0; i < Raw8<T>::kWords; ++i) r.set(i, col < n ? __ldg(reinterpret_cast<const uint4*>(row + col) + i) : make_uint4(0, 0, 0, 0));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i] = col + i < n ? row[col + i] : from_float<T>(0.f);
+  }
+  return r;
+}
+template <bool kVec, typename T> __device__ __forceinline__ void store8(T* row, int col, int n, const Raw8<T>& r) {
+  if constexpr (kVec) {
+    if (col < n) {
+#pragma unroll
+      for (int i = 0; i < Raw8<T>::kWords; ++i) reinterpret_cast<uint4*>(row + col)[i] = r.get(i);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < n) row[col + i] = r.v[i];
+  }
+}
+
+// A vector over the columns (a weight, a gate per channel) in the rows' own type T or in fp32.
+template <bool kVec, typename T> __device__ __forceinline__ void vector8(const void* vec, bool f32, int col, int n, float (&v)[8]) {
+  if (!vec) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 1.f;
+  } else if (f32) {
+    unpack(load8<kVec>(static_cast<const float*>(vec), col, n), v);
+  } else {
+    unpack(load8<kVec>(static_cast<const T*>(vec), col, n), v);
+  }
+}
+
+// ---- activations in 8 bits -------------------------------------------------------------------------
+// e4m3 times one power of two for each row and 128 columns, the smallest that holds the block's largest finite value (448 is
+// e4m3's largest): a power of two loses nothing, neither here nor on the way back, and it is one byte (exponent + 127).  Sixteen
+// neighbouring lanes hold a block, eight columns each.  Infinities come back as NaN; e4m3 has none.
+__device__ __forceinline__ float block_scale_bits(uint32_t e) { return __uint_as_float(e << 23); }
+// Subnormal numbers count here, whatever the compiler does with them elsewhere.
+__device__ __forceinline__ float mul_exact(float a, float b) {
+  float r;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// The largest exponent byte of a type's blocks.  Only there could a value round up to a power of two that the type does not have
+// (2^128, 2^16 for fp16): such values stay at 240 steps instead of 256.
+template <typename T> constexpr uint32_t kTopExponent = 247;
+template <> constexpr uint32_t kTopExponent<__half> = 135;
+
+// All 32 lanes take part.  The eight bytes of this lane's values, which are of type T, and the block's exponent byte.
+template <typename T> __device__ __forceinline__ uint2 encode8(const float (&v)[8], uint32_t& e) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
+    top = max(top, a < 0x7f800000u ? a : 0u);
+  }
+#pragma unroll
+  for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  // largest = m * 2^(E - 127), m in [1, 2), and 448 = 1.75 * 2^8
+  const int b = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u);
+  e = (uint32_t)max(b, 1);
+  const float down = block_scale_bits(254u - e), most = e == kTopExponent<T> ? 240.f : 448.f;
+  uint32_t out[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint16_t two;
+      const float lo = fminf(fmaxf(mul_exact(v[4 * h + 2 * i], down), -most), most);
+      const float hi = fminf(fmaxf(mul_exact(v[4 * h + 2 * i + 1], down), -most), most);
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(hi), "f"(lo));
+      word |= (uint32_t)two << (16 * i);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)                       // the limits made a number of what is none
+      if ((__float_as_uint(v[4 * h + i]) & 0x7fffffffu) >= 0x7f800000u) word |= 0x7fu << (8 * i);
+    out[h] = word;
+  }
+  return make_uint2(out[0], out[1]);
+}
+__device__ __forceinline__ void decode8(uint2 q, uint32_t e, float (&v)[8]) {
+  const float up = block_scale_bits(e);
+  const uint32_t w[2] = {q.x, q.y};
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t two;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(two) : "h"((uint16_t)(w[h] >> (16 * i))));
+      __half2 pair;
+      memcpy(&pair, &two, 4);
+      const float2 f = __half22float2(pair);
+      v[4 * h + 2 * i] = mul_exact(f.x, up);
+      v[4 * h + 2 * i + 1] = mul_exact(f.y, up);
+    }
+}
+
+// ---- sums over a row -----------------------------------------------------------------------------------
+// blockDim.x threads (whole warps) work on one row, blockDim.y rows on a block.  One barrier per sum: the words of two
+// sums in a row differ, so a warp that is ahead writes where nobody reads any more.
+constexpr int kMaxWarps = 32;
+struct RowSum {
+  float* words;                                       // [2][kMaxWarps], shared
+  int turn = 0;
+  __device__ __forceinline__ explicit RowSum(float* w) : words(w) {}
+  __device__ __forceinline__ float operator()(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int warps = blockDim.x >> 5;
+    if (warps == 1) return v;
+    float* mine = words + turn * kMaxWarps;
+    turn ^= 1;
+    const int first = threadIdx.y * warps;
+    if ((threadIdx.x & 31) == 0) mine[first + (threadIdx.x >> 5)] = v;
+    __syncthreads();
+    float s = 0.f;
+    for (int i = 0; i < warps; ++i) s += mine[first + i];
+    return s;
+  }
+};
+
+}  // namespace rows
+}  // namespace bshmem

@@ -1,0 +1,200 @@
+"""Activations kept in 8 bits between the forward and the backward pass.
+
+An activation that is only read again for a gradient is stored as e4m3 with one power of two per row and 128 columns:
+half the bytes of bf16, and a relative error of at most 2^-4 for values down to 2^-13 of their block's largest.  ``store``
+and ``restore`` are the way there and back; ``swiglu`` is the gated activation that keeps its input so; ``Linear`` and the norms
+take ``checkpoint=True``.  Values that e4m3 does not have come back as NaN (infinities too).
+
+The reference is a communication runtime without activations, so there is no parity citation.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from .. import _native
+from .gemm import _raw_stream, current_stream
+
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_declared = False
+_store = _restore = _swiglu_store = _swiglu_backward = None
+
+
+def block_lib() -> C.CDLL:
+    """The library of the norms, the 8-bit activations and the 4-bit weights."""
+    return _native.load("libbshmem_block.so")
+
+
+def _lib() -> C.CDLL:
+    global _declared, _store, _restore, _swiglu_store, _swiglu_backward
+    lib = block_lib()
+    if not _declared:
+        VP, I, L = C.c_void_p, C.c_int, C.c_longlong
+        lib.bshmem_ckpt8_last_error.restype = C.c_char_p
+        for name, args in (("store", [I, VP, L, VP, VP, L, I, VP]), ("restore", [I, VP, VP, VP, L, L, I, VP]),
+                           ("swiglu_store", [VP, VP, VP, VP, L, I, VP]), ("swiglu_backward", [VP, VP, VP, VP, VP, L, I, VP])):
+            fn = getattr(lib, "bshmem_ckpt8_" + name)
+            fn.restype, fn.argtypes = I, args
+        _swiglu_store, _swiglu_backward = _native.fast(lib, "bshmem_ckpt8_swiglu_store"), _native.fast(lib, "bshmem_ckpt8_swiglu_backward")
+        _restore, _store = _native.fast(lib, "bshmem_ckpt8_restore"), _native.fast(lib, "bshmem_ckpt8_store")
+        _declared = True
+    return lib
+
+
+def _check(st: int, what: str) -> None:
+    if st != 0:
+        raise RuntimeError(f"{what} failed ({st}): {_lib().bshmem_ckpt8_last_error().decode()}")
+
+
+def on_current_device(t: torch.Tensor) -> bool:
+    """Whether `t` is on the current CUDA device, whose current stream the kernels are launched on."""
+    return t.get_device() == torch._C._cuda_getDevice()
+
+
+@dataclass
+class Checkpoint8:
+    """``q`` [rows, columns rounded up to 16] e4m3 bytes, ``e`` [rows, blocks of 128 columns] biased exponents: the value of a byte
+    is e4m3 * 2^(e - 127).  ``shape`` and ``dtype`` are those of the tensor that was stored."""
+    q: torch.Tensor
+    e: torch.Tensor
+    shape: torch.Size
+    dtype: torch.dtype
+
+    def restore(self, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return restore(self, dtype, out)
+
+    @property
+    def nbytes(self) -> int:
+        return self.q.nbytes + self.e.nbytes
+
+
+def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
+    """x as [rows, columns] with neighbouring columns side by side; rows may be apart."""
+    if not x.is_cuda or x.dtype not in _TYPES:
+        raise ValueError(f"{what} needs a bf16, fp16 or fp32 CUDA tensor, got {x.dtype} on {x.device}")
+    if x.dim() < 1 or x.shape[-1] < 1 or x.shape[-1] >= 1 << 30:
+        raise ValueError(f"{what} needs rows of 1 to 2^30 columns, got {tuple(x.shape)}")
+    m = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    return m if m.stride(1) == 1 else m.contiguous()
+
+
+def _empty_kept(rows: int, cols: int, device, norms: int = 1) -> tuple:
+    q = torch.empty((norms * rows, (cols + 15) // 16 * 16), dtype=torch.uint8, device=device)
+    return q, torch.empty((norms * rows, (cols + 127) // 128), dtype=torch.uint8, device=device)
+
+
+def store(x: torch.Tensor) -> Checkpoint8:
+    """bf16, fp16 or fp32 [..., columns] → 8 bits."""
+    m = _rows(x, "store")
+    if not on_current_device(x):
+        with torch.cuda.device(x.device):
+            return store(x)
+    if _store is None:
+        _lib()
+    rows, cols = m.shape
+    q, e = _empty_kept(rows, cols, x.device)
+    _check(_store(_TYPES[x.dtype], m.data_ptr(), m.stride(0), q.data_ptr(), e.data_ptr(), rows, cols, current_stream()), "store")
+    return Checkpoint8(q, e, x.shape, x.dtype)
+
+
+def restore(kept: Checkpoint8, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The stored values in `dtype` (default: what was stored), into `out` if given ([rows, columns] with columns side by side)."""
+    dtype = dtype or (out.dtype if out is not None else kept.dtype)
+    if dtype not in _TYPES:
+        raise ValueError(f"restore gives bf16, fp16 or fp32, not {dtype}")
+    if not on_current_device(kept.q):
+        with torch.cuda.device(kept.q.device):
+            return restore(kept, dtype, out)
+    if _restore is None:
+        _lib()
+    cols = kept.shape[-1]
+    rows = kept.q.shape[0]
+    if out is None:
+        out = torch.empty(kept.shape, dtype=dtype, device=kept.q.device)
+        ld = cols
+    else:
+        if out.shape != (rows, cols) or out.dtype != dtype or out.device != kept.q.device or out.stride(1) != 1 or (rows > 1 and out.stride(0) < cols):
+            raise ValueError("bad output tensor")
+        ld = out.stride(0)
+    _check(_restore(_TYPES[dtype], kept.q.data_ptr(), kept.e.data_ptr(), out.data_ptr(), ld, rows, cols, current_stream()), "restore")
+    return out
+
+
+def _check_gu(gu: torch.Tensor) -> None:
+    if not gu.is_cuda or gu.dtype is not torch.bfloat16 or gu.dim() < 1 or gu.shape[-1] < 64 or gu.shape[-1] % 64:
+        raise ValueError(f"swiglu needs bf16 CUDA rows of 32 gate and 32 up columns in turn, got {gu.dtype} {tuple(gu.shape)} on {gu.device}")
+
+
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+def swiglu_store(gu: torch.Tensor) -> tuple[torch.Tensor, Checkpoint8]:
+    """act [..., F] = silu(gate) * up of gu [..., 2F] (32 columns of the gate, then the 32 of ``up``, see
+    ``interleave_gate_up``), and gu in 8 bits, in one pass."""
+    _check_gu(gu)
+    if not on_current_device(gu):
+        with torch.cuda.device(gu.device):
+            return swiglu_store(gu)
+    if _swiglu_store is None:
+        _lib()
+    g = _aligned(gu)
+    F = gu.shape[-1] // 2
+    rows = gu.numel() // (2 * F)
+    act = torch.empty((*gu.shape[:-1], F), dtype=torch.bfloat16, device=gu.device)
+    q, e = _empty_kept(rows, 2 * F, gu.device)
+    _check(_swiglu_store(g.data_ptr(), act.data_ptr(), q.data_ptr(), e.data_ptr(), rows, F, current_stream()), "swiglu_store")
+    return act, Checkpoint8(q, e, gu.shape, gu.dtype)
+
+
+def swiglu_backward(kept: Checkpoint8, dact: torch.Tensor, *, act: bool = False, dgu_out: Optional[torch.Tensor] = None,
+                    act_out: Optional[torch.Tensor] = None):
+    """Gradient of gu from its 8 bits and the activation's gradient; with `act` also the activation again, of the same 8 bits (what
+    the next layer's weight gradient reads).  `dgu_out`, `act_out`: contiguous buffers for them."""
+    if not on_current_device(kept.q):
+        with torch.cuda.device(kept.q.device):
+            return swiglu_backward(kept, dact, act=act, dgu_out=dgu_out, act_out=act_out)
+    F = kept.shape[-1] // 2
+    if kept.shape[-1] % 64 or dact.dtype is not torch.bfloat16 or dact.shape != (*kept.shape[:-1], F) or dact.device != kept.q.device:
+        raise ValueError(f"swiglu_backward: a bf16 gradient of {(*kept.shape[:-1], F)} belongs to this checkpoint, got {dact.dtype} {tuple(dact.shape)}")
+    if _swiglu_backward is None:
+        _lib()
+    d = _aligned(dact)
+    rows = kept.q.shape[0]
+    bf = torch.bfloat16
+    dgu = torch.empty(kept.shape, dtype=bf, device=d.device) if dgu_out is None else dgu_out
+    again = None
+    if act or act_out is not None:
+        again = torch.empty(dact.shape, dtype=bf, device=d.device) if act_out is None else act_out
+    for t, shape in ((dgu, kept.shape), (again, dact.shape)):
+        if t is not None and (t.shape != shape or t.dtype is not bf or t.device != d.device or not t.is_contiguous() or t.data_ptr() % 16):
+            raise ValueError("bad output tensor")
+    _check(_swiglu_backward(kept.q.data_ptr(), kept.e.data_ptr(), d.data_ptr(), dgu.data_ptr(), 0 if again is None else again.data_ptr(), rows, F,
+                            current_stream()), "swiglu_backward")
+    return dgu if again is None else (dgu, again)
+
+
+class _SwigluFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gu):
+        act, kept = swiglu_store(gu)
+        ctx.save_for_backward(kept.q, kept.e)
+        ctx.shape = gu.shape
+        return act
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dact):
+        q, e = ctx.saved_tensors
+        return swiglu_backward(Checkpoint8(q, e, ctx.shape, torch.bfloat16), dact)
+
+
+def swiglu(gu: torch.Tensor) -> torch.Tensor:
+    """silu(gate) * up of the interleaved gu [..., 2F]; what the gradient needs of gu is kept in 8 bits."""
+    if torch.is_grad_enabled() and gu.requires_grad:
+        return _SwigluFn.apply(gu)
+    return swiglu_store(gu)[0]
