@@ -48,7 +48,7 @@ CUDA_TARGETS = {
     "libbshmem_fused.so": (["cuda/fused_tp.cu"], []),
     "libbshmem_moe.so": (["cuda/moe_kernels.cu", "cuda/moe_gemm.cu"], []),
     "libbshmem_fp8.so": (["cuda/gemm_fp8.cu"], []),
-    "libbshmem_block.so": (["cuda/norm_bf16.cu", "cuda/norm_fp16.cu", "cuda/norm_fp32.cu", "cuda/norm_api.cu", "cuda/checkpoint8.cu"], []),
+    "libbshmem_block.so": (["cuda/norm_bf16.cu", "cuda/norm_fp16.cu", "cuda/norm_fp32.cu", "cuda/norm_api.cu", "cuda/checkpoint8.cu", "cuda/gemm_w4.cu"], []),
 }
 
 

@@ -1,0 +1,162 @@
+"""Linear layers with weights of 4 bits: ``out = x @ w.T``, w[n, k] = (q[n, k] - z) * s with one bf16 scale s, and optionally one zero
+point z of 4 bits, per row and group of columns.
+
+Few tokens (a decode step) run on a kernel that streams the 4 bits and multiplies them as they are; with many the weights are
+widened to bf16 once and the bf16 tcgen05 GEMM takes them.  The reference contains no GEMM, so there is no parity citation.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from .. import _native
+from .checkpoint8 import block_lib, on_current_device
+from .gemm import current_stream, gemm_bf16
+
+FEW_TOKENS = 32
+_declared = False
+_few = _widen = None
+
+
+def _lib() -> C.CDLL:
+    global _declared, _few, _widen
+    lib = block_lib()
+    if not _declared:
+        VP, I, L = C.c_void_p, C.c_int, C.c_longlong
+        lib.bshmem_w4_last_error.restype = C.c_char_p
+        lib.bshmem_w4_few.restype = I
+        lib.bshmem_w4_few.argtypes = [VP, L, VP, VP, VP, VP, I, I, I, I, VP]
+        lib.bshmem_w4_widen.restype = I
+        lib.bshmem_w4_widen.argtypes = [VP, VP, VP, VP, I, I, I, VP]
+        lib.bshmem_w4_quant.restype = I
+        lib.bshmem_w4_quant.argtypes = [VP, L, VP, VP, VP, I, I, I, VP]
+        _widen, _few = _native.fast(lib, "bshmem_w4_widen"), _native.fast(lib, "bshmem_w4_few")
+        _declared = True
+    return lib
+
+
+def _check(st: int, what: str) -> None:
+    if st != 0:
+        raise RuntimeError(f"{what} failed ({st}): {_lib().bshmem_w4_last_error().decode()}")
+
+
+@dataclass
+class W4Tensor:
+    """A [N, K] weight in 4 bits: ``q`` [N, K/2] bytes (the column of even number in the low half), ``scales`` [N, K/group] bf16 and
+    ``zeros`` [N, K/group] bytes 0..15, or None for 8 everywhere.  Groups have 32, 64 or a multiple of 128 columns."""
+    q: torch.Tensor
+    scales: torch.Tensor
+    zeros: Optional[torch.Tensor] = None
+
+    @property
+    def group(self) -> int:
+        return 2 * self.q.shape[1] // max(1, self.scales.shape[1])
+
+    def dequantize(self) -> torch.Tensor:
+        """fp32 [N, K] (for tests and reference computations)."""
+        q = torch.stack((self.q & 15, self.q >> 4), dim=2).flatten(1).float()
+        z = 8.0 if self.zeros is None else self.zeros.float().repeat_interleave(self.group, dim=1)
+        return (q - z) * self.scales.float().repeat_interleave(self.group, dim=1)
+
+
+def _checked(w: W4Tensor, what: str) -> tuple[int, int, int]:
+    q, s, z = w.q, w.scales, w.zeros
+    if q.dtype is not torch.uint8 or s.dtype is not torch.bfloat16 or (z is not None and z.dtype is not torch.uint8) or not q.is_cuda:
+        raise ValueError(f"{what} needs CUDA tensors q (uint8), scales (bf16) and zeros (uint8 or None)")
+    if q.dim() != 2 or s.dim() != 2 or q.shape[0] != s.shape[0] or s.shape[1] < 1 or (z is not None and z.shape != s.shape):
+        raise ValueError(f"{what}: shapes do not belong together: q {tuple(q.shape)}, scales {tuple(s.shape)}")
+    N, K = q.shape[0], 2 * q.shape[1]
+    group = K // s.shape[1]
+    if N < 1 or group * s.shape[1] != K or not (group in (32, 64) or (group and group % 128 == 0)):
+        raise ValueError(f"{what} needs whole groups of 32, 64 or a multiple of 128 columns, got K {K} in {s.shape[1]} groups")
+    if s.device != q.device or (z is not None and z.device != q.device):
+        raise ValueError(f"{what}: q, scales and zeros must be on one device")
+    if not (q.is_contiguous() and s.is_contiguous() and (z is None or z.is_contiguous())) or q.data_ptr() % 16:
+        raise ValueError(f"{what} needs contiguous tensors and q on a 16-byte boundary")
+    return N, K, group
+
+
+def quantize_w4(w: torch.Tensor, group: int = 128, *, zeros: bool = False) -> W4Tensor:
+    """bf16 [N, K] → 4 bits.  Without zero points a group's scale is (largest magnitude) / 7; with them (largest - smallest) / 15, of a range
+    that holds zero; both rounded to bf16, and every value goes to the nearest that they can say."""
+    if not w.is_cuda or w.dtype is not torch.bfloat16 or w.dim() != 2 or w.stride(1) != 1:
+        raise ValueError("quantize_w4 needs a K-major bf16 CUDA matrix")
+    N, K = w.shape
+    if N < 1 or not (group in (32, 64) or (group > 0 and group % 128 == 0)) or K < group or K % group:
+        raise ValueError(f"quantize_w4 needs rows of whole groups of 32, 64 or a multiple of 128 columns, got K {K}, group {group}")
+    if not on_current_device(w):
+        with torch.cuda.device(w.device):
+            return quantize_w4(w, group, zeros=zeros)
+    lib = _lib()
+    q = torch.empty((N, K // 2), dtype=torch.uint8, device=w.device)
+    s = torch.empty((N, K // group), dtype=torch.bfloat16, device=w.device)
+    z = torch.empty((N, K // group), dtype=torch.uint8, device=w.device) if zeros else None
+    _check(lib.bshmem_w4_quant(w.data_ptr(), w.stride(0), q.data_ptr(), s.data_ptr(), 0 if z is None else z.data_ptr(), N, K, group,
+                               current_stream()), "quantize_w4")
+    return W4Tensor(q, s, z)
+
+
+def widen_w4(w: W4Tensor) -> torch.Tensor:
+    """The weight in bf16 [N, K], each value rounded once."""
+    N, K, group = _checked(w, "widen_w4")
+    if not on_current_device(w.q):
+        with torch.cuda.device(w.q.device):
+            return widen_w4(w)
+    if _widen is None:
+        _lib()
+    out = torch.empty((N, K), dtype=torch.bfloat16, device=w.q.device)
+    _check(_widen(w.q.data_ptr(), w.scales.data_ptr(), 0 if w.zeros is None else w.zeros.data_ptr(), out.data_ptr(), N, K, group,
+                  current_stream()), "widen_w4")
+    return out
+
+
+def linear_w4(x: torch.Tensor, w: W4Tensor) -> torch.Tensor:
+    """x [..., K] bf16 times the weight [N, K] of 4 bits, in bf16 [..., N] (forward only)."""
+    N, K, group = _checked(w, "linear_w4")
+    if not x.is_cuda or x.dtype is not torch.bfloat16 or x.dim() < 1 or x.shape[-1] != K or x.device != w.q.device:
+        raise ValueError(f"linear_w4 needs bf16 [..., {K}] on {w.q.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError("linear_w4 has no gradient: detach x, or call it under torch.no_grad()")
+    if not on_current_device(x):
+        with torch.cuda.device(x.device):
+            return linear_w4(x, w)
+    m = x if x.dim() == 2 else x.reshape(-1, K)
+    T = m.shape[0]
+    if T > 1 and (m.stride(1) != 1 or m.stride(0) % 8) or m.stride(1) != 1 or m.data_ptr() % 16:
+        m = m.contiguous()
+        if m.data_ptr() % 16:
+            m = m.clone()
+    if T > FEW_TOKENS and N % 8 == 0:                        # the bf16 GEMM's columns come in eights
+        out = gemm_bf16(m, widen_w4(w))
+    else:
+        if _few is None:
+            _lib()
+        out = torch.empty((T, N), dtype=torch.bfloat16, device=x.device)
+        _check(_few(m.data_ptr(), m.stride(0) if T > 1 else K, w.q.data_ptr(), w.scales.data_ptr(), 0 if w.zeros is None else w.zeros.data_ptr(),
+                    out.data_ptr(), T, N, K, group, current_stream()), "linear_w4")
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], N)
+
+
+class LinearW4(torch.nn.Module):
+    """A linear layer (no bias) with a weight of 4 bits, for serving."""
+
+    def __init__(self, weight: W4Tensor):
+        super().__init__()
+        N, K, _ = _checked(weight, "LinearW4")
+        self.in_features, self.out_features = K, N
+        self.register_buffer("q", weight.q)
+        self.register_buffer("scales", weight.scales)
+        self.register_buffer("zeros", weight.zeros)
+
+    @classmethod
+    def from_linear(cls, layer: torch.nn.Module, group: int = 128, *, zeros: bool = False) -> "LinearW4":
+        """The same layer in 4 bits; `layer` has a bf16 ``weight`` [out, in] and no bias."""
+        if getattr(layer, "bias", None) is not None:
+            raise ValueError("LinearW4 has no bias")
+        return cls(quantize_w4(layer.weight.detach(), group, zeros=zeros))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return linear_w4(x, W4Tensor(self.q, self.scales, self.zeros))
