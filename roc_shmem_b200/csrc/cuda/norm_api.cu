@@ -12,9 +12,9 @@ namespace norms {
 extern template int forward<__nv_bfloat16>(int, bool, const Params&, cudaStream_t);
 extern template int forward<__half>(int, bool, const Params&, cudaStream_t);
 extern template int forward<float>(int, bool, const Params&, cudaStream_t);
-extern template int backward<__nv_bfloat16>(int, bool, bool, int, const BwdParams&, cudaStream_t);
-extern template int backward<__half>(int, bool, bool, int, const BwdParams&, cudaStream_t);
-extern template int backward<float>(int, bool, bool, int, const BwdParams&, cudaStream_t);
+extern template int backward<__nv_bfloat16>(int, bool, const Shape&, const BwdParams&, cudaStream_t);
+extern template int backward<__half>(int, bool, const Shape&, const BwdParams&, cudaStream_t);
+extern template int backward<float>(int, bool, const Shape&, const BwdParams&, cudaStream_t);
 }  // namespace norms
 }  // namespace bshmem
 
@@ -88,14 +88,12 @@ template <typename T> __global__ void __launch_bounds__(32 * kFinishRows) norm_b
 bool aligned(const void* p) { return !(reinterpret_cast<uintptr_t>(p) & 15); }
 bool aligned(const Mat& m, int size) { return aligned(m.p) && (m.ld * size) % 16 == 0; }
 
-int blocks_of(long long rows, int n, int* blocks, int* groups) {
+// The number of groups goes by the sizes alone (see backward_shape): the rows' layout chooses between forms of the same shape.
+int groups_of(long long rows, int n, int* groups) {
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  const Shape s = backward_shape(rows, n);
-  const long long need = (rows + s.rows - 1) / s.rows;
-  const long long most = (long long)sms * (1024 / (s.threads * s.rows) < 1 ? 1 : 1024 / (s.threads * s.rows));
-  *blocks = (int)(need < most ? need : most);
-  *groups = *blocks * s.rows;
+  const Shape s = backward_shape(rows, n, false, sms, [](int) { return 1; });
+  *groups = s.blocks * s.rows;
   return 0;
 }
 
@@ -109,9 +107,9 @@ int bshmem_norm_max_columns() { return kMaxColumns; }
 // Number of groups of rows whose column sums a backward pass leaves: part_w2 and part_c are [groups][n rounded up to 8] floats,
 // part_s [groups].  Negative: an error.
 int bshmem_norm_bwd_groups(long long rows, int n) {
-  int blocks = 0, groups = 0;
+  int groups = 0;
   if (rows < 1 || n < 1 || n > kMaxColumns) { host::last_error() = "norm: needs at least one row and 1 to 16384 columns"; return -1; }
-  if (blocks_of(rows, n, &blocks, &groups)) return -7;
+  if (groups_of(rows, n, &groups)) return -7;
   return groups;
 }
 
@@ -199,8 +197,9 @@ int bshmem_norm_bwd(int what, const void* dout, const void* dh, const void* z, l
                     const void* e, void* dz, void* dy, void* dgate, void* work, long long rows, int n, void* stream) {
   const Call c(what);
   if (!c.known() || rows < 1 || n < 1 || n > kMaxColumns || rows > 0x7fffffffLL) return refuse_size();
-  int blocks = 0, groups = 0;
-  if (int rc = blocks_of(rows, n, &blocks, &groups)) return rc;
+  int groups = 0, sms = 0;
+  if (int rc = groups_of(rows, n, &groups)) return rc;
+  if (int rc = sm_count(&sms)) return rc;
   BwdParams p = {};
   p.dout = {const_cast<void*>(dout), n};
   p.dh = {const_cast<void*>(dh), n};
@@ -236,8 +235,9 @@ int bshmem_norm_bwd(int what, const void* dout, const void* dh, const void* z, l
     if (c.gate == kElement) vec = vec && aligned(p.gate, c.gate_f32 ? 4 : c.size) && aligned(p.dgate, c.gate_f32 ? 4 : c.size);
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return c.type == 0 ? backward<__nv_bfloat16>(c.mode, vec, c.kept, blocks, p, s)
-         : c.type == 1 ? backward<__half>(c.mode, vec, c.kept, blocks, p, s) : backward<float>(c.mode, vec, c.kept, blocks, p, s);
+  const Shape shape = backward_shape(rows, n, vec, sms, [&](int chunks) { return backward_words(c.size, c.mode, c.kept, c.gate, c.gate_f32, chunks); });
+  return c.type == 0 ? backward<__nv_bfloat16>(c.mode, c.kept, shape, p, s)
+         : c.type == 1 ? backward<__half>(c.mode, c.kept, shape, p, s) : backward<float>(c.mode, c.kept, shape, p, s);
 }
 
 // The gradients that are sums over rows, of what bshmem_norm_bwd left in `work`; each may be null.
@@ -245,8 +245,8 @@ int bshmem_norm_bwd_finish(int what, const void* work, const void* w1, const voi
                            void* dw2, void* dgate, void* dscale, long long rows, int n, void* stream) {
   const Call c(what);
   if (!c.known() || rows < 1 || n < 1 || n > kMaxColumns || rows > 0x7fffffffLL) return refuse_size();
-  int blocks = 0, groups = 0;
-  if (int rc = blocks_of(rows, n, &blocks, &groups)) return rc;
+  int groups = 0;
+  if (int rc = groups_of(rows, n, &groups)) return rc;
   FinishParams f = {};
   float *pw, *pc, *ps;
   split_work(const_cast<void*>(work), c.mode, groups, n, pw, pc, ps);
@@ -261,8 +261,8 @@ int bshmem_norm_bwd_finish(int what, const void* work, const void* w1, const voi
   f.w1_f32 = c.w1_f32; f.w2_f32 = c.w2_f32; f.gcol_f32 = c.gate_f32;
   const dim3 grid((unsigned)((n + 31) / 32)), block(32, kFinishRows);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return c.type == 0 ? launch(norm_bwd_finish_kernel<__nv_bfloat16>, grid, block, f, s)
-         : c.type == 1 ? launch(norm_bwd_finish_kernel<__half>, grid, block, f, s) : launch(norm_bwd_finish_kernel<float>, grid, block, f, s);
+  return c.type == 0 ? launch(norm_bwd_finish_kernel<__nv_bfloat16>, grid, block, 0, f, s)
+         : c.type == 1 ? launch(norm_bwd_finish_kernel<__half>, grid, block, 0, f, s) : launch(norm_bwd_finish_kernel<float>, grid, block, 0, f, s);
 }
 
 }  // extern "C"

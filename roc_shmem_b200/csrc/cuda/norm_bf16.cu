@@ -4,6 +4,6 @@
 namespace bshmem {
 namespace norms {
 template int forward<__nv_bfloat16>(int, bool, const Params&, cudaStream_t);
-template int backward<__nv_bfloat16>(int, bool, bool, int, const BwdParams&, cudaStream_t);
+template int backward<__nv_bfloat16>(int, bool, const Shape&, const BwdParams&, cudaStream_t);
 }  // namespace norms
 }  // namespace bshmem

@@ -4,6 +4,6 @@
 namespace bshmem {
 namespace norms {
 template int forward<float>(int, bool, const Params&, cudaStream_t);
-template int backward<float>(int, bool, bool, int, const BwdParams&, cudaStream_t);
+template int backward<float>(int, bool, const Shape&, const BwdParams&, cudaStream_t);
 }  // namespace norms
 }  // namespace bshmem

@@ -41,6 +41,7 @@ struct Params {
   int n;                                // columns
   int gate_kind;
   int w1_f32, w2_f32, gcol_f32, gate_f32, scale_f32;
+  int stages, ring_words;               // see Ring
 };
 
 struct BwdParams {
@@ -55,6 +56,7 @@ struct BwdParams {
   int n;
   int gate_kind;
   int w1_f32, w2_f32, gcol_f32, gate_f32, scale_f32;
+  int stages, ring_words;
 };
 
 template <typename T> __device__ __forceinline__ float number(const void* p, int f32, float otherwise) {
@@ -62,133 +64,199 @@ template <typename T> __device__ __forceinline__ float number(const void* p, int
 }
 template <typename T> __device__ __forceinline__ T* row_of(const Mat& m, long long row) { return static_cast<T*>(m.p) + row * m.ld; }
 
-// One row per blockDim.x threads, kChunks groups of eight columns for each: the row stays in registers between the sums, so
-// memory is read once.
-template <typename T, int kMode, int kChunks, bool kVec>
+// How a kernel gets its rows.  kScalar: value by value, for rows off 16-byte boundaries or of odd sizes.  kDirect: 16-byte loads into
+// registers.  kRing: a block walks over rows, and each thread has the next rows' words that it will need itself on their way into
+// shared memory (cp.async), so nothing but its own wait is between the copy and the use.
+enum Form : int { kScalar = 0, kDirect = 1, kRing = 2 };
+
+// The words of a thread in one stage of the ring, [stage][word][thread].
+struct Ring {
+  uint4* base;
+  int words, threads, stages;
+  __device__ __forceinline__ uint32_t slot(int stage, int word) const {
+    return ptx::smem_u32(base + ((stage * words + word) * threads + threadIdx.y * blockDim.x + threadIdx.x));
+  }
+  __device__ __forceinline__ const uint4& at(int stage, int word) const {
+    return base[(stage * words + word) * threads + threadIdx.y * blockDim.x + threadIdx.x];
+  }
+  // The oldest of `stages` rows on their way has arrived.
+  __device__ __forceinline__ void wait() const {
+    if (stages == 2) ptx::cp_async_wait<1>();
+    else if (stages == 3) ptx::cp_async_wait<2>();
+    else ptx::cp_async_wait<3>();
+  }
+};
+__device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+template <typename T> __device__ __forceinline__ void fetch8(const Ring& r, int stage, int word, const T* row, int col) {
+#pragma unroll
+  for (int i = 0; i < Raw8<T>::kWords; ++i) ptx::cp_async_16(r.slot(stage, word + i), reinterpret_cast<const uint4*>(row + col) + i);
+}
+// Columns behind the last one were not fetched.
+template <typename T> __device__ __forceinline__ Raw8<T> fetched8(const Ring& r, int stage, int word, bool in) {
+  Raw8<T> v;
+#pragma unroll
+  for (int i = 0; i < Raw8<T>::kWords; ++i) v.set(i, in ? r.at(stage, word + i) : make_uint4(0, 0, 0, 0));
+  return v;
+}
+
+// ---- forward -------------------------------------------------------------------------------------------
+// A row stays in the registers of its threads, kChunks groups of eight columns for each, between the sums: memory is read once.
+template <typename T, int kMode, int kChunks, int kForm>
 __global__ void __launch_bounds__(kChunks == 4 ? 512 : 1024) norm_fwd_kernel(const Params p) {
-  __shared__ float words[2 * kMaxWarps];
-  RowSum sum(words);
+  constexpr bool kVec = kForm != kScalar;
+  constexpr int W = Raw8<T>::kWords, kX = kMode == kPre ? 0 : kChunks * W, kGate = kX + kChunks * W;
+  extern __shared__ uint4 ring_words[];
+  __shared__ float sums[2 * kMaxWarps];
+  RowSum sum(sums);
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
-  const bool live = row < p.rows;
-  const int n = live ? p.n : 0;
   const float inv_n = 1.f / (float)p.n;
-  float z[kChunks][8];
-  if constexpr (kMode != kPre) {
+  const long long step = (long long)gridDim.x * blockDim.y;
+  const Ring ring = {ring_words, p.ring_words, (int)(blockDim.x * blockDim.y), p.stages};
+  auto fetch = [&](long long row, int stage) {
+    if (row < p.rows) {
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int col = (threadIdx.x + i * blockDim.x) * 8;
+        if (col < p.n) {
+          if constexpr (kMode != kPre) fetch8(ring, stage, i * W, row_of<T>(p.y, row), col);
+          fetch8(ring, stage, kX + i * W, row_of<T>(p.x, row), col);
+          if (kMode != kPre && p.gate_kind == kElement) {
+            if (p.gate_f32) fetch8(ring, stage, kGate + i * 2, row_of<float>(p.gate, row), col);
+            else fetch8(ring, stage, kGate + i * W, row_of<T>(p.gate, row), col);
+          }
+        }
+      }
+    }
+    ptx::cp_async_commit();
+  };
+  long long first = (long long)blockIdx.x * blockDim.y;
+  int stage = 0;
+  if constexpr (kForm == kRing)
+    for (int i = 0; i < p.stages; ++i) fetch(first + threadIdx.y + i * step, i);
+  for (; first < p.rows; first += step) {                    // the same for the whole block
+    const bool live = first + threadIdx.y < p.rows;
+    const long long row = live ? first + threadIdx.y : 0;
+    const int n = live ? p.n : 0;
     Raw8<T> ry[kChunks], rx[kChunks];
-    const T *y = row_of<T>(p.y, live ? row : 0), *x = row_of<T>(p.x, live ? row : 0);
+    if constexpr (kForm == kRing) ring.wait();
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       const int col = (threadIdx.x + i * blockDim.x) * 8;
-      ry[i] = load8<kVec>(y, col, n);
-      rx[i] = load8<kVec>(x, col, n);
+      if constexpr (kForm == kRing) {
+        if constexpr (kMode != kPre) ry[i] = fetched8<T>(ring, stage, i * W, col < n);
+        rx[i] = fetched8<T>(ring, stage, kX + i * W, col < n);
+      } else {
+        if constexpr (kMode != kPre) ry[i] = load8<kVec>(row_of<T>(p.y, row), col, n);
+        rx[i] = load8<kVec>(row_of<T>(p.x, row), col, n);
+      }
     }
-    float scale = number<T>(p.scale, p.scale_f32, p.scale_value);
-    if (p.gate_kind == kRow && live) scale *= p.gate_f32 ? row_of<float>(p.gate, row)[0] : to_float<T>(row_of<T>(p.gate, row)[0]);
-    float ss = 0.f;
+    float z[kChunks][8];
+    if constexpr (kMode != kPre) {
+      float scale = number<T>(p.scale, p.scale_f32, p.scale_value);
+      if (p.gate_kind == kRow && live) scale *= p.gate_f32 ? row_of<float>(p.gate, row)[0] : to_float<T>(row_of<T>(p.gate, row)[0]);
+      float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      float v[8];
-      unpack(ry[i], v);
+      for (int i = 0; i < kChunks; ++i) {
+        float v[8];
+        unpack(ry[i], v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
-    }
-    const float rstd = rsqrtf(fmaf(sum(ss), inv_n, p.eps));
-    if (p.rstd1 && live && threadIdx.x == 0) p.rstd1[row] = rstd;
-    const float f = scale * rstd;
+        for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+      }
+      const float rstd = rsqrtf(fmaf(sum(ss), inv_n, p.eps));
+      if (p.rstd1 && live && threadIdx.x == 0) p.rstd1[row] = rstd;
+      const float f = scale * rstd;
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int col = (threadIdx.x + i * blockDim.x) * 8;
-      float v[8], w[8];
-      unpack(ry[i], v);
-      if (p.q1) {
-        uint32_t e;
-        const uint2 q = encode8<T>(v, e);
-        if (col < n) {
-          *reinterpret_cast<uint2*>(p.q1 + row * p.ldq + col) = q;
-          if (col % 128 == 0) p.e1[row * p.lde + col / 128] = (uint8_t)e;
+      for (int i = 0; i < kChunks; ++i) {
+        const int col = (threadIdx.x + i * blockDim.x) * 8;
+        float v[8], w[8];
+        unpack(ry[i], v);
+        if (p.q1) {
+          uint32_t e;
+          const uint2 q = encode8<T>(v, e);
+          if (col < n) {
+            *reinterpret_cast<uint2*>(p.q1 + row * p.ldq + col) = q;
+            if (col % 128 == 0) p.e1[row * p.lde + col / 128] = (uint8_t)e;
+          }
         }
-      }
-      vector8<kVec, T>(p.w1, p.w1_f32, col, n, w);
+        vector8<kVec, T>(p.w1, p.w1_f32, col, n, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= w[j] * f;
-      if (p.gate_kind == kColumn) {
-        vector8<kVec, T>(p.gcol, p.gcol_f32, col, n, w);
+        for (int j = 0; j < 8; ++j) v[j] *= w[j] * f;
+        if (p.gate_kind == kColumn) {
+          vector8<kVec, T>(p.gcol, p.gcol_f32, col, n, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= w[j];
-      } else if (p.gate_kind == kElement && live) {
-        if (p.gate_f32) unpack(load8<kVec>(row_of<float>(p.gate, row), col, n), w);
-        else unpack(load8<kVec>(row_of<T>(p.gate, row), col, n), w);
+          for (int j = 0; j < 8; ++j) v[j] *= w[j];
+        } else if (p.gate_kind == kElement) {
+          if constexpr (kForm == kRing) {
+            if (p.gate_f32) unpack(fetched8<float>(ring, stage, kGate + i * 2, col < n), w);
+            else unpack(fetched8<T>(ring, stage, kGate + i * W, col < n), w);
+          } else {
+            if (p.gate_f32) unpack(load8<kVec>(row_of<float>(p.gate, row), col, n), w);
+            else unpack(load8<kVec>(row_of<T>(p.gate, row), col, n), w);
+          }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= w[j];
-      }
-      unpack(rx[i], w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += w[j];
-      const Raw8<T> o = pack<T>(v);
-      store8<kVec>(row_of<T>(p.out, live ? row : 0), col, n, o);
-      unpack(o, z[i]);                                // the next norm is one of the stored sum
-    }
-  } else {
-    const T* x = row_of<T>(p.x, live ? row : 0);
-    Raw8<T> rx[kChunks];
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) rx[i] = load8<kVec>(x, (threadIdx.x + i * blockDim.x) * 8, n);
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) unpack(rx[i], z[i]);
-  }
-  if constexpr (kMode != kPost) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(z[i][j], z[i][j], ss);       // columns behind the last one are zero
-    const float rstd = rsqrtf(fmaf(sum(ss), inv_n, p.eps));
-    if (p.rstd2 && live && threadIdx.x == 0) p.rstd2[row] = rstd;
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int col = (threadIdx.x + i * blockDim.x) * 8;
-      if (p.q2) {
-        uint32_t e;
-        const uint2 q = encode8<T>(z[i], e);
-        if (col < n) {
-          *reinterpret_cast<uint2*>(p.q2 + row * p.ldq + col) = q;
-          if (col % 128 == 0) p.e2[row * p.lde + col / 128] = (uint8_t)e;
+          for (int j = 0; j < 8; ++j) v[j] *= w[j];
         }
-      }
-      float w[8];
-      vector8<kVec, T>(p.w2, p.w2_f32, col, n, w);
+        unpack(rx[i], w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] *= z[i][j] * rstd;
-      store8<kVec>(row_of<T>(p.h, live ? row : 0), col, n, pack<T>(w));
+        for (int j = 0; j < 8; ++j) v[j] += w[j];
+        const Raw8<T> o = pack<T>(v);
+        store8<kVec>(row_of<T>(p.out, row), col, n, o);
+        unpack(o, z[i]);                              // the next norm is one of the stored sum
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) unpack(rx[i], z[i]);
+    }
+    if constexpr (kForm == kRing) {
+      fetch(first + threadIdx.y + p.stages * step, stage);   // this thread has read its words of the stage
+      if (++stage == p.stages) stage = 0;
+    }
+    if constexpr (kMode != kPost) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fmaf(z[i][j], z[i][j], ss);     // columns behind the last one are zero
+      const float rstd = rsqrtf(fmaf(sum(ss), inv_n, p.eps));
+      if (p.rstd2 && live && threadIdx.x == 0) p.rstd2[row] = rstd;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int col = (threadIdx.x + i * blockDim.x) * 8;
+        if (p.q2) {
+          uint32_t e;
+          const uint2 q = encode8<T>(z[i], e);
+          if (col < n) {
+            *reinterpret_cast<uint2*>(p.q2 + row * p.ldq + col) = q;
+            if (col % 128 == 0) p.e2[row * p.lde + col / 128] = (uint8_t)e;
+          }
+        }
+        float w[8];
+        vector8<kVec, T>(p.w2, p.w2_f32, col, n, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] *= z[i][j] * rstd;
+        store8<kVec>(row_of<T>(p.h, row), col, n, pack<T>(w));
+      }
     }
   }
 }
 
-// Eight values of an operand that was kept as it was, or in 8 bits.
-template <bool kKept8, bool kVec, typename T>
-__device__ __forceinline__ void kept8(const Mat& m, const uint8_t* q, const uint8_t* e, long long ldq, long long lde, long long row,
-                                      int col, int n, float (&v)[8]) {
-  if constexpr (kKept8) {
-    uint2 b = make_uint2(0, 0);
-    uint32_t x = 1;
-    if (col < n) {
-      b = __ldg(reinterpret_cast<const uint2*>(q + row * ldq + col));
-      x = __ldg(e + row * lde + col / 128);
-    }
-    decode8(b, x, v);
-  } else {
-    unpack(load8<kVec>(row_of<T>(m, row), col, n), v);
-  }
-}
-
+// ---- backward ------------------------------------------------------------------------------------------
 // A block walks over rows and keeps the column sums of its rows in registers; norm_bwd_finish_kernel adds up the groups' sums in
 // their order, so two calls give the same bits.
-template <typename T, int kMode, int kChunks, bool kVec, bool kKept8>
+template <typename T, int kMode, int kChunks, int kForm, bool kKept8>
 __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
-  __shared__ float words[2 * kMaxWarps];
-  RowSum sum(words);
+  constexpr bool kVec = kForm != kScalar;
+  // words of a stage: dout, dh, z, y, the two 1 / sqrt(...) and the gate per element; one that is kept in 8 bits has its
+  // eight bytes and the four that its exponent byte is among in one word
+  constexpr int W = Raw8<T>::kWords, K = kKept8 ? 1 : W;
+  constexpr int kDh = kMode == kPre ? 0 : kChunks * W, kZ = kDh + (kMode == kPost ? 0 : kChunks * W);
+  constexpr int kY = kZ + (kMode == kPost ? 0 : kChunks * K), kRstd = kY + (kMode == kPre ? 0 : kChunks * K), kGate = kRstd + 1;
+  extern __shared__ uint4 ring_words[];
+  __shared__ float sums[2 * kMaxWarps];
+  RowSum sum(sums);
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const float inv_n = 1.f / (float)p.n;
@@ -202,35 +270,108 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
       if constexpr (kMode != kPre) acc_c[i][j] = 0.f;
     }
   const long long step = (long long)gridDim.x * blockDim.y;
-  for (long long first = (long long)blockIdx.x * blockDim.y; first < p.rows; first += step) {      // the same for the whole block
-    const bool live = first + threadIdx.y < p.rows;
-    const long long row = live ? first + threadIdx.y : 0;
-    const int n = live ? p.n : 0;
-    float dz[kChunks][8], ny[kMode != kPre ? kChunks : 1][8];
-    if constexpr (kMode != kPre) {
-      const float rstd = __ldg(p.rstd1 + row);
+  const Ring ring = {ring_words, p.ring_words, (int)(blockDim.x * blockDim.y), p.stages};
+  auto fetch_kept = [&](int stage, int word, const Mat& m, const uint8_t* q, const uint8_t* e, long long row, int col) {
+    if constexpr (kKept8) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(e + row * p.lde + col / 128);
+      cp_async_8(ring.slot(stage, word), q + row * p.ldq + col);
+      ptx::cp_async_4(ring.slot(stage, word) + 8, reinterpret_cast<const void*>(at & ~(uintptr_t)3));
+    } else {
+      fetch8(ring, stage, word, row_of<T>(m, row), col);
+    }
+  };
+  auto kept = [&](int stage, int word, const Mat& m, const uint8_t* q, const uint8_t* e, long long row, int col, int n, float (&v)[8]) {
+    if constexpr (kForm == kRing && kKept8) {
+      const uint4 w = col < n ? ring.at(stage, word) : make_uint4(0, 0, 0, 0);
+      const uint32_t byte = (uint32_t)reinterpret_cast<uintptr_t>(e + row * p.lde + col / 128) & 3;
+      decode8(make_uint2(w.x, w.y), w.z >> (8 * byte) & 255, v);
+    } else if constexpr (kForm == kRing) {
+      unpack(fetched8<T>(ring, stage, word, col < n), v);
+    } else if constexpr (kKept8) {
+      uint2 b = make_uint2(0, 0);
+      uint32_t x = 1;
+      if (col < n) {
+        b = __ldg(reinterpret_cast<const uint2*>(q + row * p.ldq + col));
+        x = __ldg(e + row * p.lde + col / 128);
+      }
+      decode8(b, x, v);
+    } else {
+      unpack(load8<kVec>(row_of<T>(m, row), col, n), v);
+    }
+  };
+  auto plain = [&](int stage, int word, const Mat& m, long long row, int col, int n, float (&v)[8]) {
+    if constexpr (kForm == kRing) unpack(fetched8<T>(ring, stage, word, col < n), v);
+    else unpack(load8<kVec>(row_of<T>(m, row), col, n), v);
+  };
+  auto fetch = [&](long long row, int stage) {
+    if (row < p.rows) {
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const int col = (threadIdx.x + i * blockDim.x) * 8;
-        kept8<kKept8, kVec, T>(p.y, p.q1, p.e1, p.ldq, p.lde, row, col, n, ny[i]);
+        if (col < p.n) {
+          if constexpr (kMode != kPre) {
+            if (p.dout.p) fetch8(ring, stage, i * W, row_of<T>(p.dout, row), col);
+            fetch_kept(stage, kY + i * K, p.y, p.q1, p.e1, row, col);
+            if (p.gate_kind == kElement) {
+              if (p.gate_f32) fetch8(ring, stage, kGate + i * 2, row_of<float>(p.gate, row), col);
+              else fetch8(ring, stage, kGate + i * W, row_of<T>(p.gate, row), col);
+            }
+          }
+          if constexpr (kMode != kPost) {
+            fetch8(ring, stage, kDh + i * W, row_of<T>(p.dh, row), col);
+            fetch_kept(stage, kZ + i * K, p.z, p.q2, p.e2, row, col);
+          }
+        }
+      }
+      if constexpr (kMode != kPre) ptx::cp_async_4(ring.slot(stage, kRstd), p.rstd1 + row);
+      if constexpr (kMode != kPost) ptx::cp_async_4(ring.slot(stage, kRstd) + 4, p.rstd2 + row);
+    }
+    ptx::cp_async_commit();
+  };
+  long long first = (long long)blockIdx.x * blockDim.y;
+  int stage = 0;
+  if constexpr (kForm == kRing)
+    for (int i = 0; i < p.stages; ++i) fetch(first + threadIdx.y + i * step, i);
+  for (; first < p.rows; first += step) {                    // the same for the whole block
+    const bool live = first + threadIdx.y < p.rows;
+    const long long row = live ? first + threadIdx.y : 0;
+    const int n = live ? p.n : 0;
+    float row_gate = 1.f;
+    if (kMode != kPre && p.gate_kind == kRow && live)
+      row_gate = p.gate_f32 ? row_of<float>(p.gate, row)[0] : to_float<T>(row_of<T>(p.gate, row)[0]);
+    float rstd1 = 0.f, rstd2 = 0.f;
+    if constexpr (kForm == kRing) {
+      ring.wait();
+      const uint4 r = ring.at(stage, kRstd);
+      rstd1 = live ? __uint_as_float(r.x) : 0.f;
+      rstd2 = live ? __uint_as_float(r.y) : 0.f;
+    } else {
+      if constexpr (kMode != kPre) rstd1 = __ldg(p.rstd1 + row);
+      if constexpr (kMode != kPost) rstd2 = __ldg(p.rstd2 + row);
+    }
+    float dz[kChunks][8], ny[kMode != kPre ? kChunks : 1][8];
+    if constexpr (kMode != kPre) {
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int col = (threadIdx.x + i * blockDim.x) * 8;
+        kept(stage, kY + i * K, p.y, p.q1, p.e1, row, col, n, ny[i]);
         if (p.dout.p) {
-          unpack(load8<kVec>(row_of<T>(p.dout, row), col, n), dz[i]);
+          plain(stage, i * W, p.dout, row, col, n, dz[i]);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) dz[i][j] = 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ny[i][j] *= rstd;
+        for (int j = 0; j < 8; ++j) ny[i][j] *= rstd1;
       }
     }
     if constexpr (kMode != kPost) {
       float nz[kChunks][8], t[kChunks][8], dot = 0.f;
-      const float rstd = __ldg(p.rstd2 + row);
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const int col = (threadIdx.x + i * blockDim.x) * 8;
-        kept8<kKept8, kVec, T>(p.z, p.q2, p.e2, p.ldq, p.lde, row, col, n, nz[i]);
-        unpack(load8<kVec>(row_of<T>(p.dh, row), col, n), t[i]);
+        kept(stage, kZ + i * K, p.z, p.q2, p.e2, row, col, n, nz[i]);
+        plain(stage, kDh + i * W, p.dh, row, col, n, t[i]);
       }
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
@@ -238,7 +379,7 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
         vector8<kVec, T>(p.w2, p.w2_f32, (threadIdx.x + i * blockDim.x) * 8, n, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          nz[i][j] *= rstd;
+          nz[i][j] *= rstd2;
           acc_w2[i][j] = fmaf(t[i][j], nz[i][j], acc_w2[i][j]);
           t[i][j] *= w[j];
           dot = fmaf(t[i][j], nz[i][j], dot);
@@ -249,7 +390,7 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
       for (int i = 0; i < kChunks; ++i) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float d = rstd * (t[i][j] - nz[i][j] * mean);
+          const float d = rstd2 * (t[i][j] - nz[i][j] * mean);
           if constexpr (kMode == kPre) dz[i][j] = d;
           else dz[i][j] += d;
         }
@@ -258,8 +399,6 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
     }
     if constexpr (kMode != kPre) {
       // v = dz * g * w1 without the row's gate and the scale; its sum with ny gives both of the scalar gradients and dy's mean
-      float row_gate = 1.f;
-      if (p.gate_kind == kRow && live) row_gate = p.gate_f32 ? row_of<float>(p.gate, row)[0] : to_float<T>(row_of<T>(p.gate, row)[0]);
       float dot = 0.f;
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
@@ -267,8 +406,13 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
         float w[8], g[8];
         vector8<kVec, T>(p.w1, p.w1_f32, col, n, w);
         if (p.gate_kind == kElement) {
-          if (p.gate_f32) unpack(load8<kVec>(row_of<float>(p.gate, row), col, n), g);
-          else unpack(load8<kVec>(row_of<T>(p.gate, row), col, n), g);
+          if constexpr (kForm == kRing) {
+            if (p.gate_f32) unpack(fetched8<float>(ring, stage, kGate + i * 2, col < n), g);
+            else unpack(fetched8<T>(ring, stage, kGate + i * W, col < n), g);
+          } else {
+            if (p.gate_f32) unpack(load8<kVec>(row_of<float>(p.gate, row), col, n), g);
+            else unpack(load8<kVec>(row_of<T>(p.gate, row), col, n), g);
+          }
           if (p.dgate.p) {
             float d[8];
 #pragma unroll
@@ -297,6 +441,7 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) dot = fmaf(dz[i][j], ny[i][j], dot);
       }
+      if constexpr (kForm == kRing) fetch(first + threadIdx.y + p.stages * step, stage);   // this thread has read its words
       dot = sum(dot);
       if (live) acc_s = fmaf(row_gate, dot, acc_s);
       if (p.gate_kind == kRow && p.dgate.p && live && threadIdx.x == 0) {
@@ -304,7 +449,7 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
         else row_of<T>(p.dgate, row)[0] = from_float<T>(scale * dot);
       }
       if (p.dy.p) {
-        const float f = __ldg(p.rstd1 + row) * scale * row_gate, mean = dot * inv_n;
+        const float f = rstd1 * scale * row_gate, mean = dot * inv_n;
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
           float d[8];
@@ -313,14 +458,17 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
           store8<kVec>(row_of<T>(p.dy, row), (threadIdx.x + i * blockDim.x) * 8, n, pack<T>(d));
         }
       }
+    } else if constexpr (kForm == kRing) {
+      fetch(first + threadIdx.y + p.stages * step, stage);
     }
+    if constexpr (kForm == kRing)
+      if (++stage == p.stages) stage = 0;
   }
   const long long group = (long long)blockIdx.x * blockDim.y + threadIdx.y;
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
     const int col = (threadIdx.x + i * blockDim.x) * 8;
-    // part rows are padded to a multiple of eight columns by their pitch
-    const long long at = group * ((p.n + 7) / 8 * 8) + col;
+    const long long at = group * ((p.n + 7) / 8 * 8) + col;  // a group's sums are padded to whole eights
     if (col < p.n) {
       if constexpr (kMode != kPost)
         if (p.part_w2) {
@@ -339,9 +487,10 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
   if (kMode != kPre && p.part_s && threadIdx.x == 0) p.part_s[group] = acc_s;
 }
 
-// Threads of a row, rows of a block and eights of columns per thread for rows of n columns.
-struct Shape { int threads, rows, chunks; };
+// Threads of a row, rows of a block, eights of columns per thread and blocks for rows of n columns.
+struct Shape { int threads, rows, chunks, blocks, form, stages, words; };
 constexpr int kMaxColumns = 16384;
+constexpr int kRingBytes = 216 * 1024;                // of a multiprocessor's shared memory, for all of its blocks
 
 inline int sm_count(int* out) {
   static int counts[64];                                       // racing threads write the same number
@@ -357,10 +506,13 @@ inline int sm_count(int* out) {
   return 0;
 }
 
-template <typename K, typename P> int launch(K* kernel, dim3 grid, dim3 block, const P& p, cudaStream_t stream) {
+template <typename K, typename P> int launch(K* kernel, dim3 grid, dim3 block, int shared, const P& p, cudaStream_t stream) {
+  if (shared > 40 * 1024)                             // 48 KB with the static part need no asking
+    BSHMEM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = shared;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -371,45 +523,96 @@ template <typename K, typename P> int launch(K* kernel, dim3 grid, dim3 block, c
   return 0;
 }
 
-inline Shape forward_shape(long long rows, int n, bool vec, int sms) {
-  const int eights = (n + 7) / 8;
-  // few rows: as many threads for each as it has eights; many: four eights per thread, whose loads are all on their way at once
-  int chunks = !vec || rows > 2LL * sms ? 4 : 1;
-  while (chunks < 4 && eights > 1024 * chunks) chunks *= 2;
-  int threads = ((eights + chunks - 1) / chunks + 31) / 32 * 32;
-  int per_block = threads >= 128 ? 1 : 128 / threads;
-  if (per_block > rows) per_block = rows < 1 ? 1 : (int)rows;
-  return {threads, per_block, chunks};
-}
-inline Shape backward_shape(long long rows, int n) {
-  const int eights = (n + 7) / 8;
-  const int chunks = eights > 1024 ? 4 : eights > 512 ? 2 : 1;
-  const int threads = ((eights + chunks - 1) / chunks + 31) / 32 * 32;
-  int per_block = threads >= 256 ? 1 : 256 / threads;
-  if (per_block > rows) per_block = rows < 1 ? 1 : (int)rows;
-  return {threads, per_block, chunks};
+// The ring of a block that shares its multiprocessor with `blocks - 1` others: as many stages as fit, up to four.  Fewer than two: none.
+inline void ring_of(Shape& s, int words, int blocks) {
+  s.words = words;
+  s.stages = kRingBytes / blocks / (words * 16 * s.threads * s.rows);
+  if (s.stages > 4) s.stages = 4;
 }
 
-template <typename T, int kMode> int forward_mode(bool vec, const Params& p, cudaStream_t stream) {
+// words(chunks): 16-byte words that a thread needs for one row.
+template <typename F> Shape forward_shape(long long rows, int n, bool vec, int sms, F words) {
+  const int eights = (n + 7) / 8;
+  Shape s = {};
+  auto divide = [&](int chunks, int block) {
+    s.chunks = chunks;
+    s.threads = ((eights + chunks - 1) / chunks + 31) / 32 * 32;
+    s.rows = s.threads >= block ? 1 : block / s.threads;
+    if (s.rows > rows) s.rows = rows < 1 ? 1 : (int)rows;
+  };
+  if (vec) {
+    divide(2, 256);
+    const int per_sm = 1024 / (s.threads * s.rows);   // 64 registers a thread
+    const long long most = (long long)sms * per_sm;
+    ring_of(s, words(2), per_sm);
+    if (s.stages >= 2 && rows > 2 * most * s.rows) {
+      s.form = kRing;
+      s.blocks = (int)most;
+      return s;
+    }
+  }
+  // few rows: as many threads for each as it has eights; many: four eights per thread, whose loads are all on their way at once
+  divide(vec && rows <= 2LL * sms && eights <= 1024 ? 1 : 4, 128);
+  s.form = vec ? kDirect : kScalar;
+  s.blocks = (int)((rows + s.rows - 1) / s.rows);
+  return s;
+}
+template <typename F> Shape backward_shape(long long rows, int n, bool vec, int sms, F words) {
+  const int eights = (n + 7) / 8;
+  Shape s = {};
+  s.chunks = eights > 1024 ? 4 : eights > 32 ? 2 : 1;
+  s.threads = ((eights + s.chunks - 1) / s.chunks + 31) / 32 * 32;
+  s.rows = s.threads >= 256 ? 1 : 256 / s.threads;
+  if (s.rows > rows) s.rows = rows < 1 ? 1 : (int)rows;
+  const long long need = (rows + s.rows - 1) / s.rows;
+  const int per_sm = 512 / (s.threads * s.rows) < 1 ? 1 : 512 / (s.threads * s.rows);        // 128 registers a thread
+  const long long most = (long long)sms * per_sm;
+  s.blocks = (int)(need < most ? need : most);
+  s.form = vec ? kDirect : kScalar;
+  if (vec && s.chunks <= 2) {
+    ring_of(s, words(s.chunks), per_sm);
+    if (s.stages >= 2 && need > most) s.form = kRing;
+  }
+  return s;
+}
+
+template <typename T, int kMode> int forward_mode(bool vec, Params p, cudaStream_t stream) {
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  const Shape s = forward_shape(p.rows, p.n, vec, sms);
-  const dim3 grid((unsigned)((p.rows + s.rows - 1) / s.rows)), block(s.threads, s.rows);
-  if (!vec) return launch(norm_fwd_kernel<T, kMode, 4, false>, grid, block, p, stream);
-  if (s.chunks == 1) return launch(norm_fwd_kernel<T, kMode, 1, true>, grid, block, p, stream);
-  if (s.chunks == 2) return launch(norm_fwd_kernel<T, kMode, 2, true>, grid, block, p, stream);
-  return launch(norm_fwd_kernel<T, kMode, 4, true>, grid, block, p, stream);
+  const int W = Raw8<T>::kWords, gate = p.gate_kind != kElement ? 0 : p.gate_f32 ? 2 : W;
+  const Shape s = forward_shape(p.rows, p.n, vec, sms, [&](int chunks) { return chunks * (W * (kMode == kPre ? 1 : 2) + gate); });
+  const dim3 grid((unsigned)s.blocks), block(s.threads, s.rows);
+  if (s.form == kRing) {
+    p.stages = s.stages;
+    p.ring_words = s.words;
+    return launch(norm_fwd_kernel<T, kMode, 2, kRing>, grid, block, s.stages * s.words * 16 * s.threads * s.rows, p, stream);
+  }
+  if (s.form == kScalar) return launch(norm_fwd_kernel<T, kMode, 4, kScalar>, grid, block, 0, p, stream);
+  if (s.chunks == 1) return launch(norm_fwd_kernel<T, kMode, 1, kDirect>, grid, block, 0, p, stream);
+  return launch(norm_fwd_kernel<T, kMode, 4, kDirect>, grid, block, 0, p, stream);
 }
-template <typename T, int kMode, bool kVec, bool kKept> int backward_form(int blocks, const BwdParams& p, cudaStream_t stream) {
-  const Shape s = backward_shape(p.rows, p.n);
-  const dim3 grid((unsigned)blocks), block(s.threads, s.rows);
-  if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kVec, kKept>, grid, block, p, stream);
-  if (s.chunks == 2) return launch(norm_bwd_kernel<T, kMode, 2, kVec, kKept>, grid, block, p, stream);
-  return launch(norm_bwd_kernel<T, kMode, 4, kVec, kKept>, grid, block, p, stream);
+// The words of norm_bwd_kernel's stages.
+inline int backward_words(int size, int mode, bool kept, int gate_kind, bool gate_f32, int chunks) {
+  const int W = size / 2, K = kept ? 1 : W;
+  return chunks * ((mode == kPostPre ? 2 : 1) * (W + K) + (gate_kind != kElement ? 0 : gate_f32 ? 2 : W)) + 1;
 }
-template <typename T, int kMode> int backward_mode(bool vec, bool kept, int blocks, const BwdParams& p, cudaStream_t stream) {
-  if (vec) return kept ? backward_form<T, kMode, true, true>(blocks, p, stream) : backward_form<T, kMode, true, false>(blocks, p, stream);
-  return kept ? backward_form<T, kMode, false, true>(blocks, p, stream) : backward_form<T, kMode, false, false>(blocks, p, stream);
+template <typename T, int kMode, bool kKept> int backward_mode(const Shape& s, BwdParams p, cudaStream_t stream) {
+  const dim3 grid((unsigned)s.blocks), block(s.threads, s.rows);
+  if (s.form == kRing) {
+    p.stages = s.stages;
+    p.ring_words = s.words;
+    const int shared = s.stages * s.words * 16 * s.threads * s.rows;
+    if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kRing, kKept>, grid, block, shared, p, stream);
+    return launch(norm_bwd_kernel<T, kMode, 2, kRing, kKept>, grid, block, shared, p, stream);
+  }
+  if (s.form == kDirect) {
+    if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kDirect, kKept>, grid, block, 0, p, stream);
+    if (s.chunks == 2) return launch(norm_bwd_kernel<T, kMode, 2, kDirect, kKept>, grid, block, 0, p, stream);
+    return launch(norm_bwd_kernel<T, kMode, 4, kDirect, kKept>, grid, block, 0, p, stream);
+  }
+  if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kScalar, kKept>, grid, block, 0, p, stream);
+  if (s.chunks == 2) return launch(norm_bwd_kernel<T, kMode, 2, kScalar, kKept>, grid, block, 0, p, stream);
+  return launch(norm_bwd_kernel<T, kMode, 4, kScalar, kKept>, grid, block, 0, p, stream);
 }
 
 // The kernels for one type of rows; norm_bf16.cu, norm_fp16.cu and norm_fp32.cu instantiate them.
@@ -417,9 +620,10 @@ template <typename T> int forward(int mode, bool vec, const Params& p, cudaStrea
   return mode == kPre ? forward_mode<T, kPre>(vec, p, stream) : mode == kPost ? forward_mode<T, kPost>(vec, p, stream)
                                                                               : forward_mode<T, kPostPre>(vec, p, stream);
 }
-template <typename T> int backward(int mode, bool vec, bool kept, int blocks, const BwdParams& p, cudaStream_t stream) {
-  return mode == kPre ? backward_mode<T, kPre>(vec, kept, blocks, p, stream)
-         : mode == kPost ? backward_mode<T, kPost>(vec, kept, blocks, p, stream) : backward_mode<T, kPostPre>(vec, kept, blocks, p, stream);
+template <typename T> int backward(int mode, bool kept, const Shape& s, const BwdParams& p, cudaStream_t stream) {
+  if (mode == kPre) return kept ? backward_mode<T, kPre, true>(s, p, stream) : backward_mode<T, kPre, false>(s, p, stream);
+  if (mode == kPost) return kept ? backward_mode<T, kPost, true>(s, p, stream) : backward_mode<T, kPost, false>(s, p, stream);
+  return kept ? backward_mode<T, kPostPre, true>(s, p, stream) : backward_mode<T, kPostPre, false>(s, p, stream);
 }
 
 }  // namespace norms
