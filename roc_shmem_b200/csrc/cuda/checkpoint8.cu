@@ -24,8 +24,7 @@ template <typename T, bool kVec> __global__ void __launch_bounds__(kThreads) sto
   const long long row = i / p.eights;
   const int col = (int)(i - row * p.eights) * 8;
   const int n = row < p.rows ? p.n : 0;
-  float v[8];
-  unpack(load8<kVec>(static_cast<const T*>(p.x) + (n ? row * p.ldx : 0), col, n), v);
+  const Vals v = unpack(load8<kVec>(static_cast<const T*>(p.x) + (n ? row * p.ldx : 0), col, n));
   uint32_t e;
   const uint2 q = encode8<T>(v, e);
   if (col < n) {
@@ -44,8 +43,7 @@ template <typename T, bool kVec> __global__ void __launch_bounds__(kThreads) res
   if (row >= p.rows) return;
   const int col = (int)(i - row * p.eights) * 8;
   if (col >= p.n) return;
-  float v[8];
-  decode8(__ldg(reinterpret_cast<const uint2*>(p.q + row * p.ldq + col)), __ldg(p.e + row * p.lde + col / 128), v);
+  const Vals v = decode8(__ldg(reinterpret_cast<const uint2*>(p.q + row * p.ldq + col)), __ldg(p.e + row * p.lde + col / 128));
   store8<kVec>(static_cast<T*>(p.x) + row * p.ldx, col, p.n, pack<T>(v));
 }
 
@@ -59,7 +57,7 @@ struct SwigluParams {
   long long eights;                                   // of a row of gu, in whole blocks of 128 columns
 };
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
+__device__ __forceinline__ float2 sigmoid2(float2 x) { return make_float2(1.f / (1.f + __expf(-x.x)), 1.f / (1.f + __expf(-x.y))); }
 
 // Thread i has eight columns of gu; four threads in a row have a gate, the next four its `up`, which they swap.
 __global__ void __launch_bounds__(kThreads) swiglu_store8_kernel(const SwigluParams p) {
@@ -70,8 +68,7 @@ __global__ void __launch_bounds__(kThreads) swiglu_store8_kernel(const SwigluPar
   const int col = (int)(i - row * p.eights) * 8;
   const int n = row < p.rows ? 2 * p.F : 0;
   const Raw8<__nv_bfloat16> r = load8<true>(p.gu + (n ? row * n : 0), col, n);
-  float v[8], u[8];
-  unpack(r, v);
+  const Vals v = unpack(r);
   uint32_t e;
   const uint2 q = encode8<__nv_bfloat16>(v, e);
   const uint4 w = r.get(0);
@@ -82,9 +79,9 @@ __global__ void __launch_bounds__(kThreads) swiglu_store8_kernel(const SwigluPar
   *reinterpret_cast<uint2*>(p.q + row * n + col) = q;
   if (col % 128 == 0) p.e[row * p.lde + col / 128] = (uint8_t)e;
   if (col & 32) return;
-  unpack(other, u);
+  Vals u = unpack(other);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) u[j] *= v[j] * sigmoid(v[j]);
+  for (int j = 0; j < 4; ++j) u.p[j] = mul2(u.p[j], mul2(v.p[j], sigmoid2(v.p[j])));
   store8<true>(p.act + row * p.F, col / 64 * 32 + col % 32, p.F, pack<__nv_bfloat16>(u));
 }
 
@@ -100,22 +97,21 @@ template <bool kAct> __global__ void __launch_bounds__(kThreads) swiglu_backward
   const int at = col / 32 * 64 + col % 32;
   const uint8_t* q = p.q + row * 2 * p.F + at;
   const uint32_t e = __ldg(p.e + row * p.lde + at / 128);
-  float g[8], u[8], d[8];
-  decode8(__ldg(reinterpret_cast<const uint2*>(q)), e, g);
-  decode8(__ldg(reinterpret_cast<const uint2*>(q + 32)), e, u);
-  unpack(load8<true>(p.dact + row * p.F, col, p.F), d);
-  float dg[8], du[8];
+  const Vals g = decode8(__ldg(reinterpret_cast<const uint2*>(q)), e), u = decode8(__ldg(reinterpret_cast<const uint2*>(q + 32)), e);
+  const Vals d = unpack(load8<true>(p.dact + row * p.F, col, p.F));
+  Vals dg, du, again;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float s = sigmoid(g[j]), silu = g[j] * s;
-    du[j] = d[j] * silu;
-    dg[j] = d[j] * u[j] * s * (1.f + g[j] * (1.f - s));
-    u[j] *= silu;
+  for (int j = 0; j < 4; ++j) {
+    const float2 s = sigmoid2(g.p[j]), silu = mul2(g.p[j], s);
+    du.p[j] = mul2(d.p[j], silu);
+    again.p[j] = mul2(u.p[j], silu);
+    // s (1 + g (1 - s)) = s + silu (1 - s)
+    dg.p[j] = mul2(mul2(d.p[j], u.p[j]), fma2(silu, make_float2(1.f - s.x, 1.f - s.y), s));
   }
   __nv_bfloat16* o = p.dgu + row * 2 * p.F + at;
   store8<true>(o, 0, 8, pack<__nv_bfloat16>(dg));
   store8<true>(o, 32, 40, pack<__nv_bfloat16>(du));
-  if constexpr (kAct) store8<true>(p.act + row * p.F, col, p.F, pack<__nv_bfloat16>(u));
+  if constexpr (kAct) store8<true>(p.act + row * p.F, col, p.F, pack<__nv_bfloat16>(again));
 }
 
 template <typename K, typename P> int launch(K* kernel, long long threads, const P& p, void* stream) {

@@ -92,7 +92,7 @@ bool aligned(const Mat& m, int size) { return aligned(m.p) && (m.ld * size) % 16
 int groups_of(long long rows, int n, int* groups) {
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  const Shape s = backward_shape(rows, n, false, sms, [](int) { return 1; });
+  const Shape s = backward_shape(rows, n, false, sms, [](int) { return 1; }, [](int) { return 0; });
   *groups = s.blocks * s.rows;
   return 0;
 }
@@ -235,7 +235,8 @@ int bshmem_norm_bwd(int what, const void* dout, const void* dh, const void* z, l
     if (c.gate == kElement) vec = vec && aligned(p.gate, c.gate_f32 ? 4 : c.size) && aligned(p.dgate, c.gate_f32 ? 4 : c.size);
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const Shape shape = backward_shape(rows, n, vec, sms, [&](int chunks) { return backward_words(c.size, c.mode, c.kept, c.gate, c.gate_f32, chunks); });
+  const Shape shape = backward_shape(rows, n, vec, sms, [&](int chunks) { return backward_words(c.size, c.mode, c.kept, c.gate, c.gate_f32, chunks); },
+                                     [&](int chunks) { return backward_held(c.mode, chunks); });
   return c.type == 0 ? backward<__nv_bfloat16>(c.mode, c.kept, shape, p, s)
          : c.type == 1 ? backward<__half>(c.mode, c.kept, shape, p, s) : backward<float>(c.mode, c.kept, shape, p, s);
 }

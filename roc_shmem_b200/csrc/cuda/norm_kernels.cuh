@@ -69,15 +69,16 @@ template <typename T> __device__ __forceinline__ T* row_of(const Mat& m, long lo
 // shared memory (cp.async), so nothing but its own wait is between the copy and the use.
 enum Form : int { kScalar = 0, kDirect = 1, kRing = 2 };
 
-// The words of a thread in one stage of the ring, [stage][word][thread].
+// The words of a thread in one stage of the ring, [stage][word][thread].  A thread reads what it copied itself.
 struct Ring {
-  uint4* base;
+  uint4* mine;
   int words, threads, stages;
-  __device__ __forceinline__ uint32_t slot(int stage, int word) const {
-    return ptx::smem_u32(base + ((stage * words + word) * threads + threadIdx.y * blockDim.x + threadIdx.x));
+  __device__ __forceinline__ Ring(uint4* base, int w, int s) : words(w), threads(blockDim.x * blockDim.y), stages(s) {
+    mine = base + threadIdx.y * blockDim.x + threadIdx.x;
   }
-  __device__ __forceinline__ const uint4& at(int stage, int word) const {
-    return base[(stage * words + word) * threads + threadIdx.y * blockDim.x + threadIdx.x];
+  __device__ __forceinline__ uint4* at(int stage, int word) const { return mine + (stage * words + word) * threads; }
+  __device__ __forceinline__ void clear(int stage) const {
+    for (int i = 0; i < words; ++i) *at(stage, i) = make_uint4(0, 0, 0, 0);
   }
   // The oldest of `stages` rows on their way has arrived.
   __device__ __forceinline__ void wait() const {
@@ -85,50 +86,59 @@ struct Ring {
     else if (stages == 3) ptx::cp_async_wait<2>();
     else ptx::cp_async_wait<3>();
   }
+  template <typename T> __device__ __forceinline__ void fetch8(int stage, int word, const T* from) const {
+#pragma unroll
+    for (int i = 0; i < Raw8<T>::kWords; ++i) ptx::cp_async_16(ptx::smem_u32(at(stage, word + i)), reinterpret_cast<const uint4*>(from) + i);
+  }
+  template <typename T> __device__ __forceinline__ Vals get8(int stage, int word) const {
+    Raw8<T> v;
+#pragma unroll
+    for (int i = 0; i < Raw8<T>::kWords; ++i) v.set(i, *at(stage, word + i));
+    return unpack(v);
+  }
 };
 __device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
-template <typename T> __device__ __forceinline__ void fetch8(const Ring& r, int stage, int word, const T* row, int col) {
-#pragma unroll
-  for (int i = 0; i < Raw8<T>::kWords; ++i) ptx::cp_async_16(r.slot(stage, word + i), reinterpret_cast<const uint4*>(row + col) + i);
-}
-// Columns behind the last one were not fetched.
-template <typename T> __device__ __forceinline__ Raw8<T> fetched8(const Ring& r, int stage, int word, bool in) {
-  Raw8<T> v;
-#pragma unroll
-  for (int i = 0; i < Raw8<T>::kWords; ++i) v.set(i, in ? r.at(stage, word + i) : make_uint4(0, 0, 0, 0));
-  return v;
-}
+__device__ __forceinline__ float sum2(float2 v) { return v.x + v.y; }
 
 // ---- forward -------------------------------------------------------------------------------------------
 // A row stays in the registers of its threads, kChunks groups of eight columns for each, between the sums: memory is read once.
+// In a ring the weights (w1 times a gate per column, and w2) stay in registers too.
 template <typename T, int kMode, int kChunks, int kForm>
-__global__ void __launch_bounds__(kChunks == 4 ? 512 : 1024) norm_fwd_kernel(const Params p) {
-  constexpr bool kVec = kForm != kScalar;
+__global__ void __launch_bounds__(kForm == kDirect && kChunks == 1 ? 1024 : 512) norm_fwd_kernel(const Params p) {
+  constexpr bool kVec = kForm != kScalar, kHeld = kForm == kRing && kChunks <= 2;
   constexpr int W = Raw8<T>::kWords, kX = kMode == kPre ? 0 : kChunks * W, kGate = kX + kChunks * W;
   extern __shared__ uint4 ring_words[];
   __shared__ float sums[2 * kMaxWarps];
   RowSum sum(sums);
+  const Ring ring(ring_words, p.ring_words, p.stages);
+  if constexpr (kForm == kRing) {
+    for (int i = 0; i < p.stages; ++i) ring.clear(i);        // columns behind the last one are never fetched
+    __syncthreads();
+  }
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const float inv_n = 1.f / (float)p.n;
   const long long step = (long long)gridDim.x * blockDim.y;
-  const Ring ring = {ring_words, p.ring_words, (int)(blockDim.x * blockDim.y), p.stages};
+  auto column = [&](int i) { return (int)(threadIdx.x + i * blockDim.x) * 8; };
   auto fetch = [&](long long row, int stage) {
     if (row < p.rows) {
+      const T *y = row_of<T>(p.y, row), *x = row_of<T>(p.x, row);
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        const int col = (threadIdx.x + i * blockDim.x) * 8;
+        const int col = column(i);
         if (col < p.n) {
-          if constexpr (kMode != kPre) fetch8(ring, stage, i * W, row_of<T>(p.y, row), col);
-          fetch8(ring, stage, kX + i * W, row_of<T>(p.x, row), col);
+          if constexpr (kMode != kPre) ring.fetch8(stage, i * W, y + col);
+          ring.fetch8(stage, kX + i * W, x + col);
           if (kMode != kPre && p.gate_kind == kElement) {
-            if (p.gate_f32) fetch8(ring, stage, kGate + i * 2, row_of<float>(p.gate, row), col);
-            else fetch8(ring, stage, kGate + i * W, row_of<T>(p.gate, row), col);
+            if (p.gate_f32) ring.fetch8(stage, kGate + i * 2, row_of<float>(p.gate, row) + col);
+            else ring.fetch8(stage, kGate + i * W, row_of<T>(p.gate, row) + col);
           }
         }
       }
+    } else {
+      ring.clear(stage);
     }
     ptx::cp_async_commit();
   };
@@ -136,95 +146,102 @@ __global__ void __launch_bounds__(kChunks == 4 ? 512 : 1024) norm_fwd_kernel(con
   int stage = 0;
   if constexpr (kForm == kRing)
     for (int i = 0; i < p.stages; ++i) fetch(first + threadIdx.y + i * step, i);
+  const float scale0 = number<T>(p.scale, p.scale_f32, p.scale_value);
+  auto weight1 = [&](int i) {
+    Vals w = vector8<kVec, T>(p.w1, p.w1_f32, column(i), p.n);
+    if (p.gate_kind == kColumn) {
+      const Vals g = vector8<kVec, T>(p.gcol, p.gcol_f32, column(i), p.n);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w.p[j] = mul2(w.p[j], g.p[j]);
+    }
+    return w;
+  };
+  Vals held1[kHeld ? kChunks : 1], held2[kHeld ? kChunks : 1];
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      if constexpr (kMode != kPre) held1[i] = weight1(i);
+      if constexpr (kMode != kPost) held2[i] = vector8<kVec, T>(p.w2, p.w2_f32, column(i), p.n);
+    }
+  }
   for (; first < p.rows; first += step) {                    // the same for the whole block
     const bool live = first + threadIdx.y < p.rows;
     const long long row = live ? first + threadIdx.y : 0;
     const int n = live ? p.n : 0;
-    Raw8<T> ry[kChunks], rx[kChunks];
     if constexpr (kForm == kRing) ring.wait();
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int col = (threadIdx.x + i * blockDim.x) * 8;
-      if constexpr (kForm == kRing) {
-        if constexpr (kMode != kPre) ry[i] = fetched8<T>(ring, stage, i * W, col < n);
-        rx[i] = fetched8<T>(ring, stage, kX + i * W, col < n);
-      } else {
-        if constexpr (kMode != kPre) ry[i] = load8<kVec>(row_of<T>(p.y, row), col, n);
-        rx[i] = load8<kVec>(row_of<T>(p.x, row), col, n);
-      }
-    }
-    float z[kChunks][8];
+    Vals z[kChunks];
     if constexpr (kMode != kPre) {
-      float scale = number<T>(p.scale, p.scale_f32, p.scale_value);
-      if (p.gate_kind == kRow && live) scale *= p.gate_f32 ? row_of<float>(p.gate, row)[0] : to_float<T>(row_of<T>(p.gate, row)[0]);
-      float ss = 0.f;
+      Vals y[kChunks], x[kForm == kRing ? 1 : kChunks];
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        float v[8];
-        unpack(ry[i], v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+        if constexpr (kForm == kRing) {
+          y[i] = ring.get8<T>(stage, i * W);
+        } else {
+          y[i] = unpack(load8<kVec>(row_of<T>(p.y, row), column(i), n));
+          x[i] = unpack(load8<kVec>(row_of<T>(p.x, row), column(i), n));
+        }
       }
-      const float rstd = rsqrtf(fmaf(sum(ss), inv_n, p.eps));
+      float scale = scale0;
+      if (p.gate_kind == kRow && live) scale *= p.gate_f32 ? row_of<float>(p.gate, row)[0] : to_float<T>(row_of<T>(p.gate, row)[0]);
+      float2 ss = both(0.f);
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ss = fma2(y[i].p[j], y[i].p[j], ss);
+      const float rstd = rsqrtf(fmaf(sum(sum2(ss)), inv_n, p.eps));
       if (p.rstd1 && live && threadIdx.x == 0) p.rstd1[row] = rstd;
-      const float f = scale * rstd;
+      const float2 f = both(scale * rstd);
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        const int col = (threadIdx.x + i * blockDim.x) * 8;
-        float v[8], w[8];
-        unpack(ry[i], v);
+        const int col = column(i);
         if (p.q1) {
           uint32_t e;
-          const uint2 q = encode8<T>(v, e);
+          const uint2 q = encode8<T>(y[i], e);
           if (col < n) {
             *reinterpret_cast<uint2*>(p.q1 + row * p.ldq + col) = q;
             if (col % 128 == 0) p.e1[row * p.lde + col / 128] = (uint8_t)e;
           }
         }
-        vector8<kVec, T>(p.w1, p.w1_f32, col, n, w);
+        Vals w, r;
+        if constexpr (kHeld) w = held1[i];
+        else w = weight1(i);
+        if constexpr (kForm == kRing) r = ring.get8<T>(stage, kX + i * W);
+        else r = x[i];
+        if (p.gate_kind == kElement) {
+          Vals g;
+          if constexpr (kForm == kRing) g = p.gate_f32 ? ring.get8<float>(stage, kGate + i * 2) : ring.get8<T>(stage, kGate + i * W);
+          else g = p.gate_f32 ? unpack(load8<kVec>(row_of<float>(p.gate, row), col, n)) : unpack(load8<kVec>(row_of<T>(p.gate, row), col, n));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= w[j] * f;
-        if (p.gate_kind == kColumn) {
-          vector8<kVec, T>(p.gcol, p.gcol_f32, col, n, w);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] *= w[j];
-        } else if (p.gate_kind == kElement) {
-          if constexpr (kForm == kRing) {
-            if (p.gate_f32) unpack(fetched8<float>(ring, stage, kGate + i * 2, col < n), w);
-            else unpack(fetched8<T>(ring, stage, kGate + i * W, col < n), w);
-          } else {
-            if (p.gate_f32) unpack(load8<kVec>(row_of<float>(p.gate, row), col, n), w);
-            else unpack(load8<kVec>(row_of<T>(p.gate, row), col, n), w);
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] *= w[j];
+          for (int j = 0; j < 4; ++j) w.p[j] = mul2(w.p[j], g.p[j]);
         }
-        unpack(rx[i], w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += w[j];
-        const Raw8<T> o = pack<T>(v);
+        for (int j = 0; j < 4; ++j) r.p[j] = fma2(mul2(y[i].p[j], f), w.p[j], r.p[j]);
+        const Raw8<T> o = pack<T>(r);
         store8<kVec>(row_of<T>(p.out, row), col, n, o);
-        unpack(o, z[i]);                              // the next norm is one of the stored sum
+        if constexpr (kMode == kPostPre) z[i] = unpack(o);   // the next norm is one of the stored sum
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) unpack(rx[i], z[i]);
+      for (int i = 0; i < kChunks; ++i) {
+        if constexpr (kForm == kRing) z[i] = ring.get8<T>(stage, i * W);
+        else z[i] = unpack(load8<kVec>(row_of<T>(p.x, row), column(i), n));
+      }
     }
     if constexpr (kForm == kRing) {
       fetch(first + threadIdx.y + p.stages * step, stage);   // this thread has read its words of the stage
       if (++stage == p.stages) stage = 0;
     }
     if constexpr (kMode != kPost) {
-      float ss = 0.f;
+      float2 ss = both(0.f);
 #pragma unroll
       for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(z[i][j], z[i][j], ss);     // columns behind the last one are zero
-      const float rstd = rsqrtf(fmaf(sum(ss), inv_n, p.eps));
+        for (int j = 0; j < 4; ++j) ss = fma2(z[i].p[j], z[i].p[j], ss);   // columns behind the last one are zero
+      const float rstd = rsqrtf(fmaf(sum(sum2(ss)), inv_n, p.eps));
       if (p.rstd2 && live && threadIdx.x == 0) p.rstd2[row] = rstd;
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        const int col = (threadIdx.x + i * blockDim.x) * 8;
+        const int col = column(i);
         if (p.q2) {
           uint32_t e;
           const uint2 q = encode8<T>(z[i], e);
@@ -233,10 +250,11 @@ __global__ void __launch_bounds__(kChunks == 4 ? 512 : 1024) norm_fwd_kernel(con
             if (col % 128 == 0) p.e2[row * p.lde + col / 128] = (uint8_t)e;
           }
         }
-        float w[8];
-        vector8<kVec, T>(p.w2, p.w2_f32, col, n, w);
+        Vals w;
+        if constexpr (kHeld) w = held2[i];
+        else w = vector8<kVec, T>(p.w2, p.w2_f32, col, n);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] *= z[i][j] * rstd;
+        for (int j = 0; j < 4; ++j) w.p[j] = mul2(mul2(z[i].p[j], both(rstd)), w.p[j]);
         store8<kVec>(row_of<T>(p.h, row), col, n, pack<T>(w));
       }
     }
@@ -245,7 +263,7 @@ __global__ void __launch_bounds__(kChunks == 4 ? 512 : 1024) norm_fwd_kernel(con
 
 // ---- backward ------------------------------------------------------------------------------------------
 // A block walks over rows and keeps the column sums of its rows in registers; norm_bwd_finish_kernel adds up the groups' sums in
-// their order, so two calls give the same bits.
+// their order, so two calls give the same bits.  In a ring the weights are fp32 words of shared memory behind the stages.
 template <typename T, int kMode, int kChunks, int kForm, bool kKept8>
 __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
   constexpr bool kVec = kForm != kScalar;
@@ -254,39 +272,46 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
   constexpr int W = Raw8<T>::kWords, K = kKept8 ? 1 : W;
   constexpr int kDh = kMode == kPre ? 0 : kChunks * W, kZ = kDh + (kMode == kPost ? 0 : kChunks * W);
   constexpr int kY = kZ + (kMode == kPost ? 0 : kChunks * K), kRstd = kY + (kMode == kPre ? 0 : kChunks * K), kGate = kRstd + 1;
+  constexpr int kW2 = kMode == kPre ? 0 : kChunks * 2;       // words of the weights: w1 times a gate per column, w2
   extern __shared__ uint4 ring_words[];
   __shared__ float sums[2 * kMaxWarps];
   RowSum sum(sums);
+  const Ring ring(ring_words, p.ring_words, p.stages);
+  const Ring weights(ring_words + p.stages * p.ring_words * ring.threads, 0, 0);
+  if constexpr (kForm == kRing) {
+    for (int i = 0; i < p.stages; ++i) ring.clear(i);
+    __syncthreads();
+  }
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const float inv_n = 1.f / (float)p.n;
   const float scale = number<T>(p.scale, p.scale_f32, p.scale_value);
-  float acc_w2[kMode != kPost ? kChunks : 1][8], acc_c[kMode != kPre ? kChunks : 1][8], acc_s = 0.f;
+  Vals acc_w2[kMode != kPost ? kChunks : 1], acc_c[kMode != kPre ? kChunks : 1];
+  float acc_s = 0.f;
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (kMode != kPost) acc_w2[i][j] = 0.f;
-      if constexpr (kMode != kPre) acc_c[i][j] = 0.f;
-    }
+  for (int i = 0; i < kChunks; ++i) {
+    if constexpr (kMode != kPost) acc_w2[i].fill(0.f);
+    if constexpr (kMode != kPre) acc_c[i].fill(0.f);
+  }
   const long long step = (long long)gridDim.x * blockDim.y;
-  const Ring ring = {ring_words, p.ring_words, (int)(blockDim.x * blockDim.y), p.stages};
+  auto column = [&](int i) { return (int)(threadIdx.x + i * blockDim.x) * 8; };
   auto fetch_kept = [&](int stage, int word, const Mat& m, const uint8_t* q, const uint8_t* e, long long row, int col) {
     if constexpr (kKept8) {
       const uintptr_t at = reinterpret_cast<uintptr_t>(e + row * p.lde + col / 128);
-      cp_async_8(ring.slot(stage, word), q + row * p.ldq + col);
-      ptx::cp_async_4(ring.slot(stage, word) + 8, reinterpret_cast<const void*>(at & ~(uintptr_t)3));
+      const uint32_t slot = ptx::smem_u32(ring.at(stage, word));
+      cp_async_8(slot, q + row * p.ldq + col);
+      ptx::cp_async_4(slot + 8, reinterpret_cast<const void*>(at & ~(uintptr_t)3));
     } else {
-      fetch8(ring, stage, word, row_of<T>(m, row), col);
+      ring.fetch8(stage, word, row_of<T>(m, row) + col);
     }
   };
-  auto kept = [&](int stage, int word, const Mat& m, const uint8_t* q, const uint8_t* e, long long row, int col, int n, float (&v)[8]) {
+  auto kept = [&](int stage, int word, const Mat& m, const uint8_t* q, const uint8_t* e, long long row, int col, int n) {
     if constexpr (kForm == kRing && kKept8) {
-      const uint4 w = col < n ? ring.at(stage, word) : make_uint4(0, 0, 0, 0);
+      const uint4 w = *ring.at(stage, word);
       const uint32_t byte = (uint32_t)reinterpret_cast<uintptr_t>(e + row * p.lde + col / 128) & 3;
-      decode8(make_uint2(w.x, w.y), w.z >> (8 * byte) & 255, v);
+      return decode8(make_uint2(w.x, w.y), w.z >> (8 * byte) & 255);
     } else if constexpr (kForm == kRing) {
-      unpack(fetched8<T>(ring, stage, word, col < n), v);
+      return ring.get8<T>(stage, word);
     } else if constexpr (kKept8) {
       uint2 b = make_uint2(0, 0);
       uint32_t x = 1;
@@ -294,44 +319,66 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
         b = __ldg(reinterpret_cast<const uint2*>(q + row * p.ldq + col));
         x = __ldg(e + row * p.lde + col / 128);
       }
-      decode8(b, x, v);
+      return decode8(b, x);
     } else {
-      unpack(load8<kVec>(row_of<T>(m, row), col, n), v);
+      return unpack(load8<kVec>(row_of<T>(m, row), col, n));
     }
   };
-  auto plain = [&](int stage, int word, const Mat& m, long long row, int col, int n, float (&v)[8]) {
-    if constexpr (kForm == kRing) unpack(fetched8<T>(ring, stage, word, col < n), v);
-    else unpack(load8<kVec>(row_of<T>(m, row), col, n), v);
+  auto plain = [&](int stage, int word, const Mat& m, long long row, int col, int n) {
+    if constexpr (kForm == kRing) return ring.get8<T>(stage, word);
+    else return unpack(load8<kVec>(row_of<T>(m, row), col, n));
   };
   auto fetch = [&](long long row, int stage) {
     if (row < p.rows) {
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        const int col = (threadIdx.x + i * blockDim.x) * 8;
+        const int col = column(i);
         if (col < p.n) {
           if constexpr (kMode != kPre) {
-            if (p.dout.p) fetch8(ring, stage, i * W, row_of<T>(p.dout, row), col);
+            if (p.dout.p) ring.fetch8(stage, i * W, row_of<T>(p.dout, row) + col);
             fetch_kept(stage, kY + i * K, p.y, p.q1, p.e1, row, col);
             if (p.gate_kind == kElement) {
-              if (p.gate_f32) fetch8(ring, stage, kGate + i * 2, row_of<float>(p.gate, row), col);
-              else fetch8(ring, stage, kGate + i * W, row_of<T>(p.gate, row), col);
+              if (p.gate_f32) ring.fetch8(stage, kGate + i * 2, row_of<float>(p.gate, row) + col);
+              else ring.fetch8(stage, kGate + i * W, row_of<T>(p.gate, row) + col);
             }
           }
           if constexpr (kMode != kPost) {
-            fetch8(ring, stage, kDh + i * W, row_of<T>(p.dh, row), col);
+            ring.fetch8(stage, kDh + i * W, row_of<T>(p.dh, row) + col);
             fetch_kept(stage, kZ + i * K, p.z, p.q2, p.e2, row, col);
           }
         }
       }
-      if constexpr (kMode != kPre) ptx::cp_async_4(ring.slot(stage, kRstd), p.rstd1 + row);
-      if constexpr (kMode != kPost) ptx::cp_async_4(ring.slot(stage, kRstd) + 4, p.rstd2 + row);
+      const uint32_t slot = ptx::smem_u32(ring.at(stage, kRstd));
+      if constexpr (kMode != kPre) ptx::cp_async_4(slot, p.rstd1 + row);
+      if constexpr (kMode != kPost) ptx::cp_async_4(slot + 4, p.rstd2 + row);
+    } else {
+      ring.clear(stage);
     }
     ptx::cp_async_commit();
   };
   long long first = (long long)blockIdx.x * blockDim.y;
   int stage = 0;
-  if constexpr (kForm == kRing)
+  auto weight1 = [&](int i, int n) {
+    Vals w = vector8<kVec, T>(p.w1, p.w1_f32, column(i), n);
+    if (p.gate_kind == kColumn) {
+      const Vals g = vector8<kVec, T>(p.gcol, p.gcol_f32, column(i), n);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w.p[j] = mul2(w.p[j], g.p[j]);
+    }
+    return w;
+  };
+  auto hold = [&](int word, const Vals& v) {
+    weights.mine[word * weights.threads] = make_uint4(__float_as_uint(v.p[0].x), __float_as_uint(v.p[0].y), __float_as_uint(v.p[1].x), __float_as_uint(v.p[1].y));
+    weights.mine[(word + 1) * weights.threads] = make_uint4(__float_as_uint(v.p[2].x), __float_as_uint(v.p[2].y), __float_as_uint(v.p[3].x), __float_as_uint(v.p[3].y));
+  };
+  if constexpr (kForm == kRing) {
     for (int i = 0; i < p.stages; ++i) fetch(first + threadIdx.y + i * step, i);
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      if constexpr (kMode != kPre) hold(i * 2, weight1(i, p.n));
+      if constexpr (kMode != kPost) hold(kW2 + i * 2, vector8<kVec, T>(p.w2, p.w2_f32, column(i), p.n));
+    }
+  }
   for (; first < p.rows; first += step) {                    // the same for the whole block
     const bool live = first + threadIdx.y < p.rows;
     const long long row = live ? first + threadIdx.y : 0;
@@ -342,107 +389,95 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
     float rstd1 = 0.f, rstd2 = 0.f;
     if constexpr (kForm == kRing) {
       ring.wait();
-      const uint4 r = ring.at(stage, kRstd);
-      rstd1 = live ? __uint_as_float(r.x) : 0.f;
-      rstd2 = live ? __uint_as_float(r.y) : 0.f;
+      const uint4 r = *ring.at(stage, kRstd);
+      rstd1 = __uint_as_float(r.x);
+      rstd2 = __uint_as_float(r.y);
     } else {
       if constexpr (kMode != kPre) rstd1 = __ldg(p.rstd1 + row);
       if constexpr (kMode != kPost) rstd2 = __ldg(p.rstd2 + row);
     }
-    float dz[kChunks][8], ny[kMode != kPre ? kChunks : 1][8];
-    if constexpr (kMode != kPre) {
+    Vals dz[kChunks], ny[kMode != kPre ? kChunks : 1];
+    // in a ring the first norm's operands are read when it is their turn; elsewhere their loads begin here
+    auto first_norm = [&](int i) {
+      ny[i] = kept(stage, kY + i * K, p.y, p.q1, p.e1, row, column(i), n);
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int col = (threadIdx.x + i * blockDim.x) * 8;
-        kept(stage, kY + i * K, p.y, p.q1, p.e1, row, col, n, ny[i]);
-        if (p.dout.p) {
-          plain(stage, i * W, p.dout, row, col, n, dz[i]);
-        } else {
+      for (int j = 0; j < 4; ++j) ny[i].p[j] = mul2(ny[i].p[j], both(rstd1));
+    };
+    auto given = [&](int i) {
+      if (p.dout.p) dz[i] = plain(stage, i * W, p.dout, row, column(i), n);
+      else dz[i].fill(0.f);
+    };
+    if constexpr (kMode == kPost || (kMode == kPostPre && kForm != kRing)) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) dz[i][j] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ny[i][j] *= rstd1;
-      }
+      for (int i = 0; i < kChunks; ++i) { first_norm(i); given(i); }
     }
     if constexpr (kMode != kPost) {
-      float nz[kChunks][8], t[kChunks][8], dot = 0.f;
+      Vals nz[kChunks], t[kChunks];
+      float2 dot = both(0.f);
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        const int col = (threadIdx.x + i * blockDim.x) * 8;
-        kept(stage, kZ + i * K, p.z, p.q2, p.e2, row, col, n, nz[i]);
-        plain(stage, kDh + i * W, p.dh, row, col, n, t[i]);
+        nz[i] = kept(stage, kZ + i * K, p.z, p.q2, p.e2, row, column(i), n);
+        t[i] = plain(stage, kDh + i * W, p.dh, row, column(i), n);
       }
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        float w[8];
-        vector8<kVec, T>(p.w2, p.w2_f32, (threadIdx.x + i * blockDim.x) * 8, n, w);
+        Vals w;
+        if constexpr (kForm == kRing) w = weights.get8<float>(0, kW2 + i * 2);
+        else w = vector8<kVec, T>(p.w2, p.w2_f32, column(i), n);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          nz[i][j] *= rstd2;
-          acc_w2[i][j] = fmaf(t[i][j], nz[i][j], acc_w2[i][j]);
-          t[i][j] *= w[j];
-          dot = fmaf(t[i][j], nz[i][j], dot);
+        for (int j = 0; j < 4; ++j) {
+          nz[i].p[j] = mul2(nz[i].p[j], both(rstd2));
+          acc_w2[i].p[j] = fma2(t[i].p[j], nz[i].p[j], acc_w2[i].p[j]);
+          t[i].p[j] = mul2(t[i].p[j], w.p[j]);
+          dot = fma2(t[i].p[j], nz[i].p[j], dot);
         }
       }
-      const float mean = sum(dot) * inv_n;
+      const float mean = sum(sum2(dot)) * inv_n;
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
+        if constexpr (kMode == kPostPre && kForm == kRing) given(i);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float d = rstd2 * (t[i][j] - nz[i][j] * mean);
-          if constexpr (kMode == kPre) dz[i][j] = d;
-          else dz[i][j] += d;
+        for (int j = 0; j < 4; ++j) {
+          const float2 d = fma2(nz[i].p[j], both(-mean), t[i].p[j]);
+          if constexpr (kMode == kPre) dz[i].p[j] = mul2(d, both(rstd2));
+          else dz[i].p[j] = fma2(d, both(rstd2), dz[i].p[j]);
         }
-        store8<kVec>(row_of<T>(p.dz, row), (threadIdx.x + i * blockDim.x) * 8, n, pack<T>(dz[i]));
+        store8<kVec>(row_of<T>(p.dz, row), column(i), n, pack<T>(dz[i]));
       }
     }
     if constexpr (kMode != kPre) {
       // v = dz * g * w1 without the row's gate and the scale; its sum with ny gives both of the scalar gradients and dy's mean
-      float dot = 0.f;
+      float2 dot2 = both(0.f);
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        const int col = (threadIdx.x + i * blockDim.x) * 8;
-        float w[8], g[8];
-        vector8<kVec, T>(p.w1, p.w1_f32, col, n, w);
+        const int col = column(i);
+        if constexpr (kMode == kPostPre && kForm == kRing) first_norm(i);
+        Vals w;
+        if constexpr (kForm == kRing) w = weights.get8<float>(0, i * 2);
+        else w = weight1(i, n);
         if (p.gate_kind == kElement) {
-          if constexpr (kForm == kRing) {
-            if (p.gate_f32) unpack(fetched8<float>(ring, stage, kGate + i * 2, col < n), g);
-            else unpack(fetched8<T>(ring, stage, kGate + i * W, col < n), g);
-          } else {
-            if (p.gate_f32) unpack(load8<kVec>(row_of<float>(p.gate, row), col, n), g);
-            else unpack(load8<kVec>(row_of<T>(p.gate, row), col, n), g);
-          }
+          Vals g;
+          if constexpr (kForm == kRing) g = p.gate_f32 ? ring.get8<float>(stage, kGate + i * 2) : ring.get8<T>(stage, kGate + i * W);
+          else g = p.gate_f32 ? unpack(load8<kVec>(row_of<float>(p.gate, row), col, n)) : unpack(load8<kVec>(row_of<T>(p.gate, row), col, n));
           if (p.dgate.p) {
-            float d[8];
+            Vals d;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) d[j] = scale * w[j] * dz[i][j] * ny[i][j];
+            for (int j = 0; j < 4; ++j) d.p[j] = mul2(mul2(both(scale), w.p[j]), mul2(dz[i].p[j], ny[i].p[j]));
             if (p.gate_f32) store8<kVec>(row_of<float>(p.dgate, row), col, n, pack<float>(d));
             else store8<kVec>(row_of<T>(p.dgate, row), col, n, pack<T>(d));
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            dz[i][j] *= g[j];
-            acc_c[i][j] = fmaf(dz[i][j], ny[i][j], acc_c[i][j]);
-            dz[i][j] *= w[j];
-          }
-        } else {
-          if (p.gate_kind == kColumn) {
-            vector8<kVec, T>(p.gcol, p.gcol_f32, col, n, g);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] *= g[j];
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            acc_c[i][j] = fmaf(dz[i][j] * row_gate, ny[i][j], acc_c[i][j]);
-            dz[i][j] *= w[j];
-          }
+          for (int j = 0; j < 4; ++j) dz[i].p[j] = mul2(dz[i].p[j], g.p[j]);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dot = fmaf(dz[i][j], ny[i][j], dot);
+        for (int j = 0; j < 4; ++j) {
+          acc_c[i].p[j] = fma2(mul2(dz[i].p[j], both(row_gate)), ny[i].p[j], acc_c[i].p[j]);
+          dz[i].p[j] = mul2(dz[i].p[j], w.p[j]);
+          dot2 = fma2(dz[i].p[j], ny[i].p[j], dot2);
+        }
       }
       if constexpr (kForm == kRing) fetch(first + threadIdx.y + p.stages * step, stage);   // this thread has read its words
-      dot = sum(dot);
+      const float dot = sum(sum2(dot2));
       if (live) acc_s = fmaf(row_gate, dot, acc_s);
       if (p.gate_kind == kRow && p.dgate.p && live && threadIdx.x == 0) {
         if (p.gate_f32) row_of<float>(p.dgate, row)[0] = scale * dot;
@@ -452,10 +487,10 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
         const float f = rstd1 * scale * row_gate, mean = dot * inv_n;
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
-          float d[8];
+          Vals d;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) d[j] = f * (dz[i][j] - ny[i][j] * mean);
-          store8<kVec>(row_of<T>(p.dy, row), (threadIdx.x + i * blockDim.x) * 8, n, pack<T>(d));
+          for (int j = 0; j < 4; ++j) d.p[j] = mul2(fma2(ny[i].p[j], both(-mean), dz[i].p[j]), both(f));
+          store8<kVec>(row_of<T>(p.dy, row), column(i), n, pack<T>(d));
         }
       }
     } else if constexpr (kForm == kRing) {
@@ -467,28 +502,20 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
   const long long group = (long long)blockIdx.x * blockDim.y + threadIdx.y;
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
-    const int col = (threadIdx.x + i * blockDim.x) * 8;
+    const int col = column(i);
     const long long at = group * ((p.n + 7) / 8 * 8) + col;  // a group's sums are padded to whole eights
     if (col < p.n) {
       if constexpr (kMode != kPost)
-        if (p.part_w2) {
-          float4* o = reinterpret_cast<float4*>(p.part_w2 + at);
-          o[0] = make_float4(acc_w2[i][0], acc_w2[i][1], acc_w2[i][2], acc_w2[i][3]);
-          o[1] = make_float4(acc_w2[i][4], acc_w2[i][5], acc_w2[i][6], acc_w2[i][7]);
-        }
+        if (p.part_w2) store8<true>(p.part_w2 + at, 0, 8, pack<float>(acc_w2[i]));
       if constexpr (kMode != kPre)
-        if (p.part_c) {
-          float4* o = reinterpret_cast<float4*>(p.part_c + at);
-          o[0] = make_float4(acc_c[i][0], acc_c[i][1], acc_c[i][2], acc_c[i][3]);
-          o[1] = make_float4(acc_c[i][4], acc_c[i][5], acc_c[i][6], acc_c[i][7]);
-        }
+        if (p.part_c) store8<true>(p.part_c + at, 0, 8, pack<float>(acc_c[i]));
     }
   }
   if (kMode != kPre && p.part_s && threadIdx.x == 0) p.part_s[group] = acc_s;
 }
 
 // Threads of a row, rows of a block, eights of columns per thread and blocks for rows of n columns.
-struct Shape { int threads, rows, chunks, blocks, form, stages, words; };
+struct Shape { int threads, rows, chunks, blocks, form, stages, words, held; };
 constexpr int kMaxColumns = 16384;
 constexpr int kRingBytes = 216 * 1024;                // of a multiprocessor's shared memory, for all of its blocks
 
@@ -523,12 +550,15 @@ template <typename K, typename P> int launch(K* kernel, dim3 grid, dim3 block, i
   return 0;
 }
 
-// The ring of a block that shares its multiprocessor with `blocks - 1` others: as many stages as fit, up to four.  Fewer than two: none.
-inline void ring_of(Shape& s, int words, int blocks) {
+// The ring of a block that shares its multiprocessor with `blocks - 1` others: as many stages as fit beside `held` words of weights,
+// up to four.  Fewer than two: none.
+inline void ring_of(Shape& s, int words, int held, int blocks) {
   s.words = words;
-  s.stages = kRingBytes / blocks / (words * 16 * s.threads * s.rows);
+  s.held = held;
+  s.stages = (kRingBytes / blocks / (16 * s.threads * s.rows) - held) / words;
   if (s.stages > 4) s.stages = 4;
 }
+inline int shared_of(const Shape& s) { return (s.stages * s.words + s.held) * 16 * s.threads * s.rows; }
 
 // words(chunks): 16-byte words that a thread needs for one row.
 template <typename F> Shape forward_shape(long long rows, int n, bool vec, int sms, F words) {
@@ -541,10 +571,10 @@ template <typename F> Shape forward_shape(long long rows, int n, bool vec, int s
     if (s.rows > rows) s.rows = rows < 1 ? 1 : (int)rows;
   };
   if (vec) {
-    divide(2, 256);
-    const int per_sm = 1024 / (s.threads * s.rows);   // 64 registers a thread
+    divide(eights > 1024 ? 4 : 2, 256);
+    const int per_sm = 512 / (s.threads * s.rows);    // 128 registers a thread
     const long long most = (long long)sms * per_sm;
-    ring_of(s, words(2), per_sm);
+    ring_of(s, words(s.chunks), 0, per_sm);
     if (s.stages >= 2 && rows > 2 * most * s.rows) {
       s.form = kRing;
       s.blocks = (int)most;
@@ -557,7 +587,7 @@ template <typename F> Shape forward_shape(long long rows, int n, bool vec, int s
   s.blocks = (int)((rows + s.rows - 1) / s.rows);
   return s;
 }
-template <typename F> Shape backward_shape(long long rows, int n, bool vec, int sms, F words) {
+template <typename F, typename G> Shape backward_shape(long long rows, int n, bool vec, int sms, F words, G held) {
   const int eights = (n + 7) / 8;
   Shape s = {};
   s.chunks = eights > 1024 ? 4 : eights > 32 ? 2 : 1;
@@ -570,7 +600,7 @@ template <typename F> Shape backward_shape(long long rows, int n, bool vec, int 
   s.blocks = (int)(need < most ? need : most);
   s.form = vec ? kDirect : kScalar;
   if (vec && s.chunks <= 2) {
-    ring_of(s, words(s.chunks), per_sm);
+    ring_of(s, words(s.chunks), held(s.chunks), per_sm);
     if (s.stages >= 2 && need > most) s.form = kRing;
   }
   return s;
@@ -585,7 +615,8 @@ template <typename T, int kMode> int forward_mode(bool vec, Params p, cudaStream
   if (s.form == kRing) {
     p.stages = s.stages;
     p.ring_words = s.words;
-    return launch(norm_fwd_kernel<T, kMode, 2, kRing>, grid, block, s.stages * s.words * 16 * s.threads * s.rows, p, stream);
+    if (s.chunks == 2) return launch(norm_fwd_kernel<T, kMode, 2, kRing>, grid, block, shared_of(s), p, stream);
+    return launch(norm_fwd_kernel<T, kMode, 4, kRing>, grid, block, shared_of(s), p, stream);
   }
   if (s.form == kScalar) return launch(norm_fwd_kernel<T, kMode, 4, kScalar>, grid, block, 0, p, stream);
   if (s.chunks == 1) return launch(norm_fwd_kernel<T, kMode, 1, kDirect>, grid, block, 0, p, stream);
@@ -596,12 +627,13 @@ inline int backward_words(int size, int mode, bool kept, int gate_kind, bool gat
   const int W = size / 2, K = kept ? 1 : W;
   return chunks * ((mode == kPostPre ? 2 : 1) * (W + K) + (gate_kind != kElement ? 0 : gate_f32 ? 2 : W)) + 1;
 }
+inline int backward_held(int mode, int chunks) { return chunks * 2 * (mode == kPostPre ? 2 : 1); }
 template <typename T, int kMode, bool kKept> int backward_mode(const Shape& s, BwdParams p, cudaStream_t stream) {
   const dim3 grid((unsigned)s.blocks), block(s.threads, s.rows);
   if (s.form == kRing) {
     p.stages = s.stages;
     p.ring_words = s.words;
-    const int shared = s.stages * s.words * 16 * s.threads * s.rows;
+    const int shared = shared_of(s);
     if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kRing, kKept>, grid, block, shared, p, stream);
     return launch(norm_bwd_kernel<T, kMode, 2, kRing, kKept>, grid, block, shared, p, stream);
   }

@@ -21,6 +21,32 @@ template <> __device__ __forceinline__ float from_float(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 
+// ---- two fp32 values at a time -------------------------------------------------------------------
+// One instruction for two: these kernels issue more than they wait for.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// Eight neighbouring values, as pairs.
+struct Vals {
+  float2 p[4];
+  __device__ __forceinline__ void fill(float v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = both(v);
+  }
+};
+
 // Eight values as they lie in memory: one 16-byte word of a 2-byte type, two of fp32.
 template <typename T> struct alignas(16) Raw8 {
   static constexpr int kWords = sizeof(T) / 2;
@@ -33,14 +59,40 @@ template <typename T> struct alignas(16) Raw8 {
   }
 };
 
-template <typename T> __device__ __forceinline__ void unpack(const Raw8<T>& r, float (&v)[8]) {
+template <typename T> __device__ __forceinline__ Vals unpack(const Raw8<T>& r) {
+  Vals v;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = to_float<T>(r.v[i]);
+  for (int i = 0; i < 4; ++i) v.p[i] = make_float2(to_float<T>(r.v[2 * i]), to_float<T>(r.v[2 * i + 1]));
+  return v;
 }
-template <typename T> __device__ __forceinline__ Raw8<T> pack(const float (&v)[8]) {
+template <> __device__ __forceinline__ Vals unpack(const Raw8<__half>& r) {
+  Vals v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v.p[i] = __half22float2(__halves2half2(r.v[2 * i], r.v[2 * i + 1]));
+  return v;
+}
+template <typename T> __device__ __forceinline__ Raw8<T> pack(const Vals& v) {
   Raw8<T> r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r.v[i] = from_float<T>(v[i]);
+  for (int i = 0; i < 4; ++i) { r.v[2 * i] = from_float<T>(v.p[i].x); r.v[2 * i + 1] = from_float<T>(v.p[i].y); }
+  return r;
+}
+template <> __device__ __forceinline__ Raw8<__nv_bfloat16> pack(const Vals& v) {
+  Raw8<__nv_bfloat16> r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 t = __float22bfloat162_rn(v.p[i]);
+    r.v[2 * i] = t.x; r.v[2 * i + 1] = t.y;
+  }
+  return r;
+}
+template <> __device__ __forceinline__ Raw8<__half> pack(const Vals& v) {
+  Raw8<__half> r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 t = __float22half2_rn(v.p[i]);
+    r.v[2 * i] = __low2half(t); r.v[2 * i + 1] = __high2half(t);
+  }
   return r;
 }
 
@@ -69,16 +121,13 @@ template <bool kVec, typename T> __device__ __forceinline__ void store8(T* row, 
   }
 }
 
-// A vector over the columns (a weight, a gate per channel) in the rows' own type T or in fp32.
-template <bool kVec, typename T> __device__ __forceinline__ void vector8(const void* vec, bool f32, int col, int n, float (&v)[8]) {
-  if (!vec) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 1.f;
-  } else if (f32) {
-    unpack(load8<kVec>(static_cast<const float*>(vec), col, n), v);
-  } else {
-    unpack(load8<kVec>(static_cast<const T*>(vec), col, n), v);
-  }
+// A vector over the columns (a weight, a gate per channel) in the rows' own type T or in fp32; ones where there is none.
+template <bool kVec, typename T> __device__ __forceinline__ Vals vector8(const void* vec, bool f32, int col, int n) {
+  Vals v;
+  if (!vec) v.fill(1.f);
+  else if (f32) v = unpack(load8<kVec>(static_cast<const float*>(vec), col, n));
+  else v = unpack(load8<kVec>(static_cast<const T*>(vec), col, n));
+  return v;
 }
 
 // ---- activations in 8 bits -------------------------------------------------------------------------
@@ -98,7 +147,8 @@ template <typename T> constexpr uint32_t kTopExponent = 247;
 template <> constexpr uint32_t kTopExponent<__half> = 135;
 
 // All 32 lanes take part.  The eight bytes of this lane's values, which are of type T, and the block's exponent byte.
-template <typename T> __device__ __forceinline__ uint2 encode8(const float (&v)[8], uint32_t& e) {
+template <typename T> __device__ __forceinline__ uint2 encode8(const Vals& pairs, uint32_t& e) {
+  const float v[8] = {pairs.p[0].x, pairs.p[0].y, pairs.p[1].x, pairs.p[1].y, pairs.p[2].x, pairs.p[2].y, pairs.p[3].x, pairs.p[3].y};
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -130,7 +180,8 @@ template <typename T> __device__ __forceinline__ uint2 encode8(const float (&v)[
   }
   return make_uint2(out[0], out[1]);
 }
-__device__ __forceinline__ void decode8(uint2 q, uint32_t e, float (&v)[8]) {
+__device__ __forceinline__ Vals decode8(uint2 q, uint32_t e) {
+  Vals v;
   const float up = block_scale_bits(e);
   const uint32_t w[2] = {q.x, q.y};
 #pragma unroll
@@ -142,9 +193,9 @@ __device__ __forceinline__ void decode8(uint2 q, uint32_t e, float (&v)[8]) {
       __half2 pair;
       memcpy(&pair, &two, 4);
       const float2 f = __half22float2(pair);
-      v[4 * h + 2 * i] = mul_exact(f.x, up);
-      v[4 * h + 2 * i + 1] = mul_exact(f.y, up);
+      v.p[2 * h + i] = make_float2(mul_exact(f.x, up), mul_exact(f.y, up));
     }
+  return v;
 }
 
 // ---- sums over a row -----------------------------------------------------------------------------------
@@ -158,16 +209,16 @@ struct RowSum {
   __device__ __forceinline__ float operator()(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    const int warps = blockDim.x >> 5;
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
     if (warps == 1) return v;
-    float* mine = words + turn * kMaxWarps;
+    float* mine = words + turn * kMaxWarps + threadIdx.y * warps;
     turn ^= 1;
-    const int first = threadIdx.y * warps;
-    if ((threadIdx.x & 31) == 0) mine[first + (threadIdx.x >> 5)] = v;
+    if (lane == 0) mine[threadIdx.x >> 5] = v;
     __syncthreads();
-    float s = 0.f;
-    for (int i = 0; i < warps; ++i) s += mine[first + i];
-    return s;
+    v = lane < warps ? mine[lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
   }
 };
 
