@@ -1,0 +1,349 @@
+// w4_stream.cuh — out[T, N] = x[T, K] · w[N, K]^T with weights of 4 bits on the tcgen05 tensor cores:
+//
+//   w[n, k] = (q[n, k] - z[n, k / group]) * s[n, k / group],   q in 0..15, z in 0..15 (8 where there is none), s bf16
+//
+// The weights are read once, half a byte each, and what counts besides is how many instructions turn one into an operand.  A
+// tile is 128 weight rows (the MMA's M) times up to 64 tokens (its N); a k-block is 128 columns.  A thread widens half a row of a
+// k-block: a nibble becomes a bf16 by or-ing it into the mantissa of 128, and 128 + q - (128 + z) is exact.  The pairs that come
+// out, columns (0,4) (1,5) (2,6) (3,7) of every eight, go to tensor memory as operand A as they are, and the activations'
+// columns are put into the same order where they lie in shared memory.  The scales never touch the weights: each group has an
+// accumulator of its own, which the thread of the row multiplies by its scale and adds up in fp32 registers.
+//
+//   warp 0      TMA producer: {128 rows x 64 bytes of weights, tokens x 128 columns} per stage, plain loads of local memory
+//   warp 1      MMA issuer: tcgen05.mma M128 x N=tokens x K16, A in tensor memory, B in shared memory
+//   warps 2-9   widen k-block i into one of two A buffers while the MMAs of i - 1 run, then add its accumulators up
+//
+// A cluster of up to 8 CTAs splits the columns of a tile where tiles are few, and adds the parts through distributed shared memory
+// in the CTAs' order: reproducible bits, no workspace.  Every wait is bounded (see gemm_core.cuh).
+#pragma once
+#include <cuda_bf16.h>
+
+#include <cstring>
+
+#include "gemm_pair.cuh"
+#include "tma_host.h"
+
+namespace bshmem {
+namespace w4 {
+
+using gemm::Guard;
+using gemm2::cluster_ctarank;
+using gemm2::cluster_sync_all;
+using gemm2::ld_cluster_f4;
+using gemm2::mapa;
+using gemm2::warp_wait;
+
+constexpr int ROWS = 128, BK = 128;                  // weight rows of a tile, columns of a k-block
+constexpr int MAX_TOKENS = 64;                       // of a tile
+constexpr int MAX_STAGES = 8, WIDENERS = 8;          // warps that widen
+constexpr int THREADS = 32 * (2 + WIDENERS);
+constexpr uint32_t W_BYTES = ROWS * BK / 2;          // 8 KiB of weights per stage
+constexpr uint32_t CTRL_BYTES = 256;
+constexpr uint32_t SMEM_HALF = 112u << 10, SMEM_FULL = 224u << 10;       // two CTAs share an SM, or one has it
+enum ErrSite : int { ERR_PRODUCER_EMPTY = 401, ERR_MMA_A = 402, ERR_WIDEN_FULL = 403, ERR_WIDEN_DONE = 404 };
+
+struct Params {
+  CUtensorMap map_w, map_x;      // weights [N, K / 2] bytes, box {64, 128}; tokens [T, K], box {64, nt}
+  const void* x; long long ldx;  // for the host
+  const __nv_bfloat16* s;
+  const uint8_t* z;              // null: 8 everywhere
+  __nv_bfloat16* out;            // [T, N]
+  long long ldo;
+  int T, N, K, group;
+  int stages, split;
+  uint32_t tmem_cols;
+  unsigned long long timeout_ns;
+};
+
+__device__ int error_word;        // site of the first wait that ran out, 0: none
+
+__host__ __device__ constexpr uint32_t stage_bytes(int nt) { return W_BYTES + (uint32_t)nt * BK * 2; }
+__host__ __device__ constexpr uint32_t smem_bytes(int nt, int stages) { return stages * stage_bytes(nt) + CTRL_BYTES + 1024; }
+// Tensor memory: two A buffers of 64 columns, then two sets of `subs` accumulators of nt columns.
+__host__ __device__ constexpr uint32_t tmem_cols(int nt, int subs) { return 128 + 2 * subs * nt <= 256 ? 256 : 512; }
+
+__device__ __forceinline__ __nv_bfloat162 as_pair(uint32_t w) {
+  __nv_bfloat162 p;
+  memcpy(&p, &w, 4);
+  return p;
+}
+__device__ __forceinline__ uint32_t as_word(__nv_bfloat162 p) {
+  uint32_t w;
+  memcpy(&w, &p, 4);
+  return w;
+}
+// Eight nibbles n0 .. n7 as bf16 pairs (n0, n4), (n1, n5), (n2, n6), (n3, n7), less `off` = 128 + z in both halves.
+__device__ __forceinline__ void widen(uint32_t w, __nv_bfloat162 off, uint32_t* o) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t v;
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(v) : "r"(w >> (4 * i)));      // (w & mask) | 128.0 in one
+    o[i] = as_word(__hsub2(as_pair(v), off));
+  }
+}
+// The same order of eight activations.
+__device__ __forceinline__ uint4 pair_up(uint4 v) {
+  return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t at, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+        "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem desc]
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
+struct Smem {
+  uint32_t base, stage, ctrl;    // 1024-byte aligned base, bytes of a stage, control block
+  uint8_t* gen;                  // generic pointer to the control block
+  __device__ __forceinline__ uint32_t w(int s) const { return base + s * stage; }
+  __device__ __forceinline__ uint32_t x(int s) const { return base + s * stage + W_BYTES; }
+  __device__ __forceinline__ uint32_t full(int s) const { return ctrl + 8 * s; }
+  __device__ __forceinline__ uint32_t empty(int s) const { return ctrl + 8 * (MAX_STAGES + s); }
+  __device__ __forceinline__ uint32_t wide(int b) const { return ctrl + 8 * (2 * MAX_STAGES + b); }        // A buffer b is written
+  __device__ __forceinline__ uint32_t done(int b) const { return ctrl + 8 * (2 * MAX_STAGES + 2 + b); }    // its MMAs are done
+  __device__ __forceinline__ uint32_t tmem_slot() const { return ctrl + 8 * (2 * MAX_STAGES + 4); }
+  __device__ __forceinline__ volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(gen + 8 * (2 * MAX_STAGES + 5)); }
+};
+
+// kNt: tokens of the tile (16, 32 or 64).  kSubs: groups of a k-block (1 for groups of 128 columns and more, 2, 4).
+template <int kNt, int kSubs>
+__global__ void __launch_bounds__(THREADS, 2) w4_stream_kernel(const __grid_constant__ Params p) {
+  static_assert(128 + 2 * kSubs * kNt <= 512, "tensor memory");
+  extern __shared__ uint8_t smem_raw[];
+  Smem L;
+  {
+    const uint32_t r = ptx::smem_u32(smem_raw);
+    L.base = (r + 1023u) & ~1023u;
+    L.stage = stage_bytes(kNt);
+    L.ctrl = L.base + p.stages * L.stage;
+    L.gen = smem_raw + (L.ctrl - r);
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, split = p.split;
+  const int rank = split > 1 ? (int)cluster_ctarank() : 0;
+  const int n0 = (int)(blockIdx.x / split) * ROWS, tok0 = (int)blockIdx.y * kNt;
+  const int kb_all = (p.K + BK - 1) / BK, kb0 = kb_all * rank / split, kb1 = kb_all * (rank + 1) / split;
+  Guard g{&error_word, L.abort_flag(), p.timeout_ns};
+
+  if (threadIdx.x == 0) {
+    *L.abort_flag() = 0;
+    for (int s = 0; s < p.stages; ++s) { ptx::mbar_init(L.full(s), 1); ptx::mbar_init(L.empty(s), 1); }
+    for (int b = 0; b < 2; ++b) { ptx::mbar_init(L.wide(b), WIDENERS); ptx::mbar_init(L.done(b), 1); }
+    ptx::fence_mbar_init();
+    ptx::prefetch_tensormap(&p.map_w);
+    ptx::prefetch_tensormap(&p.map_x);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(L.tmem_slot(), p.tmem_cols);
+    ptx::tmem_relinquish();
+  }
+  // The first weights start on their way to L2 while the previous kernel still runs; a prefetch reads nothing.
+  if (warp == 2 && lane == 0)
+    for (int kb = kb0; kb < min(kb1, kb0 + p.stages); ++kb) ptx::tma_prefetch_2d(&p.map_w, kb * (BK / 2), n0);
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(L.tmem_slot()));
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+
+  if (warp == 0) {
+    const bool leader = ptx::elect_one();
+    int s = 0; uint32_t ph = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!warp_wait(L.empty(s), ph ^ 1, g, ERR_PRODUCER_EMPTY)) break;
+      if (leader) {
+        ptx::mbar_arrive_expect_tx(L.full(s), L.stage);
+        ptx::tma_load_2d(L.w(s), &p.map_w, L.full(s), kb * (BK / 2), n0);
+        ptx::tma_load_2d(L.x(s), &p.map_x, L.full(s), kb * BK, tok0);
+        ptx::tma_load_2d(L.x(s) + kNt * 128, &p.map_x, L.full(s), kb * BK + 64, tok0);
+      }
+      if (++s == p.stages) { s = 0; ph ^= 1; }
+    }
+  } else if (warp == 1) {
+    const bool leader = ptx::elect_one();
+    constexpr uint32_t idesc = ptx::umma_idesc(1, 1, ROWS, kNt);
+    int s = 0;
+    for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+      const int b = i & 1;
+      if (!warp_wait(L.wide(b), (i >> 1) & 1, g, ERR_MMA_A)) break;
+      ptx::tc_fence_after();
+      if (leader) {
+        const uint32_t a = tmem + b * 64, d = tmem + 128 + b * kSubs * kNt;
+        const uint64_t dx = ptx::umma_desc_sw128(L.x(s));
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k) {
+          constexpr int kPer = BK / 16 / kSubs;       // MMAs of a group
+          umma_f16_ts(d + k / kPer * kNt, a + k * 8, dx + (k / 4) * (kNt * 128 / 16) + (k % 4) * 2, idesc, k % kPer ? 1u : 0u);
+        }
+        ptx::umma_commit(L.empty(s));
+        ptx::umma_commit(L.done(b));
+      }
+      __syncwarp();
+      if (++s == p.stages) s = 0;
+    }
+  } else {
+    // Thread (row, half): columns half * 64 .. + 63 of the row when it widens, tokens half * kNt / 2 .. when it adds up.
+    constexpr int kHalf = kNt / 2, kZ = kSubs == 4 ? 2 : 1;      // zero points of half a row
+    const int quarter = warp & 3, half = (warp - 2) / 4, row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const int groups = p.K / p.group;
+    const long long at0 = (long long)min(n0 + row, p.N - 1) * groups;
+    float2 acc[kHalf / 2];
+#pragma unroll
+    for (int j = 0; j < kHalf / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+    // scales of the row's groups in a k-block, zero points of its half
+    auto load = [&](int kb, uint32_t (&sc)[kSubs], uint32_t (&zp)[kZ]) {
+      const int first = kSubs == 1 ? kb * BK / p.group : kb * kSubs;
+#pragma unroll
+      for (int j = 0; j < kSubs; ++j) sc[j] = __bfloat16_as_ushort(p.s[at0 + min(first + j, groups - 1)]);
+#pragma unroll
+      for (int j = 0; j < kZ; ++j) zp[j] = p.z ? p.z[at0 + min(first + (kSubs == 1 ? 0 : half * (kSubs / 2) + j), groups - 1)] : 8;
+    };
+    auto add_up = [&](int i, const uint32_t (&sc)[kSubs]) {
+      const int b = i & 1;
+      if (!warp_wait(L.done(b), (i >> 1) & 1, g, ERR_WIDEN_DONE)) return false;
+      ptx::tc_fence_after();
+#pragma unroll
+      for (int j = 0; j < kSubs; ++j) {
+        const uint32_t d = tmem + lanes + 128 + (b * kSubs + j) * kNt + half * kHalf;
+        const float f = __uint_as_float(sc[j] << 16);
+        uint32_t v[kHalf];
+        if constexpr (kHalf == 8) tmem_ld_32x32b_x8(d, v);
+        else if constexpr (kHalf == 16) ptx::tmem_ld_32x32b_x16(d, v);
+        else ptx::tmem_ld_32x32b_x32(d, v);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int t = 0; t < kHalf / 2; ++t)
+          acc[t] = fma2(make_float2(f, f), make_float2(__uint_as_float(v[2 * t]), __uint_as_float(v[2 * t + 1])), acc[t]);
+      }
+      return true;
+    };
+    uint32_t sc[kSubs], zp[kZ], sc_next[kSubs], zp_next[kZ], sc_last[kSubs];
+    bool ok = true;
+    if (kb0 < kb1) load(kb0, sc, zp);
+    int s = 0; uint32_t ph = 0;
+    const uint32_t swz = (row >> 1) & 3;              // the 64-byte swizzle of the weights' stage
+    for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+      load(min(kb + 1, kb1 - 1), sc_next, zp_next);
+      if (!warp_wait(L.full(s), ph, g, ERR_WIDEN_FULL)) { ok = false; break; }
+      const uint32_t from = L.w(s) + row * 64;
+      const uint4 w[2] = {ld_shared_v4(from + (((half * 2) ^ swz) << 4)), ld_shared_v4(from + (((half * 2 + 1) ^ swz) << 4))};
+      for (uint32_t e = (threadIdx.x - 64) * 16; e < kNt * BK * 2; e += WIDENERS * 32 * 16) st_shared_v4(L.x(s) + e, pair_up(ld_shared_v4(L.x(s) + e)));
+      ptx::fence_proxy_async_smem();                  // the MMAs read the activations through the async proxy
+      uint32_t o[32];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t z = zp[kZ == 2 ? j : 0];
+        const __nv_bfloat162 off = as_pair(0x43004300u | z | z << 16);
+        widen(w[j].x, off, o + j * 16);
+        widen(w[j].y, off, o + j * 16 + 4);
+        widen(w[j].z, off, o + j * 16 + 8);
+        widen(w[j].w, off, o + j * 16 + 12);
+      }
+      // the buffer's last MMAs, of k-block i - 2, are done: their sums have been added up
+      tmem_st_32x32b_x32(tmem + lanes + (i & 1) * 64 + half * 32, o);
+      tmem_st_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(L.wide(i & 1));
+      if (i > 0 && !add_up(i - 1, sc_last)) { ok = false; break; }
+#pragma unroll
+      for (int j = 0; j < kSubs; ++j) { sc_last[j] = sc[j]; sc[j] = sc_next[j]; }
+#pragma unroll
+      for (int j = 0; j < kZ; ++j) zp[j] = zp_next[j];
+      if (++s == p.stages) { s = 0; ph ^= 1; }
+    }
+    if (ok && kb0 < kb1) ok = add_up(kb1 - kb0 - 1, sc_last);
+    if (ok) {
+      if (split == 1) {
+        __nv_bfloat16* out = p.out + n0 + row;
+#pragma unroll
+        for (int t = 0; t < kHalf; ++t) {             // 32 lanes = 64 neighbouring bytes of a token's row
+          const int tok = tok0 + half * kHalf + t;
+          if (n0 + row < p.N && tok < p.T) out[tok * p.ldo] = __float2bfloat16_rn(t & 1 ? acc[t / 2].y : acc[t / 2].x);
+        }
+      } else {
+        // the part as [token][row] floats over the stages: all their loads have landed and all MMAs have read them
+        const uint32_t dst = L.base + row * 4 + half * kHalf * (ROWS * 4);
+#pragma unroll
+        for (int t = 0; t < kHalf; ++t)
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + t * (ROWS * 4)), "f"(t & 1 ? acc[t / 2].y : acc[t / 2].x) : "memory");
+      }
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (split > 1) {
+    cluster_sync_all();
+    if (!*L.abort_flag()) {
+      // four rows of a token per thread; the tokens go round the cluster's CTAs
+      const int tokens = min(kNt, p.T - tok0);
+      for (int t = rank + warp * split; t < tokens; t += split * (THREADS / 32)) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r = 0; r < split; ++r) {
+          const float4 a = ld_cluster_f4(mapa(L.base + t * (ROWS * 4) + lane * 16, r));
+          v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+        }
+        const float f[4] = {v.x, v.y, v.z, v.w};
+        __nv_bfloat16* dst = p.out + (tok0 + t) * p.ldo + n0 + lane * 4;
+        if (p.N % 4 == 0) {                           // the rows of `out` begin on 8 bytes
+          if (n0 + lane * 4 < p.N)
+            *reinterpret_cast<uint2*>(dst) = make_uint2(gemm::pack_bf16(f[0], f[1]), gemm::pack_bf16(f[2], f[3]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n0 + lane * 4 + j < p.N) dst[j] = __float2bfloat16_rn(f[j]);
+        }
+      }
+    }
+    cluster_sync_all();                               // nobody's shared memory goes away while it is being read
+  }
+  if (*L.abort_flag()) {
+    // let copies and MMAs that are still in flight land before shared and tensor memory go away
+    const unsigned long long t0 = ptx::globaltimer();
+    while (ptx::globaltimer() - t0 < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, p.tmem_cols);
+  }
+}
+
+}  // namespace w4
+}  // namespace bshmem

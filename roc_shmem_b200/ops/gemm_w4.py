@@ -28,7 +28,9 @@ def _lib() -> C.CDLL:
         VP, I, L = C.c_void_p, C.c_int, C.c_longlong
         lib.bshmem_w4_last_error.restype = C.c_char_p
         lib.bshmem_w4_few.restype = I
-        lib.bshmem_w4_few.argtypes = [VP, L, VP, VP, VP, VP, I, I, I, I, VP]
+        lib.bshmem_w4_few.argtypes = [VP, L, VP, VP, VP, VP, I, I, I, I, VP, I]
+        lib.bshmem_w4_error_site.restype = I
+        lib.bshmem_w4_error_site.argtypes = [I]
         lib.bshmem_w4_widen.restype = I
         lib.bshmem_w4_widen.argtypes = [VP, VP, VP, VP, I, I, I, VP]
         lib.bshmem_w4_quant.restype = I
@@ -136,8 +138,13 @@ def linear_w4(x: torch.Tensor, w: W4Tensor) -> torch.Tensor:
             _lib()
         out = torch.empty((T, N), dtype=torch.bfloat16, device=x.device)
         _check(_few(m.data_ptr(), m.stride(0) if T > 1 else K, w.q.data_ptr(), w.scales.data_ptr(), 0 if w.zeros is None else w.zeros.data_ptr(),
-                    out.data_ptr(), T, N, K, group, current_stream()), "linear_w4")
+                    out.data_ptr(), T, N, K, group, current_stream(), 2000), "linear_w4")
     return out if x.dim() == 2 else out.view(*x.shape[:-1], N)
+
+
+def w4_error_site(clear: bool = True) -> int:
+    """0 if no in-kernel bounded wait ran out since the last clear, else the site code."""
+    return int(_lib().bshmem_w4_error_site(int(clear)))
 
 
 class LinearW4(torch.nn.Module):
