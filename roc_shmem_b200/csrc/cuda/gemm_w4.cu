@@ -119,16 +119,16 @@ int launch(K* kernel, dim3 grid, int threads, int cluster, int shared, const P& 
   return 0;
 }
 
-// How many clusters of `size` blocks of `shared` bytes the device holds at once (clusters do not span GPCs).
-int resident(void (*kernel)(w4::Params), int dev, int form, int size, int shared, int sms) {
-  static std::atomic<int> cache[64][6][9];            // racing threads write the same number
-  std::atomic<int>& slot = cache[dev][form][size];
+// How many clusters of `size` blocks the device holds at once, one block per SM (clusters do not span GPCs).
+int resident(void (*kernel)(w4::Params), int dev, int size, int threads, int sms) {
+  static std::atomic<int> cache[64][9];               // racing threads write the same number; every form takes a whole SM
+  std::atomic<int>& slot = cache[dev][size];
   int n = slot.load(std::memory_order_relaxed);
   if (n) return n;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(size * sms));
-  cfg.blockDim = dim3(w4::THREADS);
-  cfg.dynamicSmemBytes = shared;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = w4::SMEM_BYTES;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)size; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -142,17 +142,9 @@ int resident(void (*kernel)(w4::Params), int dev, int form, int size, int shared
 template <int kNt, int kSubs> int stream_product(w4::Params& p, int sms, void* stream) {
   int dev = 0;
   BSHMEM_CUDA_TRY(cudaGetDevice(&dev));
-  p.tmem_cols = w4::tmem_cols(kNt, kSubs);
-  // A block that takes all of an SM's tensor memory takes its shared memory as well: two of them on an SM, of clusters that
-  // wait for one another's other blocks, could not both allocate.
-  const uint32_t room = p.tmem_cols == 512 ? w4::SMEM_FULL : w4::SMEM_HALF;
-  p.stages = (int)((room - w4::CTRL_BYTES - 1024) / w4::stage_bytes(kNt));
-  if (p.stages > w4::MAX_STAGES) p.stages = w4::MAX_STAGES;
-  const int shared = p.tmem_cols == 512 ? (int)w4::SMEM_FULL : (int)w4::smem_bytes(kNt, p.stages);
-  constexpr int kForm = (kNt == 16 ? 0 : kNt == 32 ? 1 : 2) * 2;
   static std::atomic<bool> prepared[64];
   if (!prepared[dev].load(std::memory_order_relaxed)) {
-    BSHMEM_CUDA_TRY(cudaFuncSetAttribute(w4::w4_stream_kernel<kNt, kSubs>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)w4::SMEM_FULL));
+    BSHMEM_CUDA_TRY(cudaFuncSetAttribute(w4::w4_stream_kernel<kNt, kSubs>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)w4::SMEM_BYTES));
     prepared[dev].store(true, std::memory_order_relaxed);
   }
   int rc = host::make_tmap_2d(&p.map_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.x, p.T, p.K, p.ldx, kNt, 64);
@@ -162,15 +154,15 @@ template <int kNt, int kSubs> int stream_product(w4::Params& p, int sms, void* s
   const long long tiles = (long long)((p.N + w4::ROWS - 1) / w4::ROWS) * chunks;
   long long best = 0;
   for (int s = 1; s <= 8; ++s) {
-    const long long at_once = resident(w4::w4_stream_kernel<kNt, kSubs>, dev, kForm + (p.tmem_cols == 512), s, shared, sms);
+    const long long at_once = resident(w4::w4_stream_kernel<kNt, kSubs>, dev, s, w4::threads(kNt), sms);
     const long long cost = (tiles + at_once - 1) / at_once * ((kb + s - 1) / s) + (s > 1 ? 4 : 0);
     if (s == 1 || cost < best) { best = cost; p.split = s; }
   }
 #ifdef W4_SPLIT
   p.split = W4_SPLIT;
 #endif
-  return launch(w4::w4_stream_kernel<kNt, kSubs>, dim3((unsigned)((p.N + w4::ROWS - 1) / w4::ROWS * p.split), (unsigned)chunks), w4::THREADS, p.split,
-                shared, p, stream);
+  return launch(w4::w4_stream_kernel<kNt, kSubs>, dim3((unsigned)((p.N + w4::ROWS - 1) / w4::ROWS * p.split), (unsigned)chunks), w4::threads(kNt), p.split,
+                w4::SMEM_BYTES, p, stream);
 }
 template <int kNt> int stream_groups(w4::Params& p, int sms, void* stream) {
   // four groups of 64 tokens, twice, would be more than tensor memory has

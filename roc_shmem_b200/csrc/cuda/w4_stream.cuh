@@ -3,7 +3,7 @@
 //   w[n, k] = (q[n, k] - z[n, k / group]) * s[n, k / group],   q in 0..15, z in 0..15 (8 where there is none), s bf16
 //
 // The weights are read once, half a byte each, and what counts besides is how many instructions turn one into an operand.  A
-// tile is 128 weight rows (the MMA's M) times up to 64 tokens (its N); a k-block is 128 columns.  A thread widens half a row of a
+// tile is 128 weight rows (the MMA's M) times up to 64 tokens (its N); a k-block is 128 columns.  A thread widens a row of a
 // k-block: a nibble becomes a bf16 by or-ing it into the mantissa of 128, and 128 + q - (128 + z) is exact.  The pairs that come
 // out, columns (0,4) (1,5) (2,6) (3,7) of every eight, go to tensor memory as operand A as they are, and the activations'
 // columns are put into the same order where they lie in shared memory.  The scales never touch the weights: each group has an
@@ -11,7 +11,12 @@
 //
 //   warp 0      TMA producer: {128 rows x 64 bytes of weights, tokens x 128 columns} per stage, plain loads of local memory
 //   warp 1      MMA issuer: tcgen05.mma M128 x N=tokens x K16, A in tensor memory, B in shared memory
-//   warps 2-9   widen k-block i into one of two A buffers while the MMAs of i - 1 run, then add its accumulators up
+//   next 16     four groups of four warps, each widens every fourth k-block and orders its activations (64 tokens: three groups)
+//   last 4      add the accumulators up
+//
+// From a k-block's arrival to its sums it takes a warp of each kind some 900 cycles, and HBM brings an SM the 8 KiB of the next in 370: so several
+// are on their way (kDepth of them in tensor memory), in the hands of different warps.  The ALU is behind that: seven shifts and
+// logical operations for eight weights at half the rate of the other pipes, 230 cycles for a k-block.
 //
 // A cluster of up to 8 CTAs splits the columns of a tile where tiles are few, and adds the parts through distributed shared memory
 // in the CTAs' order: reproducible bits, no workspace.  Every wait is bounded (see gemm_core.cuh).
@@ -35,12 +40,15 @@ using gemm2::warp_wait;
 
 constexpr int ROWS = 128, BK = 128;                  // weight rows of a tile, columns of a k-block
 constexpr int MAX_TOKENS = 64;                       // of a tile
-constexpr int MAX_STAGES = 8, WIDENERS = 8;          // warps that widen
-constexpr int THREADS = 32 * (2 + WIDENERS);
+constexpr int MAX_STAGES = 12, MAX_DEPTH = 6;
+constexpr int WIDENERS = 4, ADDERS = 4;              // warps of a group that widens, and warps that add up
+__host__ __device__ constexpr int widen_groups(int nt) { return nt == 64 ? 3 : 4; }          // the sums of 64 tokens take more registers
+__host__ __device__ constexpr int threads(int nt) { return 32 * (2 + WIDENERS * widen_groups(nt) + ADDERS); }
 constexpr uint32_t W_BYTES = ROWS * BK / 2;          // 8 KiB of weights per stage
-constexpr uint32_t CTRL_BYTES = 256;
-constexpr uint32_t SMEM_HALF = 112u << 10, SMEM_FULL = 224u << 10;       // two CTAs share an SM, or one has it
-enum ErrSite : int { ERR_PRODUCER_EMPTY = 401, ERR_MMA_A = 402, ERR_WIDEN_FULL = 403, ERR_WIDEN_DONE = 404 };
+constexpr uint32_t CTRL_BYTES = 512;
+constexpr uint32_t SMEM_BYTES = 224u << 10;          // one CTA has an SM, all of its tensor memory too
+constexpr uint32_t TMEM_COLS = 512;
+enum ErrSite : int { ERR_PRODUCER_EMPTY = 401, ERR_MMA_A = 402, ERR_WIDEN_FULL = 403, ERR_WIDEN_DONE = 404, ERR_MMA_ADDED = 405, ERR_ADD_DONE = 406 };
 
 struct Params {
   CUtensorMap map_w, map_x;      // weights [N, K / 2] bytes, box {64, 128}; tokens [T, K], box {64, nt}
@@ -50,17 +58,21 @@ struct Params {
   __nv_bfloat16* out;            // [T, N]
   long long ldo;
   int T, N, K, group;
-  int stages, split;
-  uint32_t tmem_cols;
+  int split;
   unsigned long long timeout_ns;
 };
 
 __device__ int error_word;        // site of the first wait that ran out, 0: none
 
 __host__ __device__ constexpr uint32_t stage_bytes(int nt) { return W_BYTES + (uint32_t)nt * BK * 2; }
-__host__ __device__ constexpr uint32_t smem_bytes(int nt, int stages) { return stages * stage_bytes(nt) + CTRL_BYTES + 1024; }
-// Tensor memory: two A buffers of 64 columns, then two sets of `subs` accumulators of nt columns.
-__host__ __device__ constexpr uint32_t tmem_cols(int nt, int subs) { return 128 + 2 * subs * nt <= 256 ? 256 : 512; }
+__host__ __device__ constexpr int stages(int nt) {
+  return (SMEM_BYTES - CTRL_BYTES - 1024) / stage_bytes(nt) < MAX_STAGES ? (SMEM_BYTES - CTRL_BYTES - 1024) / stage_bytes(nt) : MAX_STAGES;
+}
+// k-blocks in tensor memory, each with an A buffer of 64 columns and `subs` accumulators of nt.
+__host__ __device__ constexpr int block_cols(int nt, int subs) { return 64 + subs * nt; }
+__host__ __device__ constexpr int depth(int nt, int subs) {
+  return TMEM_COLS / block_cols(nt, subs) < MAX_DEPTH ? TMEM_COLS / block_cols(nt, subs) : MAX_DEPTH;
+}
 
 __device__ __forceinline__ __nv_bfloat162 as_pair(uint32_t w) {
   __nv_bfloat162 p;
@@ -133,23 +145,26 @@ struct Smem {
   __device__ __forceinline__ uint32_t x(int s) const { return base + s * stage + W_BYTES; }
   __device__ __forceinline__ uint32_t full(int s) const { return ctrl + 8 * s; }
   __device__ __forceinline__ uint32_t empty(int s) const { return ctrl + 8 * (MAX_STAGES + s); }
-  __device__ __forceinline__ uint32_t wide(int b) const { return ctrl + 8 * (2 * MAX_STAGES + b); }        // A buffer b is written
-  __device__ __forceinline__ uint32_t done(int b) const { return ctrl + 8 * (2 * MAX_STAGES + 2 + b); }    // its MMAs are done
-  __device__ __forceinline__ uint32_t tmem_slot() const { return ctrl + 8 * (2 * MAX_STAGES + 4); }
-  __device__ __forceinline__ volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(gen + 8 * (2 * MAX_STAGES + 5)); }
+  __device__ __forceinline__ uint32_t wide(int b) const { return ctrl + 8 * (2 * MAX_STAGES + b); }                  // A buffer b is written
+  __device__ __forceinline__ uint32_t done(int b) const { return ctrl + 8 * (2 * MAX_STAGES + MAX_DEPTH + b); }      // its MMAs are done
+  __device__ __forceinline__ uint32_t added(int b) const { return ctrl + 8 * (2 * MAX_STAGES + 2 * MAX_DEPTH + b); } // its accumulators are added up
+  __device__ __forceinline__ uint32_t tmem_slot() const { return ctrl + 8 * (2 * MAX_STAGES + 3 * MAX_DEPTH); }
+  __device__ __forceinline__ volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(gen + 8 * (2 * MAX_STAGES + 3 * MAX_DEPTH + 1)); }
 };
 
 // kNt: tokens of the tile (16, 32 or 64).  kSubs: groups of a k-block (1 for groups of 128 columns and more, 2, 4).
 template <int kNt, int kSubs>
-__global__ void __launch_bounds__(THREADS, 2) w4_stream_kernel(const __grid_constant__ Params p) {
-  static_assert(128 + 2 * kSubs * kNt <= 512, "tensor memory");
+__global__ void __launch_bounds__(threads(kNt), 1) w4_stream_kernel(const __grid_constant__ Params p) {
+  constexpr int kDepth = depth(kNt, kSubs), kCols = block_cols(kNt, kSubs);        // columns of a k-block: A, then its accumulators
+  constexpr int kStages = stages(kNt), kGroups = widen_groups(kNt);
+  static_assert(kDepth >= 2 && kStages >= kGroups, "k-blocks on their way");
   extern __shared__ uint8_t smem_raw[];
   Smem L;
   {
     const uint32_t r = ptx::smem_u32(smem_raw);
     L.base = (r + 1023u) & ~1023u;
     L.stage = stage_bytes(kNt);
-    L.ctrl = L.base + p.stages * L.stage;
+    L.ctrl = L.base + kStages * L.stage;
     L.gen = smem_raw + (L.ctrl - r);
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, split = p.split;
@@ -160,19 +175,19 @@ __global__ void __launch_bounds__(THREADS, 2) w4_stream_kernel(const __grid_cons
 
   if (threadIdx.x == 0) {
     *L.abort_flag() = 0;
-    for (int s = 0; s < p.stages; ++s) { ptx::mbar_init(L.full(s), 1); ptx::mbar_init(L.empty(s), 1); }
-    for (int b = 0; b < 2; ++b) { ptx::mbar_init(L.wide(b), WIDENERS); ptx::mbar_init(L.done(b), 1); }
+    for (int s = 0; s < kStages; ++s) { ptx::mbar_init(L.full(s), 1); ptx::mbar_init(L.empty(s), 1); }
+    for (int b = 0; b < kDepth; ++b) { ptx::mbar_init(L.wide(b), WIDENERS); ptx::mbar_init(L.done(b), 1); ptx::mbar_init(L.added(b), ADDERS); }
     ptx::fence_mbar_init();
     ptx::prefetch_tensormap(&p.map_w);
     ptx::prefetch_tensormap(&p.map_x);
   }
   if (warp == 1) {
-    ptx::tmem_alloc(L.tmem_slot(), p.tmem_cols);
+    ptx::tmem_alloc(L.tmem_slot(), TMEM_COLS);
     ptx::tmem_relinquish();
   }
   // The first weights start on their way to L2 while the previous kernel still runs; a prefetch reads nothing.
   if (warp == 2 && lane == 0)
-    for (int kb = kb0; kb < min(kb1, kb0 + p.stages); ++kb) ptx::tma_prefetch_2d(&p.map_w, kb * (BK / 2), n0);
+    for (int kb = kb0; kb < min(kb1, kb0 + kStages); ++kb) ptx::tma_prefetch_2d(&p.map_w, kb * (BK / 2), n0);
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
@@ -192,18 +207,17 @@ __global__ void __launch_bounds__(THREADS, 2) w4_stream_kernel(const __grid_cons
         ptx::tma_load_2d(L.x(s), &p.map_x, L.full(s), kb * BK, tok0);
         ptx::tma_load_2d(L.x(s) + kNt * 128, &p.map_x, L.full(s), kb * BK + 64, tok0);
       }
-      if (++s == p.stages) { s = 0; ph ^= 1; }
+      if (++s == kStages) { s = 0; ph ^= 1; }
     }
   } else if (warp == 1) {
     const bool leader = ptx::elect_one();
     constexpr uint32_t idesc = ptx::umma_idesc(1, 1, ROWS, kNt);
-    int s = 0;
-    for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
-      const int b = i & 1;
-      if (!warp_wait(L.wide(b), (i >> 1) & 1, g, ERR_MMA_A)) break;
+    int s = 0, b = 0; uint32_t ph = 0;                // k-block i: stage s, buffer b in its round ph
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!warp_wait(L.added(b), ph ^ 1, g, ERR_MMA_ADDED) || !warp_wait(L.wide(b), ph, g, ERR_MMA_A)) break;
       ptx::tc_fence_after();
       if (leader) {
-        const uint32_t a = tmem + b * 64, d = tmem + 128 + b * kSubs * kNt;
+        const uint32_t a = tmem + b * kCols, d = a + 64;
         const uint64_t dx = ptx::umma_desc_sw128(L.x(s));
 #pragma unroll
         for (int k = 0; k < BK / 16; ++k) {
@@ -214,95 +228,115 @@ __global__ void __launch_bounds__(THREADS, 2) w4_stream_kernel(const __grid_cons
         ptx::umma_commit(L.done(b));
       }
       __syncwarp();
-      if (++s == p.stages) s = 0;
+      if (++s == kStages) s = 0;
+      if (++b == kDepth) { b = 0; ph ^= 1; }
     }
-  } else {
-    // Thread (row, half): columns half * 64 .. + 63 of the row when it widens, tokens half * kNt / 2 .. when it adds up.
-    constexpr int kHalf = kNt / 2, kZ = kSubs == 4 ? 2 : 1;      // zero points of half a row
-    const int quarter = warp & 3, half = (warp - 2) / 4, row = quarter * 32 + lane;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const int groups = p.K / p.group;
-    const long long at0 = (long long)min(n0 + row, p.N - 1) * groups;
-    float2 acc[kHalf / 2];
+  } else if (warp < 2 + WIDENERS * kGroups) {
+    // a thread widens its row of every kGroups-th k-block
+    const int quarter = warp & 3, group = (warp - 2) / 4, row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, swz = (row >> 1) & 3;         // swz: the 64-byte swizzle of the stage
+    const int groups = p.K / p.group, mine = (threadIdx.x - 64) % 128 * 16, tokens = min(kNt, p.T - tok0);
+    const uint8_t* const z = p.z ? p.z + (long long)min(n0 + row, p.N - 1) * groups : nullptr;
+    uint32_t zp[kSubs];                               // of the k-block's groups
+    auto load = [&](int kb) {
 #pragma unroll
-    for (int j = 0; j < kHalf / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-    // scales of the row's groups in a k-block, zero points of its half
-    auto load = [&](int kb, uint32_t (&sc)[kSubs], uint32_t (&zp)[kZ]) {
-      const int first = kSubs == 1 ? kb * BK / p.group : kb * kSubs;
-#pragma unroll
-      for (int j = 0; j < kSubs; ++j) sc[j] = __bfloat16_as_ushort(p.s[at0 + min(first + j, groups - 1)]);
-#pragma unroll
-      for (int j = 0; j < kZ; ++j) zp[j] = p.z ? p.z[at0 + min(first + (kSubs == 1 ? 0 : half * (kSubs / 2) + j), groups - 1)] : 8;
+      for (int j = 0; j < kSubs; ++j) zp[j] = z ? __ldg(z + min(kSubs == 1 ? kb * BK / p.group : kb * kSubs + j, groups - 1)) : 8;
     };
-    auto add_up = [&](int i, const uint32_t (&sc)[kSubs]) {
-      const int b = i & 1;
-      if (!warp_wait(L.done(b), (i >> 1) & 1, g, ERR_WIDEN_DONE)) return false;
-      ptx::tc_fence_after();
+    load(min(kb0 + group, kb_all - 1));
+    int s = group; uint32_t ph = 0;
+    for (int i = group; i < kb1 - kb0; i += kGroups) {
+      const int kb = kb0 + i, b = i % kDepth;
+      if (!warp_wait(L.full(s), ph, g, ERR_WIDEN_FULL)) break;
+      __nv_bfloat162 off[kSubs];
 #pragma unroll
-      for (int j = 0; j < kSubs; ++j) {
-        const uint32_t d = tmem + lanes + 128 + (b * kSubs + j) * kNt + half * kHalf;
-        const float f = __uint_as_float(sc[j] << 16);
-        uint32_t v[kHalf];
-        if constexpr (kHalf == 8) tmem_ld_32x32b_x8(d, v);
-        else if constexpr (kHalf == 16) ptx::tmem_ld_32x32b_x16(d, v);
-        else ptx::tmem_ld_32x32b_x32(d, v);
-        ptx::tmem_ld_wait();
-#pragma unroll
-        for (int t = 0; t < kHalf / 2; ++t)
-          acc[t] = fma2(make_float2(f, f), make_float2(__uint_as_float(v[2 * t]), __uint_as_float(v[2 * t + 1])), acc[t]);
-      }
-      return true;
-    };
-    uint32_t sc[kSubs], zp[kZ], sc_next[kSubs], zp_next[kZ], sc_last[kSubs];
-    bool ok = true;
-    if (kb0 < kb1) load(kb0, sc, zp);
-    int s = 0; uint32_t ph = 0;
-    const uint32_t swz = (row >> 1) & 3;              // the 64-byte swizzle of the weights' stage
-    for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
-      load(min(kb + 1, kb1 - 1), sc_next, zp_next);
-      if (!warp_wait(L.full(s), ph, g, ERR_WIDEN_FULL)) { ok = false; break; }
+      for (int j = 0; j < kSubs; ++j) off[j] = as_pair(0x43004300u | zp[j] | zp[j] << 16);
+      if (z) load(min(kb + kGroups, kb1 - 1));
       const uint32_t from = L.w(s) + row * 64;
-      const uint4 w[2] = {ld_shared_v4(from + (((half * 2) ^ swz) << 4)), ld_shared_v4(from + (((half * 2 + 1) ^ swz) << 4))};
-      for (uint32_t e = (threadIdx.x - 64) * 16; e < kNt * BK * 2; e += WIDENERS * 32 * 16) st_shared_v4(L.x(s) + e, pair_up(ld_shared_v4(L.x(s) + e)));
-      ptx::fence_proxy_async_smem();                  // the MMAs read the activations through the async proxy
-      uint32_t o[32];
+      uint4 w[4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t z = zp[kZ == 2 ? j : 0];
-        const __nv_bfloat162 off = as_pair(0x43004300u | z | z << 16);
-        widen(w[j].x, off, o + j * 16);
-        widen(w[j].y, off, o + j * 16 + 4);
-        widen(w[j].z, off, o + j * 16 + 8);
-        widen(w[j].w, off, o + j * 16 + 12);
+      for (int j = 0; j < 4; ++j) w[j] = ld_shared_v4(from + ((j ^ swz) << 4));
+#pragma unroll
+      for (int e = 0; e < kNt * BK * 2; e += 128 * 16) {
+        const int at = e + mine;
+        if (at / 128 % kNt < tokens) st_shared_v4(L.x(s) + at, pair_up(ld_shared_v4(L.x(s) + at)));      // the others are zero
       }
-      // the buffer's last MMAs, of k-block i - 2, are done: their sums have been added up
-      tmem_st_32x32b_x32(tmem + lanes + (i & 1) * 64 + half * 32, o);
+      ptx::fence_proxy_async_smem();                  // the MMAs read the activations through the async proxy
+      const uint32_t to = tmem + lanes + b * kCols;
+      bool free = true;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t o[32];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const __nv_bfloat162 f = off[(h * 2 + j) * kSubs / 4];
+          widen(w[h * 2 + j].x, f, o + j * 16);
+          widen(w[h * 2 + j].y, f, o + j * 16 + 4);
+          widen(w[h * 2 + j].z, f, o + j * 16 + 8);
+          widen(w[h * 2 + j].w, f, o + j * 16 + 12);
+        }
+        if (h == 0) {                                 // the MMAs of the buffer's last k-block are done
+          free = warp_wait(L.done(b), (i / kDepth & 1) ^ 1, g, ERR_WIDEN_DONE);
+          ptx::tc_fence_after();
+        }
+        if (free) tmem_st_32x32b_x32(to + h * 32, o);
+      }
+      if (!free) break;
       tmem_st_wait();
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(L.wide(i & 1));
-      if (i > 0 && !add_up(i - 1, sc_last)) { ok = false; break; }
-#pragma unroll
-      for (int j = 0; j < kSubs; ++j) { sc_last[j] = sc[j]; sc[j] = sc_next[j]; }
-#pragma unroll
-      for (int j = 0; j < kZ; ++j) zp[j] = zp_next[j];
-      if (++s == p.stages) { s = 0; ph ^= 1; }
+      if (lane == 0) ptx::mbar_arrive(L.wide(b));
+      if ((s += kGroups) >= kStages) { s -= kStages; ph ^= 1; }
     }
-    if (ok && kb0 < kb1) ok = add_up(kb1 - kb0 - 1, sc_last);
+  } else {
+    // a thread adds up its row's accumulators
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const int groups = p.K / p.group, tokens = min(kNt, p.T - tok0);
+    const __nv_bfloat16* const scales = p.s + (long long)min(n0 + row, p.N - 1) * groups;
+    float2 acc[kNt / 2];
+#pragma unroll
+    for (int j = 0; j < kNt / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+    float sc[kSubs];                                  // scales of the k-block that is added up next
+    auto load = [&](int kb) {
+#pragma unroll
+      for (int j = 0; j < kSubs; ++j) sc[j] = __bfloat162float(scales[min(kSubs == 1 ? kb * BK / p.group : kb * kSubs + j, groups - 1)]);
+    };
+    load(min(kb0, kb_all - 1));
+    bool ok = true;
+    int b = 0; uint32_t ph = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!warp_wait(L.done(b), ph, g, ERR_ADD_DONE)) { ok = false; break; }
+      ptx::tc_fence_after();
+      const uint32_t d = tmem + lanes + b * kCols + 64;
+#pragma unroll
+      for (int j = 0; j < kSubs; ++j)
+#pragma unroll
+        for (int c = 0; c < kNt; c += 16) {
+          uint32_t v[16];
+          ptx::tmem_ld_32x32b_x16(d + j * kNt + c, v);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int t = 0; t < 8; ++t)
+            acc[c / 2 + t] = fma2(make_float2(sc[j], sc[j]), make_float2(__uint_as_float(v[2 * t]), __uint_as_float(v[2 * t + 1])), acc[c / 2 + t]);
+        }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(L.added(b));
+      load(min(kb + 1, kb1 - 1));
+      if (++b == kDepth) { b = 0; ph ^= 1; }
+    }
     if (ok) {
       if (split == 1) {
         __nv_bfloat16* out = p.out + n0 + row;
 #pragma unroll
-        for (int t = 0; t < kHalf; ++t) {             // 32 lanes = 64 neighbouring bytes of a token's row
-          const int tok = tok0 + half * kHalf + t;
-          if (n0 + row < p.N && tok < p.T) out[tok * p.ldo] = __float2bfloat16_rn(t & 1 ? acc[t / 2].y : acc[t / 2].x);
-        }
+        for (int t = 0; t < kNt; ++t)                 // 32 lanes = 64 neighbouring bytes of a token's row
+          if (n0 + row < p.N && t < tokens) out[(tok0 + t) * p.ldo] = __float2bfloat16_rn(t & 1 ? acc[t / 2].y : acc[t / 2].x);
       } else {
         // the part as [token][row] floats over the stages: all their loads have landed and all MMAs have read them
-        const uint32_t dst = L.base + row * 4 + half * kHalf * (ROWS * 4);
 #pragma unroll
-        for (int t = 0; t < kHalf; ++t)
-          asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + t * (ROWS * 4)), "f"(t & 1 ? acc[t / 2].y : acc[t / 2].x) : "memory");
+        for (int t = 0; t < kNt; ++t)
+          if (t < tokens)
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(L.base + (t * ROWS + row) * 4), "f"(t & 1 ? acc[t / 2].y : acc[t / 2].x) : "memory");
       }
     }
   }
@@ -313,7 +347,7 @@ __global__ void __launch_bounds__(THREADS, 2) w4_stream_kernel(const __grid_cons
     if (!*L.abort_flag()) {
       // four rows of a token per thread; the tokens go round the cluster's CTAs
       const int tokens = min(kNt, p.T - tok0);
-      for (int t = rank + warp * split; t < tokens; t += split * (THREADS / 32)) {
+      for (int t = rank + warp * split; t < tokens; t += split * (threads(kNt) / 32)) {
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int r = 0; r < split; ++r) {
           const float4 a = ld_cluster_f4(mapa(L.base + t * (ROWS * 4) + lane * 16, r));
@@ -341,7 +375,7 @@ __global__ void __launch_bounds__(THREADS, 2) w4_stream_kernel(const __grid_cons
   }
   if (warp == 1) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem, p.tmem_cols);
+    ptx::tmem_dealloc(tmem, TMEM_COLS);
   }
 }
 
