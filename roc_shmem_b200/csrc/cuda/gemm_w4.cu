@@ -149,19 +149,19 @@ template <int kNt, int kSubs> int stream_product(w4::Params& p, int sms, void* s
   }
   int rc = host::make_tmap_2d(&p.map_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.x, p.T, p.K, p.ldx, kNt, 64);
   if (rc) return rc;
-  // Split the columns so that the longest block is shortest, in k-blocks; adding the parts up costs about four.
-  const int kb = (p.K + w4::BK - 1) / w4::BK, chunks = (p.T + kNt - 1) / kNt;
+  // Split the columns so that the longest block is shortest, in stages; adding the parts up costs about two.
+  const int kb = (p.K + 2 * w4::BK - 1) / (2 * w4::BK), chunks = (p.T + kNt - 1) / kNt;
   const long long tiles = (long long)((p.N + w4::ROWS - 1) / w4::ROWS) * chunks;
   long long best = 0;
   for (int s = 1; s <= 8; ++s) {
-    const long long at_once = resident(w4::w4_stream_kernel<kNt, kSubs>, dev, s, w4::threads(kNt), sms);
-    const long long cost = (tiles + at_once - 1) / at_once * ((kb + s - 1) / s) + (s > 1 ? 4 : 0);
+    const long long at_once = resident(w4::w4_stream_kernel<kNt, kSubs>, dev, s, w4::threads(kNt, kSubs), sms);
+    const long long cost = (tiles + at_once - 1) / at_once * ((kb + s - 1) / s) + (s > 1 ? 2 : 0);
     if (s == 1 || cost < best) { best = cost; p.split = s; }
   }
 #ifdef W4_SPLIT
   p.split = W4_SPLIT;
 #endif
-  return launch(w4::w4_stream_kernel<kNt, kSubs>, dim3((unsigned)((p.N + w4::ROWS - 1) / w4::ROWS * p.split), (unsigned)chunks), w4::threads(kNt), p.split,
+  return launch(w4::w4_stream_kernel<kNt, kSubs>, dim3((unsigned)((p.N + w4::ROWS - 1) / w4::ROWS * p.split), (unsigned)chunks), w4::threads(kNt, kSubs), p.split,
                 w4::SMEM_BYTES, p, stream);
 }
 template <int kNt> int stream_groups(w4::Params& p, int sms, void* stream) {
@@ -199,7 +199,7 @@ int bshmem_w4_few(const void* x, long long ldx, const void* q, const void* s, co
   p.ldo = N;
   p.T = T; p.N = N; p.K = K; p.group = group;
   p.timeout_ns = (unsigned long long)(timeout_ms > 0 ? timeout_ms : 2000) * 1000000ull;
-  if (int rc = host::make_tmap_2d(&p.map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q, N, K / 2, K / 2, w4::ROWS, w4::BK / 2, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
+  if (int rc = host::make_tmap_2d(&p.map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q, N, K / 2, K / 2, w4::ROWS, w4::BK)) return rc;
   return T <= 16 ? stream_groups<16>(p, sms, stream) : T <= 32 ? stream_groups<32>(p, sms, stream) : stream_groups<64>(p, sms, stream);
 }
 

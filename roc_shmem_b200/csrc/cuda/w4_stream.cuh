@@ -9,9 +9,10 @@
 // columns are put into the same order where they lie in shared memory.  The scales never touch the weights: each group has an
 // accumulator of its own, which the thread of the row multiplies by its scale and adds up in fp32 registers.
 //
-//   warp 0      TMA producer: {128 rows x 64 bytes of weights, tokens x 128 columns} per stage, plain loads of local memory
+//   warp 0      TMA producer: {128 rows x 128 bytes of weights, tokens x 256 columns} per stage, i.e. two k-blocks (with rows of 64
+//               bytes the TMA unit's requests, one per row, were the limit); plain loads of local memory
 //   warp 1      MMA issuer: tcgen05.mma M128 x N=tokens x K16, A in tensor memory, B in shared memory
-//   next 16     four groups of four warps, each widens every fourth k-block and orders its activations (64 tokens: three groups)
+//   next 16     up to four groups of four warps: each widens every fourth k-block and orders its activations
 //   last 4      add the accumulators up
 //
 // From a k-block's arrival to its sums it takes a warp of each kind some 900 cycles, and HBM brings an SM the 8 KiB of the next in 370: so several
@@ -40,18 +41,17 @@ using gemm2::warp_wait;
 
 constexpr int ROWS = 128, BK = 128;                  // weight rows of a tile, columns of a k-block
 constexpr int MAX_TOKENS = 64;                       // of a tile
-constexpr int MAX_STAGES = 12, MAX_DEPTH = 6;
+constexpr int MAX_STAGES = 9, MAX_DEPTH = 6;
 constexpr int WIDENERS = 4, ADDERS = 4;              // warps of a group that widens, and warps that add up
-__host__ __device__ constexpr int widen_groups(int nt) { return nt == 64 ? 3 : 4; }          // the sums of 64 tokens take more registers
-__host__ __device__ constexpr int threads(int nt) { return 32 * (2 + WIDENERS * widen_groups(nt) + ADDERS); }
-constexpr uint32_t W_BYTES = ROWS * BK / 2;          // 8 KiB of weights per stage
+constexpr int MAX_GROUPS = 4;
+constexpr uint32_t W_BYTES = ROWS * BK;              // 16 KiB of weights per stage: two k-blocks
 constexpr uint32_t CTRL_BYTES = 512;
 constexpr uint32_t SMEM_BYTES = 224u << 10;          // one CTA has an SM, all of its tensor memory too
 constexpr uint32_t TMEM_COLS = 512;
 enum ErrSite : int { ERR_PRODUCER_EMPTY = 401, ERR_MMA_A = 402, ERR_WIDEN_FULL = 403, ERR_WIDEN_DONE = 404, ERR_MMA_ADDED = 405, ERR_ADD_DONE = 406 };
 
 struct Params {
-  CUtensorMap map_w, map_x;      // weights [N, K / 2] bytes, box {64, 128}; tokens [T, K], box {64, nt}
+  CUtensorMap map_w, map_x;      // weights [N, K / 2] bytes, box {128, 128}; tokens [T, K], box {64, nt}
   const void* x; long long ldx;  // for the host
   const __nv_bfloat16* s;
   const uint8_t* z;              // null: 8 everywhere
@@ -64,7 +64,7 @@ struct Params {
 
 __device__ int error_word;        // site of the first wait that ran out, 0: none
 
-__host__ __device__ constexpr uint32_t stage_bytes(int nt) { return W_BYTES + (uint32_t)nt * BK * 2; }
+__host__ __device__ constexpr uint32_t stage_bytes(int nt) { return W_BYTES + (uint32_t)nt * BK * 4; }
 __host__ __device__ constexpr int stages(int nt) {
   return (SMEM_BYTES - CTRL_BYTES - 1024) / stage_bytes(nt) < MAX_STAGES ? (SMEM_BYTES - CTRL_BYTES - 1024) / stage_bytes(nt) : MAX_STAGES;
 }
@@ -73,6 +73,13 @@ __host__ __device__ constexpr int block_cols(int nt, int subs) { return 64 + sub
 __host__ __device__ constexpr int depth(int nt, int subs) {
   return TMEM_COLS / block_cols(nt, subs) < MAX_DEPTH ? TMEM_COLS / block_cols(nt, subs) : MAX_DEPTH;
 }
+
+// Groups that widen: no more than there are k-blocks in tensor memory, or a group could ask about a buffer's round before last and take
+// the answer for its last one; and three for 64 tokens, whose sums take more registers.
+__host__ __device__ constexpr int widen_groups(int nt, int subs) {
+  return depth(nt, subs) < MAX_GROUPS ? depth(nt, subs) : nt == 64 ? 3 : MAX_GROUPS;
+}
+__host__ __device__ constexpr int threads(int nt, int subs) { return 32 * (2 + WIDENERS * widen_groups(nt, subs) + ADDERS); }
 
 __device__ __forceinline__ __nv_bfloat162 as_pair(uint32_t w) {
   __nv_bfloat162 p;
@@ -154,10 +161,10 @@ struct Smem {
 
 // kNt: tokens of the tile (16, 32 or 64).  kSubs: groups of a k-block (1 for groups of 128 columns and more, 2, 4).
 template <int kNt, int kSubs>
-__global__ void __launch_bounds__(threads(kNt), 1) w4_stream_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(threads(kNt, kSubs), 1) w4_stream_kernel(const __grid_constant__ Params p) {
   constexpr int kDepth = depth(kNt, kSubs), kCols = block_cols(kNt, kSubs);        // columns of a k-block: A, then its accumulators
-  constexpr int kStages = stages(kNt), kGroups = widen_groups(kNt);
-  static_assert(kDepth >= 2 && kStages >= kGroups, "k-blocks on their way");
+  constexpr int kStages = stages(kNt), kGroups = widen_groups(kNt, kSubs);
+  static_assert(kDepth >= kGroups && kDepth >= 2 && 2 * kStages >= kGroups, "k-blocks on their way");
   extern __shared__ uint8_t smem_raw[];
   Smem L;
   {
@@ -170,12 +177,12 @@ __global__ void __launch_bounds__(threads(kNt), 1) w4_stream_kernel(const __grid
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, split = p.split;
   const int rank = split > 1 ? (int)cluster_ctarank() : 0;
   const int n0 = (int)(blockIdx.x / split) * ROWS, tok0 = (int)blockIdx.y * kNt;
-  const int kb_all = (p.K + BK - 1) / BK, kb0 = kb_all * rank / split, kb1 = kb_all * (rank + 1) / split;
+  const int pairs = (p.K + 2 * BK - 1) / (2 * BK), kb0 = pairs * rank / split * 2, kb1 = pairs * (rank + 1) / split * 2;       // whole stages
   Guard g{&error_word, L.abort_flag(), p.timeout_ns};
 
   if (threadIdx.x == 0) {
     *L.abort_flag() = 0;
-    for (int s = 0; s < kStages; ++s) { ptx::mbar_init(L.full(s), 1); ptx::mbar_init(L.empty(s), 1); }
+    for (int s = 0; s < kStages; ++s) { ptx::mbar_init(L.full(s), 1); ptx::mbar_init(L.empty(s), 2); }
     for (int b = 0; b < kDepth; ++b) { ptx::mbar_init(L.wide(b), WIDENERS); ptx::mbar_init(L.done(b), 1); ptx::mbar_init(L.added(b), ADDERS); }
     ptx::fence_mbar_init();
     ptx::prefetch_tensormap(&p.map_w);
@@ -187,7 +194,7 @@ __global__ void __launch_bounds__(threads(kNt), 1) w4_stream_kernel(const __grid
   }
   // The first weights start on their way to L2 while the previous kernel still runs; a prefetch reads nothing.
   if (warp == 2 && lane == 0)
-    for (int kb = kb0; kb < min(kb1, kb0 + kStages); ++kb) ptx::tma_prefetch_2d(&p.map_w, kb * (BK / 2), n0);
+    for (int kb = kb0; kb < min(kb1, kb0 + 2 * kStages); kb += 2) ptx::tma_prefetch_2d(&p.map_w, kb * (BK / 2), n0);
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
@@ -199,13 +206,13 @@ __global__ void __launch_bounds__(threads(kNt), 1) w4_stream_kernel(const __grid
   if (warp == 0) {
     const bool leader = ptx::elect_one();
     int s = 0; uint32_t ph = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
+    for (int kb = kb0; kb < kb1; kb += 2) {
       if (!warp_wait(L.empty(s), ph ^ 1, g, ERR_PRODUCER_EMPTY)) break;
       if (leader) {
         ptx::mbar_arrive_expect_tx(L.full(s), L.stage);
         ptx::tma_load_2d(L.w(s), &p.map_w, L.full(s), kb * (BK / 2), n0);
-        ptx::tma_load_2d(L.x(s), &p.map_x, L.full(s), kb * BK, tok0);
-        ptx::tma_load_2d(L.x(s) + kNt * 128, &p.map_x, L.full(s), kb * BK + 64, tok0);
+#pragma unroll
+        for (int a = 0; a < 4; ++a) ptx::tma_load_2d(L.x(s) + a * kNt * 128, &p.map_x, L.full(s), kb * BK + a * 64, tok0);
       }
       if (++s == kStages) { s = 0; ph ^= 1; }
     }
@@ -218,7 +225,7 @@ __global__ void __launch_bounds__(threads(kNt), 1) w4_stream_kernel(const __grid
       ptx::tc_fence_after();
       if (leader) {
         const uint32_t a = tmem + b * kCols, d = a + 64;
-        const uint64_t dx = ptx::umma_desc_sw128(L.x(s));
+        const uint64_t dx = ptx::umma_desc_sw128(L.x(s) + (kb & 1) * kNt * 256);
 #pragma unroll
         for (int k = 0; k < BK / 16; ++k) {
           constexpr int kPer = BK / 16 / kSubs;       // MMAs of a group
@@ -228,13 +235,13 @@ __global__ void __launch_bounds__(threads(kNt), 1) w4_stream_kernel(const __grid
         ptx::umma_commit(L.done(b));
       }
       __syncwarp();
-      if (++s == kStages) s = 0;
+      if ((kb & 1) && ++s == kStages) s = 0;
       if (++b == kDepth) { b = 0; ph ^= 1; }
     }
   } else if (warp < 2 + WIDENERS * kGroups) {
     // a thread widens its row of every kGroups-th k-block
     const int quarter = warp & 3, group = (warp - 2) / 4, row = quarter * 32 + lane;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, swz = (row >> 1) & 3;         // swz: the 64-byte swizzle of the stage
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const int groups = p.K / p.group, mine = (threadIdx.x - 64) % 128 * 16, tokens = min(kNt, p.T - tok0);
     const uint8_t* const z = p.z ? p.z + (long long)min(n0 + row, p.N - 1) * groups : nullptr;
     uint32_t zp[kSubs];                               // of the k-block's groups
@@ -242,8 +249,8 @@ __global__ void __launch_bounds__(threads(kNt), 1) w4_stream_kernel(const __grid
 #pragma unroll
       for (int j = 0; j < kSubs; ++j) zp[j] = z ? __ldg(z + min(kSubs == 1 ? kb * BK / p.group : kb * kSubs + j, groups - 1)) : 8;
     };
-    load(min(kb0 + group, kb_all - 1));
-    int s = group; uint32_t ph = 0;
+    load(kb0 + group);
+    int s = group / 2; uint32_t ph = 0;
     for (int i = group; i < kb1 - kb0; i += kGroups) {
       const int kb = kb0 + i, b = i % kDepth;
       if (!warp_wait(L.full(s), ph, g, ERR_WIDEN_FULL)) break;
@@ -251,14 +258,13 @@ __global__ void __launch_bounds__(threads(kNt), 1) w4_stream_kernel(const __grid
 #pragma unroll
       for (int j = 0; j < kSubs; ++j) off[j] = as_pair(0x43004300u | zp[j] | zp[j] << 16);
       if (z) load(min(kb + kGroups, kb1 - 1));
-      const uint32_t from = L.w(s) + row * 64;
+      const uint32_t from = L.w(s) + row * 128, x = L.x(s) + (kb & 1) * kNt * 256 + mine;
       uint4 w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = ld_shared_v4(from + ((j ^ swz) << 4));
+      for (int j = 0; j < 4; ++j) w[j] = ld_shared_v4(from + ((((kb & 1) * 4 + j) ^ (row & 7)) << 4));      // the stage's 128-byte swizzle
 #pragma unroll
       for (int e = 0; e < kNt * BK * 2; e += 128 * 16) {
-        const int at = e + mine;
-        if (at / 128 % kNt < tokens) st_shared_v4(L.x(s) + at, pair_up(ld_shared_v4(L.x(s) + at)));      // the others are zero
+        if ((e + mine) / 128 % kNt < tokens) st_shared_v4(x + e, pair_up(ld_shared_v4(x + e)));          // the others are zero
       }
       ptx::fence_proxy_async_smem();                  // the MMAs read the activations through the async proxy
       const uint32_t to = tmem + lanes + b * kCols;
@@ -285,7 +291,9 @@ __global__ void __launch_bounds__(threads(kNt), 1) w4_stream_kernel(const __grid
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(L.wide(b));
-      if ((s += kGroups) >= kStages) { s -= kStages; ph ^= 1; }
+      // kGroups k-blocks on: as many halves of stages
+      s = (i + kGroups) / 2 % kStages;
+      ph = (i + kGroups) / 2 / kStages & 1;
     }
   } else {
     // a thread adds up its row's accumulators
@@ -301,7 +309,7 @@ __global__ void __launch_bounds__(threads(kNt), 1) w4_stream_kernel(const __grid
 #pragma unroll
       for (int j = 0; j < kSubs; ++j) sc[j] = __bfloat162float(scales[min(kSubs == 1 ? kb * BK / p.group : kb * kSubs + j, groups - 1)]);
     };
-    load(min(kb0, kb_all - 1));
+    load(kb0);
     bool ok = true;
     int b = 0; uint32_t ph = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
@@ -347,7 +355,7 @@ __global__ void __launch_bounds__(threads(kNt), 1) w4_stream_kernel(const __grid
     if (!*L.abort_flag()) {
       // four rows of a token per thread; the tokens go round the cluster's CTAs
       const int tokens = min(kNt, p.T - tok0);
-      for (int t = rank + warp * split; t < tokens; t += split * (threads(kNt) / 32)) {
+      for (int t = rank + warp * split; t < tokens; t += split * (threads(kNt, kSubs) / 32)) {
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int r = 0; r < split; ++r) {
           const float4 a = ld_cluster_f4(mapa(L.base + t * (ROWS * 4) + lane * 16, r));
