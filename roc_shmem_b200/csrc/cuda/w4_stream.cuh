@@ -41,14 +41,14 @@ using gemm2::warp_wait;
 
 constexpr int ROWS = 128, BK = 128;                  // weight rows of a tile, columns of a k-block
 constexpr int MAX_TOKENS = 64;                       // of a tile
-constexpr int MAX_STAGES = 9, MAX_DEPTH = 6;
+constexpr int MAX_STAGES = 9, MAX_DEPTH = 3;
 constexpr int WIDENERS = 4, ADDERS = 4;              // warps of a group that widens, and warps that add up
 constexpr int MAX_GROUPS = 4;
 constexpr uint32_t W_BYTES = ROWS * BK;              // 16 KiB of weights per stage: two k-blocks
 constexpr uint32_t CTRL_BYTES = 512;
 constexpr uint32_t SMEM_BYTES = 224u << 10;          // one CTA has an SM, all of its tensor memory too
 constexpr uint32_t TMEM_COLS = 512;
-enum ErrSite : int { ERR_PRODUCER_EMPTY = 401, ERR_MMA_A = 402, ERR_WIDEN_FULL = 403, ERR_WIDEN_DONE = 404, ERR_MMA_ADDED = 405, ERR_ADD_DONE = 406 };
+enum ErrSite : int { ERR_PRODUCER_EMPTY = 401, ERR_MMA_A = 402, ERR_WIDEN_FULL = 403, ERR_WIDEN_ADDED = 404, ERR_ADD_DONE = 405 };
 
 struct Params {
   CUtensorMap map_w, map_x;      // weights [N, K / 2] bytes, box {128, 128}; tokens [T, K], box {64, nt}
@@ -68,16 +68,15 @@ __host__ __device__ constexpr uint32_t stage_bytes(int nt) { return W_BYTES + (u
 __host__ __device__ constexpr int stages(int nt) {
   return (SMEM_BYTES - CTRL_BYTES - 1024) / stage_bytes(nt) < MAX_STAGES ? (SMEM_BYTES - CTRL_BYTES - 1024) / stage_bytes(nt) : MAX_STAGES;
 }
-// k-blocks in tensor memory, each with an A buffer of 64 columns and `subs` accumulators of nt.
-__host__ __device__ constexpr int block_cols(int nt, int subs) { return 64 + subs * nt; }
+// Stages in tensor memory, each with two A buffers of 64 columns and `subs` accumulators of nt for either.
+__host__ __device__ constexpr int block_cols(int nt, int subs) { return 2 * (64 + subs * nt); }
 __host__ __device__ constexpr int depth(int nt, int subs) {
   return TMEM_COLS / block_cols(nt, subs) < MAX_DEPTH ? TMEM_COLS / block_cols(nt, subs) : MAX_DEPTH;
 }
-
 // Groups that widen: no more than there are k-blocks in tensor memory, or a group could ask about a buffer's round before last and take
 // the answer for its last one; and three for 64 tokens, whose sums take more registers.
 __host__ __device__ constexpr int widen_groups(int nt, int subs) {
-  return depth(nt, subs) < MAX_GROUPS ? depth(nt, subs) : nt == 64 ? 3 : MAX_GROUPS;
+  return 2 * depth(nt, subs) < MAX_GROUPS ? 2 * depth(nt, subs) : nt == 64 ? 3 : MAX_GROUPS;
 }
 __host__ __device__ constexpr int threads(int nt, int subs) { return 32 * (2 + WIDENERS * widen_groups(nt, subs) + ADDERS); }
 
@@ -154,7 +153,7 @@ struct Smem {
   __device__ __forceinline__ uint32_t empty(int s) const { return ctrl + 8 * (MAX_STAGES + s); }
   __device__ __forceinline__ uint32_t wide(int b) const { return ctrl + 8 * (2 * MAX_STAGES + b); }                  // A buffer b is written
   __device__ __forceinline__ uint32_t done(int b) const { return ctrl + 8 * (2 * MAX_STAGES + MAX_DEPTH + b); }      // its MMAs are done
-  __device__ __forceinline__ uint32_t added(int b) const { return ctrl + 8 * (2 * MAX_STAGES + 2 * MAX_DEPTH + b); } // its accumulators are added up
+  __device__ __forceinline__ uint32_t added(int b) const { return ctrl + 8 * (2 * MAX_STAGES + 2 * MAX_DEPTH + b); } // its sums are added up
   __device__ __forceinline__ uint32_t tmem_slot() const { return ctrl + 8 * (2 * MAX_STAGES + 3 * MAX_DEPTH); }
   __device__ __forceinline__ volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(gen + 8 * (2 * MAX_STAGES + 3 * MAX_DEPTH + 1)); }
 };
@@ -162,9 +161,9 @@ struct Smem {
 // kNt: tokens of the tile (16, 32 or 64).  kSubs: groups of a k-block (1 for groups of 128 columns and more, 2, 4).
 template <int kNt, int kSubs>
 __global__ void __launch_bounds__(threads(kNt, kSubs), 1) w4_stream_kernel(const __grid_constant__ Params p) {
-  constexpr int kDepth = depth(kNt, kSubs), kCols = block_cols(kNt, kSubs);        // columns of a k-block: A, then its accumulators
+  constexpr int kDepth = depth(kNt, kSubs), kCols = block_cols(kNt, kSubs);        // columns of a stage: A, then its accumulators
   constexpr int kStages = stages(kNt), kGroups = widen_groups(kNt, kSubs);
-  static_assert(kDepth >= kGroups && kDepth >= 2 && 2 * kStages >= kGroups, "k-blocks on their way");
+  static_assert(kDepth >= 1 && 2 * kDepth >= kGroups && 2 * kStages >= kGroups, "k-blocks on their way");
   extern __shared__ uint8_t smem_raw[];
   Smem L;
   {
@@ -182,8 +181,8 @@ __global__ void __launch_bounds__(threads(kNt, kSubs), 1) w4_stream_kernel(const
 
   if (threadIdx.x == 0) {
     *L.abort_flag() = 0;
-    for (int s = 0; s < kStages; ++s) { ptx::mbar_init(L.full(s), 1); ptx::mbar_init(L.empty(s), 2); }
-    for (int b = 0; b < kDepth; ++b) { ptx::mbar_init(L.wide(b), WIDENERS); ptx::mbar_init(L.done(b), 1); ptx::mbar_init(L.added(b), ADDERS); }
+    for (int s = 0; s < kStages; ++s) { ptx::mbar_init(L.full(s), 1); ptx::mbar_init(L.empty(s), 1); }
+    for (int b = 0; b < kDepth; ++b) { ptx::mbar_init(L.wide(b), 2 * WIDENERS); ptx::mbar_init(L.done(b), 1); ptx::mbar_init(L.added(b), ADDERS); }
     ptx::fence_mbar_init();
     ptx::prefetch_tensormap(&p.map_w);
     ptx::prefetch_tensormap(&p.map_x);
@@ -198,8 +197,9 @@ __global__ void __launch_bounds__(threads(kNt, kSubs), 1) w4_stream_kernel(const
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  uint32_t tmem;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(L.tmem_slot()));
+  // All of tensor memory begins at column 0.  As a constant it keeps the addresses of the MMAs in uniform registers: as a value from
+  // memory they were moved there one by one, some 60 cycles for each MMA.
+  constexpr uint32_t tmem = 0;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
@@ -219,23 +219,24 @@ __global__ void __launch_bounds__(threads(kNt, kSubs), 1) w4_stream_kernel(const
   } else if (warp == 1) {
     const bool leader = ptx::elect_one();
     constexpr uint32_t idesc = ptx::umma_idesc(1, 1, ROWS, kNt);
-    int s = 0, b = 0; uint32_t ph = 0;                // k-block i: stage s, buffer b in its round ph
-    for (int kb = kb0; kb < kb1; ++kb) {
-      if (!warp_wait(L.added(b), ph ^ 1, g, ERR_MMA_ADDED) || !warp_wait(L.wide(b), ph, g, ERR_MMA_A)) break;
+    // Two k-blocks at once: a wait that is over still takes 150 cycles, a commit 50.
+    int s = 0, b = 0; uint32_t ph = 0;                // buffer b in its round ph
+    for (int kb = kb0; kb < kb1; kb += 2) {
+      if (!warp_wait(L.wide(b), ph, g, ERR_MMA_A)) break;
       ptx::tc_fence_after();
       if (leader) {
-        const uint32_t a = tmem + b * kCols, d = a + 64;
-        const uint64_t dx = ptx::umma_desc_sw128(L.x(s) + (kb & 1) * kNt * 256);
+        const uint32_t a = tmem + b * kCols, d = a + 128;
+        const uint64_t dx = ptx::umma_desc_sw128(L.x(s));
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k) {
+        for (int k = 0; k < 2 * BK / 16; ++k) {
           constexpr int kPer = BK / 16 / kSubs;       // MMAs of a group
           umma_f16_ts(d + k / kPer * kNt, a + k * 8, dx + (k / 4) * (kNt * 128 / 16) + (k % 4) * 2, idesc, k % kPer ? 1u : 0u);
         }
-        ptx::umma_commit(L.empty(s));
         ptx::umma_commit(L.done(b));
+        ptx::umma_commit(L.empty(s));
       }
       __syncwarp();
-      if ((kb & 1) && ++s == kStages) s = 0;
+      if (++s == kStages) s = 0;
       if (++b == kDepth) { b = 0; ph ^= 1; }
     }
   } else if (warp < 2 + WIDENERS * kGroups) {
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(threads(kNt, kSubs), 1) w4_stream_kernel(const
     load(kb0 + group);
     int s = group / 2; uint32_t ph = 0;
     for (int i = group; i < kb1 - kb0; i += kGroups) {
-      const int kb = kb0 + i, b = i % kDepth;
+      const int kb = kb0 + i, b = i / 2 % kDepth;
       if (!warp_wait(L.full(s), ph, g, ERR_WIDEN_FULL)) break;
       __nv_bfloat162 off[kSubs];
 #pragma unroll
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(threads(kNt, kSubs), 1) w4_stream_kernel(const
         if ((e + mine) / 128 % kNt < tokens) st_shared_v4(x + e, pair_up(ld_shared_v4(x + e)));          // the others are zero
       }
       ptx::fence_proxy_async_smem();                  // the MMAs read the activations through the async proxy
-      const uint32_t to = tmem + lanes + b * kCols;
+      const uint32_t to = tmem + lanes + b * kCols + (kb & 1) * 64;
       bool free = true;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -280,8 +281,8 @@ __global__ void __launch_bounds__(threads(kNt, kSubs), 1) w4_stream_kernel(const
           widen(w[h * 2 + j].z, f, o + j * 16 + 8);
           widen(w[h * 2 + j].w, f, o + j * 16 + 12);
         }
-        if (h == 0) {                                 // the MMAs of the buffer's last k-block are done
-          free = warp_wait(L.done(b), (i / kDepth & 1) ^ 1, g, ERR_WIDEN_DONE);
+        if (h == 0) {                                 // the buffer's last k-block is multiplied and its sums are read
+          free = warp_wait(L.added(b), (i / 2 / kDepth & 1) ^ 1, g, ERR_WIDEN_ADDED);
           ptx::tc_fence_after();
         }
         if (free) tmem_st_32x32b_x32(to + h * 32, o);
@@ -300,38 +301,50 @@ __global__ void __launch_bounds__(threads(kNt, kSubs), 1) w4_stream_kernel(const
     const int quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const int groups = p.K / p.group, tokens = min(kNt, p.T - tok0);
-    const __nv_bfloat16* const scales = p.s + (long long)min(n0 + row, p.N - 1) * groups;
+    const unsigned short* const scales = reinterpret_cast<const unsigned short*>(p.s) + (long long)min(n0 + row, p.N - 1) * groups;
     float2 acc[kNt / 2];
 #pragma unroll
     for (int j = 0; j < kNt / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-    float sc[kSubs];                                  // scales of the k-block that is added up next
+    // The scales of eight groups ahead: a load takes as long as a k-block or two.
+    constexpr int kBatch = 8 / kSubs;                 // k-blocks
+    unsigned short sc[8], next[8];                    // as they come: a conversion would wait for its load
     auto load = [&](int kb) {
 #pragma unroll
-      for (int j = 0; j < kSubs; ++j) sc[j] = __bfloat162float(scales[min(kSubs == 1 ? kb * BK / p.group : kb * kSubs + j, groups - 1)]);
+      for (int j = 0; j < 8; ++j)
+        next[j] = __ldg(scales + min(kSubs == 1 ? (kb + j) * BK / p.group : kb * kSubs + j, groups - 1));
     };
     load(kb0);
     bool ok = true;
     int b = 0; uint32_t ph = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      if (!warp_wait(L.done(b), ph, g, ERR_ADD_DONE)) { ok = false; break; }
-      ptx::tc_fence_after();
-      const uint32_t d = tmem + lanes + b * kCols + 64;
+    for (int first = kb0; ok && first < kb1; first += kBatch) {
 #pragma unroll
-      for (int j = 0; j < kSubs; ++j)
+      for (int j = 0; j < 8; ++j) sc[j] = next[j];
+      load(first + kBatch);
 #pragma unroll
-        for (int c = 0; c < kNt; c += 16) {
-          uint32_t v[16];
-          ptx::tmem_ld_32x32b_x16(d + j * kNt + c, v);
-          ptx::tmem_ld_wait();
+      for (int u = 0; u < kBatch; u += 2) {
+        if (!ok || first + u >= kb1) break;
+        ok = warp_wait(L.done(b), ph, g, ERR_ADD_DONE);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint32_t d = tmem + lanes + b * kCols + 128;
 #pragma unroll
-          for (int t = 0; t < 8; ++t)
-            acc[c / 2 + t] = fma2(make_float2(sc[j], sc[j]), make_float2(__uint_as_float(v[2 * t]), __uint_as_float(v[2 * t + 1])), acc[c / 2 + t]);
-        }
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(L.added(b));
-      load(min(kb + 1, kb1 - 1));
-      if (++b == kDepth) { b = 0; ph ^= 1; }
+        for (int j = 0; j < 2 * kSubs; ++j)
+#pragma unroll
+          for (int c = 0; c < kNt; c += 16) {
+            uint32_t v[16];
+            ptx::tmem_ld_32x32b_x16(d + j * kNt + c, v);
+            ptx::tmem_ld_wait();
+            const float scale = __uint_as_float((uint32_t)sc[u * kSubs + j] << 16);
+            const float2 f = make_float2(scale, scale);
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+              acc[c / 2 + t] = fma2(f, make_float2(__uint_as_float(v[2 * t]), __uint_as_float(v[2 * t + 1])), acc[c / 2 + t]);
+          }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(L.added(b));
+        if (++b == kDepth) { b = 0; ph ^= 1; }
+      }
     }
     if (ok) {
       if (split == 1) {
