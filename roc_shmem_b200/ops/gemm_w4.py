@@ -16,7 +16,16 @@ from .. import _native
 from .checkpoint8 import block_lib, on_current_device
 from .gemm import current_stream, gemm_bf16
 
-FEW_TOKENS = 32
+_U8, _BF16 = torch.uint8, torch.bfloat16
+
+
+def few_tokens(group: int) -> int:
+    """Tokens up to which the weights are multiplied as they are.  us, that kernel against widening and the bf16 GEMM, 8192 to 7168 columns,
+    groups of 128: 64 tokens 23.2 / 56.6, 128 41.2 / 58.7, 192 72.6 / 63.0; 14336 to 4096, groups of 64: 128 47.0 / 58.2, 192 78.5 / 62.6.
+    Groups of 32 have four accumulators for every 128 columns, so 32 tokens are a tile: 4096 to 14336, 33 tokens 60.5 / 54.3."""
+    return 128 if group >= 64 else 32
+
+
 _declared = False
 _few = _widen = None
 
@@ -66,15 +75,16 @@ class W4Tensor:
 
 def _checked(w: W4Tensor, what: str) -> tuple[int, int, int]:
     q, s, z = w.q, w.scales, w.zeros
-    if q.dtype is not torch.uint8 or s.dtype is not torch.bfloat16 or (z is not None and z.dtype is not torch.uint8) or not q.is_cuda:
+    if not (q.dtype is _U8 and s.dtype is _BF16 and q.is_cuda and (z is None or z.dtype is _U8)):
         raise ValueError(f"{what} needs CUDA tensors q (uint8), scales (bf16) and zeros (uint8 or None)")
-    if q.dim() != 2 or s.dim() != 2 or q.shape[0] != s.shape[0] or s.shape[1] < 1 or (z is not None and z.shape != s.shape):
-        raise ValueError(f"{what}: shapes do not belong together: q {tuple(q.shape)}, scales {tuple(s.shape)}")
-    N, K = q.shape[0], 2 * q.shape[1]
-    group = K // s.shape[1]
-    if N < 1 or group * s.shape[1] != K or not (group in (32, 64) or (group and group % 128 == 0)):
-        raise ValueError(f"{what} needs whole groups of 32, 64 or a multiple of 128 columns, got K {K} in {s.shape[1]} groups")
-    if s.device != q.device or (z is not None and z.device != q.device):
+    qs, ss = q.shape, s.shape
+    if len(qs) != 2 or len(ss) != 2 or qs[0] != ss[0] or ss[1] < 1 or (z is not None and z.shape != ss):
+        raise ValueError(f"{what}: shapes do not belong together: q {tuple(qs)}, scales {tuple(ss)}")
+    N, K = qs[0], 2 * qs[1]
+    group = K // ss[1]
+    if N < 1 or group * ss[1] != K or not (group in (32, 64) or (group and group % 128 == 0)) or K > 1 << 24:
+        raise ValueError(f"{what} needs whole groups of 32, 64 or a multiple of 128 columns, got K {K} in {ss[1]} groups")
+    if s.get_device() != q.get_device() or (z is not None and z.get_device() != q.get_device()):
         raise ValueError(f"{what}: q, scales and zeros must be on one device")
     if not (q.is_contiguous() and s.is_contiguous() and (z is None or z.is_contiguous())) or q.data_ptr() % 16:
         raise ValueError(f"{what} needs contiguous tensors and q on a 16-byte boundary")
@@ -118,28 +128,35 @@ def widen_w4(w: W4Tensor) -> torch.Tensor:
 def linear_w4(x: torch.Tensor, w: W4Tensor) -> torch.Tensor:
     """x [..., K] bf16 times the weight [N, K] of 4 bits, in bf16 [..., N] (forward only)."""
     N, K, group = _checked(w, "linear_w4")
-    if not x.is_cuda or x.dtype is not torch.bfloat16 or x.dim() < 1 or x.shape[-1] != K or x.device != w.q.device:
-        raise ValueError(f"linear_w4 needs bf16 [..., {K}] on {w.q.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    if torch.is_grad_enabled() and x.requires_grad:
+    shape = x.shape
+    if x.dtype is not _BF16 or not shape or shape[-1] != K or not x.is_cuda or x.get_device() != w.q.get_device():
+        raise ValueError(f"linear_w4 needs bf16 [..., {K}] on {w.q.device}, got {x.dtype} {tuple(shape)} on {x.device}")
+    if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("linear_w4 has no gradient: detach x, or call it under torch.no_grad()")
     if not on_current_device(x):
         with torch.cuda.device(x.device):
             return linear_w4(x, w)
-    m = x if x.dim() == 2 else x.reshape(-1, K)
+    m = x if len(shape) == 2 else x.reshape(-1, K)
     T = m.shape[0]
-    if T > 1 and (m.stride(1) != 1 or m.stride(0) % 8) or m.stride(1) != 1 or m.data_ptr() % 16:
+    ld, columns = m.stride()
+    if T == 1:
+        ld = K
+    if columns != 1 or ld < K or ld % 8 or m.data_ptr() % 16:
         m = m.contiguous()
         if m.data_ptr() % 16:
             m = m.clone()
-    if T > FEW_TOKENS and N % 8 == 0:                        # the bf16 GEMM's columns come in eights
+        ld = K
+    if T > few_tokens(group) and N % 8 == 0:                 # the bf16 GEMM's columns come in eights
         out = gemm_bf16(m, widen_w4(w))
     else:
         if _few is None:
             _lib()
-        out = torch.empty((T, N), dtype=torch.bfloat16, device=x.device)
-        _check(_few(m.data_ptr(), m.stride(0) if T > 1 else K, w.q.data_ptr(), w.scales.data_ptr(), 0 if w.zeros is None else w.zeros.data_ptr(),
-                    out.data_ptr(), T, N, K, group, current_stream(), 2000), "linear_w4")
-    return out if x.dim() == 2 else out.view(*x.shape[:-1], N)
+        out = m.new_empty((T, N))
+        st = _few(m.data_ptr(), ld, w.q.data_ptr(), w.scales.data_ptr(), None if w.zeros is None else w.zeros.data_ptr(), out.data_ptr(), T, N, K,
+                  group, current_stream(), 2000)
+        if st != 0:
+            _check(st, "linear_w4")
+    return out if len(shape) == 2 else out.view(*shape[:-1], N)
 
 
 def w4_error_site(clear: bool = True) -> int:

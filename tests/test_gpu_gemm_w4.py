@@ -32,11 +32,11 @@ def _exact(w):
 def _check(x, w, got):
     """Few tokens: the products are exact, sums of K terms in fp32.  The tensor core may cut where fp32 rounds (a whole step), so each
     term counts twice.  Many: each weight is rounded to bf16 as well, half a step of it."""
-    from roc_shmem_b200.ops.gemm_w4 import FEW_TOKENS
+    from roc_shmem_b200.ops.gemm_w4 import few_tokens
     m = _exact(w)
     size = x.double().abs() @ m.abs().t()
     steps = 2 * (x.shape[1] // 16 + 16)
-    if x.shape[0] > FEW_TOKENS and m.shape[0] % 8 == 0:
+    if x.shape[0] > few_tokens(w.group) and m.shape[0] % 8 == 0:
         steps += 2.0 ** -8 / 2.0 ** -24
     close(got, x.double() @ m.t(), size, steps)
 
