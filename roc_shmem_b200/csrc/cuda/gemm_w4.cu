@@ -9,34 +9,40 @@ using namespace bshmem;
 
 namespace {
 
-// w in bf16, for products with many tokens on the bf16 kernels: each weight is rounded once (2^-9 of itself at most), as a layer
-// that keeps its weights in bf16 has them.  A thread has 32 columns, which are in one group.
+// w in bf16, for products with many tokens on the bf16 kernels: each weight is rounded once (2^-8 of itself at most), as a layer
+// that keeps its weights in bf16 has them.  A thread has four words of eight columns, a block's width apart.
 struct WidenParams {
-  const uint8_t* q;
+  const uint32_t* q;
   const __nv_bfloat16* s;
   const uint8_t* z;
   __nv_bfloat16* w;
-  long long pieces;                                   // N * K / 32
-  int K, group;
+  long long words;                                    // N * K / 8
+  int per_group;                                      // words of a group; K is whole groups, so rows need no looking at
 };
+constexpr int kWidenWords = 4;
 __global__ void __launch_bounds__(256) w4_widen_kernel(const WidenParams p) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= p.pieces) return;
-  const long long g = i * 32 / p.group;               // K is whole groups, so rows need no looking at
-  const float s = __bfloat162float(p.s[g]), z = p.z ? (float)p.z[g] : 8.f;
-  const uint4 v = ptx::ld_nc_v4(p.q + i * 16);
-  const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+  const long long first = (long long)blockIdx.x * (256 * kWidenWords) + threadIdx.x;
+  uint32_t w[kWidenWords], z[kWidenWords];
+  __nv_bfloat16 s[kWidenWords];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t w = words[j];
-    uint32_t o[4];
+  for (int j = 0; j < kWidenWords; ++j) {
+    const long long i = min(first + j * 256, p.words - 1), g = i / p.per_group;
+    w[j] = __ldg(p.q + i);
+    s[j] = p.s[g];
+    z[j] = p.z ? p.z[g] : 8;
+  }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      o[k] = w4::as_word(__floats2bfloat162_rn(((float)(w >> (8 * k) & 15) - z) * s, ((float)(w >> (8 * k + 4) & 15) - z) * s));
-    }
-    ptx::st_v4(p.w + i * 32 + j * 8, make_uint4(o[0], o[1], o[2], o[3]));
+  for (int j = 0; j < kWidenWords; ++j) {
+    uint32_t o[4];                                    // (0, 4) (1, 5) (2, 6) (3, 7)
+    w4::widen(w[j], w4::as_pair(0x43004300u | z[j] | z[j] << 16), o);
+    // a product of bf16 values rounded once is the weight rounded once: q - z is exact
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = w4::as_word(__hmul2(w4::as_pair(o[k]), __bfloat162bfloat162(s[j])));
+    if (first + j * 256 < p.words)
+      ptx::st_v4(p.w + (first + j * 256) * 8, make_uint4(__byte_perm(o[0], o[1], 0x5410), __byte_perm(o[2], o[3], 0x5410),
+                                                         __byte_perm(o[0], o[1], 0x7632), __byte_perm(o[2], o[3], 0x7632)));
   }
 }
 
@@ -215,10 +221,11 @@ int bshmem_w4_error_site(int clear) {
 int bshmem_w4_widen(const void* q, const void* s, const void* z, void* w, int N, int K, int group, void* stream) {
   if (!shape_ok(N, K, group)) return 1;
   if (!aligned(q) || !aligned(w)) { host::last_error() = "w4: needs 16-byte aligned q and w"; return 1; }
-  const WidenParams p = {static_cast<const uint8_t*>(q), static_cast<const __nv_bfloat16*>(s), static_cast<const uint8_t*>(z),
-                         static_cast<__nv_bfloat16*>(w), (long long)N * (K / 32), K, group};
-  if ((p.pieces + 255) / 256 > 0x7fffffffLL) { host::last_error() = "w4: matrix too large"; return 1; }
-  return launch(w4_widen_kernel, dim3((unsigned)((p.pieces + 255) / 256)), 256, 1, 0, p, stream);
+  const WidenParams p = {static_cast<const uint32_t*>(q), static_cast<const __nv_bfloat16*>(s), static_cast<const uint8_t*>(z),
+                         static_cast<__nv_bfloat16*>(w), (long long)N * (K / 8), group / 8};
+  const long long blocks = (p.words + 256 * kWidenWords - 1) / (256 * kWidenWords);
+  if (blocks > 0x7fffffffLL) { host::last_error() = "w4: matrix too large"; return 1; }
+  return launch(w4_widen_kernel, dim3((unsigned)blocks), 256, 1, 0, p, stream);
 }
 
 // w [N, K] bf16 with row pitch ldw -> q, s and, unless z is null, z.

@@ -135,50 +135,59 @@ template <bool kVec, typename T> __device__ __forceinline__ Vals vector8(const v
 // e4m3's largest): a power of two loses nothing, neither here nor on the way back, and it is one byte (exponent + 127).  Sixteen
 // neighbouring lanes hold a block, eight columns each.  Infinities come back as NaN; e4m3 has none.
 __device__ __forceinline__ float block_scale_bits(uint32_t e) { return __uint_as_float(e << 23); }
-// Subnormal numbers count here, whatever the compiler does with them elsewhere.
-__device__ __forceinline__ float mul_exact(float a, float b) {
-  float r;
-  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 // The largest exponent byte of a type's blocks.  Only there could a value round up to a power of two that the type does not have
 // (2^128, 2^16 for fp16): such values stay at 240 steps instead of 256.
 template <typename T> constexpr uint32_t kTopExponent = 247;
 template <> constexpr uint32_t kTopExponent<__half> = 135;
 
-// All 32 lanes take part.  The eight bytes of this lane's values, which are of type T, and the block's exponent byte.
-template <typename T> __device__ __forceinline__ uint2 encode8(const Vals& pairs, uint32_t& e) {
-  const float v[8] = {pairs.p[0].x, pairs.p[0].y, pairs.p[1].x, pairs.p[1].y, pairs.p[2].x, pairs.p[2].y, pairs.p[3].x, pairs.p[3].y};
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
-    top = max(top, a < 0x7f800000u ? a : 0u);
-  }
-#pragma unroll
-  for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  // largest = m * 2^(E - 127), m in [1, 2), and 448 = 1.75 * 2^8
-  const int b = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u);
-  e = (uint32_t)max(b, 1);
-  const float down = block_scale_bits(254u - e), most = e == kTopExponent<T> ? 240.f : 448.f;
+// The eight bytes of a lane's values; kAny: some may be no numbers, or so large that they could round up (see kTopExponent).
+template <typename T, bool kAny> __device__ __forceinline__ uint2 bytes8(const Vals& v, uint32_t e) {
+  const float2 down = both(block_scale_bits(254u - e));
+  const float most = e == kTopExponent<T> ? 240.f : 448.f;
   uint32_t out[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    uint32_t word = 0;
+    uint16_t two[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      uint16_t two;
-      const float lo = fminf(fmaxf(mul_exact(v[4 * h + 2 * i], down), -most), most);
-      const float hi = fminf(fmaxf(mul_exact(v[4 * h + 2 * i + 1], down), -most), most);
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(hi), "f"(lo));
-      word |= (uint32_t)two << (16 * i);
+      const float2 given = v.p[2 * h + i];
+      float2 f = mul2(given, down);                   // subnormal numbers count: no .ftz
+      if constexpr (kAny) f = make_float2(fminf(fmaxf(f.x, -most), most), fminf(fmaxf(f.y, -most), most));
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two[i]) : "f"(f.y), "f"(f.x));
+      if constexpr (kAny) {                           // the limits made a number of what is none
+        if ((__float_as_uint(given.x) & 0x7fffffffu) >= 0x7f800000u) two[i] |= 0x7f;
+        if ((__float_as_uint(given.y) & 0x7fffffffu) >= 0x7f800000u) two[i] |= 0x7f00;
+      }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)                       // the limits made a number of what is none
-      if ((__float_as_uint(v[4 * h + i]) & 0x7fffffffu) >= 0x7f800000u) word |= 0x7fu << (8 * i);
-    out[h] = word;
+    out[h] = two[0] | (uint32_t)two[1] << 16;
   }
   return make_uint2(out[0], out[1]);
+}
+// All 32 lanes take part.  The eight bytes of this lane's values, which are of type T, and the block's exponent byte.
+template <typename T> __device__ __forceinline__ uint2 encode8(const Vals& v, uint32_t& e) {
+  float top = 0.f;
+  float2 odd = both(0.f);                             // NaN if one of the values is no number, or infinite
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    top = fmaxf(top, fmaxf(fabsf(v.p[i].x), fabsf(v.p[i].y)));
+    odd = fma2(v.p[i], both(0.f), odd);
+  }
+  uint32_t bits = __float_as_uint(top);
+  // rare, and then for the whole warp: the largest of the finite values, and the careful conversion
+  const bool any = __any_sync(0xffffffffu, odd.x + odd.y != 0.f || bits >= (kTopExponent<T> + 7u) << 23);
+  if (any) {
+    bits = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = __float_as_uint(v.p[i].x) & 0x7fffffffu, b = __float_as_uint(v.p[i].y) & 0x7fffffffu;
+      bits = max(bits, max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u));
+    }
+  }
+#pragma unroll
+  for (int o = 8; o; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+  // largest = m * 2^(E - 127), m in [1, 2), and 448 = 1.75 * 2^8
+  e = (uint32_t)max((int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u), 1);
+  return any ? bytes8<T, true>(v, e) : bytes8<T, false>(v, e);
 }
 __device__ __forceinline__ Vals decode8(uint2 q, uint32_t e) {
   Vals v;
@@ -193,7 +202,7 @@ __device__ __forceinline__ Vals decode8(uint2 q, uint32_t e) {
       __half2 pair;
       memcpy(&pair, &two, 4);
       const float2 f = __half22float2(pair);
-      v.p[2 * h + i] = make_float2(mul_exact(f.x, up), mul_exact(f.y, up));
+      v.p[2 * h + i] = mul2(f, both(up));             // subnormal numbers count: no .ftz
     }
   return v;
 }
