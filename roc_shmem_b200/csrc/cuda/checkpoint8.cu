@@ -17,14 +17,14 @@ constexpr int kThreads = 256;
 struct StoreParams { const void* x; long long ldx; uint8_t* q; uint8_t* e; long long ldq, lde, rows; int n; long long eights; };
 
 // Thread i of the grid has the i-th eight of its row; rows are padded to whole blocks of 128 columns (16 threads).
-template <typename T, bool kVec> __global__ void __launch_bounds__(kThreads) store8_kernel(const StoreParams p) {
+template <typename T, int kAccess> __global__ void __launch_bounds__(kThreads) store8_kernel(const StoreParams p) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
   const long long row = i / p.eights;
   const int col = (int)(i - row * p.eights) * 8;
   const int n = row < p.rows ? p.n : 0;
-  const Vals v = unpack(load8<kVec>(static_cast<const T*>(p.x) + (n ? row * p.ldx : 0), col, n));
+  const Vals v = unpack(load8<kAccess>(static_cast<const T*>(p.x) + (n ? row * p.ldx : 0), col, n));
   uint32_t e;
   const uint2 q = encode8<T>(v, e);
   if (col < n) {
@@ -35,7 +35,7 @@ template <typename T, bool kVec> __global__ void __launch_bounds__(kThreads) sto
 
 struct RestoreParams { const uint8_t *q, *e; long long ldq, lde; void* x; long long ldx, rows; int n; long long eights; };
 
-template <typename T, bool kVec> __global__ void __launch_bounds__(kThreads) restore8_kernel(const RestoreParams p) {
+template <typename T, int kAccess> __global__ void __launch_bounds__(kThreads) restore8_kernel(const RestoreParams p) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
@@ -44,7 +44,7 @@ template <typename T, bool kVec> __global__ void __launch_bounds__(kThreads) res
   const int col = (int)(i - row * p.eights) * 8;
   if (col >= p.n) return;
   const Vals v = decode8(__ldg(reinterpret_cast<const uint2*>(p.q + row * p.ldq + col)), __ldg(p.e + row * p.lde + col / 128));
-  store8<kVec>(static_cast<T*>(p.x) + row * p.ldx, col, p.n, pack<T>(v));
+  store8<kAccess>(static_cast<T*>(p.x) + row * p.ldx, col, p.n, pack<T>(v));
 }
 
 // gu: [rows, 2F], 32 columns of the gate and the 32 of `up` that belong to them in turn.
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kThreads) swiglu_store8_kernel(const SwigluPar
   const long long row = i / p.eights;
   const int col = (int)(i - row * p.eights) * 8;
   const int n = row < p.rows ? 2 * p.F : 0;
-  const Raw8<__nv_bfloat16> r = load8<true>(p.gu + (n ? row * n : 0), col, n);
+  const Raw8<__nv_bfloat16> r = load8<kVector>(p.gu + (n ? row * n : 0), col, n);
   const Vals v = unpack(r);
   uint32_t e;
   const uint2 q = encode8<__nv_bfloat16>(v, e);
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kThreads) swiglu_store8_kernel(const SwigluPar
   Vals u = unpack(other);
 #pragma unroll
   for (int j = 0; j < 4; ++j) u.p[j] = mul2(u.p[j], mul2(v.p[j], sigmoid2(v.p[j])));
-  store8<true>(p.act + row * p.F, col / 64 * 32 + col % 32, p.F, pack<__nv_bfloat16>(u));
+  store8<kVector>(p.act + row * p.F, col / 64 * 32 + col % 32, p.F, pack<__nv_bfloat16>(u));
 }
 
 // Thread i has eight columns of the activation: their gate and `up` in 8 bits lie 32 columns apart in one block.
@@ -98,7 +98,7 @@ template <bool kAct> __global__ void __launch_bounds__(kThreads) swiglu_backward
   const uint8_t* q = p.q + row * 2 * p.F + at;
   const uint32_t e = __ldg(p.e + row * p.lde + at / 128);
   const Vals g = decode8(__ldg(reinterpret_cast<const uint2*>(q)), e), u = decode8(__ldg(reinterpret_cast<const uint2*>(q + 32)), e);
-  const Vals d = unpack(load8<true>(p.dact + row * p.F, col, p.F));
+  const Vals d = unpack(load8<kVector>(p.dact + row * p.F, col, p.F));
   Vals dg, du, again;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -109,9 +109,9 @@ template <bool kAct> __global__ void __launch_bounds__(kThreads) swiglu_backward
     dg.p[j] = mul2(mul2(d.p[j], u.p[j]), fma2(silu, make_float2(1.f - s.x, 1.f - s.y), s));
   }
   __nv_bfloat16* o = p.dgu + row * 2 * p.F + at;
-  store8<true>(o, 0, 8, pack<__nv_bfloat16>(dg));
-  store8<true>(o, 32, 40, pack<__nv_bfloat16>(du));
-  if constexpr (kAct) store8<true>(p.act + row * p.F, col, p.F, pack<__nv_bfloat16>(again));
+  store8<kVector>(o, 0, 8, pack<__nv_bfloat16>(dg));
+  store8<kVector>(o, 32, 40, pack<__nv_bfloat16>(du));
+  if constexpr (kAct) store8<kVector>(p.act + row * p.F, col, p.F, pack<__nv_bfloat16>(again));
 }
 
 template <typename K, typename P> int launch(K* kernel, long long threads, const P& p, void* stream) {
@@ -147,9 +147,9 @@ int bshmem_ckpt8_store(int type, const void* x, long long ldx, void* q, void* e,
   const StoreParams p = {x, ldx, static_cast<uint8_t*>(q), static_cast<uint8_t*>(e), ((long long)n + 15) / 16 * 16, blocks, rows, n, blocks * 16};
   const bool vec = n % 8 == 0 && aligned(x) && ldx * (type == 2 ? 4 : 2) % 16 == 0;
   const long long threads = rows * p.eights;
-  if (type == 0) return vec ? launch(store8_kernel<__nv_bfloat16, true>, threads, p, stream) : launch(store8_kernel<__nv_bfloat16, false>, threads, p, stream);
-  if (type == 1) return vec ? launch(store8_kernel<__half, true>, threads, p, stream) : launch(store8_kernel<__half, false>, threads, p, stream);
-  return vec ? launch(store8_kernel<float, true>, threads, p, stream) : launch(store8_kernel<float, false>, threads, p, stream);
+  if (type == 0) return vec ? launch(store8_kernel<__nv_bfloat16, kVector>, threads, p, stream) : launch(store8_kernel<__nv_bfloat16, kSingle>, threads, p, stream);
+  if (type == 1) return vec ? launch(store8_kernel<__half, kVector>, threads, p, stream) : launch(store8_kernel<__half, kSingle>, threads, p, stream);
+  return vec ? launch(store8_kernel<float, kVector>, threads, p, stream) : launch(store8_kernel<float, kSingle>, threads, p, stream);
 }
 
 // The way back; x has row pitch ldx.
@@ -160,9 +160,9 @@ int bshmem_ckpt8_restore(int type, const void* q, const void* e, void* x, long l
                            x, ldx, rows, n, ((long long)n + 7) / 8};
   const bool vec = n % 8 == 0 && aligned(x) && ldx * (type == 2 ? 4 : 2) % 16 == 0;
   const long long threads = rows * p.eights;
-  if (type == 0) return vec ? launch(restore8_kernel<__nv_bfloat16, true>, threads, p, stream) : launch(restore8_kernel<__nv_bfloat16, false>, threads, p, stream);
-  if (type == 1) return vec ? launch(restore8_kernel<__half, true>, threads, p, stream) : launch(restore8_kernel<__half, false>, threads, p, stream);
-  return vec ? launch(restore8_kernel<float, true>, threads, p, stream) : launch(restore8_kernel<float, false>, threads, p, stream);
+  if (type == 0) return vec ? launch(restore8_kernel<__nv_bfloat16, kVector>, threads, p, stream) : launch(restore8_kernel<__nv_bfloat16, kSingle>, threads, p, stream);
+  if (type == 1) return vec ? launch(restore8_kernel<__half, kVector>, threads, p, stream) : launch(restore8_kernel<__half, kSingle>, threads, p, stream);
+  return vec ? launch(restore8_kernel<float, kVector>, threads, p, stream) : launch(restore8_kernel<float, kSingle>, threads, p, stream);
 }
 
 // gu [rows, 2F] bf16 -> act [rows, F] and gu in 8 bits.  Everything contiguous and 16-byte aligned, F % 32 == 0.

@@ -57,6 +57,7 @@ struct BwdParams {
   int gate_kind;
   int w1_f32, w2_f32, gcol_f32, gate_f32, scale_f32;
   int stages, ring_words;
+  int held;                             // the weights are in shared memory
 };
 
 template <typename T> __device__ __forceinline__ float number(const void* p, int f32, float otherwise) {
@@ -107,7 +108,8 @@ __device__ __forceinline__ float sum2(float2 v) { return v.x + v.y; }
 // In a ring the weights (w1 times a gate per column, and w2) stay in registers too.
 template <typename T, int kMode, int kChunks, int kForm>
 __global__ void __launch_bounds__(kForm == kDirect && kChunks == 1 ? 1024 : 512) norm_fwd_kernel(const Params p) {
-  constexpr bool kVec = kForm != kScalar, kHeld = kForm == kRing && kChunks <= 2;
+  constexpr int kAccess = kForm == kScalar ? kStrided : kVector;
+  constexpr bool kHeld = kForm == kRing && kChunks <= 2;
   constexpr int W = Raw8<T>::kWords, kX = kMode == kPre ? 0 : kChunks * W, kGate = kX + kChunks * W;
   extern __shared__ uint4 ring_words[];
   __shared__ float sums[2 * kMaxWarps];
@@ -148,9 +150,9 @@ __global__ void __launch_bounds__(kForm == kDirect && kChunks == 1 ? 1024 : 512)
     for (int i = 0; i < p.stages; ++i) fetch(first + threadIdx.y + i * step, i);
   const float scale0 = number<T>(p.scale, p.scale_f32, p.scale_value);
   auto weight1 = [&](int i) {
-    Vals w = vector8<kVec, T>(p.w1, p.w1_f32, column(i), p.n);
+    Vals w = vector8<kAccess, T>(p.w1, p.w1_f32, column(i), p.n);
     if (p.gate_kind == kColumn) {
-      const Vals g = vector8<kVec, T>(p.gcol, p.gcol_f32, column(i), p.n);
+      const Vals g = vector8<kAccess, T>(p.gcol, p.gcol_f32, column(i), p.n);
 #pragma unroll
       for (int j = 0; j < 4; ++j) w.p[j] = mul2(w.p[j], g.p[j]);
     }
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(kForm == kDirect && kChunks == 1 ? 1024 : 512)
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       if constexpr (kMode != kPre) held1[i] = weight1(i);
-      if constexpr (kMode != kPost) held2[i] = vector8<kVec, T>(p.w2, p.w2_f32, column(i), p.n);
+      if constexpr (kMode != kPost) held2[i] = vector8<kAccess, T>(p.w2, p.w2_f32, column(i), p.n);
     }
   }
   for (; first < p.rows; first += step) {                    // the same for the whole block
@@ -177,8 +179,8 @@ __global__ void __launch_bounds__(kForm == kDirect && kChunks == 1 ? 1024 : 512)
         if constexpr (kForm == kRing) {
           y[i] = ring.get8<T>(stage, i * W);
         } else {
-          y[i] = unpack(load8<kVec>(row_of<T>(p.y, row), column(i), n));
-          x[i] = unpack(load8<kVec>(row_of<T>(p.x, row), column(i), n));
+          y[i] = unpack(load8<kAccess>(row_of<T>(p.y, row), column(i), n));
+          x[i] = unpack(load8<kAccess>(row_of<T>(p.x, row), column(i), n));
         }
       }
       float scale = scale0;
@@ -194,14 +196,7 @@ __global__ void __launch_bounds__(kForm == kDirect && kChunks == 1 ? 1024 : 512)
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const int col = column(i);
-        if (p.q1) {
-          uint32_t e;
-          const uint2 q = encode8<T>(y[i], e);
-          if (col < n) {
-            *reinterpret_cast<uint2*>(p.q1 + row * p.ldq + col) = q;
-            if (col % 128 == 0) p.e1[row * p.lde + col / 128] = (uint8_t)e;
-          }
-        }
+        if (p.q1) keep8<kAccess, T>(p.q1 + row * p.ldq, p.e1 + row * p.lde, col, n, y[i]);
         Vals w, r;
         if constexpr (kHeld) w = held1[i];
         else w = weight1(i);
@@ -210,21 +205,21 @@ __global__ void __launch_bounds__(kForm == kDirect && kChunks == 1 ? 1024 : 512)
         if (p.gate_kind == kElement) {
           Vals g;
           if constexpr (kForm == kRing) g = p.gate_f32 ? ring.get8<float>(stage, kGate + i * 2) : ring.get8<T>(stage, kGate + i * W);
-          else g = p.gate_f32 ? unpack(load8<kVec>(row_of<float>(p.gate, row), col, n)) : unpack(load8<kVec>(row_of<T>(p.gate, row), col, n));
+          else g = p.gate_f32 ? unpack(load8<kAccess>(row_of<float>(p.gate, row), col, n)) : unpack(load8<kAccess>(row_of<T>(p.gate, row), col, n));
 #pragma unroll
           for (int j = 0; j < 4; ++j) w.p[j] = mul2(w.p[j], g.p[j]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) r.p[j] = fma2(mul2(y[i].p[j], f), w.p[j], r.p[j]);
         const Raw8<T> o = pack<T>(r);
-        store8<kVec>(row_of<T>(p.out, row), col, n, o);
+        store8<kAccess>(row_of<T>(p.out, row), col, n, o);
         if constexpr (kMode == kPostPre) z[i] = unpack(o);   // the next norm is one of the stored sum
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         if constexpr (kForm == kRing) z[i] = ring.get8<T>(stage, i * W);
-        else z[i] = unpack(load8<kVec>(row_of<T>(p.x, row), column(i), n));
+        else z[i] = unpack(load8<kAccess>(row_of<T>(p.x, row), column(i), n));
       }
     }
     if constexpr (kForm == kRing) {
@@ -242,20 +237,13 @@ __global__ void __launch_bounds__(kForm == kDirect && kChunks == 1 ? 1024 : 512)
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const int col = column(i);
-        if (p.q2) {
-          uint32_t e;
-          const uint2 q = encode8<T>(z[i], e);
-          if (col < n) {
-            *reinterpret_cast<uint2*>(p.q2 + row * p.ldq + col) = q;
-            if (col % 128 == 0) p.e2[row * p.lde + col / 128] = (uint8_t)e;
-          }
-        }
+        if (p.q2) keep8<kAccess, T>(p.q2 + row * p.ldq, p.e2 + row * p.lde, col, n, z[i]);
         Vals w;
         if constexpr (kHeld) w = held2[i];
-        else w = vector8<kVec, T>(p.w2, p.w2_f32, col, n);
+        else w = vector8<kAccess, T>(p.w2, p.w2_f32, col, n);
 #pragma unroll
         for (int j = 0; j < 4; ++j) w.p[j] = mul2(mul2(z[i].p[j], both(rstd)), w.p[j]);
-        store8<kVec>(row_of<T>(p.h, row), col, n, pack<T>(w));
+        store8<kAccess>(row_of<T>(p.h, row), col, n, pack<T>(w));
       }
     }
   }
@@ -263,10 +251,13 @@ __global__ void __launch_bounds__(kForm == kDirect && kChunks == 1 ? 1024 : 512)
 
 // ---- backward ------------------------------------------------------------------------------------------
 // A block walks over rows and keeps the column sums of its rows in registers; norm_bwd_finish_kernel adds up the groups' sums in
-// their order, so two calls give the same bits.  In a ring the weights are fp32 words of shared memory behind the stages.
-template <typename T, int kMode, int kChunks, int kForm, bool kKept8>
-__global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
-  constexpr bool kVec = kForm != kScalar;
+// their order, so two calls give the same bits.  In a ring the weights are fp32 words of shared memory behind the stages, where
+// there is room.  kLong: rows of over 8192 columns on 1024 threads, whose 64 registers do not hold the column sums: words of shared
+// memory do, which only their thread touches.
+template <typename T, int kMode, int kChunks, int kForm, bool kKept8, bool kLong = false>
+__global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdParams p) {
+
+  constexpr int kAccess = kForm == kScalar ? kStrided : kVector;
   // words of a stage: dout, dh, z, y, the two 1 / sqrt(...) and the gate per element; one that is kept in 8 bits has its
   // eight bytes and the four that its exponent byte is among in one word
   constexpr int W = Raw8<T>::kWords, K = kKept8 ? 1 : W;
@@ -286,12 +277,25 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
   ptx::grid_launch_dependents();
   const float inv_n = 1.f / (float)p.n;
   const float scale = number<T>(p.scale, p.scale_f32, p.scale_value);
-  Vals acc_w2[kMode != kPost ? kChunks : 1], acc_c[kMode != kPre ? kChunks : 1];
+  Vals acc_w2[kMode != kPost && !kLong ? kChunks : 1], acc_c[kMode != kPre && !kLong ? kChunks : 1];
   float acc_s = 0.f;
+  const Ring accs(ring_words, 0, 0);                         // kLong: [sum][thread]
+  auto hold = [](const Ring& r, int word, const Vals& v) {
+    r.mine[word * r.threads] = make_uint4(__float_as_uint(v.p[0].x), __float_as_uint(v.p[0].y), __float_as_uint(v.p[1].x), __float_as_uint(v.p[1].y));
+    r.mine[(word + 1) * r.threads] = make_uint4(__float_as_uint(v.p[2].x), __float_as_uint(v.p[2].y), __float_as_uint(v.p[3].x), __float_as_uint(v.p[3].y));
+  };
+  constexpr int kAccC = kMode == kPost ? 0 : kChunks * 2;    // words of the first sum, of w2
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
-    if constexpr (kMode != kPost) acc_w2[i].fill(0.f);
-    if constexpr (kMode != kPre) acc_c[i].fill(0.f);
+    Vals zero;
+    zero.fill(0.f);
+    if constexpr (kLong) {
+      if constexpr (kMode != kPost) hold(accs, i * 2, zero);
+      if constexpr (kMode != kPre) hold(accs, kAccC + i * 2, zero);
+    } else {
+      if constexpr (kMode != kPost) acc_w2[i] = zero;
+      if constexpr (kMode != kPre) acc_c[i] = zero;
+    }
   }
   const long long step = (long long)gridDim.x * blockDim.y;
   auto column = [&](int i) { return (int)(threadIdx.x + i * blockDim.x) * 8; };
@@ -313,20 +317,14 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
     } else if constexpr (kForm == kRing) {
       return ring.get8<T>(stage, word);
     } else if constexpr (kKept8) {
-      uint2 b = make_uint2(0, 0);
-      uint32_t x = 1;
-      if (col < n) {
-        b = __ldg(reinterpret_cast<const uint2*>(q + row * p.ldq + col));
-        x = __ldg(e + row * p.lde + col / 128);
-      }
-      return decode8(b, x);
+      return kept8<kAccess>(q + row * p.ldq, e + row * p.lde, col, n);
     } else {
-      return unpack(load8<kVec>(row_of<T>(m, row), col, n));
+      return unpack(load8<kAccess>(row_of<T>(m, row), col, n));
     }
   };
   auto plain = [&](int stage, int word, const Mat& m, long long row, int col, int n) {
     if constexpr (kForm == kRing) return ring.get8<T>(stage, word);
-    else return unpack(load8<kVec>(row_of<T>(m, row), col, n));
+    else return unpack(load8<kAccess>(row_of<T>(m, row), col, n));
   };
   auto fetch = [&](long long row, int stage) {
     if (row < p.rows) {
@@ -359,24 +357,22 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
   long long first = (long long)blockIdx.x * blockDim.y;
   int stage = 0;
   auto weight1 = [&](int i, int n) {
-    Vals w = vector8<kVec, T>(p.w1, p.w1_f32, column(i), n);
+    Vals w = vector8<kAccess, T>(p.w1, p.w1_f32, column(i), n);
     if (p.gate_kind == kColumn) {
-      const Vals g = vector8<kVec, T>(p.gcol, p.gcol_f32, column(i), n);
+      const Vals g = vector8<kAccess, T>(p.gcol, p.gcol_f32, column(i), n);
 #pragma unroll
       for (int j = 0; j < 4; ++j) w.p[j] = mul2(w.p[j], g.p[j]);
     }
     return w;
   };
-  auto hold = [&](int word, const Vals& v) {
-    weights.mine[word * weights.threads] = make_uint4(__float_as_uint(v.p[0].x), __float_as_uint(v.p[0].y), __float_as_uint(v.p[1].x), __float_as_uint(v.p[1].y));
-    weights.mine[(word + 1) * weights.threads] = make_uint4(__float_as_uint(v.p[2].x), __float_as_uint(v.p[2].y), __float_as_uint(v.p[3].x), __float_as_uint(v.p[3].y));
-  };
   if constexpr (kForm == kRing) {
     for (int i = 0; i < p.stages; ++i) fetch(first + threadIdx.y + i * step, i);
+    if (p.held) {
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      if constexpr (kMode != kPre) hold(i * 2, weight1(i, p.n));
-      if constexpr (kMode != kPost) hold(kW2 + i * 2, vector8<kVec, T>(p.w2, p.w2_f32, column(i), p.n));
+      for (int i = 0; i < kChunks; ++i) {
+        if constexpr (kMode != kPre) hold(weights, i * 2, weight1(i, p.n));
+        if constexpr (kMode != kPost) hold(weights, kW2 + i * 2, vector8<kAccess, T>(p.w2, p.w2_f32, column(i), p.n));
+      }
     }
   }
   for (; first < p.rows; first += step) {                    // the same for the whole block
@@ -422,15 +418,20 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         Vals w;
-        if constexpr (kForm == kRing) w = weights.get8<float>(0, kW2 + i * 2);
-        else w = vector8<kVec, T>(p.w2, p.w2_f32, column(i), n);
+        if (kForm == kRing && p.held) w = weights.get8<float>(0, kW2 + i * 2);
+        else w = vector8<kAccess, T>(p.w2, p.w2_f32, column(i), n);
+        Vals sums_w2;
+        if constexpr (kLong) sums_w2 = accs.get8<float>(0, i * 2);
+        else sums_w2 = acc_w2[i];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           nz[i].p[j] = mul2(nz[i].p[j], both(rstd2));
-          acc_w2[i].p[j] = fma2(t[i].p[j], nz[i].p[j], acc_w2[i].p[j]);
+          sums_w2.p[j] = fma2(t[i].p[j], nz[i].p[j], sums_w2.p[j]);
           t[i].p[j] = mul2(t[i].p[j], w.p[j]);
           dot = fma2(t[i].p[j], nz[i].p[j], dot);
         }
+        if constexpr (kLong) hold(accs, i * 2, sums_w2);
+        else acc_w2[i] = sums_w2;
       }
       const float mean = sum(sum2(dot)) * inv_n;
 #pragma unroll
@@ -442,7 +443,7 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
           if constexpr (kMode == kPre) dz[i].p[j] = mul2(d, both(rstd2));
           else dz[i].p[j] = fma2(d, both(rstd2), dz[i].p[j]);
         }
-        store8<kVec>(row_of<T>(p.dz, row), column(i), n, pack<T>(dz[i]));
+        store8<kAccess>(row_of<T>(p.dz, row), column(i), n, pack<T>(dz[i]));
       }
     }
     if constexpr (kMode != kPre) {
@@ -453,28 +454,33 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
         const int col = column(i);
         if constexpr (kMode == kPostPre && kForm == kRing) first_norm(i);
         Vals w;
-        if constexpr (kForm == kRing) w = weights.get8<float>(0, i * 2);
+        if (kForm == kRing && p.held) w = weights.get8<float>(0, i * 2);
         else w = weight1(i, n);
         if (p.gate_kind == kElement) {
           Vals g;
           if constexpr (kForm == kRing) g = p.gate_f32 ? ring.get8<float>(stage, kGate + i * 2) : ring.get8<T>(stage, kGate + i * W);
-          else g = p.gate_f32 ? unpack(load8<kVec>(row_of<float>(p.gate, row), col, n)) : unpack(load8<kVec>(row_of<T>(p.gate, row), col, n));
+          else g = p.gate_f32 ? unpack(load8<kAccess>(row_of<float>(p.gate, row), col, n)) : unpack(load8<kAccess>(row_of<T>(p.gate, row), col, n));
           if (p.dgate.p) {
             Vals d;
 #pragma unroll
             for (int j = 0; j < 4; ++j) d.p[j] = mul2(mul2(both(scale), w.p[j]), mul2(dz[i].p[j], ny[i].p[j]));
-            if (p.gate_f32) store8<kVec>(row_of<float>(p.dgate, row), col, n, pack<float>(d));
-            else store8<kVec>(row_of<T>(p.dgate, row), col, n, pack<T>(d));
+            if (p.gate_f32) store8<kAccess>(row_of<float>(p.dgate, row), col, n, pack<float>(d));
+            else store8<kAccess>(row_of<T>(p.dgate, row), col, n, pack<T>(d));
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) dz[i].p[j] = mul2(dz[i].p[j], g.p[j]);
         }
+        Vals sums_c;
+        if constexpr (kLong) sums_c = accs.get8<float>(0, kAccC + i * 2);
+        else sums_c = acc_c[i];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          acc_c[i].p[j] = fma2(mul2(dz[i].p[j], both(row_gate)), ny[i].p[j], acc_c[i].p[j]);
+          sums_c.p[j] = fma2(mul2(dz[i].p[j], both(row_gate)), ny[i].p[j], sums_c.p[j]);
           dz[i].p[j] = mul2(dz[i].p[j], w.p[j]);
           dot2 = fma2(dz[i].p[j], ny[i].p[j], dot2);
         }
+        if constexpr (kLong) hold(accs, kAccC + i * 2, sums_c);
+        else acc_c[i] = sums_c;
       }
       if constexpr (kForm == kRing) fetch(first + threadIdx.y + p.stages * step, stage);   // this thread has read its words
       const float dot = sum(sum2(dot2));
@@ -490,7 +496,7 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
           Vals d;
 #pragma unroll
           for (int j = 0; j < 4; ++j) d.p[j] = mul2(fma2(ny[i].p[j], both(-mean), dz[i].p[j]), both(f));
-          store8<kVec>(row_of<T>(p.dy, row), column(i), n, pack<T>(d));
+          store8<kAccess>(row_of<T>(p.dy, row), column(i), n, pack<T>(d));
         }
       }
     } else if constexpr (kForm == kRing) {
@@ -500,15 +506,16 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const BwdParams p) {
       if (++stage == p.stages) stage = 0;
   }
   const long long group = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  const long long at = group * ((p.n + 7) / 8 * 8);          // a group's sums are padded to whole eights
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
-    const int col = column(i);
-    const long long at = group * ((p.n + 7) / 8 * 8) + col;  // a group's sums are padded to whole eights
-    if (col < p.n) {
-      if constexpr (kMode != kPost)
-        if (p.part_w2) store8<true>(p.part_w2 + at, 0, 8, pack<float>(acc_w2[i]));
-      if constexpr (kMode != kPre)
-        if (p.part_c) store8<true>(p.part_c + at, 0, 8, pack<float>(acc_c[i]));
+    if constexpr (kMode != kPost) {
+      if constexpr (kLong) acc_w2[0] = accs.get8<float>(0, i * 2);
+      if (p.part_w2) store8<kAccess>(p.part_w2 + at, column(i), p.n, pack<float>(acc_w2[kLong ? 0 : i]));
+    }
+    if constexpr (kMode != kPre) {
+      if constexpr (kLong) acc_c[0] = accs.get8<float>(0, kAccC + i * 2);
+      if (p.part_c) store8<kAccess>(p.part_c + at, column(i), p.n, pack<float>(acc_c[kLong ? 0 : i]));
     }
   }
   if (kMode != kPre && p.part_s && threadIdx.x == 0) p.part_s[group] = acc_s;
@@ -590,7 +597,7 @@ template <typename F> Shape forward_shape(long long rows, int n, bool vec, int s
 template <typename F, typename G> Shape backward_shape(long long rows, int n, bool vec, int sms, F words, G held) {
   const int eights = (n + 7) / 8;
   Shape s = {};
-  s.chunks = eights > 1024 ? 4 : eights > 32 ? 2 : 1;
+  s.chunks = eights > 32 ? 2 : 1;
   s.threads = ((eights + s.chunks - 1) / s.chunks + 31) / 32 * 32;
   s.rows = s.threads >= 256 ? 1 : 256 / s.threads;
   if (s.rows > rows) s.rows = rows < 1 ? 1 : (int)rows;
@@ -599,8 +606,12 @@ template <typename F, typename G> Shape backward_shape(long long rows, int n, bo
   const long long most = (long long)sms * per_sm;
   s.blocks = (int)(need < most ? need : most);
   s.form = vec ? kDirect : kScalar;
-  if (vec && s.chunks <= 2) {
+  if (eights > 1024) {
+    s.words = 0;
+    s.held = held(s.chunks);                          // as many words as the weights: the column sums
+  } else if (vec) {
     ring_of(s, words(s.chunks), held(s.chunks), per_sm);
+    if (s.stages < 2) ring_of(s, words(s.chunks), 0, per_sm);
     if (s.stages >= 2 && need > most) s.form = kRing;
   }
   return s;
@@ -630,21 +641,24 @@ inline int backward_words(int size, int mode, bool kept, int gate_kind, bool gat
 inline int backward_held(int mode, int chunks) { return chunks * 2 * (mode == kPostPre ? 2 : 1); }
 template <typename T, int kMode, bool kKept> int backward_mode(const Shape& s, BwdParams p, cudaStream_t stream) {
   const dim3 grid((unsigned)s.blocks), block(s.threads, s.rows);
+  if (s.threads > 512) {
+    if (s.form == kDirect) return launch(norm_bwd_kernel<T, kMode, 2, kDirect, kKept, true>, grid, block, shared_of(s), p, stream);
+    return launch(norm_bwd_kernel<T, kMode, 2, kScalar, kKept, true>, grid, block, shared_of(s), p, stream);
+  }
   if (s.form == kRing) {
     p.stages = s.stages;
     p.ring_words = s.words;
+    p.held = s.held != 0;
     const int shared = shared_of(s);
     if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kRing, kKept>, grid, block, shared, p, stream);
     return launch(norm_bwd_kernel<T, kMode, 2, kRing, kKept>, grid, block, shared, p, stream);
   }
   if (s.form == kDirect) {
     if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kDirect, kKept>, grid, block, 0, p, stream);
-    if (s.chunks == 2) return launch(norm_bwd_kernel<T, kMode, 2, kDirect, kKept>, grid, block, 0, p, stream);
-    return launch(norm_bwd_kernel<T, kMode, 4, kDirect, kKept>, grid, block, 0, p, stream);
+    return launch(norm_bwd_kernel<T, kMode, 2, kDirect, kKept>, grid, block, 0, p, stream);
   }
   if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kScalar, kKept>, grid, block, 0, p, stream);
-  if (s.chunks == 2) return launch(norm_bwd_kernel<T, kMode, 2, kScalar, kKept>, grid, block, 0, p, stream);
-  return launch(norm_bwd_kernel<T, kMode, 4, kScalar, kKept>, grid, block, 0, p, stream);
+  return launch(norm_bwd_kernel<T, kMode, 2, kScalar, kKept>, grid, block, 0, p, stream);
 }
 
 // The kernels for one type of rows; norm_bf16.cu, norm_fp16.cu and norm_fp32.cu instantiate them.

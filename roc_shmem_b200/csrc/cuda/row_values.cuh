@@ -96,37 +96,44 @@ template <> __device__ __forceinline__ Raw8<__half> pack(const Vals& v) {
   return r;
 }
 
-// Columns col .. col + 7 of the row at `row`, zeros from column n on.  kVec: the row is 16-byte aligned and n % 8 == 0.
-template <bool kVec, typename T> __device__ __forceinline__ Raw8<T> load8(const T* row, int col, int n) {
+// How eight values lie in a row.  kVector: columns col .. col + 7, the row is 16-byte aligned and the row's length n % 8 == 0.  kSingle:
+// the same columns, one by one.  kStrided: one by one too, but for a warp on 256 neighbouring columns the lanes' j-th values are
+// neighbours (lane, lane + 32, ...), so that each access of the warp is whole sectors.
+enum Access : int { kSingle = 0, kVector = 1, kStrided = 2 };
+template <int kAccess> __device__ __forceinline__ int column_of(int col, int j) {
+  return kAccess == kStrided ? (col & ~255) + (col >> 3 & 31) + 32 * j : col + j;
+}
+// Columns from n on are zeros.
+template <int kAccess, typename T> __device__ __forceinline__ Raw8<T> load8(const T* row, int col, int n) {
   Raw8<T> r;
-  if constexpr (kVec) {
+  if constexpr (kAccess == kVector) {
 #pragma unroll
     for (int i = 0; i < Raw8<T>::kWords; ++i) r.set(i, col < n ? __ldg(reinterpret_cast<const uint4*>(row + col) + i) : make_uint4(0, 0, 0, 0));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = col + i < n ? row[col + i] : from_float<T>(0.f);
+    for (int j = 0; j < 8; ++j) r.v[j] = column_of<kAccess>(col, j) < n ? row[column_of<kAccess>(col, j)] : from_float<T>(0.f);
   }
   return r;
 }
-template <bool kVec, typename T> __device__ __forceinline__ void store8(T* row, int col, int n, const Raw8<T>& r) {
-  if constexpr (kVec) {
+template <int kAccess, typename T> __device__ __forceinline__ void store8(T* row, int col, int n, const Raw8<T>& r) {
+  if constexpr (kAccess == kVector) {
     if (col < n) {
 #pragma unroll
       for (int i = 0; i < Raw8<T>::kWords; ++i) reinterpret_cast<uint4*>(row + col)[i] = r.get(i);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (col + i < n) row[col + i] = r.v[i];
+    for (int j = 0; j < 8; ++j)
+      if (column_of<kAccess>(col, j) < n) row[column_of<kAccess>(col, j)] = r.v[j];
   }
 }
 
 // A vector over the columns (a weight, a gate per channel) in the rows' own type T or in fp32; ones where there is none.
-template <bool kVec, typename T> __device__ __forceinline__ Vals vector8(const void* vec, bool f32, int col, int n) {
+template <int kAccess, typename T> __device__ __forceinline__ Vals vector8(const void* vec, bool f32, int col, int n) {
   Vals v;
   if (!vec) v.fill(1.f);
-  else if (f32) v = unpack(load8<kVec>(static_cast<const float*>(vec), col, n));
-  else v = unpack(load8<kVec>(static_cast<const T*>(vec), col, n));
+  else if (f32) v = unpack(load8<kAccess>(static_cast<const float*>(vec), col, n));
+  else v = unpack(load8<kAccess>(static_cast<const T*>(vec), col, n));
   return v;
 }
 
@@ -163,7 +170,15 @@ template <typename T, bool kAny> __device__ __forceinline__ uint2 bytes8(const V
   }
   return make_uint2(out[0], out[1]);
 }
-// All 32 lanes take part.  The eight bytes of this lane's values, which are of type T, and the block's exponent byte.
+// largest = m * 2^(E - 127), m in [1, 2), and 448 = 1.75 * 2^8
+__device__ __forceinline__ uint32_t exponent_byte(uint32_t largest) {
+  return (uint32_t)max((int)(largest >> 23) - 8 + ((largest & 0x7fffffu) > 0x600000u), 1);
+}
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t a = __float_as_uint(v) & 0x7fffffffu;
+  return a < 0x7f800000u ? a : 0u;
+}
+// All 32 lanes take part; sixteen of them hold a block.  The eight bytes of this lane's values, which are of type T, and the block's exponent byte.
 template <typename T> __device__ __forceinline__ uint2 encode8(const Vals& v, uint32_t& e) {
   float top = 0.f;
   float2 odd = both(0.f);                             // NaN if one of the values is no number, or infinite
@@ -178,15 +193,11 @@ template <typename T> __device__ __forceinline__ uint2 encode8(const Vals& v, ui
   if (any) {
     bits = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t a = __float_as_uint(v.p[i].x) & 0x7fffffffu, b = __float_as_uint(v.p[i].y) & 0x7fffffffu;
-      bits = max(bits, max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u));
-    }
+    for (int i = 0; i < 4; ++i) bits = max(bits, max(finite_bits(v.p[i].x), finite_bits(v.p[i].y)));
   }
 #pragma unroll
   for (int o = 8; o; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
-  // largest = m * 2^(E - 127), m in [1, 2), and 448 = 1.75 * 2^8
-  e = (uint32_t)max((int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u), 1);
+  e = exponent_byte(bits);
   return any ? bytes8<T, true>(v, e) : bytes8<T, false>(v, e);
 }
 __device__ __forceinline__ Vals decode8(uint2 q, uint32_t e) {
@@ -205,6 +216,61 @@ __device__ __forceinline__ Vals decode8(uint2 q, uint32_t e) {
       v.p[2 * h + i] = mul2(f, both(up));             // subnormal numbers count: no .ftz
     }
   return v;
+}
+
+// A lane's eight values into a row of bytes and exponents, and back.  kStrided: the warp's 256 columns are two blocks, of the lanes'
+// first four and last four values.
+template <int kAccess, typename T> __device__ __forceinline__ void keep8(uint8_t* q, uint8_t* e, int col, int n, const Vals& v) {
+  if constexpr (kAccess == kVector) {
+    uint32_t x;
+    const uint2 b = encode8<T>(v, x);
+    if (col < n) {
+      *reinterpret_cast<uint2*>(q + col) = b;
+      if (col % 128 == 0) e[col / 128] = (uint8_t)x;
+    }
+  } else {
+    uint32_t x[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i / 2] = max(x[i / 2], max(finite_bits(v.p[i].x), finite_bits(v.p[i].y)));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      x[0] = max(x[0], __shfl_xor_sync(0xffffffffu, x[0], o));
+      x[1] = max(x[1], __shfl_xor_sync(0xffffffffu, x[1], o));
+    }
+    const uint32_t e0 = exponent_byte(x[0]), e1 = exponent_byte(x[1]), low = bytes8<T, true>(v, e0).x, high = bytes8<T, true>(v, e1).y;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (column_of<kAccess>(col, j) < n) q[column_of<kAccess>(col, j)] = (uint8_t)((j < 4 ? low : high) >> (8 * (j & 3)));
+    if (col % 256 == 0) {
+      if (col < n) e[col / 128] = (uint8_t)e0;
+      if (col + 128 < n) e[col / 128 + 1] = (uint8_t)e1;
+    }
+  }
+}
+template <int kAccess> __device__ __forceinline__ Vals kept8(const uint8_t* q, const uint8_t* e, int col, int n) {
+  if constexpr (kAccess == kVector) {
+    uint2 b = make_uint2(0, 0);
+    uint32_t x = 1;
+    if (col < n) {
+      b = __ldg(reinterpret_cast<const uint2*>(q + col));
+      x = __ldg(e + col / 128);
+    }
+    return decode8(b, x);
+  } else {
+    const int block = (col & ~255) / 128;
+    const uint32_t e0 = col - (col & 255) < n ? e[block] : 1, e1 = col - (col & 255) + 128 < n ? e[block + 1] : 1;
+    uint2 b = make_uint2(0, 0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t x = column_of<kAccess>(col, j) < n ? q[column_of<kAccess>(col, j)] : 0;
+      if (j < 4) b.x |= x << (8 * j);
+      else b.y |= x << (8 * (j - 4));
+    }
+    const Vals low = decode8(b, e0), high = decode8(b, e1);
+    Vals v;
+    v.p[0] = low.p[0]; v.p[1] = low.p[1]; v.p[2] = high.p[2]; v.p[3] = high.p[3];
+    return v;
+  }
 }
 
 // ---- sums over a row -----------------------------------------------------------------------------------
