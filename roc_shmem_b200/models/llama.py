@@ -16,9 +16,11 @@ from typing import Optional
 
 import torch
 
+from ..ops.checkpoint8 import Checkpoint8, restore, store, swiglu_backward
 from ..ops.gemm import current_stream, gemm_bf16
 from ..ops.moe import _fast as moe_fast
 from ..ops.moe import (grouped_gemm, grouped_gemm_act, grouped_gemm_swiglu_bwd, grouped_gemm_tn, interleave_gate_up, moe_lib)
+from ..ops.norms import post_norm, rms_norm
 from ..parallel.tp import ColumnParallelLinear, RowParallelLinear
 
 
@@ -109,11 +111,19 @@ class LlamaMLP:
             return x
         return buffer.copy_(x)
 
-    def backward(self, dy_shard: torch.Tensor) -> torch.Tensor:
-        """Returns dx_shard [M/P, H]; weight gradients land in ``dw13`` / ``dw2``.  Must follow forward()."""
+    def keep(self) -> tuple[Checkpoint8, Checkpoint8]:
+        """What the backward pass of the last forward() needs of it, in 8 bits: the rows that went in (all ranks') and the
+        pre-activations.  With it backward() may come after further forward() calls; it takes up (H + 2F/P) bytes a token where the
+        block's own buffers have 2H + 6F/P."""
+        assert self.training
+        return store(self.up.gathered), store(self.gu)
+
+    def backward(self, dy_shard: torch.Tensor, kept: Optional[tuple[Checkpoint8, Checkpoint8]] = None) -> torch.Tensor:
+        """Returns dx_shard [M/P, H]; weight gradients land in ``dw13`` / ``dw2``.  Must follow forward(), unless it gets what keep()
+        gave after the forward() that it belongs to: the gradients are then those at the kept values."""
         assert self.training
         s = current_stream()
-        fused = self.P == 1 and self._fills(self.Fp)
+        fused = self.P == 1 and self._fills(self.Fp) and kept is None
         if self.P == 1:
             dy = self._operand(dy_shard, self.dgrad_h.x_shard)                     # nothing to gather
             if fused:
@@ -123,13 +133,16 @@ class LlamaMLP:
         else:
             dh = self.dgrad_h(dy_shard, weight=self.w2_t)                          # [M, F/P], gathers dy
             dy = self.dgrad_h.gathered
+        if kept is not None:
+            restore(kept[0], out=self.up.gathered)
+            swiglu_backward(kept[1], dh, dgu_out=self.dgu, act_out=self.h)         # SwiGLU' and the activations again
         grouped_gemm_tn(dy, self.h, self.dw2, 1, self.rows)                        # dW2 = dy^T h
-        if not fused:
+        if not fused and kept is None:
             self._chk(moe_fast.swiglu_bwd(self.gu.data_ptr(), dh.data_ptr(), self.rows.data_ptr(), 1, self.M, self.Fp,
                                           self.dgu.data_ptr(), s), "swiglu bwd")
         grouped_gemm_tn(self.dgu, self.up.gathered, self.dw13, 1, self.rows)       # dW13 = dgu^T x
         dx = self.dgrad_x(self.dgu, weight=self.w13_t)
-        self.launches += 4 if fused else 5
+        self.launches += 4 if fused else 5 if kept is None else 6
         return dx
 
     def check(self) -> None:
@@ -144,30 +157,53 @@ class _LlamaMLPFn(torch.autograd.Function):
     """autograd bridge: the block's hand-written backward supplies every gradient."""
 
     @staticmethod
-    def forward(ctx, x, w13, w2, block):
-        ctx.block = block
-        return block.forward(x).clone()
+    def forward(ctx, x, w13, w2, block, checkpoint):
+        ctx.block, ctx.shapes = block, None
+        y = block.forward(x).clone()
+        if checkpoint:
+            kept = block.keep()
+            ctx.save_for_backward(*(t for c in kept for t in (c.q, c.e)))
+            ctx.shapes = [(c.shape, c.dtype) for c in kept]
+        return y
 
     @staticmethod
     def backward(ctx, dy):
-        block = ctx.block
-        dx = block.backward(dy.contiguous())
-        return dx.clone(), block.dw13.clone(), block.dw2.clone(), None
+        block, kept = ctx.block, None
+        if ctx.shapes is not None:
+            t = ctx.saved_tensors
+            kept = Checkpoint8(t[0], t[1], *ctx.shapes[0]), Checkpoint8(t[2], t[3], *ctx.shapes[1])
+        dx = block.backward(dy.contiguous(), kept)
+        return dx.clone(), block.dw13.clone(), block.dw2.clone(), None, None
 
 
 class LlamaMLPModule(torch.nn.Module):
     """``torch.nn.Module`` face of ``LlamaMLP``: parameters alias the block's weight buffers, gradients come
     from the block's own backward kernels.  Call ``block.sync_transposes()`` (or ``after_step()``) after
-    every optimiser step."""
+    every optimiser step.
 
-    def __init__(self, rt, hidden: int = 8192, ffn: int = 28672, max_tokens: int = 8192):
+    ``norms``: the whole residual block, x + scale * norm(MLP(norm(x))), with weights ``pre`` and ``post`` and a learned
+    ``scale``; the norms are of this rank's rows, so with several ranks their gradients are to be added up over them.
+    ``checkpoint``: every forward keeps what its backward needs in 8 bits instead of the block's buffers, so that several may come before
+    their backwards (micro-batches)."""
+
+    def __init__(self, rt, hidden: int = 8192, ffn: int = 28672, max_tokens: int = 8192, *, norms: bool = False, checkpoint: bool = False,
+                 eps: float = 1e-6):
         super().__init__()
         self.block = LlamaMLP(rt, hidden, ffn, max_tokens, training=True)
         self.w13 = torch.nn.Parameter(self.block.w13)
         self.w2 = torch.nn.Parameter(self.block.w2)
+        self.norms, self.checkpoint, self.eps = norms, checkpoint, eps
+        if norms:
+            self.pre = torch.nn.Parameter(torch.ones((hidden,), dtype=torch.bfloat16, device=rt.device))
+            self.post = torch.nn.Parameter(torch.ones((hidden,), dtype=torch.bfloat16, device=rt.device))
+            self.scale = torch.nn.Parameter(torch.ones((1,), dtype=torch.float32, device=rt.device))
 
     def forward(self, x_shard: torch.Tensor) -> torch.Tensor:
-        return _LlamaMLPFn.apply(x_shard, self.w13, self.w2, self.block)
+        if not self.norms:
+            return _LlamaMLPFn.apply(x_shard, self.w13, self.w2, self.block, self.checkpoint)
+        h = rms_norm(x_shard, self.pre, self.eps, checkpoint=self.checkpoint)
+        y = _LlamaMLPFn.apply(h, self.w13, self.w2, self.block, self.checkpoint)
+        return post_norm(y, x_shard, self.post, scale=self.scale, eps=self.eps, checkpoint=self.checkpoint)
 
     def after_step(self) -> None:
         self.block.sync_transposes()

@@ -1,0 +1,173 @@
+"""Norms, 8-bit activations and 4-bit weights together, as a block's training and serving use them."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+@pytest.fixture
+def rt():
+    import roc_shmem_b200 as shmem
+    r = shmem.init("device", rank=0, world_size=1, heap_bytes=256 << 20)
+    yield r
+    shmem.finalize()
+
+
+def _rand(*shape, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, device="cuda", generator=g) * scale).to(BF)
+
+
+def _reference(x, pre, post, scale, wg, wu, wd, eps):
+    n = lambda v: v / (v.pow(2).mean(-1, keepdim=True) + eps).sqrt()  # noqa: E731
+    h = n(x) * pre
+    y = (torch.nn.functional.silu(h @ wg.t()) * (h @ wu.t())) @ wd.t()
+    return x + scale * n(y) * post
+
+
+def _near(got, ref, limit):
+    assert (got.double() - ref).norm() <= limit * ref.norm(), float((got.double() - ref).norm() / ref.norm())
+
+
+@pytest.mark.parametrize("M,F", [(512, 768), (2560, 1024)])
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_residual_block_trains(rt, M, F, checkpoint):
+    """Relative errors in the 2-norm.  A rounding to bf16 is within 2^-8 and uniform in its step, so below 2^-8 / sqrt(3) in the norm; a pass
+    goes through about ten: under 2^-8 * 6.  One to 8 bits is within 2^-4, below 2^-4 / sqrt(3) = 0.036 in the norm; of what a gradient
+    is made of, at most the norm's input, the norm's output and the pre-activations (which count twice, as factor and derivative) are kept
+    so: under 0.036 * 4.  The scale's gradient is one sum of M * H terms of either sign, so it may be far smaller than they: with errors of
+    the terms that are independent and below the limit in the norm, the sum is off by a normal number whose deviation is below the
+    limit times the terms' 2-norm; four of those are exceeded once in 16000."""
+    from roc_shmem_b200.models.llama import LlamaMLPModule
+    from roc_shmem_b200.ops.moe import interleave_gate_up
+    H = 512
+    mod = LlamaMLPModule(rt, H, F, M, norms=True, checkpoint=checkpoint)
+    wg, wu, wd = _rand(F, H, seed=1, scale=0.05), _rand(F, H, seed=2, scale=0.05), _rand(H, F, seed=3, scale=0.05)
+    mod.block.load(wg, wu, wd)
+    with torch.no_grad():
+        mod.pre.copy_(1 + _rand(H, seed=4, scale=0.1))
+        mod.post.copy_(1 + _rand(H, seed=5, scale=0.1))
+        mod.scale.fill_(0.7)
+    x, dy = _rand(M, H, seed=6), _rand(M, H, seed=7)
+    other = _rand(M, H, seed=8)
+    leaf = x.clone().requires_grad_(True)
+    out = mod(leaf)
+    if checkpoint:
+        mod(other)                                            # another forward before the first one's backward
+    params = (leaf, mod.pre, mod.post, mod.scale, mod.w13, mod.w2)
+    got = torch.autograd.grad(out, params, dy)
+    mod.block.check()
+    ref = [t.detach().double().requires_grad_(True) for t in (x, mod.pre, mod.post, mod.scale, wg, wu, wd)]
+    r = _reference(*ref, mod.eps)
+    grads = torch.autograd.grad(r, ref, dy.double())
+    expect = [*grads[:4], interleave_gate_up(grads[4], grads[5]), grads[6]]
+    _near(out, r.detach(), 2.0 ** -8 * 6)
+    limit = 2.0 ** -8 * 6 + (0.036 * 4 if checkpoint else 0)
+    for g, e in zip(got[:3] + got[4:], expect[:3] + expect[4:]):
+        _near(g, e, limit)
+    terms = dy.double() * (r.detach() - x.double()) / 0.7
+    assert (terms.sum() - expect[3]).abs() <= 1e-6 * terms.norm() and (got[3].double() - expect[3]).abs() <= 4 * limit * terms.norm()
+
+
+def test_checkpointed_block_equals_its_own_recomputation(rt):
+    """The backward from 8 bits is the unfused backward at exactly the kept values."""
+    from roc_shmem_b200.models.llama import LlamaMLP
+    M, H, F = 512, 512, 768
+    block = LlamaMLP(rt, H, F, M)
+    block.load(_rand(F, H, seed=1, scale=0.05), _rand(F, H, seed=2, scale=0.05), _rand(H, F, seed=3, scale=0.05))
+    x, dy = _rand(M, H, seed=6), _rand(M, H, seed=7)
+    block.forward(x)
+    kept = block.keep()
+    assert kept[0].nbytes + kept[1].nbytes < 0.52 * 2 * M * (H + 2 * F)
+    block.forward(_rand(M, H, seed=9))
+    dx, dw13, dw2 = block.backward(dy, kept).clone(), block.dw13.clone(), block.dw2.clone()
+    block.check()
+    xk, gu = kept[0].restore().double(), kept[1].restore().double().unflatten(1, (-1, 2, 32))
+    g, u = gu[:, :, 0].flatten(1), gu[:, :, 1].flatten(1)
+    dh = dy.double() @ block.w2.double()
+    s = torch.sigmoid(g)
+    dgu = torch.stack(((dh * u * s * (1 + g * (1 - s))).unflatten(1, (-1, 32)), (dh * g * s).unflatten(1, (-1, 32))), dim=2).flatten(1)
+    for got, ref in ((dw2, dy.double().t() @ (g * s * u)), (dw13, dgu.t() @ xk), (dx, dgu @ block.w13.double())):
+        _near(got, ref, 2.0 ** -8 * 3)                        # dh, dgu or the activations, and the result are rounded to bf16
+
+
+@pytest.mark.parametrize("rows", [8, 1000])
+def test_linear_with_kept_input(rows):
+    from roc_shmem_b200.ops.checkpoint8 import restore, store
+    from roc_shmem_b200.ops.torch_ops import Linear
+    plain, kept = Linear(512, 264, device="cuda"), Linear(512, 264, device="cuda", checkpoint=True)
+    kept.load_state_dict(plain.state_dict())
+    x, dy = _rand(rows, 512, seed=1), _rand(rows, 264, seed=2)
+    grads = []
+    for layer in (plain, kept):
+        leaf = x.clone().requires_grad_(True)
+        y = layer(leaf)
+        grads.append((y, *torch.autograd.grad(y, (leaf, layer.weight), dy)))
+    assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
+    assert torch.equal(grads[1][2], torch.ops.bshmem.linear_wgrad(dy, restore(store(x))))
+    leaf = x.view(2, -1, 512).clone().requires_grad_(True)   # a frozen weight, more dimensions
+    kept.weight.requires_grad_(False)
+    g, = torch.autograd.grad(kept(leaf), leaf, dy.view(2, -1, 264))
+    assert torch.equal(g.view(rows, 512), grads[0][1])
+    with torch.no_grad():
+        assert torch.equal(kept(x), plain(x))
+
+
+def test_decode_step_in_a_graph():
+    """norm, gate + up in 4 bits, SwiGLU, down in 4 bits, norm with residual and the next block's norm: captured once, replayed on new tokens."""
+    from roc_shmem_b200.ops.checkpoint8 import swiglu
+    from roc_shmem_b200.ops.gemm_w4 import linear_w4, quantize_w4, w4_error_site
+    from roc_shmem_b200.ops.moe import interleave_gate_up
+    from roc_shmem_b200.ops.norms import post_pre_norm, rms_norm
+    H, F, T = 1024, 2048, 5
+    wg, wu, wd = _rand(F, H, seed=1, scale=0.03), _rand(F, H, seed=2, scale=0.03), _rand(H, F, seed=3, scale=0.03)
+    up, down = quantize_w4(interleave_gate_up(wg, wu), 64, zeros=True), quantize_w4(wd, 128)
+    w = [1 + _rand(H, seed=s, scale=0.1) for s in (4, 5, 6)]
+    x = _rand(T, H, seed=7)
+
+    def step():
+        h = rms_norm(x, w[0])
+        y = linear_w4(swiglu(linear_w4(h, up)), down)
+        return post_pre_norm(y, x, w[1], w[2], scale=0.5)
+    with torch.no_grad():
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, h = step()
+        for seed in (8, 9):
+            x.copy_(_rand(T, H, seed=seed))
+            graph.replay()
+            eager = step()
+            assert torch.equal(out, eager[0]) and torch.equal(h, eager[1])
+    assert w4_error_site() == 0
+    g = up.dequantize().double().unflatten(0, (-1, 2, 32))
+    wg, wu = g[:, 0].flatten(0, 1), g[:, 1].flatten(0, 1)
+    ref = _reference(x.double(), w[0].double(), w[1].double(), 0.5, wg, wu, down.dequantize().double(), 1e-6)
+    _near(out, ref, 2.0 ** -8 * 6)
+    _near(h, ref / (ref.pow(2).mean(-1, keepdim=True) + 1e-6).sqrt() * w[2].double(), 2.0 ** -8 * 7)
+
+
+def test_modules():
+    from roc_shmem_b200.ops.norms import RMSNorm, rms_norm
+    norm = RMSNorm(264, device="cuda", checkpoint=True)
+    x = _rand(7, 264, seed=1)
+    assert torch.equal(norm(x), rms_norm(x, norm.weight))
+    norm(x.requires_grad_(True)).float().sum().backward()
+    assert norm.weight.grad.shape == (264,) and x.grad.shape == x.shape
+
+
+def test_long_offsets():
+    """Rows whose bytes lie beyond 2^32 of the tensor's beginning."""
+    from roc_shmem_b200.ops.checkpoint8 import restore, store
+    from roc_shmem_b200.ops.norms import rms_norm
+    rows, n = 140000, 16384                                   # 4.6 GB
+    x = torch.zeros(rows, n, dtype=BF, device="cuda")
+    last = _rand(3, n, seed=1)
+    x[-3:] = last
+    w = 1 + _rand(n, seed=2, scale=0.1)
+    h = rms_norm(x, w)
+    assert torch.equal(h[-3:], rms_norm(last, w)) and not h[:-3].any()
+    del h
+    assert torch.equal(restore(store(x))[-3:], restore(store(last)))
