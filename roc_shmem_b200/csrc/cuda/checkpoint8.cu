@@ -138,13 +138,15 @@ extern "C" {
 
 const char* bshmem_ckpt8_last_error() { return host::last_error().c_str(); }
 
-// x: [rows, n] of type 0 bf16, 1 fp16, 2 fp32 with row pitch ldx -> q [rows][n rounded up to 16], e [rows][blocks of 128 columns].
-// Bytes of q behind the last eight columns are not written.
-int bshmem_ckpt8_store(int type, const void* x, long long ldx, void* q, void* e, long long rows, int n, void* stream) {
+// x: [rows, n] of type 0 bf16, 1 fp16, 2 fp32 with row pitch ldx -> kept: q [rows][n rounded up to 16], then e [rows][blocks of 128
+// columns].  Bytes of q behind the last eight columns are not written.
+int bshmem_ckpt8_store(int type, const void* x, long long ldx, void* kept, long long rows, int n, void* stream) {
   if (type < 0 || type > 2 || n < 1) { host::last_error() = "checkpoint: unknown type or no columns"; return 1; }
   if (rows <= 0) return 0;
   const long long blocks = ((long long)n + 127) / 128;
-  const StoreParams p = {x, ldx, static_cast<uint8_t*>(q), static_cast<uint8_t*>(e), ((long long)n + 15) / 16 * 16, blocks, rows, n, blocks * 16};
+  const long long ldq = ((long long)n + 15) / 16 * 16;
+  uint8_t* const q = static_cast<uint8_t*>(kept);
+  const StoreParams p = {x, ldx, q, q + rows * ldq, ldq, blocks, rows, n, blocks * 16};
   const bool vec = n % 8 == 0 && aligned(x) && ldx * (type == 2 ? 4 : 2) % 16 == 0;
   const long long threads = rows * p.eights;
   if (type == 0) return vec ? launch(store8_kernel<__nv_bfloat16, kVector>, threads, p, stream) : launch(store8_kernel<__nv_bfloat16, kSingle>, threads, p, stream);
@@ -153,11 +155,12 @@ int bshmem_ckpt8_store(int type, const void* x, long long ldx, void* q, void* e,
 }
 
 // The way back; x has row pitch ldx.
-int bshmem_ckpt8_restore(int type, const void* q, const void* e, void* x, long long ldx, long long rows, int n, void* stream) {
+int bshmem_ckpt8_restore(int type, const void* kept, void* x, long long ldx, long long rows, int n, void* stream) {
   if (type < 0 || type > 2 || n < 1) { host::last_error() = "checkpoint: unknown type or no columns"; return 1; }
   if (rows <= 0) return 0;
-  const RestoreParams p = {static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(e), ((long long)n + 15) / 16 * 16, ((long long)n + 127) / 128,
-                           x, ldx, rows, n, ((long long)n + 7) / 8};
+  const long long ldq = ((long long)n + 15) / 16 * 16;
+  const uint8_t* const q = static_cast<const uint8_t*>(kept);
+  const RestoreParams p = {q, q + rows * ldq, ldq, ((long long)n + 127) / 128, x, ldx, rows, n, ((long long)n + 7) / 8};
   const bool vec = n % 8 == 0 && aligned(x) && ldx * (type == 2 ? 4 : 2) % 16 == 0;
   const long long threads = rows * p.eights;
   if (type == 0) return vec ? launch(restore8_kernel<__nv_bfloat16, kVector>, threads, p, stream) : launch(restore8_kernel<__nv_bfloat16, kSingle>, threads, p, stream);
@@ -166,23 +169,23 @@ int bshmem_ckpt8_restore(int type, const void* q, const void* e, void* x, long l
 }
 
 // gu [rows, 2F] bf16 -> act [rows, F] and gu in 8 bits.  Everything contiguous and 16-byte aligned, F % 32 == 0.
-int bshmem_ckpt8_swiglu_store(const void* gu, void* act, void* q, void* e, long long rows, int F, void* stream) {
+int bshmem_ckpt8_swiglu_store(const void* gu, void* act, void* kept, long long rows, int F, void* stream) {
   if (F < 32 || F % 32 || F > 1 << 29 || !aligned(gu) || !aligned(act)) { host::last_error() = "checkpoint: swiglu needs F % 32 == 0 and 16-byte aligned rows"; return 1; }
   if (rows <= 0) return 0;
   SwigluParams p = {};
   p.gu = static_cast<const __nv_bfloat16*>(gu);
   p.act = static_cast<__nv_bfloat16*>(act);
-  p.q = static_cast<uint8_t*>(q); p.e = static_cast<uint8_t*>(e);
+  p.q = static_cast<uint8_t*>(kept); p.e = p.q + rows * 2 * F;
   p.lde = (2LL * F + 127) / 128; p.rows = rows; p.F = F; p.eights = p.lde * 16;
   return launch(swiglu_store8_kernel, rows * p.eights, p, stream);
 }
 
 // dgu [rows, 2F] from gu in 8 bits and dact [rows, F]; act (may be null): the activation again, of the same 8 bits.
-int bshmem_ckpt8_swiglu_backward(const void* q, const void* e, const void* dact, void* dgu, void* act, long long rows, int F, void* stream) {
+int bshmem_ckpt8_swiglu_backward(const void* kept, const void* dact, void* dgu, void* act, long long rows, int F, void* stream) {
   if (F < 32 || F % 32 || F > 1 << 29 || !aligned(dact) || !aligned(dgu) || !aligned(act)) { host::last_error() = "checkpoint: swiglu needs F % 32 == 0 and 16-byte aligned rows"; return 1; }
   if (rows <= 0) return 0;
   SwigluParams p = {};
-  p.q = static_cast<uint8_t*>(const_cast<void*>(q)); p.e = static_cast<uint8_t*>(const_cast<void*>(e));
+  p.q = static_cast<uint8_t*>(const_cast<void*>(kept)); p.e = p.q + rows * 2 * F;
   p.dact = static_cast<const __nv_bfloat16*>(dact);
   p.dgu = static_cast<__nv_bfloat16*>(dgu);
   p.act = static_cast<__nv_bfloat16*>(act);

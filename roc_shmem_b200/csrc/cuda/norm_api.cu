@@ -92,7 +92,7 @@ bool aligned(const Mat& m, int size) { return aligned(m.p) && (m.ld * size) % 16
 int groups_of(long long rows, int n, int* groups) {
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  const Shape s = backward_shape(rows, n, false, sms, [](int) { return 1; }, [](int) { return 0; });
+  const Shape s = backward_shape(rows, n, false, sms, [](int) { return 1; }, [](int) { return 0; }, false);
   *groups = s.blocks * s.rows;
   return 0;
 }
@@ -134,11 +134,11 @@ static int refuse_size() {
   return 1;
 }
 
-// out and h are contiguous; rstd: [rows], in kPostPre [2][rows] (y's, then out's), or null.  q, e: [kept norms][rows][n rounded up
-// to 16] and [kept norms][rows][blocks of 128 columns], in the same order.  numbers: the bits of eps, and of a scale that is not
+// out and h are contiguous; rstd: [rows], in kPostPre [2][rows] (y's, then out's), or null.  kept: q [norms][rows][n rounded up to 16],
+// then e [norms][rows][blocks of 128 columns], in the same order.  numbers: the bits of eps, and of a scale that is not
 // in memory above them.
 int bshmem_norm_fwd(int what, const void* y, long long ldy, const void* x, long long ldx, void* out, void* h, const void* w1,
-                    const void* w2, const void* gate, long long ldg, const void* scale, uint64_t numbers, void* rstd, void* q, void* e,
+                    const void* w2, const void* gate, long long ldg, const void* scale, uint64_t numbers, void* rstd, void* kept,
                     long long rows, int n, void* stream) {
   const Call c(what);
   if (!c.known() || n < 1 || n > kMaxColumns || rows > 0x7fffffffLL) return refuse_size();
@@ -165,7 +165,7 @@ int bshmem_norm_fwd(int what, const void* y, long long ldy, const void* x, long 
   if (c.kept) {
     p.ldq = (n + 15) / 16 * 16;
     p.lde = (n + 127) / 128;
-    uint8_t *qb = static_cast<uint8_t*>(q), *eb = static_cast<uint8_t*>(e);
+    uint8_t *qb = static_cast<uint8_t*>(kept), *eb = qb + (c.mode == kPostPre ? 2 : 1) * rows * p.ldq;
     if (c.mode != kPre) { p.q1 = qb; p.e1 = eb; }
     if (c.mode != kPost) { p.q2 = qb + (c.mode == kPre ? 0 : rows * p.ldq); p.e2 = eb + (c.mode == kPre ? 0 : rows * p.lde); }
   }
@@ -193,8 +193,8 @@ static void split_work(void* work, int mode, long long groups, int n, float*& w2
 // The rows' part of a backward pass: dz (kPre, kPostPre), dy and the gradient of a gate per row or element.  Everything but z, y
 // and a gate per row is contiguous.  dout, dy and dgate may be null.
 int bshmem_norm_bwd(int what, const void* dout, const void* dh, const void* z, long long ldz, const void* y, long long ldy, const void* w1,
-                    const void* w2, const void* gate, long long ldg, const void* scale, uint64_t scale_bits, const void* rstd, const void* q,
-                    const void* e, void* dz, void* dy, void* dgate, void* work, long long rows, int n, void* stream) {
+                    const void* w2, const void* gate, long long ldg, const void* scale, uint64_t scale_bits, const void* rstd, const void* kept,
+                    int norms_kept, void* dz, void* dy, void* dgate, void* work, long long rows, int n, void* stream) {
   const Call c(what);
   if (!c.known() || rows < 1 || n < 1 || n > kMaxColumns || rows > 0x7fffffffLL) return refuse_size();
   int groups = 0, sms = 0;
@@ -222,8 +222,8 @@ int bshmem_norm_bwd(int what, const void* dout, const void* dh, const void* z, l
   if (c.kept) {
     p.ldq = (n + 15) / 16 * 16;
     p.lde = (n + 127) / 128;
-    p.q1 = static_cast<const uint8_t*>(q);
-    p.e1 = static_cast<const uint8_t*>(e);
+    p.q1 = static_cast<const uint8_t*>(kept);
+    p.e1 = p.q1 + norms_kept * rows * p.ldq;
     p.q2 = p.q1 + (c.mode == kPostPre ? rows * p.ldq : 0);
     p.e2 = p.e1 + (c.mode == kPostPre ? rows * p.lde : 0);
   }
@@ -236,7 +236,7 @@ int bshmem_norm_bwd(int what, const void* dout, const void* dh, const void* z, l
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const Shape shape = backward_shape(rows, n, vec, sms, [&](int chunks) { return backward_words(c.size, c.mode, c.kept, c.gate, c.gate_f32, chunks); },
-                                     [&](int chunks) { return backward_held(c.mode, chunks); });
+                                     [&](int chunks) { return backward_held(c.mode, chunks); }, backward_raw(p, c.size));
   return c.type == 0 ? backward<__nv_bfloat16>(c.mode, c.kept, shape, p, s)
          : c.type == 1 ? backward<__half>(c.mode, c.kept, shape, p, s) : backward<float>(c.mode, c.kept, shape, p, s);
 }

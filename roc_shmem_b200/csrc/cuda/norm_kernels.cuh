@@ -57,7 +57,7 @@ struct BwdParams {
   int gate_kind;
   int w1_f32, w2_f32, gcol_f32, gate_f32, scale_f32;
   int stages, ring_words;
-  int held;                             // the weights are in shared memory
+  int held;                             // the weights are in shared memory: 1 in fp32, 2 as they are (see backward_raw)
 };
 
 template <typename T> __device__ __forceinline__ float number(const void* p, int f32, float otherwise) {
@@ -107,7 +107,7 @@ __device__ __forceinline__ float sum2(float2 v) { return v.x + v.y; }
 // A row stays in the registers of its threads, kChunks groups of eight columns for each, between the sums: memory is read once.
 // In a ring the weights (w1 times a gate per column, and w2) stay in registers too.
 template <typename T, int kMode, int kChunks, int kForm>
-__global__ void __launch_bounds__(kForm == kDirect && kChunks == 1 ? 1024 : 512) norm_fwd_kernel(const Params p) {
+__global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512) norm_fwd_kernel(const Params p) {
   constexpr int kAccess = kForm == kScalar ? kStrided : kVector;
   constexpr bool kHeld = kForm == kRing && kChunks <= 2;
   constexpr int W = Raw8<T>::kWords, kX = kMode == kPre ? 0 : kChunks * W, kGate = kX + kChunks * W;
@@ -365,13 +365,18 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
     }
     return w;
   };
+  auto keep = [&](int i, int from, const Vals& v) {
+    if (p.held == 1) hold(weights, from + i * 2, v);
+    else weights.mine[(from / 2 + i) * weights.threads] = pack<T>(v).get(0);
+  };
+  auto held = [&](int i, int from) { return p.held == 1 ? weights.get8<float>(0, from + i * 2) : weights.get8<T>(0, from / 2 + i); };
   if constexpr (kForm == kRing) {
     for (int i = 0; i < p.stages; ++i) fetch(first + threadIdx.y + i * step, i);
     if (p.held) {
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        if constexpr (kMode != kPre) hold(weights, i * 2, weight1(i, p.n));
-        if constexpr (kMode != kPost) hold(weights, kW2 + i * 2, vector8<kAccess, T>(p.w2, p.w2_f32, column(i), p.n));
+        if constexpr (kMode != kPre) keep(i, 0, weight1(i, p.n));
+        if constexpr (kMode != kPost) keep(i, kW2, vector8<kAccess, T>(p.w2, p.w2_f32, column(i), p.n));
       }
     }
   }
@@ -418,7 +423,7 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         Vals w;
-        if (kForm == kRing && p.held) w = weights.get8<float>(0, kW2 + i * 2);
+        if (kForm == kRing && p.held) w = held(i, kW2);
         else w = vector8<kAccess, T>(p.w2, p.w2_f32, column(i), n);
         Vals sums_w2;
         if constexpr (kLong) sums_w2 = accs.get8<float>(0, i * 2);
@@ -454,7 +459,7 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
         const int col = column(i);
         if constexpr (kMode == kPostPre && kForm == kRing) first_norm(i);
         Vals w;
-        if (kForm == kRing && p.held) w = weights.get8<float>(0, i * 2);
+        if (kForm == kRing && p.held) w = held(i, 0);
         else w = weight1(i, n);
         if (p.gate_kind == kElement) {
           Vals g;
@@ -579,7 +584,9 @@ template <typename F> Shape forward_shape(long long rows, int n, bool vec, int s
   };
   if (vec) {
     divide(eights > 1024 ? 4 : 2, 256);
-    const int per_sm = 512 / (s.threads * s.rows);    // 128 registers a thread
+    // 64 registers a thread, some of the weights spilled: with 86 and half as many threads 16384 x 4096 takes 110 us for 104, 12000 x 5120,
+    // of which then one block fits, 144
+    const int per_sm = (s.chunks == 2 ? 1024 : 512) / (s.threads * s.rows);
     const long long most = (long long)sms * per_sm;
     ring_of(s, words(s.chunks), 0, per_sm);
     if (s.stages >= 2 && rows > 2 * most * s.rows) {
@@ -594,7 +601,7 @@ template <typename F> Shape forward_shape(long long rows, int n, bool vec, int s
   s.blocks = (int)((rows + s.rows - 1) / s.rows);
   return s;
 }
-template <typename F, typename G> Shape backward_shape(long long rows, int n, bool vec, int sms, F words, G held) {
+template <typename F, typename G> Shape backward_shape(long long rows, int n, bool vec, int sms, F words, G held, bool raw) {
   const int eights = (n + 7) / 8;
   Shape s = {};
   s.chunks = eights > 32 ? 2 : 1;
@@ -611,6 +618,7 @@ template <typename F, typename G> Shape backward_shape(long long rows, int n, bo
     s.held = held(s.chunks);                          // as many words as the weights: the column sums
   } else if (vec) {
     ring_of(s, words(s.chunks), held(s.chunks), per_sm);
+    if (s.stages < 2 && raw) ring_of(s, words(s.chunks), held(s.chunks) / 2, per_sm);
     if (s.stages < 2) ring_of(s, words(s.chunks), 0, per_sm);
     if (s.stages >= 2 && need > most) s.form = kRing;
   }
@@ -639,6 +647,10 @@ inline int backward_words(int size, int mode, bool kept, int gate_kind, bool gat
   return chunks * ((mode == kPostPre ? 2 : 1) * (W + K) + (gate_kind != kElement ? 0 : gate_f32 ? 2 : W)) + 1;
 }
 inline int backward_held(int mode, int chunks) { return chunks * 2 * (mode == kPostPre ? 2 : 1); }
+// Whether half of that will do: 2-byte rows, weights of their type or none, no gate per column, which is multiplied into w1.
+inline bool backward_raw(const BwdParams& p, int size) {
+  return size == 2 && p.gate_kind != kColumn && !(p.w1 && p.w1_f32) && !(p.w2 && p.w2_f32);
+}
 template <typename T, int kMode, bool kKept> int backward_mode(const Shape& s, BwdParams p, cudaStream_t stream) {
   const dim3 grid((unsigned)s.blocks), block(s.threads, s.rows);
   if (s.threads > 512) {
@@ -648,7 +660,7 @@ template <typename T, int kMode, bool kKept> int backward_mode(const Shape& s, B
   if (s.form == kRing) {
     p.stages = s.stages;
     p.ring_words = s.words;
-    p.held = s.held != 0;
+    p.held = s.held == 0 ? 0 : s.held == backward_held(kMode, s.chunks) ? 1 : 2;
     const int shared = shared_of(s);
     if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kRing, kKept>, grid, block, shared, p, stream);
     return launch(norm_bwd_kernel<T, kMode, 2, kRing, kKept>, grid, block, shared, p, stream);

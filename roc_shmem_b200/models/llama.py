@@ -162,7 +162,7 @@ class _LlamaMLPFn(torch.autograd.Function):
         y = block.forward(x).clone()
         if checkpoint:
             kept = block.keep()
-            ctx.save_for_backward(*(t for c in kept for t in (c.q, c.e)))
+            ctx.save_for_backward(*(c.data for c in kept))
             ctx.shapes = [(c.shape, c.dtype) for c in kept]
         return y
 
@@ -170,8 +170,7 @@ class _LlamaMLPFn(torch.autograd.Function):
     def backward(ctx, dy):
         block, kept = ctx.block, None
         if ctx.shapes is not None:
-            t = ctx.saved_tensors
-            kept = Checkpoint8(t[0], t[1], *ctx.shapes[0]), Checkpoint8(t[2], t[3], *ctx.shapes[1])
+            kept = tuple(Checkpoint8(data, *shape) for data, shape in zip(ctx.saved_tensors, ctx.shapes))
         dx = block.backward(dy.contiguous(), kept)
         return dx.clone(), block.dw13.clone(), block.dw2.clone(), None, None
 

@@ -34,8 +34,8 @@ def _lib() -> C.CDLL:
     if not _declared:
         VP, I, L = C.c_void_p, C.c_int, C.c_longlong
         lib.bshmem_ckpt8_last_error.restype = C.c_char_p
-        for name, args in (("store", [I, VP, L, VP, VP, L, I, VP]), ("restore", [I, VP, VP, VP, L, L, I, VP]),
-                           ("swiglu_store", [VP, VP, VP, VP, L, I, VP]), ("swiglu_backward", [VP, VP, VP, VP, VP, L, I, VP])):
+        for name, args in (("store", [I, VP, L, VP, L, I, VP]), ("restore", [I, VP, VP, L, L, I, VP]),
+                           ("swiglu_store", [VP, VP, VP, L, I, VP]), ("swiglu_backward", [VP, VP, VP, VP, L, I, VP])):
             fn = getattr(lib, "bshmem_ckpt8_" + name)
             fn.restype, fn.argtypes = I, args
         _swiglu_store, _swiglu_backward = _native.fast(lib, "bshmem_ckpt8_swiglu_store"), _native.fast(lib, "bshmem_ckpt8_swiglu_backward")
@@ -54,21 +54,38 @@ def on_current_device(t: torch.Tensor) -> bool:
     return t.get_device() == torch._C._cuda_getDevice()
 
 
+def kept_bytes(rows: int, cols: int) -> int:
+    """Bytes of a [rows, cols] activation in 8 bits: its values, rows padded to 16 columns, then an exponent per row and 128 columns."""
+    return rows * ((cols + 15) // 16 * 16 + (cols + 127) // 128)
+
+
 @dataclass
 class Checkpoint8:
-    """``q`` [rows, columns rounded up to 16] e4m3 bytes, ``e`` [rows, blocks of 128 columns] biased exponents: the value of a byte
-    is e4m3 * 2^(e - 127).  ``shape`` and ``dtype`` are those of the tensor that was stored."""
-    q: torch.Tensor
-    e: torch.Tensor
+    """An activation in 8 bits.  ``data`` holds ``q`` [rows, columns rounded up to 16], e4m3 bytes, and behind it ``e`` [rows, blocks of 128
+    columns], biased exponents: the value of a byte is e4m3 * 2^(e - 127).  ``shape`` and ``dtype`` are those of the tensor that was stored."""
+    data: torch.Tensor
     shape: torch.Size
     dtype: torch.dtype
+
+    @property
+    def rows(self) -> int:
+        return self.data.numel() // kept_bytes(1, self.shape[-1])
+
+    @property
+    def q(self) -> torch.Tensor:
+        width = (self.shape[-1] + 15) // 16 * 16
+        return self.data[:self.rows * width].view(-1, width)
+
+    @property
+    def e(self) -> torch.Tensor:
+        return self.data[self.rows * ((self.shape[-1] + 15) // 16 * 16):].view(-1, (self.shape[-1] + 127) // 128)
 
     def restore(self, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         return restore(self, dtype, out)
 
     @property
     def nbytes(self) -> int:
-        return self.q.nbytes + self.e.nbytes
+        return self.data.nbytes
 
 
 def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
@@ -81,11 +98,6 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     return m if m.stride(1) == 1 else m.contiguous()
 
 
-def _empty_kept(rows: int, cols: int, device, norms: int = 1) -> tuple:
-    q = torch.empty((norms * rows, (cols + 15) // 16 * 16), dtype=torch.uint8, device=device)
-    return q, torch.empty((norms * rows, (cols + 127) // 128), dtype=torch.uint8, device=device)
-
-
 def store(x: torch.Tensor) -> Checkpoint8:
     """bf16, fp16 or fp32 [..., columns] → 8 bits."""
     m = _rows(x, "store")
@@ -95,31 +107,35 @@ def store(x: torch.Tensor) -> Checkpoint8:
     if _store is None:
         _lib()
     rows, cols = m.shape
-    q, e = _empty_kept(rows, cols, x.device)
-    _check(_store(_TYPES[x.dtype], m.data_ptr(), m.stride(0), q.data_ptr(), e.data_ptr(), rows, cols, current_stream()), "store")
-    return Checkpoint8(q, e, x.shape, x.dtype)
+    data = x.new_empty((kept_bytes(rows, cols),), dtype=torch.uint8)
+    st = _store(_TYPES[x.dtype], m.data_ptr(), m.stride(0), data.data_ptr(), rows, cols, current_stream())
+    if st != 0:
+        _check(st, "store")
+    return Checkpoint8(data, x.shape, x.dtype)
 
 
 def restore(kept: Checkpoint8, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The stored values in `dtype` (default: what was stored), into `out` if given ([rows, columns] with columns side by side)."""
     dtype = dtype or (out.dtype if out is not None else kept.dtype)
+    data = kept.data
     if dtype not in _TYPES:
         raise ValueError(f"restore gives bf16, fp16 or fp32, not {dtype}")
-    if not on_current_device(kept.q):
-        with torch.cuda.device(kept.q.device):
+    if not on_current_device(data):
+        with torch.cuda.device(data.device):
             return restore(kept, dtype, out)
     if _restore is None:
         _lib()
-    cols = kept.shape[-1]
-    rows = kept.q.shape[0]
+    cols, rows = kept.shape[-1], kept.rows
     if out is None:
-        out = torch.empty(kept.shape, dtype=dtype, device=kept.q.device)
+        out = data.new_empty(kept.shape, dtype=dtype)
         ld = cols
     else:
-        if out.shape != (rows, cols) or out.dtype != dtype or out.device != kept.q.device or out.stride(1) != 1 or (rows > 1 and out.stride(0) < cols):
+        if out.shape != (rows, cols) or out.dtype != dtype or out.device != data.device or out.stride(1) != 1 or (rows > 1 and out.stride(0) < cols):
             raise ValueError("bad output tensor")
         ld = out.stride(0)
-    _check(_restore(_TYPES[dtype], kept.q.data_ptr(), kept.e.data_ptr(), out.data_ptr(), ld, rows, cols, current_stream()), "restore")
+    st = _restore(_TYPES[dtype], data.data_ptr(), out.data_ptr(), ld, rows, cols, current_stream())
+    if st != 0:
+        _check(st, "restore")
     return out
 
 
@@ -145,36 +161,41 @@ def swiglu_store(gu: torch.Tensor) -> tuple[torch.Tensor, Checkpoint8]:
     g = _aligned(gu)
     F = gu.shape[-1] // 2
     rows = gu.numel() // (2 * F)
-    act = torch.empty((*gu.shape[:-1], F), dtype=torch.bfloat16, device=gu.device)
-    q, e = _empty_kept(rows, 2 * F, gu.device)
-    _check(_swiglu_store(g.data_ptr(), act.data_ptr(), q.data_ptr(), e.data_ptr(), rows, F, current_stream()), "swiglu_store")
-    return act, Checkpoint8(q, e, gu.shape, gu.dtype)
+    act = gu.new_empty((*gu.shape[:-1], F))
+    data = gu.new_empty((kept_bytes(rows, 2 * F),), dtype=torch.uint8)
+    st = _swiglu_store(g.data_ptr(), act.data_ptr(), data.data_ptr(), rows, F, current_stream())
+    if st != 0:
+        _check(st, "swiglu_store")
+    return act, Checkpoint8(data, gu.shape, gu.dtype)
 
 
 def swiglu_backward(kept: Checkpoint8, dact: torch.Tensor, *, act: bool = False, dgu_out: Optional[torch.Tensor] = None,
                     act_out: Optional[torch.Tensor] = None):
     """Gradient of gu from its 8 bits and the activation's gradient; with `act` also the activation again, of the same 8 bits (what
     the next layer's weight gradient reads).  `dgu_out`, `act_out`: contiguous buffers for them."""
-    if not on_current_device(kept.q):
-        with torch.cuda.device(kept.q.device):
+    data, shape = kept.data, kept.shape
+    if not on_current_device(data):
+        with torch.cuda.device(data.device):
             return swiglu_backward(kept, dact, act=act, dgu_out=dgu_out, act_out=act_out)
-    F = kept.shape[-1] // 2
-    if kept.shape[-1] % 64 or dact.dtype is not torch.bfloat16 or dact.shape != (*kept.shape[:-1], F) or dact.device != kept.q.device:
-        raise ValueError(f"swiglu_backward: a bf16 gradient of {(*kept.shape[:-1], F)} belongs to this checkpoint, got {dact.dtype} {tuple(dact.shape)}")
+    F = shape[-1] // 2
+    bf = torch.bfloat16
+    if shape[-1] % 64 or dact.dtype is not bf or dact.shape != (*shape[:-1], F) or dact.get_device() != data.get_device():
+        raise ValueError(f"swiglu_backward: a bf16 gradient of {(*shape[:-1], F)} belongs to this checkpoint, got {dact.dtype} {tuple(dact.shape)}")
     if _swiglu_backward is None:
         _lib()
     d = _aligned(dact)
-    rows = kept.q.shape[0]
-    bf = torch.bfloat16
-    dgu = torch.empty(kept.shape, dtype=bf, device=d.device) if dgu_out is None else dgu_out
-    again = None
-    if act or act_out is not None:
-        again = torch.empty(dact.shape, dtype=bf, device=d.device) if act_out is None else act_out
-    for t, shape in ((dgu, kept.shape), (again, dact.shape)):
-        if t is not None and (t.shape != shape or t.dtype is not bf or t.device != d.device or not t.is_contiguous() or t.data_ptr() % 16):
+
+    def buffer(given, like):
+        if given is None:
+            return d.new_empty(like)
+        if given.shape != like or given.dtype is not bf or given.device != d.device or not given.is_contiguous() or given.data_ptr() % 16:
             raise ValueError("bad output tensor")
-    _check(_swiglu_backward(kept.q.data_ptr(), kept.e.data_ptr(), d.data_ptr(), dgu.data_ptr(), 0 if again is None else again.data_ptr(), rows, F,
-                            current_stream()), "swiglu_backward")
+        return given
+    dgu = buffer(dgu_out, shape)
+    again = buffer(act_out, dact.shape) if act or act_out is not None else None
+    st = _swiglu_backward(data.data_ptr(), d.data_ptr(), dgu.data_ptr(), None if again is None else again.data_ptr(), kept.rows, F, current_stream())
+    if st != 0:
+        _check(st, "swiglu_backward")
     return dgu if again is None else (dgu, again)
 
 
@@ -182,15 +203,14 @@ class _SwigluFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gu):
         act, kept = swiglu_store(gu)
-        ctx.save_for_backward(kept.q, kept.e)
+        ctx.save_for_backward(kept.data)
         ctx.shape = gu.shape
         return act
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dact):
-        q, e = ctx.saved_tensors
-        return swiglu_backward(Checkpoint8(q, e, ctx.shape, torch.bfloat16), dact)
+        return swiglu_backward(Checkpoint8(*ctx.saved_tensors, ctx.shape, torch.bfloat16), dact)
 
 
 def swiglu(gu: torch.Tensor) -> torch.Tensor:

@@ -23,7 +23,7 @@ from typing import Optional, Union
 import torch
 
 from .. import _native
-from .checkpoint8 import _TYPES, _empty_kept, block_lib, on_current_device
+from .checkpoint8 import _TYPES, block_lib, kept_bytes, on_current_device
 from .gemm import current_stream
 
 PRE, POST, POST_PRE = range(3)
@@ -42,9 +42,9 @@ def _lib() -> C.CDLL:
         VP, I, L, U = C.c_void_p, C.c_int, C.c_longlong, C.c_uint64
         lib.bshmem_norm_last_error.restype = C.c_char_p
         lib.bshmem_norm_fwd.restype = I
-        lib.bshmem_norm_fwd.argtypes = [I, VP, L, VP, L, VP, VP, VP, VP, VP, L, VP, U, VP, VP, VP, L, I, VP]
+        lib.bshmem_norm_fwd.argtypes = [I, VP, L, VP, L, VP, VP, VP, VP, VP, L, VP, U, VP, VP, L, I, VP]
         lib.bshmem_norm_bwd.restype = I
-        lib.bshmem_norm_bwd.argtypes = [I, VP, VP, VP, L, VP, L, VP, VP, VP, L, VP, U, VP, VP, VP, VP, VP, VP, VP, L, I, VP]
+        lib.bshmem_norm_bwd.argtypes = [I, VP, VP, VP, L, VP, L, VP, VP, VP, L, VP, U, VP, VP, I, VP, VP, VP, VP, L, I, VP]
         lib.bshmem_norm_bwd_finish.restype = I
         lib.bshmem_norm_bwd_finish.argtypes = [I, VP, VP, VP, VP, U, VP, VP, VP, VP, L, I, VP]
         lib.bshmem_norm_bwd_groups.restype = I
@@ -146,27 +146,27 @@ class _Call:
 
 
 def _forward(c: _Call, mode: int, train: bool):
-    """(out, h, rstd, q, e); what the call does not give is None."""
+    """(out, h, rstd, kept); what the call does not give is None."""
     if _fwd is None:
         _lib()
     rows, n, like, what = c.rows, c.n, c.like, c.what
     out = _new_like(like, memory_format=_CONTIGUOUS) if mode != PRE else None
     h = _new_like(like, memory_format=_CONTIGUOUS) if mode != POST else None
-    rstd = q = e = None
+    rstd = kept = None
     if train:
         norms = 2 if mode == POST_PRE else 1
         rstd = torch.empty((norms, rows), dtype=_F32, device=like.device)
         if what & KEPT:
-            q, e = _empty_kept(rows, n, like.device, norms)
+            kept = like.new_empty((norms * kept_bytes(rows, n),), dtype=torch.uint8)
     else:
         what &= ~KEPT
     y, x = c.y, c.x
     st = _fwd(what, None if y is None else y.data_ptr(), 0 if y is None else y.stride(0), x.data_ptr(), x.stride(0),
               None if out is None else out.data_ptr(), None if h is None else h.data_ptr(), _p(c.w1), _p(c.w2), _p(c.gate), c.gate_ld, _p(c.scale),
-              _numbers(c.eps, c.number), _p(rstd), _p(q), _p(e), rows, n, current_stream())
+              _numbers(c.eps, c.number), _p(rstd), _p(kept), rows, n, current_stream())
     if st != 0:
         _check(st, "norm")
-    return out, h, rstd, q, e
+    return out, h, rstd, kept
 
 
 def _backward(ctx, *grads):
@@ -219,7 +219,7 @@ def _backward(ctx, *grads):
     stream = current_stream()
     if mode != POST or dy is not None or sums or dgate is not None:
         st = _bwd(what, _p(dout), _p(dh), _p(z), 0 if z is None else z.stride(0), _p(y), 0 if y is None else y.stride(0), _p(w1), _p(w2),
-                  _p(gate_m), gate_ld, _p(scale), number, rstd.data_ptr(), _p(a) if kept8 else None, _p(b) if kept8 else None,
+                  _p(gate_m), gate_ld, _p(scale), number, rstd.data_ptr(), _p(a) if kept8 else None, 2 if ctx.call[0] == POST_PRE else 1,
                   _p(dz) if mode != POST else None, _p(dy), None if column else _p(dgate), _p(work), rows, n, stream)
         if st != 0:
             _check(st, "norm backward")
@@ -242,10 +242,10 @@ class _NormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, x, w1, w2, gate, scale, c, mode):
         ctx.set_materialize_grads(False)
-        out, h, rstd, q, e = _forward(c, mode, True)
+        out, h, rstd, kept = _forward(c, mode, True)
         ctx.call = mode, c.what, c.n, c.rows, c.kind, _bits(c.number)
-        if q is not None:
-            ctx.save_for_backward(w1, w2, gate, scale, rstd, q, e)
+        if kept is not None:
+            ctx.save_for_backward(w1, w2, gate, scale, rstd, kept, None)
         else:
             ctx.save_for_backward(w1, w2, gate, scale, rstd, y, x if mode == PRE else None if mode == POST else out)
         return (out, h) if mode == POST_PRE else out if mode == POST else h
@@ -266,7 +266,7 @@ def _run(name, mode, y, x, w1, w2, gate, scale, eps, checkpoint):
             return _run(name, mode, y, x, w1, w2, gate, scale, eps, checkpoint)
     if torch.is_grad_enabled() and (x.requires_grad or _wants_grad(y) or _wants_grad(w2) or _wants_grad(w1) or _wants_grad(gate) or _wants_grad(c.scale)):
         return _NormFn.apply(y, x, w1, w2, gate, c.scale, c, mode)
-    out, h, _, _, _ = _forward(c, mode, False)
+    out, h, _, _ = _forward(c, mode, False)
     return (out, h) if mode == POST_PRE else out if mode == POST else h
 
 

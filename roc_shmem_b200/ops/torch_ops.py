@@ -119,7 +119,7 @@ class _LinearKeptFn(torch.autograd.Function):
     def forward(ctx, x, w):
         _check_linear(x, w)
         kept = store(x) if ctx.needs_input_grad[1] else None
-        ctx.save_for_backward(w, *(() if kept is None else (kept.q, kept.e)))
+        ctx.save_for_backward(w, *(() if kept is None else (kept.data,)))
         ctx.shape = x.shape
         return gemm_bf16(x.contiguous(), w.contiguous())
 

@@ -27,19 +27,19 @@ def test_native_entries_refuse_bad_sizes():
     """Sizes and types are looked at before CUDA is."""
     from roc_shmem_b200.ops import checkpoint8, gemm_w4, norms
     n, c, w = norms._lib(), checkpoint8._lib(), gemm_w4._lib()
-    assert n.bshmem_norm_fwd(3, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, 8, 0) == 1          # type
-    assert n.bshmem_norm_fwd(3 << 2, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, 8, 0) == 1     # mode
+    assert n.bshmem_norm_fwd(3, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, 8, 0) == 1          # type
+    assert n.bshmem_norm_fwd(3 << 2, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, 8, 0) == 1     # mode
     for rows, cols in ((1, 0), (1, 16385), (1 << 31, 8)):
-        assert n.bshmem_norm_fwd(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, rows, cols, 0) == 1
+        assert n.bshmem_norm_fwd(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, rows, cols, 0) == 1
         assert n.bshmem_norm_bwd(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, rows, cols, 0) == 1
     assert b"16384" in n.bshmem_norm_last_error()
-    assert n.bshmem_norm_fwd(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 8, 0) == 0           # no rows: nothing to do
+    assert n.bshmem_norm_fwd(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 8, 0) == 0           # no rows: nothing to do
     assert n.bshmem_norm_bwd_groups(0, 8) < 0 and n.bshmem_norm_bwd_groups(1, 16385) < 0
-    assert c.bshmem_ckpt8_store(3, 0, 8, 0, 0, 1, 8, 0) == 1 and c.bshmem_ckpt8_store(0, 0, 8, 0, 0, 1, 0, 0) == 1
-    assert c.bshmem_ckpt8_store(0, 0, 8, 0, 0, 0, 8, 0) == 0 and c.bshmem_ckpt8_restore(3, 0, 0, 0, 8, 1, 8, 0) == 1
+    assert c.bshmem_ckpt8_store(3, 0, 8, 0, 1, 8, 0) == 1 and c.bshmem_ckpt8_store(0, 0, 8, 0, 1, 0, 0) == 1
+    assert c.bshmem_ckpt8_store(0, 0, 8, 0, 0, 8, 0) == 0 and c.bshmem_ckpt8_restore(3, 0, 0, 8, 1, 8, 0) == 1
     for F in (0, 31, 48):
-        assert c.bshmem_ckpt8_swiglu_store(0, 0, 0, 0, 1, F, 0) == 1 and c.bshmem_ckpt8_swiglu_backward(0, 0, 0, 0, 0, 1, F, 0) == 1
-    assert c.bshmem_ckpt8_swiglu_store(8, 0, 0, 0, 1, 64, 0) == 1                                    # off a 16-byte boundary
+        assert c.bshmem_ckpt8_swiglu_store(0, 0, 0, 1, F, 0) == 1 and c.bshmem_ckpt8_swiglu_backward(0, 0, 0, 0, 1, F, 0) == 1
+    assert c.bshmem_ckpt8_swiglu_store(8, 0, 0, 1, 64, 0) == 1                                    # off a 16-byte boundary
     for N, K, group in ((0, 64, 32), (8, 48, 48), (8, 96, 64), (8, 192, 128), (8, 64, 0), (8, 1 << 25, 128)):
         assert w.bshmem_w4_few(0, K, 0, 0, 0, 0, 1, N, K, group, 0, 0) == 1
         assert w.bshmem_w4_widen(0, 0, 0, 0, N, K, group, 0) == 1 and w.bshmem_w4_quant(0, K, 0, 0, 0, N, K, group, 0) == 1
