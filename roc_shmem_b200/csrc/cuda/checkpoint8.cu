@@ -14,37 +14,71 @@ namespace {
 
 constexpr int kThreads = 256;
 
-struct StoreParams { const void* x; long long ldx; uint8_t* q; uint8_t* e; long long ldq, lde, rows; int n; long long eights; };
+// A thread has kPer eights of the matrix, a block's width apart, whose loads are all on their way before the first is used: one alone
+// leaves 32 KB of an SM on their way, and 16384 x 4096 there and back took 83 us.  Rows are padded to whole blocks of 128 columns (16
+// eights), so the eights of a block are neighbours in a warp.
+constexpr int kPer = 4;
+struct Eights { long long total; uint32_t per_row; };
+// Row and column of the i-th eight; a 64-bit division only where there are that many.
+__device__ __forceinline__ void place(const Eights& s, long long i, long long& row, int& col) {
+  uint32_t in;
+  if (s.total <= 0xffffffffLL) {
+    const uint32_t r = (uint32_t)i / s.per_row;
+    in = (uint32_t)i - r * s.per_row;
+    row = r;
+  } else {
+    row = i / s.per_row;
+    in = (uint32_t)(i - row * s.per_row);
+  }
+  col = (int)in * 8;
+}
 
-// Thread i of the grid has the i-th eight of its row; rows are padded to whole blocks of 128 columns (16 threads).
+struct StoreParams { const void* x; long long ldx; uint8_t* q; uint8_t* e; long long ldq, lde; int n; Eights size; };
+
 template <typename T, int kAccess> __global__ void __launch_bounds__(kThreads) store8_kernel(const StoreParams p) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-  const long long row = i / p.eights;
-  const int col = (int)(i - row * p.eights) * 8;
-  const int n = row < p.rows ? p.n : 0;
-  const Vals v = unpack(load8<kAccess>(static_cast<const T*>(p.x) + (n ? row * p.ldx : 0), col, n));
-  uint32_t e;
-  const uint2 q = encode8<T>(v, e);
-  if (col < n) {
-    *reinterpret_cast<uint2*>(p.q + row * p.ldq + col) = q;
-    if (col % 128 == 0) p.e[row * p.lde + col / 128] = (uint8_t)e;
+  const long long first = (long long)blockIdx.x * (kThreads * kPer) + threadIdx.x;
+  long long row[kPer];
+  int col[kPer], n[kPer];
+  Raw8<T> r[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const long long i = first + j * kThreads;
+    n[j] = i < p.size.total ? p.n : 0;
+    place(p.size, n[j] ? i : 0, row[j], col[j]);
+    r[j] = load8<kAccess>(static_cast<const T*>(p.x) + row[j] * p.ldx, col[j], n[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    uint32_t e;
+    const uint2 q = encode8<T>(unpack(r[j]), e);
+    if (col[j] < n[j]) {
+      *reinterpret_cast<uint2*>(p.q + row[j] * p.ldq + col[j]) = q;
+      if (col[j] % 128 == 0) p.e[row[j] * p.lde + col[j] / 128] = (uint8_t)e;
+    }
   }
 }
 
-struct RestoreParams { const uint8_t *q, *e; long long ldq, lde; void* x; long long ldx, rows; int n; long long eights; };
+struct RestoreParams { const uint8_t *q, *e; long long ldq, lde; void* x; long long ldx; int n; Eights size; };
 
 template <typename T, int kAccess> __global__ void __launch_bounds__(kThreads) restore8_kernel(const RestoreParams p) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-  const long long row = i / p.eights;
-  if (row >= p.rows) return;
-  const int col = (int)(i - row * p.eights) * 8;
-  if (col >= p.n) return;
-  const Vals v = decode8(__ldg(reinterpret_cast<const uint2*>(p.q + row * p.ldq + col)), __ldg(p.e + row * p.lde + col / 128));
-  store8<kAccess>(static_cast<T*>(p.x) + row * p.ldx, col, p.n, pack<T>(v));
+  const long long first = (long long)blockIdx.x * (kThreads * kPer) + threadIdx.x;
+  long long row[kPer];
+  int col[kPer];
+  uint2 q[kPer];
+  uint32_t e[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    place(p.size, min(first + j * kThreads, p.size.total - 1), row[j], col[j]);
+    q[j] = __ldg(reinterpret_cast<const uint2*>(p.q + row[j] * p.ldq + col[j]));
+    e[j] = __ldg(p.e + row[j] * p.lde + col[j] / 128);
+  }
+#pragma unroll
+  for (int j = 0; j < kPer; ++j)
+    if (first + j * kThreads < p.size.total) store8<kAccess>(static_cast<T*>(p.x) + row[j] * p.ldx, col[j], p.n, pack<T>(decode8(q[j], e[j])));
 }
 
 // gu: [rows, 2F], 32 columns of the gate and the 32 of `up` that belong to them in turn.
@@ -52,70 +86,91 @@ struct SwigluParams {
   const __nv_bfloat16 *gu, *dact;
   __nv_bfloat16 *act, *dgu;
   uint8_t *q, *e;
-  long long lde, rows;
+  long long lde;
   int F;
-  long long eights;                                   // of a row of gu, in whole blocks of 128 columns
+  Eights size;                                        // forward: of gu, in whole blocks of 128 columns; backward: of the activation
 };
 
 __device__ __forceinline__ float2 sigmoid2(float2 x) { return make_float2(1.f / (1.f + __expf(-x.x)), 1.f / (1.f + __expf(-x.y))); }
 
-// Thread i has eight columns of gu; four threads in a row have a gate, the next four its `up`, which they swap.
+// Four threads in a row have a gate, the next four its `up`, which they swap.
 __global__ void __launch_bounds__(kThreads) swiglu_store8_kernel(const SwigluParams p) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-  const long long row = i / p.eights;
-  const int col = (int)(i - row * p.eights) * 8;
-  const int n = row < p.rows ? 2 * p.F : 0;
-  const Raw8<__nv_bfloat16> r = load8<kVector>(p.gu + (n ? row * n : 0), col, n);
-  const Vals v = unpack(r);
-  uint32_t e;
-  const uint2 q = encode8<__nv_bfloat16>(v, e);
-  const uint4 w = r.get(0);
-  Raw8<__nv_bfloat16> other;
-  other.set(0, make_uint4(__shfl_xor_sync(0xffffffffu, w.x, 4), __shfl_xor_sync(0xffffffffu, w.y, 4), __shfl_xor_sync(0xffffffffu, w.z, 4),
-                          __shfl_xor_sync(0xffffffffu, w.w, 4)));
-  if (col >= n) return;
-  *reinterpret_cast<uint2*>(p.q + row * n + col) = q;
-  if (col % 128 == 0) p.e[row * p.lde + col / 128] = (uint8_t)e;
-  if (col & 32) return;
-  Vals u = unpack(other);
+  const long long first = (long long)blockIdx.x * (kThreads * kPer) + threadIdx.x;
+  long long row[kPer];
+  int col[kPer], n[kPer];
+  Raw8<__nv_bfloat16> r[kPer];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) u.p[j] = mul2(u.p[j], mul2(v.p[j], sigmoid2(v.p[j])));
-  store8<kVector>(p.act + row * p.F, col / 64 * 32 + col % 32, p.F, pack<__nv_bfloat16>(u));
+  for (int j = 0; j < kPer; ++j) {
+    const long long i = first + j * kThreads;
+    n[j] = i < p.size.total ? 2 * p.F : 0;
+    place(p.size, n[j] ? i : 0, row[j], col[j]);
+    r[j] = load8<kVector>(p.gu + row[j] * 2 * p.F, col[j], n[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const Vals v = unpack(r[j]);
+    uint32_t e;
+    const uint2 q = encode8<__nv_bfloat16>(v, e);
+    const uint4 w = r[j].get(0);
+    Raw8<__nv_bfloat16> other;
+    other.set(0, make_uint4(__shfl_xor_sync(0xffffffffu, w.x, 4), __shfl_xor_sync(0xffffffffu, w.y, 4), __shfl_xor_sync(0xffffffffu, w.z, 4),
+                            __shfl_xor_sync(0xffffffffu, w.w, 4)));
+    if (col[j] >= n[j]) continue;
+    *reinterpret_cast<uint2*>(p.q + row[j] * 2 * p.F + col[j]) = q;
+    if (col[j] % 128 == 0) p.e[row[j] * p.lde + col[j] / 128] = (uint8_t)e;
+    if (col[j] & 32) continue;
+    Vals u = unpack(other);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u.p[k] = mul2(u.p[k], mul2(v.p[k], sigmoid2(v.p[k])));
+    store8<kVector>(p.act + row[j] * p.F, col[j] / 64 * 32 + col[j] % 32, p.F, pack<__nv_bfloat16>(u));
+  }
 }
 
-// Thread i has eight columns of the activation: their gate and `up` in 8 bits lie 32 columns apart in one block.
+// A thread has eights of the activation, whose gate and `up` lie 32 bytes apart in one block.
+constexpr int kPerBack = 2;
 template <bool kAct> __global__ void __launch_bounds__(kThreads) swiglu_backward8_kernel(const SwigluParams p) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-  const long long row = i / p.eights;
-  if (row >= p.rows) return;
-  const int col = (int)(i - row * p.eights) * 8;
-  if (col >= p.F) return;
-  const int at = col / 32 * 64 + col % 32;
-  const uint8_t* q = p.q + row * 2 * p.F + at;
-  const uint32_t e = __ldg(p.e + row * p.lde + at / 128);
-  const Vals g = decode8(__ldg(reinterpret_cast<const uint2*>(q)), e), u = decode8(__ldg(reinterpret_cast<const uint2*>(q + 32)), e);
-  const Vals d = unpack(load8<kVector>(p.dact + row * p.F, col, p.F));
-  Vals dg, du, again;
+  const long long first = (long long)blockIdx.x * (kThreads * kPerBack) + threadIdx.x;
+  long long row[kPerBack];
+  int col[kPerBack], at[kPerBack];
+  uint2 qg[kPerBack], qu[kPerBack];
+  uint32_t e[kPerBack];
+  Raw8<__nv_bfloat16> rd[kPerBack];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 s = sigmoid2(g.p[j]), silu = mul2(g.p[j], s);
-    du.p[j] = mul2(d.p[j], silu);
-    again.p[j] = mul2(u.p[j], silu);
-    // s (1 + g (1 - s)) = s + silu (1 - s)
-    dg.p[j] = mul2(mul2(d.p[j], u.p[j]), fma2(silu, make_float2(1.f - s.x, 1.f - s.y), s));
+  for (int j = 0; j < kPerBack; ++j) {
+    place(p.size, min(first + j * kThreads, p.size.total - 1), row[j], col[j]);
+    at[j] = col[j] / 32 * 64 + col[j] % 32;
+    const uint8_t* q = p.q + row[j] * 2 * p.F + at[j];
+    e[j] = __ldg(p.e + row[j] * p.lde + at[j] / 128);
+    qg[j] = __ldg(reinterpret_cast<const uint2*>(q));
+    qu[j] = __ldg(reinterpret_cast<const uint2*>(q + 32));
+    rd[j] = load8<kVector>(p.dact + row[j] * p.F, col[j], p.F);
   }
-  __nv_bfloat16* o = p.dgu + row * 2 * p.F + at;
-  store8<kVector>(o, 0, 8, pack<__nv_bfloat16>(dg));
-  store8<kVector>(o, 32, 40, pack<__nv_bfloat16>(du));
-  if constexpr (kAct) store8<kVector>(p.act + row * p.F, col, p.F, pack<__nv_bfloat16>(again));
+#pragma unroll
+  for (int j = 0; j < kPerBack; ++j) {
+    if (first + j * kThreads >= p.size.total) continue;
+    const Vals g = decode8(qg[j], e[j]), u = decode8(qu[j], e[j]), d = unpack(rd[j]);
+    Vals dg, du, again;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 s = sigmoid2(g.p[k]), silu = mul2(g.p[k], s);
+      du.p[k] = mul2(d.p[k], silu);
+      again.p[k] = mul2(u.p[k], silu);
+      // s (1 + g (1 - s)) = s + silu (1 - s)
+      dg.p[k] = mul2(mul2(d.p[k], u.p[k]), fma2(silu, make_float2(1.f - s.x, 1.f - s.y), s));
+    }
+    __nv_bfloat16* o = p.dgu + row[j] * 2 * p.F + at[j];
+    store8<kVector>(o, 0, 8, pack<__nv_bfloat16>(dg));
+    store8<kVector>(o, 32, 40, pack<__nv_bfloat16>(du));
+    if constexpr (kAct) store8<kVector>(p.act + row[j] * p.F, col[j], p.F, pack<__nv_bfloat16>(again));
+  }
 }
 
-template <typename K, typename P> int launch(K* kernel, long long threads, const P& p, void* stream) {
-  const long long blocks = (threads + kThreads - 1) / kThreads;
+template <typename K, typename P> int launch(K* kernel, int per, const P& p, void* stream) {
+  const long long blocks = (p.size.total + kThreads * per - 1) / (kThreads * per);
   if (blocks > 0x7fffffffLL) { host::last_error() = "checkpoint: too many elements for one call"; return 1; }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
@@ -146,12 +201,11 @@ int bshmem_ckpt8_store(int type, const void* x, long long ldx, void* kept, long 
   const long long blocks = ((long long)n + 127) / 128;
   const long long ldq = ((long long)n + 15) / 16 * 16;
   uint8_t* const q = static_cast<uint8_t*>(kept);
-  const StoreParams p = {x, ldx, q, q + rows * ldq, ldq, blocks, rows, n, blocks * 16};
+  const StoreParams p = {x, ldx, q, q + rows * ldq, ldq, blocks, n, {rows * blocks * 16, (uint32_t)(blocks * 16)}};
   const bool vec = n % 8 == 0 && aligned(x) && ldx * (type == 2 ? 4 : 2) % 16 == 0;
-  const long long threads = rows * p.eights;
-  if (type == 0) return vec ? launch(store8_kernel<__nv_bfloat16, kVector>, threads, p, stream) : launch(store8_kernel<__nv_bfloat16, kSingle>, threads, p, stream);
-  if (type == 1) return vec ? launch(store8_kernel<__half, kVector>, threads, p, stream) : launch(store8_kernel<__half, kSingle>, threads, p, stream);
-  return vec ? launch(store8_kernel<float, kVector>, threads, p, stream) : launch(store8_kernel<float, kSingle>, threads, p, stream);
+  if (type == 0) return vec ? launch(store8_kernel<__nv_bfloat16, kVector>, kPer, p, stream) : launch(store8_kernel<__nv_bfloat16, kSingle>, kPer, p, stream);
+  if (type == 1) return vec ? launch(store8_kernel<__half, kVector>, kPer, p, stream) : launch(store8_kernel<__half, kSingle>, kPer, p, stream);
+  return vec ? launch(store8_kernel<float, kVector>, kPer, p, stream) : launch(store8_kernel<float, kSingle>, kPer, p, stream);
 }
 
 // The way back; x has row pitch ldx.
@@ -160,12 +214,12 @@ int bshmem_ckpt8_restore(int type, const void* kept, void* x, long long ldx, lon
   if (rows <= 0) return 0;
   const long long ldq = ((long long)n + 15) / 16 * 16;
   const uint8_t* const q = static_cast<const uint8_t*>(kept);
-  const RestoreParams p = {q, q + rows * ldq, ldq, ((long long)n + 127) / 128, x, ldx, rows, n, ((long long)n + 7) / 8};
+  const RestoreParams p = {q, q + rows * ldq, ldq, ((long long)n + 127) / 128, x, ldx, n,
+                           {rows * (((long long)n + 7) / 8), (uint32_t)(((long long)n + 7) / 8)}};
   const bool vec = n % 8 == 0 && aligned(x) && ldx * (type == 2 ? 4 : 2) % 16 == 0;
-  const long long threads = rows * p.eights;
-  if (type == 0) return vec ? launch(restore8_kernel<__nv_bfloat16, kVector>, threads, p, stream) : launch(restore8_kernel<__nv_bfloat16, kSingle>, threads, p, stream);
-  if (type == 1) return vec ? launch(restore8_kernel<__half, kVector>, threads, p, stream) : launch(restore8_kernel<__half, kSingle>, threads, p, stream);
-  return vec ? launch(restore8_kernel<float, kVector>, threads, p, stream) : launch(restore8_kernel<float, kSingle>, threads, p, stream);
+  if (type == 0) return vec ? launch(restore8_kernel<__nv_bfloat16, kVector>, kPer, p, stream) : launch(restore8_kernel<__nv_bfloat16, kSingle>, kPer, p, stream);
+  if (type == 1) return vec ? launch(restore8_kernel<__half, kVector>, kPer, p, stream) : launch(restore8_kernel<__half, kSingle>, kPer, p, stream);
+  return vec ? launch(restore8_kernel<float, kVector>, kPer, p, stream) : launch(restore8_kernel<float, kSingle>, kPer, p, stream);
 }
 
 // gu [rows, 2F] bf16 -> act [rows, F] and gu in 8 bits.  Everything contiguous and 16-byte aligned, F % 32 == 0.
@@ -176,8 +230,9 @@ int bshmem_ckpt8_swiglu_store(const void* gu, void* act, void* kept, long long r
   p.gu = static_cast<const __nv_bfloat16*>(gu);
   p.act = static_cast<__nv_bfloat16*>(act);
   p.q = static_cast<uint8_t*>(kept); p.e = p.q + rows * 2 * F;
-  p.lde = (2LL * F + 127) / 128; p.rows = rows; p.F = F; p.eights = p.lde * 16;
-  return launch(swiglu_store8_kernel, rows * p.eights, p, stream);
+  p.lde = (2LL * F + 127) / 128; p.F = F;
+  p.size = {rows * p.lde * 16, (uint32_t)(p.lde * 16)};
+  return launch(swiglu_store8_kernel, kPer, p, stream);
 }
 
 // dgu [rows, 2F] from gu in 8 bits and dact [rows, F]; act (may be null): the activation again, of the same 8 bits.
@@ -189,8 +244,9 @@ int bshmem_ckpt8_swiglu_backward(const void* kept, const void* dact, void* dgu, 
   p.dact = static_cast<const __nv_bfloat16*>(dact);
   p.dgu = static_cast<__nv_bfloat16*>(dgu);
   p.act = static_cast<__nv_bfloat16*>(act);
-  p.lde = (2LL * F + 127) / 128; p.rows = rows; p.F = F; p.eights = F / 8;
-  return act ? launch(swiglu_backward8_kernel<true>, rows * p.eights, p, stream) : launch(swiglu_backward8_kernel<false>, rows * p.eights, p, stream);
+  p.lde = (2LL * F + 127) / 128; p.F = F;
+  p.size = {rows * (F / 8), (uint32_t)(F / 8)};
+  return act ? launch(swiglu_backward8_kernel<true>, kPerBack, p, stream) : launch(swiglu_backward8_kernel<false>, kPerBack, p, stream);
 }
 
 }  // extern "C"
