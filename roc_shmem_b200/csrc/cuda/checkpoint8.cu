@@ -93,8 +93,8 @@ struct SwigluParams {
 
 __device__ __forceinline__ float2 sigmoid2(float2 x) { return make_float2(1.f / (1.f + __expf(-x.x)), 1.f / (1.f + __expf(-x.y))); }
 
-// Four threads in a row have a gate, the next four its `up`, which they swap.
-__global__ void __launch_bounds__(kThreads) swiglu_store8_kernel(const SwigluParams p) {
+// Four threads in a row have a gate, the next four its `up`, which they swap.  Without kKeep only the activation is written.
+template <bool kKeep> __global__ void __launch_bounds__(kThreads) swiglu_store8_kernel(const SwigluParams p) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const long long first = (long long)blockIdx.x * (kThreads * kPer) + threadIdx.x;
@@ -112,14 +112,17 @@ __global__ void __launch_bounds__(kThreads) swiglu_store8_kernel(const SwigluPar
   for (int j = 0; j < kPer; ++j) {
     const Vals v = unpack(r[j]);
     uint32_t e;
-    const uint2 q = encode8<__nv_bfloat16>(v, e);
+    uint2 q;
+    if constexpr (kKeep) q = encode8<__nv_bfloat16>(v, e);
     const uint4 w = r[j].get(0);
     Raw8<__nv_bfloat16> other;
     other.set(0, make_uint4(__shfl_xor_sync(0xffffffffu, w.x, 4), __shfl_xor_sync(0xffffffffu, w.y, 4), __shfl_xor_sync(0xffffffffu, w.z, 4),
                             __shfl_xor_sync(0xffffffffu, w.w, 4)));
     if (col[j] >= n[j]) continue;
-    *reinterpret_cast<uint2*>(p.q + row[j] * 2 * p.F + col[j]) = q;
-    if (col[j] % 128 == 0) p.e[row[j] * p.lde + col[j] / 128] = (uint8_t)e;
+    if constexpr (kKeep) {
+      *reinterpret_cast<uint2*>(p.q + row[j] * 2 * p.F + col[j]) = q;
+      if (col[j] % 128 == 0) p.e[row[j] * p.lde + col[j] / 128] = (uint8_t)e;
+    }
     if (col[j] & 32) continue;
     Vals u = unpack(other);
 #pragma unroll
@@ -222,7 +225,7 @@ int bshmem_ckpt8_restore(int type, const void* kept, void* x, long long ldx, lon
   return vec ? launch(restore8_kernel<float, kVector>, kPer, p, stream) : launch(restore8_kernel<float, kSingle>, kPer, p, stream);
 }
 
-// gu [rows, 2F] bf16 -> act [rows, F] and gu in 8 bits.  Everything contiguous and 16-byte aligned, F % 32 == 0.
+// gu [rows, 2F] bf16 -> act [rows, F] and, unless kept is null, gu in 8 bits.  Everything contiguous and 16-byte aligned, F % 32 == 0.
 int bshmem_ckpt8_swiglu_store(const void* gu, void* act, void* kept, long long rows, int F, void* stream) {
   if (F < 32 || F % 32 || F > 1 << 29 || !aligned(gu) || !aligned(act)) { host::last_error() = "checkpoint: swiglu needs F % 32 == 0 and 16-byte aligned rows"; return 1; }
   if (rows <= 0) return 0;
@@ -232,7 +235,7 @@ int bshmem_ckpt8_swiglu_store(const void* gu, void* act, void* kept, long long r
   p.q = static_cast<uint8_t*>(kept); p.e = p.q + rows * 2 * F;
   p.lde = (2LL * F + 127) / 128; p.F = F;
   p.size = {rows * p.lde * 16, (uint32_t)(p.lde * 16)};
-  return launch(swiglu_store8_kernel, kPer, p, stream);
+  return kept ? launch(swiglu_store8_kernel<true>, kPer, p, stream) : launch(swiglu_store8_kernel<false>, kPer, p, stream);
 }
 
 // dgu [rows, 2F] from gu in 8 bits and dact [rows, F]; act (may be null): the activation again, of the same 8 bits.

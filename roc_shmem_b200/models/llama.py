@@ -133,14 +133,15 @@ class LlamaMLP:
         else:
             dh = self.dgrad_h(dy_shard, weight=self.w2_t)                          # [M, F/P], gathers dy
             dy = self.dgrad_h.gathered
-        if kept is not None:
-            restore(kept[0], out=self.up.gathered)
-            swiglu_backward(kept[1], dh, dgu_out=self.dgu, act_out=self.h)         # SwiGLU' and the activations again
-        grouped_gemm_tn(dy, self.h, self.dw2, 1, self.rows)                        # dW2 = dy^T h
+        h, x = self.h, self.up.gathered
+        if kept is not None:                                                       # the last forward's own buffers stay as they are
+            _, h = swiglu_backward(kept[1], dh, act=True, dgu_out=self.dgu)        # SwiGLU' and the activations again
+            x = restore(kept[0])
+        grouped_gemm_tn(dy, h, self.dw2, 1, self.rows)                             # dW2 = dy^T h
         if not fused and kept is None:
             self._chk(moe_fast.swiglu_bwd(self.gu.data_ptr(), dh.data_ptr(), self.rows.data_ptr(), 1, self.M, self.Fp,
                                           self.dgu.data_ptr(), s), "swiglu bwd")
-        grouped_gemm_tn(self.dgu, self.up.gathered, self.dw13, 1, self.rows)       # dW13 = dgu^T x
+        grouped_gemm_tn(self.dgu, x, self.dw13, 1, self.rows)                      # dW13 = dgu^T x
         dx = self.dgrad_x(self.dgu, weight=self.w13_t)
         self.launches += 4 if fused else 5 if kept is None else 6
         return dx

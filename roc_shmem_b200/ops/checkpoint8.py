@@ -149,23 +149,28 @@ def _aligned(x: torch.Tensor) -> torch.Tensor:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
-def swiglu_store(gu: torch.Tensor) -> tuple[torch.Tensor, Checkpoint8]:
-    """act [..., F] = silu(gate) * up of gu [..., 2F] (32 columns of the gate, then the 32 of ``up``, see
-    ``interleave_gate_up``), and gu in 8 bits, in one pass."""
+def _swiglu_forward(gu: torch.Tensor, keep: bool) -> tuple[torch.Tensor, Optional[torch.Tensor]]:
     _check_gu(gu)
     if not on_current_device(gu):
         with torch.cuda.device(gu.device):
-            return swiglu_store(gu)
+            return _swiglu_forward(gu, keep)
     if _swiglu_store is None:
         _lib()
     g = _aligned(gu)
     F = gu.shape[-1] // 2
     rows = gu.numel() // (2 * F)
     act = gu.new_empty((*gu.shape[:-1], F))
-    data = gu.new_empty((kept_bytes(rows, 2 * F),), dtype=torch.uint8)
-    st = _swiglu_store(g.data_ptr(), act.data_ptr(), data.data_ptr(), rows, F, current_stream())
+    data = gu.new_empty((kept_bytes(rows, 2 * F),), dtype=torch.uint8) if keep else None
+    st = _swiglu_store(g.data_ptr(), act.data_ptr(), None if data is None else data.data_ptr(), rows, F, current_stream())
     if st != 0:
         _check(st, "swiglu_store")
+    return act, data
+
+
+def swiglu_store(gu: torch.Tensor) -> tuple[torch.Tensor, Checkpoint8]:
+    """act [..., F] = silu(gate) * up of gu [..., 2F] (32 columns of the gate, then the 32 of ``up``, see
+    ``interleave_gate_up``), and gu in 8 bits, in one pass."""
+    act, data = _swiglu_forward(gu, True)
     return act, Checkpoint8(data, gu.shape, gu.dtype)
 
 
@@ -217,4 +222,4 @@ def swiglu(gu: torch.Tensor) -> torch.Tensor:
     """silu(gate) * up of the interleaved gu [..., 2F]; what the gradient needs of gu is kept in 8 bits."""
     if torch.is_grad_enabled() and gu.requires_grad:
         return _SwigluFn.apply(gu)
-    return swiglu_store(gu)[0]
+    return _swiglu_forward(gu, False)[0]

@@ -92,6 +92,65 @@ def test_checkpointed_block_equals_its_own_recomputation(rt):
         _near(got, ref, 2.0 ** -8 * 3)                        # dh, dgu or the activations, and the result are rounded to bf16
 
 
+@pytest.mark.parametrize("M,F", [(512, 768), (2560, 1024)])
+def test_kept_backward_leaves_the_last_forward_alone(rt, M, F):
+    """A (kept), B (not kept), A's backward, B's backward: B's gradients are those without A in between."""
+    from roc_shmem_b200.models.llama import LlamaMLP
+    H = 512
+    block = LlamaMLP(rt, H, F, M)
+    block.load(_rand(F, H, seed=1, scale=0.05), _rand(F, H, seed=2, scale=0.05), _rand(H, F, seed=3, scale=0.05))
+    a, b, dy = (_rand(M, H, seed=s) for s in (4, 5, 6))
+    block.forward(b)
+    expect = [t.clone() for t in (block.backward(dy), block.dw13, block.dw2)]
+    block.forward(a)
+    kept = block.keep()
+    block.forward(b)
+    block.backward(dy, kept)
+    got = (block.backward(dy), block.dw13, block.dw2)
+    assert all(torch.equal(x, y) for x, y in zip(got, expect))
+    block.check()
+
+
+_FIRST_CALLS = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from roc_shmem_b200.ops.checkpoint8 import restore, store, swiglu_backward, swiglu_store
+from roc_shmem_b200.ops.gemm_w4 import W4Tensor, linear_w4
+from roc_shmem_b200.ops.norms import post_pre_norm
+bf = torch.bfloat16
+x = torch.randn(600, 1024, device="cuda").to(bf)
+w = torch.ones(1024, device="cuda", dtype=bf)
+leaves = [t.clone().requires_grad_(True) for t in (x, x, w, w)]
+q = W4Tensor(torch.randint(0, 256, (512, 512), device="cuda", dtype=torch.uint8), torch.ones(512, 8, device="cuda", dtype=bf))
+few = x[:3].clone()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out, h = post_pre_norm(*leaves, checkpoint=True)
+    grads = torch.autograd.grad((out, h), leaves, (x, x))
+    y = linear_w4(few, q)
+    act, kept = swiglu_store(x)
+    dgu = swiglu_backward(kept, act)
+    back = restore(store(x))
+graph.replay()
+torch.cuda.synchronize()
+out2, h2 = post_pre_norm(*leaves, checkpoint=True)
+grads2 = torch.autograd.grad((out2, h2), leaves, (x, x))
+same = [torch.equal(a, b) for a, b in zip((out, h, *grads, y, dgu, back), (out2, h2, *grads2, linear_w4(few, q), swiglu_backward(swiglu_store(x)[1], act), restore(store(x))))]
+print("same", all(same))
+"""
+
+
+def test_first_calls_inside_a_capture():
+    """A program whose first use of each operator is recorded into a graph."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = str(Path(__file__).resolve().parent.parent)
+    done = subprocess.run([sys.executable, "-c", _FIRST_CALLS, root], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same True" in done.stdout, done.stderr[-2000:]
+
+
 @pytest.mark.parametrize("rows", [8, 1000])
 def test_linear_with_kept_input(rows):
     from roc_shmem_b200.ops.checkpoint8 import restore, store
