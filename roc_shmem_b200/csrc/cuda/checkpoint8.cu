@@ -14,10 +14,10 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// A thread has kPer eights of the matrix, a block's width apart, whose loads are all on their way before the first is used: one alone
-// leaves 32 KB of an SM on their way, and 16384 x 4096 there and back took 83 us.  Rows are padded to whole blocks of 128 columns (16
-// eights), so the eights of a block are neighbours in a warp.
-constexpr int kPer = 4;
+// A thread has several eights, whose loads are all on their way before the first is used: with one alone, 32 KB of an SM on their way,
+// 16384 x 4096 there and back took 83 us, for 76 with four.  Two of them are of one block of 128 columns, whose largest value takes
+// eight threads then: the way there is bound by issue (three instructions a cycle with one eight of a block for each of sixteen threads).
+constexpr int kPer = 4, kPairs = 2;
 struct Eights { long long total; uint32_t per_row; };
 // Row and column of the i-th eight; a 64-bit division only where there are that many.
 __device__ __forceinline__ void place(const Eights& s, long long i, long long& row, int& col) {
@@ -35,28 +35,32 @@ __device__ __forceinline__ void place(const Eights& s, long long i, long long& r
 
 struct StoreParams { const void* x; long long ldx; uint8_t* q; uint8_t* e; long long ldq, lde; int n; Eights size; };
 
+// The size counts pairs of eights: the j-th and the (j + 8)-th of a block are thread j's.
 template <typename T, int kAccess> __global__ void __launch_bounds__(kThreads) store8_kernel(const StoreParams p) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const long long first = (long long)blockIdx.x * (kThreads * kPer) + threadIdx.x;
-  long long row[kPer];
-  int col[kPer], n[kPer];
-  Raw8<T> r[kPer];
+  const long long first = (long long)blockIdx.x * (kThreads * kPairs) + threadIdx.x;
+  long long row[kPairs];
+  int col[kPairs], n[kPairs];
+  Raw8<T> r[kPairs][2];
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
+  for (int j = 0; j < kPairs; ++j) {
     const long long i = first + j * kThreads;
     n[j] = i < p.size.total ? p.n : 0;
     place(p.size, n[j] ? i : 0, row[j], col[j]);
-    r[j] = load8<kAccess>(static_cast<const T*>(p.x) + row[j] * p.ldx, col[j], n[j]);
+    col[j] = col[j] / 64 * 128 + col[j] % 64;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) r[j][k] = load8<kAccess>(static_cast<const T*>(p.x) + row[j] * p.ldx, col[j] + 64 * k, n[j]);
   }
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
+  for (int j = 0; j < kPairs; ++j) {
     uint32_t e;
-    const uint2 q = encode8<T>(unpack(r[j]), e);
-    if (col[j] < n[j]) {
-      *reinterpret_cast<uint2*>(p.q + row[j] * p.ldq + col[j]) = q;
-      if (col[j] % 128 == 0) p.e[row[j] * p.lde + col[j] / 128] = (uint8_t)e;
-    }
+    uint2 q[2];
+    encode<T, 2>({unpack(r[j][0]), unpack(r[j][1])}, q, e);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (col[j] + 64 * k < n[j]) *reinterpret_cast<uint2*>(p.q + row[j] * p.ldq + col[j] + 64 * k) = q[k];
+    if (col[j] % 128 == 0 && col[j] < n[j]) p.e[row[j] * p.lde + col[j] / 128] = (uint8_t)e;
   }
 }
 
@@ -88,46 +92,46 @@ struct SwigluParams {
   uint8_t *q, *e;
   long long lde;
   int F;
-  Eights size;                                        // forward: of gu, in whole blocks of 128 columns; backward: of the activation
+  Eights size;                                        // of the activation; forward: in whole blocks
 };
 
 __device__ __forceinline__ float2 sigmoid2(float2 x) { return make_float2(1.f / (1.f + __expf(-x.x)), 1.f / (1.f + __expf(-x.y))); }
 
-// Four threads in a row have a gate, the next four its `up`, which they swap.  Without kKeep only the activation is written.
+// A thread has eights of the activation; the gate and `up` of eight threads are a block.  Without kKeep only the activation is written.
 template <bool kKeep> __global__ void __launch_bounds__(kThreads) swiglu_store8_kernel(const SwigluParams p) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const long long first = (long long)blockIdx.x * (kThreads * kPer) + threadIdx.x;
-  long long row[kPer];
-  int col[kPer], n[kPer];
-  Raw8<__nv_bfloat16> r[kPer];
+  const long long first = (long long)blockIdx.x * (kThreads * kPairs) + threadIdx.x;
+  long long row[kPairs];
+  int col[kPairs], at[kPairs];
+  bool in[kPairs];
+  Raw8<__nv_bfloat16> r[kPairs][2];
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
+  for (int j = 0; j < kPairs; ++j) {
     const long long i = first + j * kThreads;
-    n[j] = i < p.size.total ? 2 * p.F : 0;
-    place(p.size, n[j] ? i : 0, row[j], col[j]);
-    r[j] = load8<kVector>(p.gu + row[j] * 2 * p.F, col[j], n[j]);
+    place(p.size, i < p.size.total ? i : 0, row[j], col[j]);
+    in[j] = i < p.size.total && col[j] < p.F;
+    at[j] = col[j] / 32 * 64 + col[j] % 32;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) r[j][k] = load8<kVector>(p.gu + row[j] * 2 * p.F, at[j] + 32 * k, in[j] ? 2 * p.F : 0);
   }
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const Vals v = unpack(r[j]);
-    uint32_t e;
-    uint2 q;
-    if constexpr (kKeep) q = encode8<__nv_bfloat16>(v, e);
-    const uint4 w = r[j].get(0);
-    Raw8<__nv_bfloat16> other;
-    other.set(0, make_uint4(__shfl_xor_sync(0xffffffffu, w.x, 4), __shfl_xor_sync(0xffffffffu, w.y, 4), __shfl_xor_sync(0xffffffffu, w.z, 4),
-                            __shfl_xor_sync(0xffffffffu, w.w, 4)));
-    if (col[j] >= n[j]) continue;
+  for (int j = 0; j < kPairs; ++j) {
+    const Vals g = unpack(r[j][0]), u = unpack(r[j][1]);
     if constexpr (kKeep) {
-      *reinterpret_cast<uint2*>(p.q + row[j] * 2 * p.F + col[j]) = q;
-      if (col[j] % 128 == 0) p.e[row[j] * p.lde + col[j] / 128] = (uint8_t)e;
-    }
-    if (col[j] & 32) continue;
-    Vals u = unpack(other);
+      uint32_t e;
+      uint2 q[2];
+      encode<__nv_bfloat16, 2>({g, u}, q, e);
+      if (in[j]) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) u.p[k] = mul2(u.p[k], mul2(v.p[k], sigmoid2(v.p[k])));
-    store8<kVector>(p.act + row[j] * p.F, col[j] / 64 * 32 + col[j] % 32, p.F, pack<__nv_bfloat16>(u));
+        for (int k = 0; k < 2; ++k) *reinterpret_cast<uint2*>(p.q + row[j] * 2 * p.F + at[j] + 32 * k) = q[k];
+        if (at[j] % 128 == 0) p.e[row[j] * p.lde + at[j] / 128] = (uint8_t)e;
+      }
+    }
+    Vals o;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o.p[k] = mul2(u.p[k], mul2(g.p[k], sigmoid2(g.p[k])));
+    if (in[j]) store8<kVector>(p.act + row[j] * p.F, col[j], p.F, pack<__nv_bfloat16>(o));
   }
 }
 
@@ -204,11 +208,11 @@ int bshmem_ckpt8_store(int type, const void* x, long long ldx, void* kept, long 
   const long long blocks = ((long long)n + 127) / 128;
   const long long ldq = ((long long)n + 15) / 16 * 16;
   uint8_t* const q = static_cast<uint8_t*>(kept);
-  const StoreParams p = {x, ldx, q, q + rows * ldq, ldq, blocks, n, {rows * blocks * 16, (uint32_t)(blocks * 16)}};
+  const StoreParams p = {x, ldx, q, q + rows * ldq, ldq, blocks, n, {rows * blocks * 8, (uint32_t)(blocks * 8)}};
   const bool vec = n % 8 == 0 && aligned(x) && ldx * (type == 2 ? 4 : 2) % 16 == 0;
-  if (type == 0) return vec ? launch(store8_kernel<__nv_bfloat16, kVector>, kPer, p, stream) : launch(store8_kernel<__nv_bfloat16, kSingle>, kPer, p, stream);
-  if (type == 1) return vec ? launch(store8_kernel<__half, kVector>, kPer, p, stream) : launch(store8_kernel<__half, kSingle>, kPer, p, stream);
-  return vec ? launch(store8_kernel<float, kVector>, kPer, p, stream) : launch(store8_kernel<float, kSingle>, kPer, p, stream);
+  if (type == 0) return vec ? launch(store8_kernel<__nv_bfloat16, kVector>, kPairs, p, stream) : launch(store8_kernel<__nv_bfloat16, kSingle>, kPairs, p, stream);
+  if (type == 1) return vec ? launch(store8_kernel<__half, kVector>, kPairs, p, stream) : launch(store8_kernel<__half, kSingle>, kPairs, p, stream);
+  return vec ? launch(store8_kernel<float, kVector>, kPairs, p, stream) : launch(store8_kernel<float, kSingle>, kPairs, p, stream);
 }
 
 // The way back; x has row pitch ldx.
@@ -234,8 +238,8 @@ int bshmem_ckpt8_swiglu_store(const void* gu, void* act, void* kept, long long r
   p.act = static_cast<__nv_bfloat16*>(act);
   p.q = static_cast<uint8_t*>(kept); p.e = p.q + rows * 2 * F;
   p.lde = (2LL * F + 127) / 128; p.F = F;
-  p.size = {rows * p.lde * 16, (uint32_t)(p.lde * 16)};
-  return kept ? launch(swiglu_store8_kernel<true>, kPer, p, stream) : launch(swiglu_store8_kernel<false>, kPer, p, stream);
+  p.size = {rows * p.lde * 8, (uint32_t)(p.lde * 8)};
+  return kept ? launch(swiglu_store8_kernel<true>, kPairs, p, stream) : launch(swiglu_store8_kernel<false>, kPairs, p, stream);
 }
 
 // dgu [rows, 2F] from gu in 8 bits and dact [rows, F]; act (may be null): the activation again, of the same 8 bits.

@@ -178,27 +178,38 @@ __device__ __forceinline__ uint32_t finite_bits(float v) {
   const uint32_t a = __float_as_uint(v) & 0x7fffffffu;
   return a < 0x7f800000u ? a : 0u;
 }
-// All 32 lanes take part; sixteen of them hold a block.  The eight bytes of this lane's values, which are of type T, and the block's exponent byte.
-template <typename T> __device__ __forceinline__ uint2 encode8(const Vals& v, uint32_t& e) {
+// All 32 lanes take part; 16 / kEach neighbours hold a block, kEach eights of it each.  The bytes of this lane's values, which are of type T, and
+// the block's exponent byte.
+template <typename T, int kEach> __device__ __forceinline__ void encode(const Vals (&v)[kEach], uint2 (&q)[kEach], uint32_t& e) {
   float top = 0.f;
   float2 odd = both(0.f);                             // NaN if one of the values is no number, or infinite
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    top = fmaxf(top, fmaxf(fabsf(v.p[i].x), fabsf(v.p[i].y)));
-    odd = fma2(v.p[i], both(0.f), odd);
-  }
+  for (int k = 0; k < kEach; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      top = fmaxf(top, fmaxf(fabsf(v[k].p[i].x), fabsf(v[k].p[i].y)));
+      odd = fma2(v[k].p[i], both(0.f), odd);
+    }
   uint32_t bits = __float_as_uint(top);
   // rare, and then for the whole warp: the largest of the finite values, and the careful conversion
   const bool any = __any_sync(0xffffffffu, odd.x + odd.y != 0.f || bits >= (kTopExponent<T> + 7u) << 23);
   if (any) {
     bits = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bits = max(bits, max(finite_bits(v.p[i].x), finite_bits(v.p[i].y)));
+    for (int k = 0; k < kEach; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bits = max(bits, max(finite_bits(v[k].p[i].x), finite_bits(v[k].p[i].y)));
   }
 #pragma unroll
-  for (int o = 8; o; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+  for (int o = 8 / kEach; o; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
   e = exponent_byte(bits);
-  return any ? bytes8<T, true>(v, e) : bytes8<T, false>(v, e);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) q[k] = any ? bytes8<T, true>(v[k], e) : bytes8<T, false>(v[k], e);
+}
+template <typename T> __device__ __forceinline__ uint2 encode8(const Vals& v, uint32_t& e) {
+  uint2 q[1];
+  encode<T, 1>({v}, q, e);
+  return q[0];
 }
 __device__ __forceinline__ Vals decode8(uint2 q, uint32_t e) {
   Vals v;
