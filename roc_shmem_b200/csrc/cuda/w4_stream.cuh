@@ -163,7 +163,10 @@ template <int kNt, int kSubs>
 __global__ void __launch_bounds__(threads(kNt, kSubs), 1) w4_stream_kernel(const __grid_constant__ Params p) {
   constexpr int kDepth = depth(kNt, kSubs), kCols = block_cols(kNt, kSubs);        // columns of a stage: A, then its accumulators
   constexpr int kStages = stages(kNt), kGroups = widen_groups(kNt, kSubs);
-  static_assert(kDepth >= 1 && 2 * kDepth >= kGroups && 2 * kStages >= kGroups, "k-blocks on their way");
+  // A wait knows a barrier's rounds by their parity only, so nobody may come to one two rounds early.  A group is (kGroups + 1) / 2 stages
+  // at most behind its last k-block, when it knew all sums of kDepth stages before that to be added up (and so their loads, too).
+  constexpr int kStride = (kGroups + 1) / 2;
+  static_assert(kDepth >= kStride && kStages >= kStride + kDepth, "rounds of the barriers");
   extern __shared__ uint8_t smem_raw[];
   Smem L;
   {
