@@ -77,8 +77,8 @@ template <typename T, int kAccess> __global__ void __launch_bounds__(kThreads) r
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     place(p.size, min(first + j * kThreads, p.size.total - 1), row[j], col[j]);
-    q[j] = __ldg(reinterpret_cast<const uint2*>(p.q + row[j] * p.ldq + col[j]));
-    e[j] = __ldg(p.e + row[j] * p.lde + col[j] / 128);
+    q[j] = *reinterpret_cast<const uint2*>(p.q + row[j] * p.ldq + col[j]);
+    e[j] = p.e[row[j] * p.lde + col[j] / 128];
   }
 #pragma unroll
   for (int j = 0; j < kPer; ++j)
@@ -151,9 +151,9 @@ template <bool kAct> __global__ void __launch_bounds__(kThreads) swiglu_backward
     place(p.size, min(first + j * kThreads, p.size.total - 1), row[j], col[j]);
     at[j] = col[j] / 32 * 64 + col[j] % 32;
     const uint8_t* q = p.q + row[j] * 2 * p.F + at[j];
-    e[j] = __ldg(p.e + row[j] * p.lde + at[j] / 128);
-    qg[j] = __ldg(reinterpret_cast<const uint2*>(q));
-    qu[j] = __ldg(reinterpret_cast<const uint2*>(q + 32));
+    e[j] = p.e[row[j] * p.lde + at[j] / 128];
+    qg[j] = *reinterpret_cast<const uint2*>(q);
+    qu[j] = *reinterpret_cast<const uint2*>(q + 32);
     rd[j] = load8<kVector>(p.dact + row[j] * p.F, col[j], p.F);
   }
 #pragma unroll

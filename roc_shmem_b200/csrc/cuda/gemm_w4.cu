@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(256) w4_widen_kernel(const WidenParams p) {
 #pragma unroll
   for (int j = 0; j < kWidenWords; ++j) {
     const long long i = min(first + j * 256, p.words - 1), g = i / p.per_group;
-    w[j] = __ldg(p.q + i);
+    w[j] = p.q[i];
     s[j] = p.s[g];
     z[j] = p.z ? p.z[g] : 8;
   }

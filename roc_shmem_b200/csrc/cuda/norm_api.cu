@@ -56,8 +56,8 @@ template <typename T> __global__ void __launch_bounds__(kFinishCols * kFinishLan
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const long long at = g + i * kFinishLanes;
-        va[i] = p.part_w2 && at < p.groups ? __ldg(p.part_w2 + at * pitch + col) : 0.f;
-        vc[i] = p.part_c && at < p.groups ? __ldg(p.part_c + at * pitch + col) : 0.f;
+        va[i] = p.part_w2 && at < p.groups ? p.part_w2[at * pitch + col] : 0.f;
+        vc[i] = p.part_c && at < p.groups ? p.part_c[at * pitch + col] : 0.f;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) { a += va[i]; c += vc[i]; }

@@ -394,8 +394,8 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
       rstd1 = __uint_as_float(r.x);
       rstd2 = __uint_as_float(r.y);
     } else {
-      if constexpr (kMode != kPre) rstd1 = __ldg(p.rstd1 + row);
-      if constexpr (kMode != kPost) rstd2 = __ldg(p.rstd2 + row);
+      if constexpr (kMode != kPre) rstd1 = p.rstd1[row];
+      if constexpr (kMode != kPost) rstd2 = p.rstd2[row];
     }
     Vals dz[kChunks], ny[kMode != kPre ? kChunks : 1];
     // in a ring the first norm's operands are read when it is their turn; elsewhere their loads begin here

@@ -103,12 +103,13 @@ enum Access : int { kSingle = 0, kVector = 1, kStrided = 2 };
 template <int kAccess> __device__ __forceinline__ int column_of(int col, int j) {
   return kAccess == kStrided ? (col & ~255) + (col >> 3 & 31) + 32 * j : col + j;
 }
-// Columns from n on are zeros.
+// Columns from n on are zeros.  Plain loads: a kernel that starts while the one before still writes its operands may not say that they are read
+// only, or the compiler could move a load in front of the wait for that kernel.
 template <int kAccess, typename T> __device__ __forceinline__ Raw8<T> load8(const T* row, int col, int n) {
   Raw8<T> r;
   if constexpr (kAccess == kVector) {
 #pragma unroll
-    for (int i = 0; i < Raw8<T>::kWords; ++i) r.set(i, col < n ? __ldg(reinterpret_cast<const uint4*>(row + col) + i) : make_uint4(0, 0, 0, 0));
+    for (int i = 0; i < Raw8<T>::kWords; ++i) r.set(i, col < n ? reinterpret_cast<const uint4*>(row + col)[i] : make_uint4(0, 0, 0, 0));
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) r.v[j] = column_of<kAccess>(col, j) < n ? row[column_of<kAccess>(col, j)] : from_float<T>(0.f);
@@ -263,8 +264,8 @@ template <int kAccess> __device__ __forceinline__ Vals kept8(const uint8_t* q, c
     uint2 b = make_uint2(0, 0);
     uint32_t x = 1;
     if (col < n) {
-      b = __ldg(reinterpret_cast<const uint2*>(q + col));
-      x = __ldg(e + col / 128);
+      b = *reinterpret_cast<const uint2*>(q + col);
+      x = e[col / 128];
     }
     return decode8(b, x);
   } else {

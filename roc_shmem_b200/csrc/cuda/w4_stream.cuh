@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(threads(kNt, kSubs), 1) w4_stream_kernel(const
     uint32_t zp[kSubs];                               // of the k-block's groups
     auto load = [&](int kb) {
 #pragma unroll
-      for (int j = 0; j < kSubs; ++j) zp[j] = z ? __ldg(z + min(kSubs == 1 ? kb * BK / p.group : kb * kSubs + j, groups - 1)) : 8;
+      for (int j = 0; j < kSubs; ++j) zp[j] = z ? z[min(kSubs == 1 ? kb * BK / p.group : kb * kSubs + j, groups - 1)] : 8;
     };
     load(kb0 + group);
     int s = group / 2; uint32_t ph = 0;
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(threads(kNt, kSubs), 1) w4_stream_kernel(const
     auto load = [&](int kb) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        next[j] = __ldg(scales + min(kSubs == 1 ? (kb + j) * BK / p.group : kb * kSubs + j, groups - 1));
+        next[j] = scales[min(kSubs == 1 ? (kb + j) * BK / p.group : kb * kSubs + j, groups - 1)];
     };
     load(kb0);
     bool ok = true;

@@ -90,8 +90,8 @@ class _Call:
             raise ValueError(f"{name} needs bf16, fp16 or fp32 CUDA tensors, got {dt} on {x.device}")
         if not shape or not 1 <= shape[-1] <= MAX_COLUMNS:
             raise ValueError(f"{name} needs rows of 1 to {MAX_COLUMNS} columns, got {tuple(shape)}")
-        if not eps > 0:
-            raise ValueError(f"{name} needs eps > 0")
+        if not 1.2e-38 < eps < 3.4e38:
+            raise ValueError(f"{name} needs eps > 0, a normal fp32 number")
         n, dev = shape[-1], x.get_device()
         what |= mode << 2
         if checkpoint:

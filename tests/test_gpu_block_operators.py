@@ -230,3 +230,49 @@ def test_long_offsets():
     assert torch.equal(h[-3:], rms_norm(last, w)) and not h[:-3].any()
     del h
     assert torch.equal(restore(store(x))[-3:], restore(store(last)))
+
+
+def test_two_streams_at_once():
+    """4-bit products, the bf16 GEMM and norms of two streams in each other's way: what takes whole multiprocessors waits, nothing else changes."""
+    from roc_shmem_b200.ops.gemm import gemm_bf16, gemm_error_site
+    from roc_shmem_b200.ops.gemm_w4 import linear_w4, quantize_w4, w4_error_site
+    from roc_shmem_b200.ops.norms import post_pre_norm
+    a, b = quantize_w4(_rand(2048, 4096, seed=1), 128), quantize_w4(_rand(4104, 2048, seed=2), 32, zeros=True)
+    x, y, w = _rand(3, 4096, seed=3), _rand(40, 2048, seed=4), _rand(512, 2048, seed=5)
+    r, one = _rand(300, 2048, seed=6), torch.ones(2048, dtype=BF, device="cuda")
+    jobs = [lambda: linear_w4(x, a), lambda: linear_w4(y, b), lambda: gemm_bf16(y, w), lambda: post_pre_norm(r, r, one, one)[1]]
+    expect = [j() for j in jobs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(60):
+        for s, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                k = (i + 2 * s) % 4
+                got.append((k, jobs[k]()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, expect[k]) for k, v in got) and w4_error_site() == 0 and gemm_error_site() == 0
+
+
+def test_extreme_shapes():
+    """One column and a million rows; a million columns of a few 4-bit rows; many rows of few columns."""
+    from block_reference import close
+    from roc_shmem_b200.ops.gemm_w4 import W4Tensor, linear_w4
+    from roc_shmem_b200.ops.norms import rms_norm
+    x = _rand(1000003, 1, seed=1).requires_grad_(True)
+    w = torch.full((1,), 0.5, dtype=torch.float32, device="cuda", requires_grad=True)
+    h = rms_norm(x, w, 1e-3)
+    d = x.detach().double()
+    n = d / (d * d + 1e-3).sqrt()
+    close(h, n * 0.5, (n * 0.5).abs())
+    gw, = torch.autograd.grad(h, w, torch.ones_like(h))
+    close(gw, n.sum().view(1), n.abs().sum().view(1), 64 + 1000003 // 4)
+    K = 1 << 20
+    q = torch.randint(0, 256, (24, K // 2), device="cuda", dtype=torch.uint8, generator=torch.Generator(device="cuda").manual_seed(2))
+    t = W4Tensor(q, torch.full((24, K // 128), 0.01, dtype=BF, device="cuda"))
+    v = _rand(3, K, seed=3)
+    m = ((torch.stack((q & 15, q >> 4), 2).flatten(1).double() - 8) * t.scales[0, 0].double())
+    close(linear_w4(v, t), v.double() @ m.t(), v.double().abs() @ m.abs().t(), 2 * (K // 16 + 16))
+    tall = W4Tensor(q.view(-1, 32)[:100003].contiguous(), torch.full((100003, 1), 0.01, dtype=BF, device="cuda"))
+    u = _rand(2, 64, seed=4)
+    m = ((torch.stack((tall.q & 15, tall.q >> 4), 2).flatten(1).double() - 8) * tall.scales[0, 0].double())
+    close(linear_w4(u, tall), u.double() @ m.t(), u.double().abs() @ m.abs().t(), 2 * (64 // 16 + 16))
