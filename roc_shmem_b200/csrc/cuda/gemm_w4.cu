@@ -164,9 +164,6 @@ template <int kNt, int kSubs> int stream_product(w4::Params& p, int sms, void* s
     const long long cost = (tiles + at_once - 1) / at_once * ((kb + s - 1) / s) + (s > 1 ? 2 : 0);
     if (s == 1 || cost < best) { best = cost; p.split = s; }
   }
-#ifdef W4_SPLIT
-  p.split = W4_SPLIT;
-#endif
   return launch(w4::w4_stream_kernel<kNt, kSubs>, dim3((unsigned)((p.N + w4::ROWS - 1) / w4::ROWS * p.split), (unsigned)chunks), w4::threads(kNt, kSubs), p.split,
                 w4::SMEM_BYTES, p, stream);
 }

@@ -12,7 +12,7 @@
 //   warp 0      TMA producer: {128 rows x 128 bytes of weights, tokens x 256 columns} per stage, i.e. two k-blocks (with rows of 64
 //               bytes the TMA unit's requests, one per row, were the limit); plain loads of local memory
 //   warp 1      MMA issuer: tcgen05.mma M128 x N=tokens x K16, A in tensor memory, B in shared memory
-//   next 16     up to four groups of four warps: each widens every fourth k-block and orders its activations
+//   then        three to five groups of four warps: each widens every third to fifth k-block and orders its activations
 //   last 4      add the accumulators up
 //
 // From a k-block's arrival to its sums it takes a warp of each kind some 900 cycles, and HBM brings an SM the 8 KiB of the next in 370: so several
@@ -40,10 +40,8 @@ using gemm2::mapa;
 using gemm2::warp_wait;
 
 constexpr int ROWS = 128, BK = 128;                  // weight rows of a tile, columns of a k-block
-constexpr int MAX_TOKENS = 64;                       // of a tile
 constexpr int MAX_STAGES = 9, MAX_DEPTH = 3;
 constexpr int WIDENERS = 4, ADDERS = 4;              // warps of a group that widens, and warps that add up
-constexpr int MAX_GROUPS = 4;
 constexpr uint32_t W_BYTES = ROWS * BK;              // 16 KiB of weights per stage: two k-blocks
 constexpr uint32_t CTRL_BYTES = 512;
 constexpr uint32_t SMEM_BYTES = 224u << 10;          // one CTA has an SM, all of its tensor memory too
@@ -74,9 +72,11 @@ __host__ __device__ constexpr int depth(int nt, int subs) {
   return TMEM_COLS / block_cols(nt, subs) < MAX_DEPTH ? TMEM_COLS / block_cols(nt, subs) : MAX_DEPTH;
 }
 // Groups that widen: no more than there are k-blocks in tensor memory, or a group could ask about a buffer's round before last and take
-// the answer for its last one; and three for 64 tokens, whose sums take more registers.
+// the answer for its last one; three for 64 tokens, whose sums take more registers; five for 16 tokens in groups of 128 columns and
+// more, whose sums take fewest (7168 rows of 8192, one token: 14.1 us with four, 13.7 with five or six; 4096 of 4096: 6.8, 6.8, 7.2).
 __host__ __device__ constexpr int widen_groups(int nt, int subs) {
-  return 2 * depth(nt, subs) < MAX_GROUPS ? 2 * depth(nt, subs) : nt == 64 ? 3 : MAX_GROUPS;
+  const int most = nt == 64 ? 3 : nt == 16 && subs == 1 ? 5 : 4;
+  return 2 * depth(nt, subs) < most ? 2 * depth(nt, subs) : most;
 }
 __host__ __device__ constexpr int threads(int nt, int subs) { return 32 * (2 + WIDENERS * widen_groups(nt, subs) + ADDERS); }
 
@@ -123,10 +123,6 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
-}
 // D[tmem] (+)= A[tmem] * B[smem desc]
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
