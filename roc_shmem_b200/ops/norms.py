@@ -79,6 +79,10 @@ def _matrix(t: torch.Tensor, cols: int) -> torch.Tensor:
     return m if m.stride(1) == 1 or cols == 1 else m.contiguous()
 
 
+def _refuse_vector(name, label, t, x):
+    raise ValueError(f"{name}: {label} must be {x.dtype} or fp32 of shape ({x.shape[-1]},) on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
 class _Call:
     """A call's operands, checked: what they are in one word, and their addresses and pitches."""
     __slots__ = ("what", "y", "x", "w1", "w2", "gate", "scale", "number", "eps", "rows", "n", "like", "gate_ld", "kind")
@@ -102,34 +106,40 @@ class _Call:
         if self.rows > 0x7fffffff:
             raise ValueError(f"{name} takes less than 2^31 rows")
 
-        def vector(t, label, bit):
-            nonlocal what
-            if t.shape != (n,) or t.get_device() != dev or (t.dtype is not dt and t.dtype is not _F32):
-                raise ValueError(f"{name}: {label} must be {dt} or fp32 of shape ({n},) on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-            if t.dtype is _F32:
-                what |= 1 << bit
-            return t if t.is_contiguous() else t.contiguous()
-        self.w1 = None if w1 is None else vector(w1, "weight", 8)
-        self.w2 = None if w2 is None else vector(w2, "weight" if mode == PRE else "next_weight", 9)
-        self.gate, self.gate_ld, self.scale, self.number = None, 0, None, 1.0
+        column = (n,)
+        if w1 is not None:
+            if w1.shape != column or w1.get_device() != dev or (w1.dtype is not dt and w1.dtype is not _F32):
+                _refuse_vector(name, "weight", w1, x)
+            if w1.dtype is _F32:
+                what |= 1 << 8
+            if not w1.is_contiguous():
+                w1 = w1.contiguous()
+        if w2 is not None:
+            if w2.shape != column or w2.get_device() != dev or (w2.dtype is not dt and w2.dtype is not _F32):
+                _refuse_vector(name, "weight" if mode == PRE else "next_weight", w2, x)
+            if w2.dtype is _F32:
+                what |= 1 << 9
+            if not w2.is_contiguous():
+                w2 = w2.contiguous()
+        self.w1, self.w2, self.gate, self.gate_ld, self.scale, self.number = w1, w2, None, 0, None, 1.0
         if mode != PRE:
             if y.shape != shape or y.dtype is not dt or y.get_device() != dev:
                 raise ValueError(f"{name}: y and residual must be alike, got {y.dtype} {tuple(y.shape)} on {y.device} and {dt} {tuple(shape)} on {x.device}")
             self.y = _matrix(y, n)
             if gate is not None:
-                if gate.shape == (n,):
-                    self.kind, self.gate = COLUMN, vector(gate, "gate", 10)
+                if gate.get_device() != dev or (gate.dtype is not dt and gate.dtype is not _F32):
+                    raise ValueError(f"{name}: gate must be {dt} or fp32 on {x.device}, got {gate.dtype} on {gate.device}")
+                if gate.dtype is _F32:
+                    what |= 1 << 10
+                if gate.shape == column:
+                    self.kind, self.gate = COLUMN, gate.contiguous()
                 else:
-                    if gate.get_device() != dev or (gate.dtype is not dt and gate.dtype is not _F32):
-                        raise ValueError(f"{name}: gate must be {dt} or fp32 on {x.device}, got {gate.dtype} on {gate.device}")
                     if gate.shape == shape:
                         self.kind, self.gate = ELEMENT, _matrix(gate, n)
                     elif gate.shape == (*shape[:-1], 1):
                         self.kind, self.gate = ROW, _matrix(gate, 1)
                     else:
                         raise ValueError(f"{name}: gate must be ({n},), {(*shape[:-1], 1)} or {tuple(shape)}, got {tuple(gate.shape)}")
-                    if gate.dtype is _F32:
-                        what |= 1 << 10
                     self.gate_ld = self.gate.stride(0)
                 what |= self.kind << 4
             if scale is None:
@@ -162,7 +172,8 @@ def _forward(c: _Call, mode: int, train: bool):
         what &= ~KEPT
     y, x = c.y, c.x
     st = _fwd(what, None if y is None else y.data_ptr(), 0 if y is None else y.stride(0), x.data_ptr(), x.stride(0),
-              None if out is None else out.data_ptr(), None if h is None else h.data_ptr(), _p(c.w1), _p(c.w2), _p(c.gate), c.gate_ld, _p(c.scale),
+              None if out is None else out.data_ptr(), None if h is None else h.data_ptr(), None if c.w1 is None else c.w1.data_ptr(),
+              None if c.w2 is None else c.w2.data_ptr(), None if c.gate is None else c.gate.data_ptr(), c.gate_ld, _p(c.scale),
               _numbers(c.eps, c.number), _p(rstd), _p(kept), rows, n, current_stream())
     if st != 0:
         _check(st, "norm")
@@ -255,16 +266,12 @@ class _NormFn(torch.autograd.Function):
         return _backward_once(ctx, *grads) if torch.is_grad_enabled() else _backward(ctx, *grads)
 
 
-def _wants_grad(t) -> bool:
-    return t is not None and t.requires_grad
-
-
 def _run(name, mode, y, x, w1, w2, gate, scale, eps, checkpoint):
     c = _Call(name, mode, y, x, w1, w2, gate, scale, eps, checkpoint)
     if not on_current_device(x):
         with torch.cuda.device(x.device):
             return _run(name, mode, y, x, w1, w2, gate, scale, eps, checkpoint)
-    if torch.is_grad_enabled() and (x.requires_grad or _wants_grad(y) or _wants_grad(w2) or _wants_grad(w1) or _wants_grad(gate) or _wants_grad(c.scale)):
+    if torch.is_grad_enabled() and any([t.requires_grad for t in (x, y, w1, w2, gate, c.scale) if t is not None]):
         return _NormFn.apply(y, x, w1, w2, gate, c.scale, c, mode)
     out, h, _, _ = _forward(c, mode, False)
     return (out, h) if mode == POST_PRE else out if mode == POST else h
