@@ -122,6 +122,8 @@ class LlamaMLP:
         """Returns dx_shard [M/P, H]; weight gradients land in ``dw13`` / ``dw2``.  Must follow forward(), unless it gets what keep()
         gave after the forward() that it belongs to: the gradients are then those at the kept values."""
         assert self.training
+        if kept is not None and (kept[0].shape != self.up.gathered.shape or kept[1].shape != self.gu.shape):
+            raise ValueError(f"these are not what a forward() of this block kept: {tuple(kept[0].shape)}, {tuple(kept[1].shape)}")
         s = current_stream()
         fused = self.P == 1 and self._fills(self.Fp) and kept is None
         if self.P == 1:
@@ -185,6 +187,7 @@ class LlamaMLPModule(torch.nn.Module):
     ``scale``; the norms are of this rank's rows, so with several ranks their gradients are to be added up over them.
     ``checkpoint``: every forward keeps what its backward needs in 8 bits instead of the block's buffers, so that several may come before
     their backwards (micro-batches)."""
+    norms = checkpoint = False                           # of modules saved before there were any
 
     def __init__(self, rt, hidden: int = 8192, ffn: int = 28672, max_tokens: int = 8192, *, norms: bool = False, checkpoint: bool = False,
                  eps: float = 1e-6):
@@ -199,10 +202,11 @@ class LlamaMLPModule(torch.nn.Module):
             self.scale = torch.nn.Parameter(torch.ones((1,), dtype=torch.float32, device=rt.device))
 
     def forward(self, x_shard: torch.Tensor) -> torch.Tensor:
+        checkpoint = self.checkpoint and torch.is_grad_enabled()
         if not self.norms:
-            return _LlamaMLPFn.apply(x_shard, self.w13, self.w2, self.block, self.checkpoint)
+            return _LlamaMLPFn.apply(x_shard, self.w13, self.w2, self.block, checkpoint)
         h = rms_norm(x_shard, self.pre, self.eps, checkpoint=self.checkpoint)
-        y = _LlamaMLPFn.apply(h, self.w13, self.w2, self.block, self.checkpoint)
+        y = _LlamaMLPFn.apply(h, self.w13, self.w2, self.block, checkpoint)
         return post_norm(y, x_shard, self.post, scale=self.scale, eps=self.eps, checkpoint=self.checkpoint)
 
     def after_step(self) -> None:

@@ -98,6 +98,18 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     return m if m.stride(1) == 1 else m.contiguous()
 
 
+def _held(kept: Checkpoint8, what: str) -> tuple[torch.Tensor, int, int]:
+    """(bytes, rows, columns) of `kept`, whose shape says what the kernels write."""
+    data, shape = kept.data, kept.shape
+    cols = shape[-1] if shape else 0
+    rows = shape.numel() // cols if cols else 0
+    if not cols or data.numel() != kept_bytes(rows, cols) or data.dtype is not torch.uint8 or not data.is_contiguous() or data.data_ptr() % 16:
+        raise ValueError(f"{what}: the checkpoint does not hold a {tuple(shape)}")
+    if not data.is_cuda:
+        raise ValueError(f"{what} needs a checkpoint of a CUDA tensor, got one on {data.device}")
+    return data, rows, cols
+
+
 def store(x: torch.Tensor) -> Checkpoint8:
     """bf16, fp16 or fp32 [..., columns] → 8 bits."""
     m = _rows(x, "store")
@@ -117,7 +129,7 @@ def store(x: torch.Tensor) -> Checkpoint8:
 def restore(kept: Checkpoint8, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The stored values in `dtype` (default: what was stored), into `out` if given ([rows, columns] with columns side by side)."""
     dtype = dtype or (out.dtype if out is not None else kept.dtype)
-    data = kept.data
+    data, rows, cols = _held(kept, "restore")
     if dtype not in _TYPES:
         raise ValueError(f"restore gives bf16, fp16 or fp32, not {dtype}")
     if not on_current_device(data):
@@ -125,7 +137,6 @@ def restore(kept: Checkpoint8, dtype: Optional[torch.dtype] = None, out: Optiona
             return restore(kept, dtype, out)
     if _restore is None:
         _lib()
-    cols, rows = kept.shape[-1], kept.rows
     if out is None:
         out = data.new_empty(kept.shape, dtype=dtype)
         ld = cols
@@ -178,13 +189,14 @@ def swiglu_backward(kept: Checkpoint8, dact: torch.Tensor, *, act: bool = False,
                     act_out: Optional[torch.Tensor] = None):
     """Gradient of gu from its 8 bits and the activation's gradient; with `act` also the activation again, of the same 8 bits (what
     the next layer's weight gradient reads).  `dgu_out`, `act_out`: contiguous buffers for them."""
-    data, shape = kept.data, kept.shape
+    shape = kept.shape
+    data, rows, cols = _held(kept, "swiglu_backward")
     if not on_current_device(data):
         with torch.cuda.device(data.device):
             return swiglu_backward(kept, dact, act=act, dgu_out=dgu_out, act_out=act_out)
-    F = shape[-1] // 2
+    F = cols // 2
     bf = torch.bfloat16
-    if shape[-1] % 64 or dact.dtype is not bf or dact.shape != (*shape[:-1], F) or dact.get_device() != data.get_device():
+    if cols % 64 or dact.dtype is not bf or dact.shape != (*shape[:-1], F) or dact.get_device() != data.get_device():
         raise ValueError(f"swiglu_backward: a bf16 gradient of {(*shape[:-1], F)} belongs to this checkpoint, got {dact.dtype} {tuple(dact.shape)}")
     if _swiglu_backward is None:
         _lib()
@@ -198,7 +210,7 @@ def swiglu_backward(kept: Checkpoint8, dact: torch.Tensor, *, act: bool = False,
         return given
     dgu = buffer(dgu_out, shape)
     again = buffer(act_out, dact.shape) if act or act_out is not None else None
-    st = _swiglu_backward(data.data_ptr(), d.data_ptr(), dgu.data_ptr(), None if again is None else again.data_ptr(), kept.rows, F, current_stream())
+    st = _swiglu_backward(data.data_ptr(), d.data_ptr(), dgu.data_ptr(), None if again is None else again.data_ptr(), rows, F, current_stream())
     if st != 0:
         _check(st, "swiglu_backward")
     return dgu if again is None else (dgu, again)

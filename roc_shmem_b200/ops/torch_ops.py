@@ -148,6 +148,7 @@ def _unwatched() -> bool:
 class Linear(torch.nn.Module):
     """Drop-in bf16 ``nn.Linear`` (no bias) whose forward and both gradients run on the tcgen05 kernels.  ``checkpoint``: calls of plain
     tensors keep their input for the weight's gradient in 8 bits (``checkpoint8``), half of what bf16 takes."""
+    checkpoint = False                                   # of modules saved before there was one
 
     def __init__(self, in_features: int, out_features: int, device=None, *, checkpoint: bool = False):
         super().__init__()

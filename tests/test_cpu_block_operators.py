@@ -75,3 +75,31 @@ def test_few_tokens_rule():
     from roc_shmem_b200.ops.gemm_w4 import few_tokens
     assert [few_tokens(g) for g in (32, 64, 128, 256)] == [32, 128, 128, 128]
     assert C.sizeof(C.c_longlong) == 8
+
+
+def test_checkpoints_that_do_not_hold_their_shape():
+    """The kernels write as many rows as the shape has, so bytes for another number of them are refused, and whatever is not on a GPU."""
+    from roc_shmem_b200.ops.checkpoint8 import Checkpoint8, kept_bytes, restore, swiglu_backward
+    bf, shape = torch.bfloat16, torch.Size((4, 64))
+    data = torch.zeros(kept_bytes(4, 64) + 16, dtype=torch.uint8)
+    size, dact = kept_bytes(4, 64), torch.zeros(4, 32, dtype=bf)
+    assert size == 4 * 65 and Checkpoint8(data[:size], shape, bf).rows == 4
+    for kept in (Checkpoint8(data, shape, bf), Checkpoint8(data[:size - 1], shape, bf), Checkpoint8(data[:size], torch.Size((5, 64)), bf),
+                 Checkpoint8(data[:size], torch.Size((3, 64)), bf), Checkpoint8(data[:size], torch.Size(()), bf),
+                 Checkpoint8(data[:size], torch.Size((4, 0)), bf), Checkpoint8(data[1:size + 1], shape, bf),
+                 Checkpoint8(data[:size].view(torch.int8), shape, bf)):
+        for call in (lambda: restore(kept), lambda: swiglu_backward(kept, dact)):
+            with pytest.raises(ValueError, match="does not hold"):
+                call()
+    for call in (lambda: restore(Checkpoint8(data[:size], shape, bf)), lambda: swiglu_backward(Checkpoint8(data[:size], shape, bf), dact)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+
+
+def test_modules_saved_before_there_were_checkpoints():
+    """What unpickling makes of a layer that was saved without the attributes."""
+    from roc_shmem_b200.models.llama import LlamaMLPModule
+    from roc_shmem_b200.ops.torch_ops import Linear
+    assert Linear.__new__(Linear).checkpoint is False
+    old = LlamaMLPModule.__new__(LlamaMLPModule)
+    assert old.checkpoint is False and old.norms is False

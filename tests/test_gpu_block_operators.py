@@ -276,3 +276,26 @@ def test_extreme_shapes():
     u = _rand(2, 64, seed=4)
     m = ((torch.stack((tall.q & 15, tall.q >> 4), 2).flatten(1).double() - 8) * tall.scales[0, 0].double())
     close(linear_w4(u, tall), u.double() @ m.t(), u.double().abs() @ m.abs().t(), 2 * (64 // 16 + 16))
+
+
+def test_kept_of_another_block_is_refused(rt):
+    from roc_shmem_b200.models.llama import LlamaMLP
+    M, H = 512, 512
+    one, other = LlamaMLP(rt, H, 768, M), LlamaMLP(rt, H, 1024, M)
+    x = _rand(M, H, seed=1)
+    one.forward(x), other.forward(x)
+    a, b = one.keep(), other.keep()
+    for kept in (b, (a[0], b[1]), (a[1], a[0])):
+        with pytest.raises(ValueError, match="forward"):
+            one.backward(x, kept)
+
+
+def test_no_gradient_nothing_kept(rt, monkeypatch):
+    from roc_shmem_b200.models.llama import LlamaMLPModule
+    mod = LlamaMLPModule(rt, 512, 768, 512, norms=True, checkpoint=True)
+    mod.block.load(_rand(768, 512, seed=1, scale=0.05), _rand(768, 512, seed=2, scale=0.05), _rand(512, 768, seed=3, scale=0.05))
+    x = _rand(512, 512, seed=4)
+    expect = mod(x).detach()
+    monkeypatch.setattr(mod.block, "keep", lambda: pytest.fail("kept without a gradient"))
+    with torch.no_grad():
+        assert torch.equal(mod(x), expect)
