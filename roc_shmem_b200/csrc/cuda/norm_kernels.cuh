@@ -256,7 +256,6 @@ __global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512)
 // memory do, which only their thread touches.
 template <typename T, int kMode, int kChunks, int kForm, bool kKept8, bool kLong = false>
 __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdParams p) {
-
   constexpr int kAccess = kForm == kScalar ? kStrided : kVector;
   // words of a stage: dout, dh, z, y, the two 1 / sqrt(...) and the gate per element; one that is kept in 8 bits has its
   // eight bytes and the four that its exponent byte is among in one word
@@ -546,8 +545,8 @@ inline int sm_count(int* out) {
 }
 
 template <typename K, typename P> int launch(K* kernel, dim3 grid, dim3 block, int shared, const P& p, cudaStream_t stream) {
-  if (shared > 40 * 1024)                             // 48 KB with the static part need no asking
-    BSHMEM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
+  if (shared > 40 * 1024)                             // 48 KB with the static part need no asking; the same for every call, or one of two at once lowered it
+    BSHMEM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;

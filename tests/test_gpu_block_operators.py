@@ -299,3 +299,30 @@ def test_no_gradient_nothing_kept(rt, monkeypatch):
     monkeypatch.setattr(mod.block, "keep", lambda: pytest.fail("kept without a gradient"))
     with torch.no_grad():
         assert torch.equal(mod(x), expect)
+
+
+def test_two_threads_at_once():
+    """Widths whose kernels are the same but for their shared memory, from two threads: what one asks for does not become the other's."""
+    import threading
+    from roc_shmem_b200.ops.norms import post_pre_norm
+    inputs = [torch.randn(rows, n, device="cuda", generator=torch.Generator("cuda").manual_seed(n)).to(BF) for rows, n in ((1300, 4096), (700, 8192))]
+    weights = [torch.ones(x.shape[1], dtype=BF, device="cuda") for x in inputs]
+    expect = [post_pre_norm(x, x, w, w)[1] for x, w in zip(inputs, weights)]
+    torch.cuda.synchronize()
+    start, failed = threading.Barrier(2), []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for _ in range(3000):
+                    got = post_pre_norm(inputs[i], inputs[i], weights[i], weights[i])[1]
+                assert torch.equal(got, expect[i])
+        except Exception as e:
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
