@@ -1,8 +1,8 @@
 // checkpoint8.cu — activations in 8 bits between the forward and the backward pass (the form is in row_values.cuh): to it and
 // back, and the gated activation act = silu(gate) * up that keeps its input so.
 //
-// Every kernel reads and writes each byte once and computes next to nothing: memory bounds them.  A thread has eight columns and
-// sixteen threads a block of 128, so the largest value of a block is found by four shuffles.
+// Every kernel reads and writes each byte once: memory bounds them, but for the way to the form, where conversions come close to what the
+// multiprocessors issue.  8192 x 3584 of the gated activation, forward and backward: 84 us (6.3 TB/s).
 #include "ptx.cuh"
 #include "row_values.cuh"
 #include "tma_host.h"
@@ -15,8 +15,9 @@ namespace {
 constexpr int kThreads = 256;
 
 // A thread has several eights, whose loads are all on their way before the first is used: with one alone, 32 KB of an SM on their way,
-// 16384 x 4096 there and back took 83 us, for 76 with four.  Two of them are of one block of 128 columns, whose largest value takes
-// eight threads then: the way there is bound by issue (three instructions a cycle with one eight of a block for each of sixteen threads).
+// 16384 x 4096 there and back took 83 us, for 76 with four.  On the way there two of them are of one block of 128 columns, whose largest value
+// takes eight threads then: it is bound by issue (three instructions a cycle with one eight of a block for each of sixteen threads), and there and
+// back take 70 us so, 67 with plain loads (6.1 TB/s).
 constexpr int kPer = 4, kPairs = 2;
 struct Eights { long long total; uint32_t per_row; };
 // Row and column of the i-th eight; a 64-bit division only where there are that many.
