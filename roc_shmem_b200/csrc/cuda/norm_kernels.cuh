@@ -105,8 +105,10 @@ __device__ __forceinline__ float sum2(float2 v) { return v.x + v.y; }
 
 // ---- forward -------------------------------------------------------------------------------------------
 // A row stays in the registers of its threads, kChunks groups of eight columns for each, between the sums: memory is read once.
-// In a ring the weights (w1 times a gate per column, and w2) stay in registers too.
-template <typename T, int kMode, int kChunks, int kForm>
+// In a ring the weights (w1 times a gate per column, and w2) stay in registers too, and what a call has besides is known when the kernel is
+// built: kKeep, its inputs are kept in 8 bits; kElement, it has a gate per element.  8192 x 8192 with neither takes 93 us so, 110 where
+// the kernel asks at every row (elsewhere true means that it asks).
+template <typename T, int kMode, int kChunks, int kForm, bool kKeep = true, bool kElement = true>
 __global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512) norm_fwd_kernel(const Params p) {
   constexpr int kAccess = kForm == kScalar ? kStrided : kVector;
   constexpr bool kHeld = kForm == kRing && kChunks <= 2;
@@ -114,6 +116,8 @@ __global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512)
   extern __shared__ uint4 ring_words[];
   __shared__ float sums[2 * kMaxWarps];
   RowSum sum(sums);
+  const bool keep = kForm == kRing ? kKeep : (p.q1 || p.q2),
+             per_element = kMode != kPre && (kForm == kRing ? kElement : p.gate_kind == Gate::kElement);
   const Ring ring(ring_words, p.ring_words, p.stages);
   if constexpr (kForm == kRing) {
     for (int i = 0; i < p.stages; ++i) ring.clear(i);        // columns behind the last one are never fetched
@@ -133,7 +137,7 @@ __global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512)
         if (col < p.n) {
           if constexpr (kMode != kPre) ring.fetch8(stage, i * W, y + col);
           ring.fetch8(stage, kX + i * W, x + col);
-          if (kMode != kPre && p.gate_kind == kElement) {
+          if (per_element) {
             if (p.gate_f32) ring.fetch8(stage, kGate + i * 2, row_of<float>(p.gate, row) + col);
             else ring.fetch8(stage, kGate + i * W, row_of<T>(p.gate, row) + col);
           }
@@ -196,13 +200,13 @@ __global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512)
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const int col = column(i);
-        if (p.q1) keep8<kAccess, T>(p.q1 + row * p.ldq, p.e1 + row * p.lde, col, n, y[i]);
+        if (keep) keep8<kAccess, T>(p.q1 + row * p.ldq, p.e1 + row * p.lde, col, n, y[i]);
         Vals w, r;
         if constexpr (kHeld) w = held1[i];
         else w = weight1(i);
         if constexpr (kForm == kRing) r = ring.get8<T>(stage, kX + i * W);
         else r = x[i];
-        if (p.gate_kind == kElement) {
+        if (per_element) {
           Vals g;
           if constexpr (kForm == kRing) g = p.gate_f32 ? ring.get8<float>(stage, kGate + i * 2) : ring.get8<T>(stage, kGate + i * W);
           else g = p.gate_f32 ? unpack(load8<kAccess>(row_of<float>(p.gate, row), col, n)) : unpack(load8<kAccess>(row_of<T>(p.gate, row), col, n));
@@ -237,7 +241,7 @@ __global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512)
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const int col = column(i);
-        if (p.q2) keep8<kAccess, T>(p.q2 + row * p.ldq, p.e2 + row * p.lde, col, n, z[i]);
+        if (keep) keep8<kAccess, T>(p.q2 + row * p.ldq, p.e2 + row * p.lde, col, n, z[i]);
         Vals w;
         if constexpr (kHeld) w = held2[i];
         else w = vector8<kAccess, T>(p.w2, p.w2_f32, col, n);
@@ -253,8 +257,8 @@ __global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512)
 // A block walks over rows and keeps the column sums of its rows in registers; norm_bwd_finish_kernel adds up the groups' sums in
 // their order, so two calls give the same bits.  In a ring the weights are fp32 words of shared memory behind the stages, where
 // there is room.  kLong: rows of over 8192 columns on 1024 threads, whose 64 registers do not hold the column sums: words of shared
-// memory do, which only their thread touches.
-template <typename T, int kMode, int kChunks, int kForm, bool kKept8, bool kLong = false>
+// memory do, which only their thread touches.  kElement: as in norm_fwd_kernel (8192 x 8192: 156 us for 162).
+template <typename T, int kMode, int kChunks, int kForm, bool kKept8, bool kElement = true, bool kLong = false>
 __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdParams p) {
   constexpr int kAccess = kForm == kScalar ? kStrided : kVector;
   // words of a stage: dout, dh, z, y, the two 1 / sqrt(...) and the gate per element; one that is kept in 8 bits has its
@@ -266,6 +270,7 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
   extern __shared__ uint4 ring_words[];
   __shared__ float sums[2 * kMaxWarps];
   RowSum sum(sums);
+  const bool per_element = kMode != kPre && (kForm == kRing ? kElement : p.gate_kind == Gate::kElement);
   const Ring ring(ring_words, p.ring_words, p.stages);
   const Ring weights(ring_words + p.stages * p.ring_words * ring.threads, 0, 0);
   if constexpr (kForm == kRing) {
@@ -334,7 +339,7 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
           if constexpr (kMode != kPre) {
             if (p.dout.p) ring.fetch8(stage, i * W, row_of<T>(p.dout, row) + col);
             fetch_kept(stage, kY + i * K, p.y, p.q1, p.e1, row, col);
-            if (p.gate_kind == kElement) {
+            if (per_element) {
               if (p.gate_f32) ring.fetch8(stage, kGate + i * 2, row_of<float>(p.gate, row) + col);
               else ring.fetch8(stage, kGate + i * W, row_of<T>(p.gate, row) + col);
             }
@@ -460,7 +465,7 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
         Vals w;
         if (kForm == kRing && p.held) w = held(i, 0);
         else w = weight1(i, n);
-        if (p.gate_kind == kElement) {
+        if (per_element) {
           Vals g;
           if constexpr (kForm == kRing) g = p.gate_f32 ? ring.get8<float>(stage, kGate + i * 2) : ring.get8<T>(stage, kGate + i * W);
           else g = p.gate_f32 ? unpack(load8<kAccess>(row_of<float>(p.gate, row), col, n)) : unpack(load8<kAccess>(row_of<T>(p.gate, row), col, n));
@@ -624,6 +629,16 @@ template <typename F, typename G> Shape backward_shape(long long rows, int n, bo
   return s;
 }
 
+template <typename T, int kMode, bool kKeep, bool kElement> int forward_ring(const Shape& s, const Params& p, dim3 grid, dim3 block, cudaStream_t stream) {
+  if (s.chunks == 2) return launch(norm_fwd_kernel<T, kMode, 2, kRing, kKeep, kElement>, grid, block, shared_of(s), p, stream);
+  return launch(norm_fwd_kernel<T, kMode, 4, kRing, kKeep, kElement>, grid, block, shared_of(s), p, stream);
+}
+template <typename T, int kMode, bool kKeep> int forward_ring(const Shape& s, const Params& p, dim3 grid, dim3 block, cudaStream_t stream) {
+  if constexpr (kMode != kPre) {
+    if (p.gate_kind == Gate::kElement) return forward_ring<T, kMode, kKeep, true>(s, p, grid, block, stream);
+  }
+  return forward_ring<T, kMode, kKeep, false>(s, p, grid, block, stream);
+}
 template <typename T, int kMode> int forward_mode(bool vec, Params p, cudaStream_t stream) {
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
@@ -633,8 +648,7 @@ template <typename T, int kMode> int forward_mode(bool vec, Params p, cudaStream
   if (s.form == kRing) {
     p.stages = s.stages;
     p.ring_words = s.words;
-    if (s.chunks == 2) return launch(norm_fwd_kernel<T, kMode, 2, kRing>, grid, block, shared_of(s), p, stream);
-    return launch(norm_fwd_kernel<T, kMode, 4, kRing>, grid, block, shared_of(s), p, stream);
+    return p.q1 || p.q2 ? forward_ring<T, kMode, true>(s, p, grid, block, stream) : forward_ring<T, kMode, false>(s, p, grid, block, stream);
   }
   if (s.form == kScalar) return launch(norm_fwd_kernel<T, kMode, 4, kScalar>, grid, block, 0, p, stream);
   if (s.chunks == 1) return launch(norm_fwd_kernel<T, kMode, 1, kDirect>, grid, block, 0, p, stream);
@@ -653,16 +667,22 @@ inline bool backward_raw(const BwdParams& p, int size) {
 template <typename T, int kMode, bool kKept> int backward_mode(const Shape& s, BwdParams p, cudaStream_t stream) {
   const dim3 grid((unsigned)s.blocks), block(s.threads, s.rows);
   if (s.threads > 512) {
-    if (s.form == kDirect) return launch(norm_bwd_kernel<T, kMode, 2, kDirect, kKept, true>, grid, block, shared_of(s), p, stream);
-    return launch(norm_bwd_kernel<T, kMode, 2, kScalar, kKept, true>, grid, block, shared_of(s), p, stream);
+    if (s.form == kDirect) return launch(norm_bwd_kernel<T, kMode, 2, kDirect, kKept, true, true>, grid, block, shared_of(s), p, stream);
+    return launch(norm_bwd_kernel<T, kMode, 2, kScalar, kKept, true, true>, grid, block, shared_of(s), p, stream);
   }
   if (s.form == kRing) {
     p.stages = s.stages;
     p.ring_words = s.words;
     p.held = s.held == 0 ? 0 : s.held == backward_held(kMode, s.chunks) ? 1 : 2;
     const int shared = shared_of(s);
-    if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kRing, kKept>, grid, block, shared, p, stream);
-    return launch(norm_bwd_kernel<T, kMode, 2, kRing, kKept>, grid, block, shared, p, stream);
+    if constexpr (kMode != kPre) {
+      if (p.gate_kind == Gate::kElement) {
+        if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kRing, kKept, true>, grid, block, shared, p, stream);
+        return launch(norm_bwd_kernel<T, kMode, 2, kRing, kKept, true>, grid, block, shared, p, stream);
+      }
+    }
+    if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kRing, kKept, false>, grid, block, shared, p, stream);
+    return launch(norm_bwd_kernel<T, kMode, 2, kRing, kKept, false>, grid, block, shared, p, stream);
   }
   if (s.form == kDirect) {
     if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kDirect, kKept>, grid, block, 0, p, stream);

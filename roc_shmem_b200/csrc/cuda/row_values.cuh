@@ -65,6 +65,14 @@ template <typename T> __device__ __forceinline__ Vals unpack(const Raw8<T>& r) {
   for (int i = 0; i < 4; ++i) v.p[i] = make_float2(to_float<T>(r.v[2 * i]), to_float<T>(r.v[2 * i + 1]));
   return v;
 }
+template <> __device__ __forceinline__ Vals unpack(const Raw8<__nv_bfloat16>& r) {      // a bf16 is the high half of its fp32
+  Vals v;
+  const uint4 w = r.get(0);
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v.p[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+  return v;
+}
 template <> __device__ __forceinline__ Vals unpack(const Raw8<__half>& r) {
   Vals v;
 #pragma unroll
@@ -140,8 +148,8 @@ template <int kAccess, typename T> __device__ __forceinline__ Vals vector8(const
 
 // ---- activations in 8 bits -------------------------------------------------------------------------
 // e4m3 times one power of two for each row and 128 columns, the smallest that holds the block's largest finite value (448 is
-// e4m3's largest): a power of two loses nothing, neither here nor on the way back, and it is one byte (exponent + 127).  Sixteen
-// neighbouring lanes hold a block, eight columns each.  Infinities come back as NaN; e4m3 has none.
+// e4m3's largest): a power of two loses nothing, neither here nor on the way back, and it is one byte (exponent + 127).
+// Infinities come back as NaN; e4m3 has none.
 __device__ __forceinline__ float block_scale_bits(uint32_t e) { return __uint_as_float(e << 23); }
 // The largest exponent byte of a type's blocks.  Only there could a value round up to a power of two that the type does not have
 // (2^128, 2^16 for fp16): such values stay at 240 steps instead of 256.
