@@ -70,6 +70,11 @@ template <typename T> __device__ __forceinline__ T* row_of(const Mat& m, long lo
 // shared memory (cp.async), so nothing but its own wait is between the copy and the use.
 enum Form : int { kScalar = 0, kDirect = 1, kRing = 2 };
 
+// What is known of a gate per element when a kernel is built: that there is none, that it has the rows' type, that it is fp32, or nothing.
+enum Element : int { kNone = 0, kOfT = 1, kOfF32 = 2, kAsk = 3 };
+template <int kElement> __device__ __forceinline__ bool element_gate(int gate_kind) { return kElement == kAsk ? gate_kind == Gate::kElement : kElement != kNone; }
+template <int kElement> __device__ __forceinline__ bool element_f32(int gate_f32) { return kElement == kAsk ? gate_f32 : kElement == kOfF32; }
+
 // The words of a thread in one stage of the ring, [stage][word][thread].  A thread reads what it copied itself.
 struct Ring {
   uint4* mine;
@@ -105,10 +110,10 @@ __device__ __forceinline__ float sum2(float2 v) { return v.x + v.y; }
 
 // ---- forward -------------------------------------------------------------------------------------------
 // A row stays in the registers of its threads, kChunks groups of eight columns for each, between the sums: memory is read once.
-// In a ring the weights (w1 times a gate per column, and w2) stay in registers too, and what a call has besides is known when the kernel is
-// built: kKeep, its inputs are kept in 8 bits; kElement, it has a gate per element.  8192 x 8192 with neither takes 93 us so, 110 where
-// the kernel asks at every row (elsewhere true means that it asks).
-template <typename T, int kMode, int kChunks, int kForm, bool kKeep = true, bool kElement = true>
+// In a ring the weights (w1 times a gate per column, and w2) stay in registers too, and whether the inputs are kept in 8 bits (kKeep) and
+// what gate per element there is are known when the kernel is built: 8192 x 8192 with neither takes 95 us so, 110 where the kernel asks at
+// every row.  In the other forms it asks.
+template <typename T, int kMode, int kChunks, int kForm, bool kKeep = true, int kElement = kAsk>
 __global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512) norm_fwd_kernel(const Params p) {
   constexpr int kAccess = kForm == kScalar ? kStrided : kVector;
   constexpr bool kHeld = kForm == kRing && kChunks <= 2;
@@ -116,8 +121,8 @@ __global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512)
   extern __shared__ uint4 ring_words[];
   __shared__ float sums[2 * kMaxWarps];
   RowSum sum(sums);
-  const bool keep = kForm == kRing ? kKeep : (p.q1 || p.q2),
-             per_element = kMode != kPre && (kForm == kRing ? kElement : p.gate_kind == Gate::kElement);
+  const bool keep = kForm == kRing ? kKeep : p.q1 || p.q2, per_element = kMode != kPre && element_gate<kElement>(p.gate_kind);
+  const bool f32 = element_f32<kElement>(p.gate_f32);
   const Ring ring(ring_words, p.ring_words, p.stages);
   if constexpr (kForm == kRing) {
     for (int i = 0; i < p.stages; ++i) ring.clear(i);        // columns behind the last one are never fetched
@@ -138,7 +143,7 @@ __global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512)
           if constexpr (kMode != kPre) ring.fetch8(stage, i * W, y + col);
           ring.fetch8(stage, kX + i * W, x + col);
           if (per_element) {
-            if (p.gate_f32) ring.fetch8(stage, kGate + i * 2, row_of<float>(p.gate, row) + col);
+            if (f32) ring.fetch8(stage, kGate + i * 2, row_of<float>(p.gate, row) + col);
             else ring.fetch8(stage, kGate + i * W, row_of<T>(p.gate, row) + col);
           }
         }
@@ -208,8 +213,8 @@ __global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512)
         else r = x[i];
         if (per_element) {
           Vals g;
-          if constexpr (kForm == kRing) g = p.gate_f32 ? ring.get8<float>(stage, kGate + i * 2) : ring.get8<T>(stage, kGate + i * W);
-          else g = p.gate_f32 ? unpack(load8<kAccess>(row_of<float>(p.gate, row), col, n)) : unpack(load8<kAccess>(row_of<T>(p.gate, row), col, n));
+          if constexpr (kForm == kRing) g = f32 ? ring.get8<float>(stage, kGate + i * 2) : ring.get8<T>(stage, kGate + i * W);
+          else g = f32 ? unpack(load8<kAccess>(row_of<float>(p.gate, row), col, n)) : unpack(load8<kAccess>(row_of<T>(p.gate, row), col, n));
 #pragma unroll
           for (int j = 0; j < 4; ++j) w.p[j] = mul2(w.p[j], g.p[j]);
         }
@@ -257,8 +262,10 @@ __global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512)
 // A block walks over rows and keeps the column sums of its rows in registers; norm_bwd_finish_kernel adds up the groups' sums in
 // their order, so two calls give the same bits.  In a ring the weights are fp32 words of shared memory behind the stages, where
 // there is room.  kLong: rows of over 8192 columns on 1024 threads, whose 64 registers do not hold the column sums: words of shared
-// memory do, which only their thread touches.  kElement: as in norm_fwd_kernel (8192 x 8192: 156 us for 162).
-template <typename T, int kMode, int kChunks, int kForm, bool kKept8, bool kElement = true, bool kLong = false>
+// memory do, which only their thread touches.  kHeld: the usual call of a ring, known when the kernel is built: the weights are held (1, 2: see
+// BwdParams), dout is there, dy is wanted, and what gate per element there is; 0: the kernel asks.  8192 x 8192 with its forward pass 243 us
+// for 251, 16384 x 4096 with 8 bits and a gate per element 379 for 397.
+template <typename T, int kMode, int kChunks, int kForm, bool kKept8, int kHeld = 0, int kElement = kAsk, bool kLong = false>
 __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdParams p) {
   constexpr int kAccess = kForm == kScalar ? kStrided : kVector;
   // words of a stage: dout, dh, z, y, the two 1 / sqrt(...) and the gate per element; one that is kept in 8 bits has its
@@ -270,7 +277,9 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
   extern __shared__ uint4 ring_words[];
   __shared__ float sums[2 * kMaxWarps];
   RowSum sum(sums);
-  const bool per_element = kMode != kPre && (kForm == kRing ? kElement : p.gate_kind == Gate::kElement);
+  const bool per_element = kMode != kPre && element_gate<kElement>(p.gate_kind), f32 = element_f32<kElement>(p.gate_f32);
+  const bool has_dout = kHeld || p.dout.p, wants_dy = kHeld || p.dy.p;
+  const bool in_fp32 = kHeld ? kHeld == 1 : p.held == 1;
   const Ring ring(ring_words, p.ring_words, p.stages);
   const Ring weights(ring_words + p.stages * p.ring_words * ring.threads, 0, 0);
   if constexpr (kForm == kRing) {
@@ -337,10 +346,10 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
         const int col = column(i);
         if (col < p.n) {
           if constexpr (kMode != kPre) {
-            if (p.dout.p) ring.fetch8(stage, i * W, row_of<T>(p.dout, row) + col);
+            if (has_dout) ring.fetch8(stage, i * W, row_of<T>(p.dout, row) + col);
             fetch_kept(stage, kY + i * K, p.y, p.q1, p.e1, row, col);
             if (per_element) {
-              if (p.gate_f32) ring.fetch8(stage, kGate + i * 2, row_of<float>(p.gate, row) + col);
+              if (f32) ring.fetch8(stage, kGate + i * 2, row_of<float>(p.gate, row) + col);
               else ring.fetch8(stage, kGate + i * W, row_of<T>(p.gate, row) + col);
             }
           }
@@ -370,13 +379,13 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
     return w;
   };
   auto keep = [&](int i, int from, const Vals& v) {
-    if (p.held == 1) hold(weights, from + i * 2, v);
+    if (in_fp32) hold(weights, from + i * 2, v);
     else weights.mine[(from / 2 + i) * weights.threads] = pack<T>(v).get(0);
   };
-  auto held = [&](int i, int from) { return p.held == 1 ? weights.get8<float>(0, from + i * 2) : weights.get8<T>(0, from / 2 + i); };
+  auto held = [&](int i, int from) { return in_fp32 ? weights.get8<float>(0, from + i * 2) : weights.get8<T>(0, from / 2 + i); };
   if constexpr (kForm == kRing) {
     for (int i = 0; i < p.stages; ++i) fetch(first + threadIdx.y + i * step, i);
-    if (p.held) {
+    if (kHeld || p.held) {
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         if constexpr (kMode != kPre) keep(i, 0, weight1(i, p.n));
@@ -409,7 +418,7 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
       for (int j = 0; j < 4; ++j) ny[i].p[j] = mul2(ny[i].p[j], both(rstd1));
     };
     auto given = [&](int i) {
-      if (p.dout.p) dz[i] = plain(stage, i * W, p.dout, row, column(i), n);
+      if (has_dout) dz[i] = plain(stage, i * W, p.dout, row, column(i), n);
       else dz[i].fill(0.f);
     };
     if constexpr (kMode == kPost || (kMode == kPostPre && kForm != kRing)) {
@@ -427,7 +436,7 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         Vals w;
-        if (kForm == kRing && p.held) w = held(i, kW2);
+        if (kForm == kRing && (kHeld || p.held)) w = held(i, kW2);
         else w = vector8<kAccess, T>(p.w2, p.w2_f32, column(i), n);
         Vals sums_w2;
         if constexpr (kLong) sums_w2 = accs.get8<float>(0, i * 2);
@@ -463,17 +472,17 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
         const int col = column(i);
         if constexpr (kMode == kPostPre && kForm == kRing) first_norm(i);
         Vals w;
-        if (kForm == kRing && p.held) w = held(i, 0);
+        if (kForm == kRing && (kHeld || p.held)) w = held(i, 0);
         else w = weight1(i, n);
         if (per_element) {
           Vals g;
-          if constexpr (kForm == kRing) g = p.gate_f32 ? ring.get8<float>(stage, kGate + i * 2) : ring.get8<T>(stage, kGate + i * W);
-          else g = p.gate_f32 ? unpack(load8<kAccess>(row_of<float>(p.gate, row), col, n)) : unpack(load8<kAccess>(row_of<T>(p.gate, row), col, n));
+          if constexpr (kForm == kRing) g = f32 ? ring.get8<float>(stage, kGate + i * 2) : ring.get8<T>(stage, kGate + i * W);
+          else g = f32 ? unpack(load8<kAccess>(row_of<float>(p.gate, row), col, n)) : unpack(load8<kAccess>(row_of<T>(p.gate, row), col, n));
           if (p.dgate.p) {
             Vals d;
 #pragma unroll
             for (int j = 0; j < 4; ++j) d.p[j] = mul2(mul2(both(scale), w.p[j]), mul2(dz[i].p[j], ny[i].p[j]));
-            if (p.gate_f32) store8<kAccess>(row_of<float>(p.dgate, row), col, n, pack<float>(d));
+            if (f32) store8<kAccess>(row_of<float>(p.dgate, row), col, n, pack<float>(d));
             else store8<kAccess>(row_of<T>(p.dgate, row), col, n, pack<T>(d));
           }
 #pragma unroll
@@ -498,7 +507,7 @@ __global__ void __launch_bounds__(kLong ? 1024 : 512) norm_bwd_kernel(const BwdP
         if (p.gate_f32) row_of<float>(p.dgate, row)[0] = scale * dot;
         else row_of<T>(p.dgate, row)[0] = from_float<T>(scale * dot);
       }
-      if (p.dy.p) {
+      if (wants_dy) {
         const float f = rstd1 * scale * row_gate, mean = dot * inv_n;
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
@@ -629,15 +638,20 @@ template <typename F, typename G> Shape backward_shape(long long rows, int n, bo
   return s;
 }
 
-template <typename T, int kMode, bool kKeep, bool kElement> int forward_ring(const Shape& s, const Params& p, dim3 grid, dim3 block, cudaStream_t stream) {
+template <typename T, int kMode, bool kKeep, int kElement> int forward_ring(const Shape& s, const Params& p, dim3 grid, dim3 block, cudaStream_t stream) {
   if (s.chunks == 2) return launch(norm_fwd_kernel<T, kMode, 2, kRing, kKeep, kElement>, grid, block, shared_of(s), p, stream);
   return launch(norm_fwd_kernel<T, kMode, 4, kRing, kKeep, kElement>, grid, block, shared_of(s), p, stream);
 }
 template <typename T, int kMode, bool kKeep> int forward_ring(const Shape& s, const Params& p, dim3 grid, dim3 block, cudaStream_t stream) {
   if constexpr (kMode != kPre) {
-    if (p.gate_kind == Gate::kElement) return forward_ring<T, kMode, kKeep, true>(s, p, grid, block, stream);
+    if (p.gate_kind == Gate::kElement) {
+      if constexpr (sizeof(T) == 2) {
+        if (p.gate_f32) return forward_ring<T, kMode, kKeep, kOfF32>(s, p, grid, block, stream);
+      }
+      return forward_ring<T, kMode, kKeep, kOfT>(s, p, grid, block, stream);
+    }
   }
-  return forward_ring<T, kMode, kKeep, false>(s, p, grid, block, stream);
+  return forward_ring<T, kMode, kKeep, kNone>(s, p, grid, block, stream);
 }
 template <typename T, int kMode> int forward_mode(bool vec, Params p, cudaStream_t stream) {
   int sms = 0;
@@ -664,25 +678,32 @@ inline int backward_held(int mode, int chunks) { return chunks * 2 * (mode == kP
 inline bool backward_raw(const BwdParams& p, int size) {
   return size == 2 && p.gate_kind != kColumn && !(p.w1 && p.w1_f32) && !(p.w2 && p.w2_f32);
 }
+template <typename T, int kMode, bool kKept, int kHeld> int backward_usual(dim3 grid, dim3 block, int shared, const BwdParams& p, cudaStream_t stream) {
+  if constexpr (kMode != kPre) {
+    if (p.gate_kind == Gate::kElement) {
+      if (sizeof(T) == 2 && p.gate_f32) return launch(norm_bwd_kernel<T, kMode, 2, kRing, kKept>, grid, block, shared, p, stream);
+      return launch(norm_bwd_kernel<T, kMode, 2, kRing, kKept, kHeld, kOfT>, grid, block, shared, p, stream);
+    }
+  }
+  return launch(norm_bwd_kernel<T, kMode, 2, kRing, kKept, kHeld, kNone>, grid, block, shared, p, stream);
+}
 template <typename T, int kMode, bool kKept> int backward_mode(const Shape& s, BwdParams p, cudaStream_t stream) {
   const dim3 grid((unsigned)s.blocks), block(s.threads, s.rows);
   if (s.threads > 512) {
-    if (s.form == kDirect) return launch(norm_bwd_kernel<T, kMode, 2, kDirect, kKept, true, true>, grid, block, shared_of(s), p, stream);
-    return launch(norm_bwd_kernel<T, kMode, 2, kScalar, kKept, true, true>, grid, block, shared_of(s), p, stream);
+    if (s.form == kDirect) return launch(norm_bwd_kernel<T, kMode, 2, kDirect, kKept, 0, kAsk, true>, grid, block, shared_of(s), p, stream);
+    return launch(norm_bwd_kernel<T, kMode, 2, kScalar, kKept, 0, kAsk, true>, grid, block, shared_of(s), p, stream);
   }
   if (s.form == kRing) {
     p.stages = s.stages;
     p.ring_words = s.words;
     p.held = s.held == 0 ? 0 : s.held == backward_held(kMode, s.chunks) ? 1 : 2;
     const int shared = shared_of(s);
-    if constexpr (kMode != kPre) {
-      if (p.gate_kind == Gate::kElement) {
-        if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kRing, kKept, true>, grid, block, shared, p, stream);
-        return launch(norm_bwd_kernel<T, kMode, 2, kRing, kKept, true>, grid, block, shared, p, stream);
-      }
+    if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kRing, kKept>, grid, block, shared, p, stream);
+    if (p.held == 0 || (kMode != kPre && !(p.dout.p && p.dy.p))) return launch(norm_bwd_kernel<T, kMode, 2, kRing, kKept>, grid, block, shared, p, stream);
+    if constexpr (sizeof(T) == 2) {
+      if (p.held == 2) return backward_usual<T, kMode, kKept, 2>(grid, block, shared, p, stream);
     }
-    if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kRing, kKept, false>, grid, block, shared, p, stream);
-    return launch(norm_bwd_kernel<T, kMode, 2, kRing, kKept, false>, grid, block, shared, p, stream);
+    return backward_usual<T, kMode, kKept, 1>(grid, block, shared, p, stream);
   }
   if (s.form == kDirect) {
     if (s.chunks == 1) return launch(norm_bwd_kernel<T, kMode, 1, kDirect, kKept>, grid, block, 0, p, stream);

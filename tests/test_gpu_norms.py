@@ -305,3 +305,35 @@ def test_refusals():
     g, = torch.autograd.grad(rms_norm(leaf, w).float().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.float().sum(), leaf)
+
+
+# Rows enough for blocks that walk over them, with every kind of call that has a kernel of its own.
+@pytest.mark.parametrize("rows,n", [(5000, 520), (700, 8192), (400, 8208), (5001, 232)])
+@pytest.mark.parametrize("mode,dtype,w,gate,scale,kept8,absent", [
+    ("post_pre", BF, BF, "element", "tensor", True, None), ("post_pre", BF, BF, "element", 0.5, False, None),
+    ("post_pre", BF, F32, "element", 0.5, False, None), ("post_pre", HF, F32, "element", "tensor", True, None),
+    ("post_pre", HF, HF, None, "tensor", False, "dout"), ("post_pre", BF, BF, "row", None, True, "dh"),
+    ("post_pre", F32, F32, "column", "tensor", False, None), ("post_pre", BF, BF, None, None, True, None),
+    ("post", F32, F32, "element", "tensor", True, None), ("post", BF, BF, "column", 0.5, False, None), ("post", HF, HF, "row", "tensor", True, None),
+    ("pre", HF, F32, None, None, True, None), ("pre", BF, BF, None, None, False, None), ("pre", F32, F32, None, None, True, None)])
+def test_many_rows_of_every_kind(rows, n, mode, dtype, w, gate, scale, kept8, absent):
+    c = _case(rows, n, dtype, gate, w, scale, seed=n + rows)
+    if absent:
+        c[absent] = None
+    got, grads = _train(mode, c, kept8)
+    _check_forward(mode, c, got)
+    if absent == "dh":
+        assert not grads.pop("w2").any()
+        mode, got = "post", got[0]
+    _check_backward(mode, c, got[0] if mode == "post_pre" else got, grads, kept8, rows)
+
+
+@pytest.mark.parametrize("kept8", [False, True])
+def test_many_rows_whose_first_norm_has_no_gradient(kept8):
+    c = _case(2000, 1024, BF, "element", BF, "tensor", seed=3)
+    names = ("x", "w1", "w2", "gate", "scale")
+    for name in names:
+        c[name] = c[name].requires_grad_(True)
+    out, h = _call("post_pre", c, kept8)
+    grads = torch.autograd.grad([out, h], [c[name] for name in names], [c["dout"], c["dh"]])
+    _check_backward("post_pre", c, out, dict(zip(names, grads)), kept8, 2000)
