@@ -109,12 +109,17 @@ __device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src) {
 __device__ __forceinline__ float sum2(float2 v) { return v.x + v.y; }
 
 // ---- forward -------------------------------------------------------------------------------------------
+// Threads of a multiprocessor for rows in a ring.  1024 have 64 registers each, which holds two eights of a row and of its weights: 16384 x
+// 4096 before a block 47 us.  `more` (8 bits or a gate per element) with both norms does not fit: 8192 x 8192 with a gate per
+// element takes 109 us with 512, 118 with 1024; one norm with 8 bits, 16384 x 4096 with its gradient, 231 with 512, 176 with 1024.
+constexpr int ring_threads(int mode, int chunks, bool more) { return chunks > 2 || (mode == kPostPre && more) ? 512 : 1024; }
 // A row stays in the registers of its threads, kChunks groups of eight columns for each, between the sums: memory is read once.
 // In a ring the weights (w1 times a gate per column, and w2) stay in registers too, and whether the inputs are kept in 8 bits (kKeep) and
 // what gate per element there is are known when the kernel is built: 8192 x 8192 with neither takes 95 us so, 110 where the kernel asks at
 // every row.  In the other forms it asks.
 template <typename T, int kMode, int kChunks, int kForm, bool kKeep = true, int kElement = kAsk>
-__global__ void __launch_bounds__(kForm != kScalar && kChunks <= 2 ? 1024 : 512) norm_fwd_kernel(const Params p) {
+__global__ void __launch_bounds__(kForm == kRing ? ring_threads(kMode, kChunks, kKeep || kElement != kNone) : kForm == kDirect && kChunks == 1 ? 1024 : 512)
+    norm_fwd_kernel(const Params p) {
   constexpr int kAccess = kForm == kScalar ? kStrided : kVector;
   constexpr bool kHeld = kForm == kRing && kChunks <= 2;
   constexpr int W = Raw8<T>::kWords, kX = kMode == kPre ? 0 : kChunks * W, kGate = kX + kChunks * W;
@@ -586,7 +591,7 @@ inline void ring_of(Shape& s, int words, int held, int blocks) {
 inline int shared_of(const Shape& s) { return (s.stages * s.words + s.held) * 16 * s.threads * s.rows; }
 
 // words(chunks): 16-byte words that a thread needs for one row.
-template <typename F> Shape forward_shape(long long rows, int n, bool vec, int sms, F words) {
+template <typename F, typename G> Shape forward_shape(long long rows, int n, bool vec, int sms, F words, G ring_threads) {
   const int eights = (n + 7) / 8;
   Shape s = {};
   auto divide = [&](int chunks, int block) {
@@ -597,9 +602,7 @@ template <typename F> Shape forward_shape(long long rows, int n, bool vec, int s
   };
   if (vec) {
     divide(eights > 1024 ? 4 : 2, 256);
-    // 64 registers a thread, some of the weights spilled: with 86 and half as many threads 16384 x 4096 takes 110 us for 104, 12000 x 5120,
-    // of which then one block fits, 144
-    const int per_sm = (s.chunks == 2 ? 1024 : 512) / (s.threads * s.rows);
+    const int per_sm = ring_threads(s.chunks) / (s.threads * s.rows);
     const long long most = (long long)sms * per_sm;
     ring_of(s, words(s.chunks), 0, per_sm);
     if (s.stages >= 2 && rows > 2 * most * s.rows) {
@@ -657,7 +660,8 @@ template <typename T, int kMode> int forward_mode(bool vec, Params p, cudaStream
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const int W = Raw8<T>::kWords, gate = p.gate_kind != kElement ? 0 : p.gate_f32 ? 2 : W;
-  const Shape s = forward_shape(p.rows, p.n, vec, sms, [&](int chunks) { return chunks * (W * (kMode == kPre ? 1 : 2) + gate); });
+  const Shape s = forward_shape(p.rows, p.n, vec, sms, [&](int chunks) { return chunks * (W * (kMode == kPre ? 1 : 2) + gate); },
+                                [&](int chunks) { return ring_threads(kMode, chunks, p.q1 || p.q2 || gate); });
   const dim3 grid((unsigned)s.blocks), block(s.threads, s.rows);
   if (s.form == kRing) {
     p.stages = s.stages;
