@@ -89,8 +89,7 @@ struct Ring {
   // The oldest of `stages` rows on their way has arrived.
   __device__ __forceinline__ void wait() const {
     if (stages == 2) ptx::cp_async_wait<1>();
-    else if (stages == 3) ptx::cp_async_wait<2>();
-    else ptx::cp_async_wait<3>();
+    else ptx::cp_async_wait<2>();
   }
   template <typename T> __device__ __forceinline__ void fetch8(int stage, int word, const T* from) const {
 #pragma unroll
@@ -581,12 +580,12 @@ template <typename K, typename P> int launch(K* kernel, dim3 grid, dim3 block, i
 }
 
 // The ring of a block that shares its multiprocessor with `blocks - 1` others: as many stages as fit beside `held` words of weights,
-// up to four.  Fewer than two: none.
+// up to three (16384 x 4096 with a gate per element: 106 us with three, 108 with four, 109 with six).  Fewer than two: none.
 inline void ring_of(Shape& s, int words, int held, int blocks) {
   s.words = words;
   s.held = held;
   s.stages = (kRingBytes / blocks / (16 * s.threads * s.rows) - held) / words;
-  if (s.stages > 4) s.stages = 4;
+  if (s.stages > 3) s.stages = 3;
 }
 inline int shared_of(const Shape& s) { return (s.stages * s.words + s.held) * 16 * s.threads * s.rows; }
 
