@@ -600,7 +600,8 @@ template <typename F, typename G> Shape forward_shape(long long rows, int n, boo
     if (s.rows > rows) s.rows = rows < 1 ? 1 : (int)rows;
   };
   if (vec) {
-    divide(eights > 1024 ? 4 : 2, 256);
+    // two eights a thread keep the weights in registers (4096 x 16384: 88 us for 153 with four); with 512 threads they end at 8192 columns
+    divide(eights > 1024 && ring_threads(2) == 512 ? 4 : 2, 256);
     const int per_sm = ring_threads(s.chunks) / (s.threads * s.rows);
     const long long most = (long long)sms * per_sm;
     ring_of(s, words(s.chunks), 0, per_sm);

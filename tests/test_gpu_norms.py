@@ -337,3 +337,10 @@ def test_many_rows_whose_first_norm_has_no_gradient(kept8):
     out, h = _call("post_pre", c, kept8)
     grads = torch.autograd.grad([out, h], [c[name] for name in names], [c["dout"], c["dh"]])
     _check_backward("post_pre", c, out, dict(zip(names, grads)), kept8, 2000)
+
+
+@pytest.mark.parametrize("n", [8200, 12288, 16384])
+@pytest.mark.parametrize("mode,dtype,w,gate", [("post_pre", BF, BF, "column"), ("post_pre", F32, F32, None), ("post", HF, F32, "element"), ("pre", BF, F32, None)])
+def test_many_long_rows(mode, dtype, w, gate, n):
+    c = _case(450, n, dtype, gate, w, 0.5, seed=n)
+    _check_forward(mode, c, _call(mode, c))
