@@ -75,6 +75,15 @@ enum Element : int { kNone = 0, kOfT = 1, kOfF32 = 2, kAsk = 3 };
 template <int kElement> __device__ __forceinline__ bool element_gate(int gate_kind) { return kElement == kAsk ? gate_kind == Gate::kElement : kElement != kNone; }
 template <int kElement> __device__ __forceinline__ bool element_f32(int gate_f32) { return kElement == kAsk ? gate_f32 : kElement == kOfF32; }
 
+__device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+// Through L1: the two halves of a sector of fp32 come with two copies, and the second finds it there.  One norm of 16384 x 4096 in fp32 takes
+// 103 us so, 129 past L1.
+__device__ __forceinline__ void cp_async_16_near(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // The words of a thread in one stage of the ring, [stage][word][thread].  A thread reads what it copied itself.
 struct Ring {
   uint4* mine;
@@ -93,7 +102,11 @@ struct Ring {
   }
   template <typename T> __device__ __forceinline__ void fetch8(int stage, int word, const T* from) const {
 #pragma unroll
-    for (int i = 0; i < Raw8<T>::kWords; ++i) ptx::cp_async_16(ptx::smem_u32(at(stage, word + i)), reinterpret_cast<const uint4*>(from) + i);
+    for (int i = 0; i < Raw8<T>::kWords; ++i) {
+      const uint32_t to = ptx::smem_u32(at(stage, word + i));
+      if constexpr (Raw8<T>::kWords == 1) ptx::cp_async_16(to, from);
+      else cp_async_16_near(to, reinterpret_cast<const uint4*>(from) + i);
+    }
   }
   template <typename T> __device__ __forceinline__ Vals get8(int stage, int word) const {
     Raw8<T> v;
@@ -102,9 +115,6 @@ struct Ring {
     return unpack(v);
   }
 };
-__device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ float sum2(float2 v) { return v.x + v.y; }
 
 // ---- forward -------------------------------------------------------------------------------------------
