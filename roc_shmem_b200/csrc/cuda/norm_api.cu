@@ -145,8 +145,8 @@ static int refuse_size() {
 }
 
 // out and h are contiguous; rstd: [rows], in kPostPre [2][rows] (y's, then out's), or null.  kept: q [norms][rows][n rounded up to 16],
-// then e [norms][rows][blocks of 128 columns], in the same order.  numbers: the bits of eps, and of a scale that is not
-// in memory above them.
+// then e [norms][rows][blocks of 128 columns], in the same order, 16-byte aligned and in whole 4-byte words.  numbers: the bits of eps,
+// and of a scale that is not in memory above them.
 int bshmem_norm_fwd(int what, const void* y, long long ldy, const void* x, long long ldx, void* out, void* h, const void* w1,
                     const void* w2, const void* gate, long long ldg, const void* scale, uint64_t numbers, void* rstd, void* kept,
                     long long rows, int n, void* stream) {
@@ -201,7 +201,8 @@ static void split_work(void* work, int mode, long long groups, int n, float*& w2
 }
 
 // The rows' part of a backward pass: dz (kPre, kPostPre), dy and the gradient of a gate per row or element.  Everything but z, y
-// and a gate per row is contiguous.  dout, dy and dgate may be null.
+// and a gate per row is contiguous.  dout, dy and dgate may be null.  kept: as bshmem_norm_fwd has it; exponents are read by the whole
+// 4-byte word that they are in, so up to three bytes behind the last one have to be there.
 int bshmem_norm_bwd(int what, const void* dout, const void* dh, const void* z, long long ldz, const void* y, long long ldy, const void* w1,
                     const void* w2, const void* gate, long long ldg, const void* scale, uint64_t scale_bits, const void* rstd, const void* kept,
                     int norms_kept, void* dz, void* dy, void* dgate, void* work, long long rows, int n, void* stream) {

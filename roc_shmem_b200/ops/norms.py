@@ -156,6 +156,11 @@ class _Call:
         self.what = what
 
 
+def kept_size(norms: int, rows: int, n: int) -> int:
+    """Bytes that a call of `norms` norms keeps in 8 bits: values, then exponents, which the backward pass reads in whole words."""
+    return (norms * kept_bytes(rows, n) + 3) // 4 * 4
+
+
 def _forward(c: _Call, mode: int, train: bool):
     """(out, h, rstd, kept); what the call does not give is None."""
     if _fwd is None:
@@ -168,7 +173,7 @@ def _forward(c: _Call, mode: int, train: bool):
         norms = 2 if mode == POST_PRE else 1
         rstd = torch.empty((norms, rows), dtype=_F32, device=like.device)
         if what & KEPT:
-            kept = like.new_empty((norms * kept_bytes(rows, n),), dtype=torch.uint8)
+            kept = like.new_empty((kept_size(norms, rows, n),), dtype=torch.uint8)
     else:
         what &= ~KEPT
     y, x = c.y, c.x

@@ -103,3 +103,22 @@ def test_modules_saved_before_there_were_checkpoints():
     assert Linear.__new__(Linear).checkpoint is False
     old = LlamaMLPModule.__new__(LlamaMLPModule)
     assert old.checkpoint is False and old.norms is False
+
+
+def test_kept_norms_hold_every_word_that_is_read(monkeypatch):
+    """The backward pass reads an exponent by the aligned word of four bytes that it is in, the last one's too: the buffer that the call
+    makes has them all."""
+    from types import SimpleNamespace
+
+    from roc_shmem_b200.ops import norms
+    monkeypatch.setattr(norms, "_fwd", lambda *_: 0)
+    monkeypatch.setattr(norms, "current_stream", lambda: 0)
+    for mode in (norms.PRE, norms.POST, norms.POST_PRE):
+        for rows in (1, 2, 3, 501):
+            for n in (8, 128, 136, 232, 520, 8200):
+                x = torch.empty(rows, n, dtype=torch.bfloat16)
+                c = SimpleNamespace(rows=rows, n=n, like=x, what=norms.KEPT, y=x, x=x, w1=None, w2=None, gate=None, gate_ld=0, scale=None, eps=1e-6, number=1.0)
+                kept = norms._forward(c, mode, True)[3]
+                count = 2 if mode == norms.POST_PRE else 1
+                last = count * rows * ((n + 15) // 16 * 16 + (n + 127) // 128) - 1
+                assert last // 4 * 4 + 4 <= kept.numel() < last + 5
