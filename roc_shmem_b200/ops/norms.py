@@ -11,6 +11,8 @@ element.  Every tensor has a gradient; sums over rows are added in a fixed order
 kept values.  Rows have 1 to 16384 columns and may be apart (any stride of the leading dimension); rows of a multiple of 8 columns on
 16-byte boundaries are the fast ones.  A backward pass that a CUDA graph captures wants every eager graph of the same leaves gone: torch
 keeps their gradients' accumulators as long, and with them the stream that they were made on.  Squares are fp32: rows whose squares leave its range give what that gives.
+Traced, compiled, fake and watched calls are the registered operators ``torch.ops.bshmem.norm`` and ``norm_backward``; there is no forward-mode
+derivative.
 
 The reference is a communication runtime without models, so there is no parity citation.
 """
@@ -26,11 +28,13 @@ import torch
 from .. import _native
 from .checkpoint8 import _TYPES, block_lib, kept_bytes, on_current_device
 from .gemm import current_stream
+from .watched import direct, direct_gradients
 
 PRE, POST, POST_PRE = range(3)
 NO_GATE, COLUMN, ROW, ELEMENT = range(4)
 MAX_COLUMNS = 16384
 KEPT = 1 << 12                                           # the call keeps its norms' inputs in 8 bits
+_NAMES = ("rms_norm", "post_norm", "post_pre_norm")
 _F32, _CONTIGUOUS, _new_like = torch.float32, torch.contiguous_format, torch.empty_like
 _declared = False
 _fwd = _bwd = _groups = _finish = None
@@ -186,14 +190,13 @@ def _forward(c: _Call, mode: int, train: bool):
     return out, h, rstd, kept
 
 
-def _backward(ctx, *grads):
-    w1, w2, gate, scale, rstd, a, b = ctx.saved_tensors
-    need_y, need_x, need_w1, need_w2, need_gate, need_scale = ctx.needs_input_grad[:6]
-    mode, what, n, rows, kind, number = ctx.call
-    dout = grads[0] if mode != PRE else None
-    dh = grads[-1] if mode != POST else None
+def _gradients(call, need, saved, dout, dh):
+    """Gradients of y, x, w1, w2, gate and scale, as far as `need` asks for them, from what _NormFn keeps."""
+    w1, w2, gate, scale, rstd, a, b = saved
+    need_y, need_x, need_w1, need_w2, need_gate, need_scale = need
+    mode, what, n, rows, kind, number = call
     if dout is None and dh is None:
-        return (None,) * 8
+        return (None,) * 6
     like = dout if dout is not None else dh
     dw_next = None
     if mode == POST_PRE and dh is None:                 # nobody used h: the first norm alone
@@ -203,7 +206,7 @@ def _backward(ctx, *grads):
     if rows == 0:
         return (torch.zeros_like(like) if need_y else None, torch.zeros_like(like) if need_x else None, torch.zeros_like(w1) if need_w1 else None,
                 dw_next if dw_next is not None else torch.zeros_like(w2) if need_w2 else None, torch.zeros_like(gate) if need_gate else None,
-                torch.zeros_like(scale) if need_scale else None, None, None)
+                torch.zeros_like(scale) if need_scale else None)
     if dout is not None and not dout.is_contiguous():
         dout = dout.contiguous()
     if dh is not None and not dh.is_contiguous():
@@ -236,7 +239,7 @@ def _backward(ctx, *grads):
     stream = current_stream()
     if mode != POST or dy is not None or sums or dgate is not None:
         st = _bwd(what, _p(dout), _p(dh), _p(z), 0 if z is None else z.stride(0), _p(y), 0 if y is None else y.stride(0), _p(w1), _p(w2),
-                  _p(gate_m), gate_ld, _p(scale), number, rstd.data_ptr(), _p(a) if kept8 else None, 2 if ctx.call[0] == POST_PRE else 1,
+                  _p(gate_m), gate_ld, _p(scale), number, rstd.data_ptr(), _p(a) if kept8 else None, 2 if call[0] == POST_PRE else 1,
                   _p(dz) if mode != POST else None, _p(dy), None if column else _p(dgate), _p(work), rows, n, stream)
         if st != 0:
             _check(st, "norm backward")
@@ -249,7 +252,15 @@ def _backward(ctx, *grads):
                      _p(dgate) if column else None, _p(dscale), rows, n, stream)
         if st != 0:
             _check(st, "norm backward")
-    return dy, dz if need_x else None, dw1, dw2 if dw_next is None else dw_next, dgate, dscale, None, None
+    return dy, dz if need_x else None, dw1, dw2 if dw_next is None else dw_next, dgate, dscale
+
+
+def _given(mode, grads):
+    return grads[0] if mode != PRE else None, grads[-1] if mode != POST else None
+
+
+def _backward(ctx, *grads):
+    return *_gradients(ctx.call, ctx.needs_input_grad[:6], ctx.saved_tensors, *_given(ctx.call[0], grads)), None, None
 
 
 _backward_once = torch.autograd.function.once_differentiable(_backward)
@@ -269,10 +280,104 @@ class _NormFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
+        mode, what = ctx.call[:2]
+        if not direct_gradients(_NAMES[mode], *grads):
+            number = struct.unpack("<f", struct.pack("<I", ctx.call[5]))[0]
+            return *_registered_gradients(mode, bool(what & KEPT), number, ctx.needs_input_grad[:6], ctx.saved_tensors, *_given(mode, grads)), None, None
         return _backward_once(ctx, *grads) if torch.is_grad_enabled() else _backward(ctx, *grads)
 
 
+# ---- registered operators: calls that somebody watches, traces or transforms ------------------------------------------------
+
+def _registered(name, mode, y, x, w1, w2, gate, scale, eps, checkpoint):
+    from . import torch_ops  # noqa: F401
+    number = 1.0
+    if scale is not None and not isinstance(scale, torch.Tensor):
+        scale, number = None, float(scale)
+    out, h, _, _ = torch.ops.bshmem.norm(y, x, w1, w2, gate, scale, number, float(eps), mode, bool(checkpoint))
+    return (out, h) if mode == POST_PRE else out if mode == POST else h
+
+
+def _registered_gradients(mode, checkpoint, number, need, saved, dout, dh):
+    from . import torch_ops  # noqa: F401
+    need = list(need)
+    if dout is None and dh is None:
+        return (None,) * 6
+    dx = dout if mode == POST and need[1] else None      # an operator may not return what it was given
+    need[1] = need[1] and mode != POST
+    found = torch.ops.bshmem.norm_backward(dout, dh, *saved, number, mode, checkpoint, need)
+    found = [g if wanted else None for g, wanted in zip(found, need)]
+    return found[0], found[1] if dx is None else dx, *found[2:]
+
+
+def _only_its_own(what, mode, w1, w2, gate, scale) -> None:
+    if (mode == PRE and not (w1 is gate is scale is None)) or (mode == POST and w2 is not None):
+        raise ValueError(f"{what}: operands that do not belong to the mode")
+
+
+def _whole_call(mode, y, x, w1, w2, gate, scale, number, eps, checkpoint) -> _Call:
+    if mode not in (PRE, POST, POST_PRE) or (y is None) != (mode == PRE):
+        raise ValueError("norm: unknown mode, or y does not belong to it")
+    _only_its_own("norm", mode, w1, w2, gate, scale)
+    return _Call(_NAMES[mode], mode, y, x, w1, w2, gate, number if scale is None else scale, eps, checkpoint)
+
+
+def operator_forward(y, x, w1, w2, gate, scale, number, eps, mode, checkpoint):
+    """torch.ops.bshmem.norm: (out, h, rstd, kept) of a call; what it does not have is empty."""
+    c = _whole_call(mode, y, x, w1, w2, gate, scale, number, eps, checkpoint)
+    with torch.cuda.device(x.device):
+        found = _forward(c, mode, True)
+    return tuple(x.new_empty(0) if t is None else t for t in found)
+
+
+def operator_forward_fake(y, x, w1, w2, gate, scale, number, eps, mode, checkpoint):
+    c = _whole_call(mode, y, x, w1, w2, gate, scale, number, eps, checkpoint)
+    norms = 2 if mode == POST_PRE else 1
+    return (_new_like(x, memory_format=_CONTIGUOUS) if mode != PRE else x.new_empty(0), _new_like(x, memory_format=_CONTIGUOUS) if mode != POST else x.new_empty(0),
+            x.new_empty((norms, c.rows), dtype=_F32),
+            x.new_empty((kept_size(norms, c.rows, c.n),), dtype=torch.uint8) if checkpoint else x.new_empty(0))
+
+
+def _whole_gradients(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need):
+    """The call that these belong to, checked: the kernels go by its sizes."""
+    like = dout if dout is not None else dh
+    if mode not in (PRE, POST, POST_PRE) or like is None or (mode == PRE and dout is not None) or (mode == POST and dh is not None) or len(need) != 6:
+        raise ValueError("norm_backward: unknown mode, or gradients that do not belong to it")
+    _only_its_own("norm_backward", mode, w1, w2, gate, scale)
+    y = like if mode != PRE else None
+    c = _Call("norm_backward", mode, y, like, w1, w2, gate, number if scale is None else scale, 1.0, checkpoint)
+    norms = 2 if mode == POST_PRE else 1
+    alike = [t for t in (dout, dh) if t is not None]
+    if checkpoint:
+        sized = a is not None and b is None and a.dtype is torch.uint8 and a.shape == (kept_size(norms, c.rows, c.n),) and a.is_contiguous()
+        sized = sized and a.get_device() == like.get_device()
+    else:
+        sized = (a is not None) == (mode != PRE) and (b is not None) == (mode != POST)
+        alike += [t for t in (a, b) if t is not None]
+    if not (sized and rstd.shape == (norms, c.rows) and rstd.dtype is _F32 and rstd.is_contiguous() and rstd.get_device() == like.get_device()
+            and all([t.shape == like.shape and t.dtype is like.dtype and t.get_device() == like.get_device() for t in alike])):
+        raise ValueError("norm_backward: these are not what a call of this form kept")
+    if any([wanted and t is None for wanted, t in zip(need, (y, like if mode != POST else None, w1, w2, gate, scale))]):
+        raise ValueError("norm_backward: a gradient of an operand that the call does not have")
+    return c
+
+
+def operator_backward(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need):
+    """torch.ops.bshmem.norm_backward: gradients of y, x, w1, w2, gate and scale; what `need` does not ask for is empty."""
+    c = _whole_gradients(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need)
+    with torch.cuda.device(rstd.device):
+        found = _gradients((mode, c.what, c.n, c.rows, c.kind, _bits(number)), need, (w1, w2, gate, scale, rstd, a, b), dout, dh)
+    return tuple(g if wanted else rstd.new_empty(0) for g, wanted in zip(found, need))
+
+
+def operator_backward_fake(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need):
+    c = _whole_gradients(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need)
+    return tuple(_new_like(t, memory_format=_CONTIGUOUS) if wanted else rstd.new_empty(0) for t, wanted in zip((c.like, c.like, w1, w2, gate, scale), need))
+
+
 def _run(name, mode, y, x, w1, w2, gate, scale, eps, checkpoint):
+    if not direct(name, y, x, w1, w2, gate, scale):
+        return _registered(name, mode, y, x, w1, w2, gate, scale, eps, checkpoint)
     c = _Call(name, mode, y, x, w1, w2, gate, scale, eps, checkpoint)
     if not on_current_device(x):
         with torch.cuda.device(x.device):

@@ -8,12 +8,15 @@ the fp8 kernel (forward only).  The reference has no PyTorch layer.
 """
 from __future__ import annotations
 
-import torch
-from torch.utils._device import DeviceContext
+from typing import Optional, Sequence
 
+import torch
+
+from . import norms
 from .checkpoint8 import Checkpoint8, restore, store
 from .gemm import gemm_bf16
 from .gemm_fp8 import gemm_fp8, quantize_act, quantize_weight
+from .watched import _PLAIN, _unwatched
 
 
 def _check_linear(x: torch.Tensor, w: torch.Tensor) -> None:
@@ -91,6 +94,49 @@ def _(x, w):
     return x.new_empty((x.shape[0], w.shape[0]))
 
 
+# ---- norms: what the calls of ops.norms are where somebody watches them -------------------------------------------
+
+_Optional = Optional[torch.Tensor]
+
+
+@torch.library.custom_op("bshmem::norm", mutates_args=())
+def norm(y: _Optional, x: torch.Tensor, w1: _Optional, w2: _Optional, gate: _Optional, scale: _Optional, number: float, eps: float, mode: int,
+         checkpoint: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return norms.operator_forward(y, x, w1, w2, gate, scale, number, eps, mode, checkpoint)
+
+
+norm.register_fake(norms.operator_forward_fake)
+
+
+@torch.library.custom_op("bshmem::norm_backward", mutates_args=())
+def norm_backward(dout: _Optional, dh: _Optional, w1: _Optional, w2: _Optional, gate: _Optional, scale: _Optional, rstd: torch.Tensor, a: _Optional,
+                  b: _Optional, number: float, mode: int, checkpoint: bool, need: Sequence[bool]) -> tuple[
+                      torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return norms.operator_backward(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need)
+
+
+norm_backward.register_fake(norms.operator_backward_fake)
+
+
+def _norm_setup(ctx, inputs, output):
+    y, x, w1, w2, gate, scale, number, _, mode, checkpoint = inputs
+    out, _, rstd, kept = output
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(rstd, kept)
+    a, b = (kept, None) if checkpoint else (y, x if mode == norms.PRE else None if mode == norms.POST else out)
+    ctx.save_for_backward(w1, w2, gate, scale, rstd, a, b)
+    ctx.call = mode, checkpoint, number
+
+
+def _norm_gradients(ctx, dout, dh, *_):
+    mode = ctx.call[0]
+    given = dout if mode != norms.PRE else None, dh if mode != norms.POST else None
+    return *norms._registered_gradients(*ctx.call, ctx.needs_input_grad[:6], ctx.saved_tensors, *given), None, None, None, None
+
+
+norm.register_autograd(_norm_gradients, setup_context=_norm_setup)
+
+
 class _LinearFn(torch.autograd.Function):
     """The same layer without the dispatcher: a custom operator costs 60 to 100 us of host time per call (fake-tensor
     and schema machinery), a training step of the layer makes three of them."""
@@ -131,18 +177,6 @@ class _LinearKeptFn(torch.autograd.Function):
         dx = gemm_bf16(dy, w.contiguous(), b_mn=True) if ctx.needs_input_grad[0] else None
         dw = gemm_bf16(dy, restore(Checkpoint8(*kept, ctx.shape, torch.bfloat16)), a_mn=True, b_mn=True) if ctx.needs_input_grad[1] else None
         return dx, dw
-
-
-_PLAIN = (torch.Tensor, torch.nn.Parameter)
-
-
-def _unwatched() -> bool:
-    """Nobody watches or rewrites operators: no compilation or tracing, no dispatch or function mode (fake tensors, make_fx,
-    counters; the one of a default device only adds an argument to factories), no functorch transform (vmap, grad, jvp)."""
-    C = torch._C
-    modes = C._len_torch_function_stack()
-    return (C._len_torch_dispatch_stack() == 0 and C._functorch.peek_interpreter_stack() is None and C._get_tracing_state() is None
-            and (modes == 0 or modes == 1 and type(C._get_function_stack_at(0)) is DeviceContext) and not torch.compiler.is_compiling())
 
 
 class Linear(torch.nn.Module):

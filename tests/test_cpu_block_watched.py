@@ -1,0 +1,179 @@
+"""Norms on anything but plain tensors that nobody watches: fake tensors, tracing, transforms, modes that see operators and
+forward-mode derivatives, with the formulas in the kernels' place.  Nothing there may reach a native entry, which would read addresses that
+are not there."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.autograd import forward_ad
+
+from roc_shmem_b200.ops import norms, torch_ops  # noqa: F401
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _native(*_):
+    pytest.fail("a native entry was reached")
+
+
+@pytest.fixture(autouse=True)
+def no_native(monkeypatch):
+    for entry in ("_fwd", "_bwd", "_groups", "_finish"):
+        monkeypatch.setattr(norms, entry, _native)
+
+
+def _n(v, eps):
+    return v * torch.rsqrt(v.pow(2).mean(-1, keepdim=True) + eps)
+
+
+@pytest.fixture
+def formulas(monkeypatch):
+    """The operators' own bodies on the CPU; the gradients are the norm's before a block."""
+    def forward(y, x, w1, w2, gate, scale, number, eps, mode, checkpoint):
+        one = lambda t: 1.0 if t is None else t  # noqa: E731
+        out = h = None
+        z = x
+        if mode != norms.PRE:
+            out = z = x + (number if scale is None else scale) * one(gate) * one(w1) * _n(y, eps)
+        if mode != norms.POST:
+            h = one(w2) * _n(z, eps)
+        return tuple(x.new_empty(0) if t is None else t for t in (out, h, x.new_full((1,), eps), None))
+
+    def backward(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need):
+        assert mode == norms.PRE
+        r = torch.rsqrt(b.pow(2).mean(-1, keepdim=True) + rstd[0])
+        n, t = b * r, dh * w2
+        found = (None, r * (t - n * (t * n).mean(-1, keepdim=True)), None, (dh * n).sum(0), None, None)
+        return tuple(f if n else dh.new_empty(0) for f, n in zip(found, need))
+    monkeypatch.setattr(norms, "operator_forward", forward)
+    monkeypatch.setattr(norms, "operator_backward", backward)
+
+
+def _fakes(*shapes, dtype=BF):
+    return [torch.empty(s, dtype=dtype, device="cuda") for s in shapes]
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_fake_norms_launch_nothing(checkpoint):
+    with FakeTensorMode():
+        x, y, w, g = _fakes((4, 6, 72), (4, 6, 72), (72,), (4, 6, 1))
+        h = norms.rms_norm(x, w, checkpoint=checkpoint)
+        out = norms.post_norm(y, x, w, gate=g, scale=0.5)
+        both = norms.post_pre_norm(y, x, w, w, checkpoint=checkpoint)
+        assert all(t.shape == x.shape and t.dtype is BF and t.device.type == "cuda" for t in (h, out, *both))
+        s = torch.ones(1, device="cuda")                         # the backward pass as autograd calls it (its engine asks for a GPU)
+        for mode, grads, need in ((norms.POST_PRE, (x, y), [True] * 6), (norms.POST_PRE, (x, None), [True] * 6),
+                                  (norms.POST, (x, None), [True, True, True, False, True, True]), (norms.PRE, (None, y), [False, True, False, True, False, False])):
+            operands = (y if mode != norms.PRE else None, x, w if mode != norms.PRE else None, w if mode != norms.POST else None,
+                        g if mode != norms.PRE else None, s if mode != norms.PRE else None)
+            _, _, rstd, kept = torch.ops.bshmem.norm(*operands, 1.0, 1e-6, mode, checkpoint)
+            saved = (*operands[2:], rstd, *((kept, None) if checkpoint else (operands[0], x if mode != norms.POST else None)))
+            found = norms._registered_gradients(mode, checkpoint, 1.0, need, saved, *grads)
+            assert [None if t is None else t.shape for t in found] == [t.shape if n else None for t, n in zip(operands, need)]
+        for bad in (lambda: norms.rms_norm(x, w[:71]), lambda: norms.post_norm(y[:3], x), lambda: norms.rms_norm(x, w.double()), lambda: norms.rms_norm(x, eps=0.0)):
+            with pytest.raises(ValueError):
+                bad()
+
+
+def _close(a, b):
+    assert torch.allclose(a, b, rtol=1e-5, atol=1e-6)
+
+
+def test_norms_are_traced(formulas):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, y, w = torch.randn(5, 8), torch.randn(5, 8), torch.randn(8)
+    cases = (lambda a, b: norms.rms_norm(a, w), lambda a, b: norms.post_norm(b, a, w, scale=0.5), lambda a, b: norms.post_pre_norm(b, a, w, w)[1])
+    expect = (w * _n(x, 1e-6), x + 0.5 * w * _n(y, 1e-6), w * _n(x + w * _n(y, 1e-6), 1e-6))
+    for f, e in zip(cases, expect):
+        for traced in (make_fx(f)(torch.zeros(5, 8), torch.zeros(5, 8)), torch.jit.trace(f, (torch.zeros(5, 8), torch.zeros(5, 8)), check_trace=False)):
+            assert "bshmem" in str(traced.graph) and "norm" in str(traced.graph)
+            _close(traced(x, y), e)
+
+
+def test_norms_with_gradients_are_traced(formulas):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def step(a, b):
+        a, b = a.detach().requires_grad_(True), b.detach().requires_grad_(True)
+        return torch.autograd.grad(norms.rms_norm(a, b), (a, b), torch.ones_like(a))
+    x, w = torch.randn(5, 8), torch.randn(8)
+    graph = make_fx(step)(torch.zeros(5, 8), torch.zeros(8))
+    assert "norm_backward" in str(graph.graph)
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    for got, e in zip(graph(x, w), torch.autograd.grad(b * _n(a, 1e-6), (a, b), torch.ones_like(a))):
+        _close(got, e)
+
+
+def test_transforms_and_modes(formulas):
+    from torch.utils._python_dispatch import TorchDispatchMode
+    x, w = torch.randn(3, 5, 8), torch.randn(8)
+    e = w * _n(x, 1e-6)
+    _close(torch.func.vmap(lambda v: norms.rms_norm(v, w))(x), e)
+    with pytest.raises(RuntimeError, match="functorch"):      # torch's own refusal of a registered operator's gradient there
+        torch.func.grad(lambda v: norms.rms_norm(v, w).pow(2).sum())(x)
+    seen = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+    with Watch():
+        _close(norms.rms_norm(x, w), e)
+    assert "bshmem.norm.default" in seen
+
+
+def test_no_forward_mode_derivative():
+    """A tangent is refused, not dropped; tensors without one pass on to the usual checks."""
+    x, w = torch.randn(5, 8), torch.randn(8)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        g = forward_ad.make_dual(w, torch.ones_like(w))
+        for call in (lambda: norms.rms_norm(d, w), lambda: norms.rms_norm(x, g), lambda: norms.post_norm(d, x), lambda: norms.post_norm(x, x, gate=d),
+                     lambda: norms.post_pre_norm(x, x, scale=forward_ad.make_dual(w[:1], w[:1]))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(ValueError, match="CUDA"):
+            norms.rms_norm(x, w)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda v: norms.rms_norm(v, w), (x,), (x,))
+
+
+def _graph(monkeypatch, x, w):
+    """A result of the direct call whose backward pass is still to come, with the formula in the kernel's place."""
+    def forward(c, mode, train):
+        return None, w.detach() * _n(x.detach(), 1e-6), torch.full((1,), 1e-6), None
+    monkeypatch.setattr(norms, "_forward", forward)
+    return norms._NormFn.apply(None, x, None, w, None, None, SimpleNamespace(what=2, n=8, rows=5, kind=norms.NO_GATE, number=1.0), norms.PRE)
+
+
+def test_watched_backward_of_a_direct_call(formulas, monkeypatch):
+    """The forward pass went past the dispatcher, the backward pass is batched, fake or of dual numbers."""
+    x, w = torch.randn(5, 8, requires_grad=True), torch.randn(8, requires_grad=True)
+    h = _graph(monkeypatch, x, w)
+    d = torch.randn(3, 5, 8)
+    got = torch.autograd.grad(h, (x, w), d, is_grads_batched=True, retain_graph=True)
+    e = [torch.autograd.grad(w * _n(x, 1e-6), (x, w), v) for v in d]
+    _close(got[0], torch.stack([v[0] for v in e]))
+    _close(got[1], torch.stack([v[1] for v in e]))
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.autograd.grad(h, x, forward_ad.make_dual(d[0], d[1]), retain_graph=True)
+
+
+def test_operators_refuse_what_does_not_belong_together():
+    with FakeTensorMode():
+        x, w = _fakes((4, 8), (8,))
+        r, two = torch.empty(1, 4, device="cuda"), torch.empty(2, 4, device="cuda")
+        op, back = torch.ops.bshmem.norm, torch.ops.bshmem.norm_backward
+        need = [False, True, False, False, False, False]
+        assert back(None, x, None, w, None, None, r, None, x, 1.0, norms.PRE, False, need)[1].shape == x.shape
+        for bad in (lambda: op(None, x, None, w, None, None, 1.0, 1e-6, 3, False), lambda: op(x, x, None, w, None, None, 1.0, 1e-6, norms.PRE, False),
+                    lambda: op(None, x, None, w, None, None, 1.0, 1e-6, norms.POST, False), lambda: op(None, x, w, w, None, None, 1.0, 1e-6, norms.PRE, False),
+                    lambda: back(None, x, None, w, None, None, two, None, x, 1.0, norms.PRE, False, need),
+                    lambda: back(None, x, None, w, None, None, r, None, x[:3], 1.0, norms.PRE, False, need),
+                    lambda: back(None, x, None, w, None, None, r, x, None, 1.0, norms.PRE, True, need),
+                    lambda: back(x, x, None, w, None, None, r, None, x, 1.0, norms.PRE, False, need),
+                    lambda: back(None, None, None, w, None, None, r, None, x, 1.0, norms.PRE, False, need),
+                    lambda: back(None, x, None, None, None, None, r, None, x, 1.0, norms.PRE, False, [False, True, False, True, False, False])):
+            with pytest.raises(ValueError):
+                bad()
