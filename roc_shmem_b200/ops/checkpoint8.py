@@ -3,7 +3,9 @@
 An activation that is only read again for a gradient is stored as e4m3 with one power of two per row and 128 columns:
 half the bytes of bf16, and a relative error of at most 2^-4 for values down to 2^-13 of their block's largest.  ``store``
 and ``restore`` are the way there and back; ``swiglu`` is the gated activation that keeps its input so; ``Linear`` and the norms
-take ``checkpoint=True``.  Values that e4m3 does not have come back as NaN (infinities too).
+take ``checkpoint=True``.  Values that e4m3 does not have come back as NaN (infinities too).  No gradient goes through ``store`` and
+``restore``.  Traced, compiled, fake and watched calls are the registered operators ``torch.ops.bshmem.store8``, ``restore8``, ``swiglu8`` and
+``swiglu8_backward``; there is no forward-mode derivative.
 
 The reference is a communication runtime without activations, so there is no parity citation.
 """
@@ -16,7 +18,8 @@ from typing import Optional
 import torch
 
 from .. import _native
-from .gemm import _raw_stream, current_stream
+from .gemm import current_stream
+from .watched import direct, direct_gradients
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _declared = False
@@ -98,13 +101,22 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     return m if m.stride(1) == 1 else m.contiguous()
 
 
-def _held(kept: Checkpoint8, what: str) -> tuple[torch.Tensor, int, int]:
-    """(bytes, rows, columns) of `kept`, whose shape says what the kernels write."""
+def _sized(kept: Checkpoint8, what: str) -> tuple[int, int]:
+    """Rows and columns of `kept`, whose shape says what the kernels write."""
     data, shape = kept.data, kept.shape
     cols = shape[-1] if shape else 0
     rows = shape.numel() // cols if cols else 0
-    if not cols or data.numel() != kept_bytes(rows, cols) or data.dtype is not torch.uint8 or not data.is_contiguous() or data.data_ptr() % 16:
+    if not cols or data.numel() != kept_bytes(rows, cols) or data.dtype is not torch.uint8 or not data.is_contiguous():
         raise ValueError(f"{what}: the checkpoint does not hold a {tuple(shape)}")
+    return rows, cols
+
+
+def _held(kept: Checkpoint8, what: str) -> tuple[torch.Tensor, int, int]:
+    """(bytes, rows, columns) of `kept`."""
+    rows, cols = _sized(kept, what)
+    data = kept.data
+    if data.data_ptr() % 16:
+        raise ValueError(f"{what}: the checkpoint does not hold a {tuple(kept.shape)}")
     if not data.is_cuda:
         raise ValueError(f"{what} needs a checkpoint of a CUDA tensor, got one on {data.device}")
     return data, rows, cols
@@ -112,10 +124,16 @@ def _held(kept: Checkpoint8, what: str) -> tuple[torch.Tensor, int, int]:
 
 def store(x: torch.Tensor) -> Checkpoint8:
     """bf16, fp16 or fp32 [..., columns] → 8 bits."""
+    if not direct("store", x):
+        return Checkpoint8(_operators().store8(x), x.shape, x.dtype)
+    return Checkpoint8(store_direct(x), x.shape, x.dtype)
+
+
+def store_direct(x: torch.Tensor) -> torch.Tensor:
     m = _rows(x, "store")
     if not on_current_device(x):
         with torch.cuda.device(x.device):
-            return store(x)
+            return store_direct(x)
     if _store is None:
         _lib()
     rows, cols = m.shape
@@ -123,26 +141,45 @@ def store(x: torch.Tensor) -> Checkpoint8:
     st = _store(_TYPES[x.dtype], m.data_ptr(), m.stride(0), data.data_ptr(), rows, cols, current_stream())
     if st != 0:
         _check(st, "store")
-    return Checkpoint8(data, x.shape, x.dtype)
+    return data
 
 
 def restore(kept: Checkpoint8, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The stored values in `dtype` (default: what was stored), into `out` if given ([rows, columns] with columns side by side)."""
     dtype = dtype or (out.dtype if out is not None else kept.dtype)
-    data, rows, cols = _held(kept, "restore")
+    if direct("restore", kept.data, out):
+        return restore_direct(kept, dtype, out)
+    _check_dtype(dtype)
+    rows, cols = _sized(kept, "restore")
+    if out is not None:
+        _check_out(out, rows, cols, dtype, kept.data)
+    got = _operators().restore8(kept.data, cols, dtype)
+    return got.view(kept.shape) if out is None else out.copy_(got)
+
+
+def _check_dtype(dtype: torch.dtype) -> None:
     if dtype not in _TYPES:
         raise ValueError(f"restore gives bf16, fp16 or fp32, not {dtype}")
+
+
+def _check_out(out: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, data: torch.Tensor) -> None:
+    if out.shape != (rows, cols) or out.dtype != dtype or out.device != data.device or out.stride(1) != 1 or (rows > 1 and out.stride(0) < cols):
+        raise ValueError("bad output tensor")
+
+
+def restore_direct(kept: Checkpoint8, dtype: torch.dtype, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    data, rows, cols = _held(kept, "restore")
+    _check_dtype(dtype)
     if not on_current_device(data):
         with torch.cuda.device(data.device):
-            return restore(kept, dtype, out)
+            return restore_direct(kept, dtype, out)
     if _restore is None:
         _lib()
     if out is None:
         out = data.new_empty(kept.shape, dtype=dtype)
         ld = cols
     else:
-        if out.shape != (rows, cols) or out.dtype != dtype or out.device != data.device or out.stride(1) != 1 or (rows > 1 and out.stride(0) < cols):
-            raise ValueError("bad output tensor")
+        _check_out(out, rows, cols, dtype, data)
         ld = out.stride(0)
     st = _restore(_TYPES[dtype], data.data_ptr(), out.data_ptr(), ld, rows, cols, current_stream())
     if st != 0:
@@ -181,7 +218,7 @@ def _swiglu_forward(gu: torch.Tensor, keep: bool) -> tuple[torch.Tensor, Optiona
 def swiglu_store(gu: torch.Tensor) -> tuple[torch.Tensor, Checkpoint8]:
     """act [..., F] = silu(gate) * up of gu [..., 2F] (32 columns of the gate, then the 32 of ``up``, see
     ``interleave_gate_up``), and gu in 8 bits, in one pass."""
-    act, data = _swiglu_forward(gu, True)
+    act, data = _swiglu_forward(gu, True) if direct("swiglu_store", gu) else _operators().swiglu8(gu.detach(), True)
     return act, Checkpoint8(data, gu.shape, gu.dtype)
 
 
@@ -189,15 +226,36 @@ def swiglu_backward(kept: Checkpoint8, dact: torch.Tensor, *, act: bool = False,
                     act_out: Optional[torch.Tensor] = None):
     """Gradient of gu from its 8 bits and the activation's gradient; with `act` also the activation again, of the same 8 bits (what
     the next layer's weight gradient reads).  `dgu_out`, `act_out`: contiguous buffers for them."""
-    shape = kept.shape
+    act = act or act_out is not None
+    if direct("swiglu_backward", kept.data, dact, dgu_out, act_out):
+        return swiglu_backward_direct(kept, dact, act, dgu_out, act_out)
+    _check_dact(kept, _sized(kept, "swiglu_backward")[1], dact)
+    for given, like in ((dgu_out, kept.shape), (act_out, dact.shape)):
+        if given is not None:
+            _check_buffer(given, like, dact)
+    dgu, again = _operators().swiglu8_backward(kept.data, dact, act)
+    dgu = dgu if dgu_out is None else dgu_out.copy_(dgu)
+    return (dgu, again if act_out is None else act_out.copy_(again)) if act else dgu
+
+
+def _check_dact(kept: Checkpoint8, cols: int, dact: torch.Tensor) -> None:
+    like = (*kept.shape[:-1], cols // 2)
+    if cols % 64 or dact.dtype is not torch.bfloat16 or dact.shape != like or dact.get_device() != kept.data.get_device():
+        raise ValueError(f"swiglu_backward: a bf16 gradient of {like} belongs to this checkpoint, got {dact.dtype} {tuple(dact.shape)}")
+
+
+def _check_buffer(given: torch.Tensor, like: torch.Size, d: torch.Tensor) -> None:
+    if given.shape != like or given.dtype is not torch.bfloat16 or given.device != d.device or not given.is_contiguous():
+        raise ValueError("bad output tensor")
+
+
+def swiglu_backward_direct(kept: Checkpoint8, dact: torch.Tensor, act: bool, dgu_out: Optional[torch.Tensor] = None,
+                           act_out: Optional[torch.Tensor] = None):
     data, rows, cols = _held(kept, "swiglu_backward")
     if not on_current_device(data):
         with torch.cuda.device(data.device):
-            return swiglu_backward(kept, dact, act=act, dgu_out=dgu_out, act_out=act_out)
-    F = cols // 2
-    bf = torch.bfloat16
-    if cols % 64 or dact.dtype is not bf or dact.shape != (*shape[:-1], F) or dact.get_device() != data.get_device():
-        raise ValueError(f"swiglu_backward: a bf16 gradient of {(*shape[:-1], F)} belongs to this checkpoint, got {dact.dtype} {tuple(dact.shape)}")
+            return swiglu_backward_direct(kept, dact, act, dgu_out, act_out)
+    _check_dact(kept, cols, dact)
     if _swiglu_backward is None:
         _lib()
     d = _aligned(dact)
@@ -205,12 +263,14 @@ def swiglu_backward(kept: Checkpoint8, dact: torch.Tensor, *, act: bool = False,
     def buffer(given, like):
         if given is None:
             return d.new_empty(like)
-        if given.shape != like or given.dtype is not bf or given.device != d.device or not given.is_contiguous() or given.data_ptr() % 16:
+        _check_buffer(given, like, d)
+        if given.data_ptr() % 16:
             raise ValueError("bad output tensor")
         return given
-    dgu = buffer(dgu_out, shape)
-    again = buffer(act_out, dact.shape) if act or act_out is not None else None
-    st = _swiglu_backward(data.data_ptr(), d.data_ptr(), dgu.data_ptr(), None if again is None else again.data_ptr(), rows, F, current_stream())
+    dgu = buffer(dgu_out, kept.shape)
+    again = buffer(act_out, dact.shape) if act else None
+    st = _swiglu_backward(data.data_ptr(), d.data_ptr(), dgu.data_ptr(), None if again is None else again.data_ptr(), rows, cols // 2,
+                          current_stream())
     if st != 0:
         _check(st, "swiglu_backward")
     return dgu if again is None else (dgu, again)
@@ -219,19 +279,79 @@ def swiglu_backward(kept: Checkpoint8, dact: torch.Tensor, *, act: bool = False,
 class _SwigluFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gu):
-        act, kept = swiglu_store(gu)
-        ctx.save_for_backward(kept.data)
+        act, data = _swiglu_forward(gu, True)
+        ctx.save_for_backward(data)
         ctx.shape = gu.shape
         return act
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dact):
-        return swiglu_backward(Checkpoint8(*ctx.saved_tensors, ctx.shape, torch.bfloat16), dact)
+        data, = ctx.saved_tensors
+        if not direct_gradients("swiglu", dact):
+            return _operators().swiglu8_backward(data, dact, False)[0]
+        return swiglu_backward_direct(Checkpoint8(data, ctx.shape, torch.bfloat16), dact, False)
 
 
 def swiglu(gu: torch.Tensor) -> torch.Tensor:
     """silu(gate) * up of the interleaved gu [..., 2F]; what the gradient needs of gu is kept in 8 bits."""
-    if torch.is_grad_enabled() and gu.requires_grad:
-        return _SwigluFn.apply(gu)
-    return _swiglu_forward(gu, False)[0]
+    train = torch.is_grad_enabled() and gu.requires_grad
+    if not direct("swiglu", gu):
+        return _operators().swiglu8(gu, train)[0]
+    return _SwigluFn.apply(gu) if train else _swiglu_forward(gu, False)[0]
+
+
+# ---- registered operators: calls that somebody watches, traces or transforms ------------------------------------------------
+
+def _operators():
+    from . import torch_ops  # noqa: F401
+    return torch.ops.bshmem
+
+
+def operator_store_fake(x):
+    rows, cols = _rows(x, "store").shape
+    return x.new_empty((kept_bytes(rows, cols),), dtype=torch.uint8)
+
+
+def _kept_rows(data, cols, dtype):
+    if cols < 1 or data.numel() % kept_bytes(1, cols):
+        raise ValueError(f"restore8: the checkpoint does not hold rows of {cols}")
+    return Checkpoint8(data, torch.Size((data.numel() // kept_bytes(1, cols), cols)), dtype)
+
+
+def operator_restore(data, cols, dtype):
+    return restore_direct(_kept_rows(data, cols, dtype), dtype)
+
+
+def operator_restore_fake(data, cols, dtype):
+    _check_dtype(dtype)
+    return data.new_empty(_kept_rows(data, cols, dtype).shape, dtype=dtype)
+
+
+def operator_swiglu(gu, keep):
+    act, data = _swiglu_forward(gu, keep)
+    return act, gu.new_empty((0,), dtype=torch.uint8) if data is None else data
+
+
+def operator_swiglu_fake(gu, keep):
+    _check_gu(gu)
+    cols = gu.shape[-1]
+    size = kept_bytes(gu.numel() // cols, cols) if keep else 0
+    return gu.new_empty((*gu.shape[:-1], cols // 2)), gu.new_empty((size,), dtype=torch.uint8)
+
+
+def _kept_gu(data, dact):
+    if dact.dim() < 1:
+        raise ValueError("swiglu8_backward needs rows")
+    return Checkpoint8(data, torch.Size((*dact.shape[:-1], 2 * dact.shape[-1])), torch.bfloat16)
+
+
+def operator_swiglu_backward(data, dact, act):
+    got = swiglu_backward_direct(_kept_gu(data, dact), dact, act)
+    return got if act else (got, dact.new_empty((0,)))
+
+
+def operator_swiglu_backward_fake(data, dact, act):
+    kept = _kept_gu(data, dact)
+    _check_dact(kept, _sized(kept, "swiglu_backward")[1], dact)
+    return dact.new_empty(kept.shape), dact.new_empty(dact.shape if act else (0,))

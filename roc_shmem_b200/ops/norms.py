@@ -305,7 +305,7 @@ def _registered_gradients(mode, checkpoint, number, need, saved, dout, dh):
         return (None,) * 6
     dx = dout if mode == POST and need[1] else None      # an operator may not return what it was given
     need[1] = need[1] and mode != POST
-    found = torch.ops.bshmem.norm_backward(dout, dh, *saved, number, mode, checkpoint, need)
+    found = torch.ops.bshmem.norm_backward(dout, dh, *saved, number, mode, checkpoint, sum(1 << i for i, wanted in enumerate(need) if wanted))
     found = [g if wanted else None for g, wanted in zip(found, need)]
     return found[0], found[1] if dx is None else dx, *found[2:]
 
@@ -338,10 +338,14 @@ def operator_forward_fake(y, x, w1, w2, gate, scale, number, eps, mode, checkpoi
             x.new_empty((kept_size(norms, c.rows, c.n),), dtype=torch.uint8) if checkpoint else x.new_empty(0))
 
 
+def _asked(need: int) -> list[bool]:
+    return [bool(need >> i & 1) for i in range(6)]
+
+
 def _whole_gradients(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need):
     """The call that these belong to, checked: the kernels go by its sizes."""
     like = dout if dout is not None else dh
-    if mode not in (PRE, POST, POST_PRE) or like is None or (mode == PRE and dout is not None) or (mode == POST and dh is not None) or len(need) != 6:
+    if mode not in (PRE, POST, POST_PRE) or like is None or (mode == PRE and dout is not None) or (mode == POST and dh is not None) or not 0 <= need < 64:
         raise ValueError("norm_backward: unknown mode, or gradients that do not belong to it")
     _only_its_own("norm_backward", mode, w1, w2, gate, scale)
     y = like if mode != PRE else None
@@ -357,22 +361,22 @@ def _whole_gradients(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, ch
     if not (sized and rstd.shape == (norms, c.rows) and rstd.dtype is _F32 and rstd.is_contiguous() and rstd.get_device() == like.get_device()
             and all([t.shape == like.shape and t.dtype is like.dtype and t.get_device() == like.get_device() for t in alike])):
         raise ValueError("norm_backward: these are not what a call of this form kept")
-    if any([wanted and t is None for wanted, t in zip(need, (y, like if mode != POST else None, w1, w2, gate, scale))]):
+    if any([wanted and t is None for wanted, t in zip(_asked(need), (y, like if mode != POST else None, w1, w2, gate, scale))]):
         raise ValueError("norm_backward: a gradient of an operand that the call does not have")
     return c
 
 
 def operator_backward(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need):
-    """torch.ops.bshmem.norm_backward: gradients of y, x, w1, w2, gate and scale; what `need` does not ask for is empty."""
+    """torch.ops.bshmem.norm_backward: gradients of y, x, w1, w2, gate and scale; what the bits of `need` do not ask for is empty."""
     c = _whole_gradients(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need)
     with torch.cuda.device(rstd.device):
-        found = _gradients((mode, c.what, c.n, c.rows, c.kind, _bits(number)), need, (w1, w2, gate, scale, rstd, a, b), dout, dh)
-    return tuple(g if wanted else rstd.new_empty(0) for g, wanted in zip(found, need))
+        found = _gradients((mode, c.what, c.n, c.rows, c.kind, _bits(number)), _asked(need), (w1, w2, gate, scale, rstd, a, b), dout, dh)
+    return tuple(g if wanted else rstd.new_empty(0) for g, wanted in zip(found, _asked(need)))
 
 
 def operator_backward_fake(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need):
     c = _whole_gradients(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need)
-    return tuple(_new_like(t, memory_format=_CONTIGUOUS) if wanted else rstd.new_empty(0) for t, wanted in zip((c.like, c.like, w1, w2, gate, scale), need))
+    return tuple(_new_like(t, memory_format=_CONTIGUOUS) if wanted else rstd.new_empty(0) for t, wanted in zip((c.like, c.like, w1, w2, gate, scale), _asked(need)))
 
 
 def _run(name, mode, y, x, w1, w2, gate, scale, eps, checkpoint):

@@ -8,15 +8,15 @@ the fp8 kernel (forward only).  The reference has no PyTorch layer.
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence
+from typing import Optional
 
 import torch
 
-from . import norms
-from .checkpoint8 import Checkpoint8, restore, store
+from . import checkpoint8, norms
+from .checkpoint8 import Checkpoint8
 from .gemm import gemm_bf16
 from .gemm_fp8 import gemm_fp8, quantize_act, quantize_weight
-from .watched import _PLAIN, _unwatched
+from .watched import _PLAIN, _unwatched, direct_gradients
 
 
 def _check_linear(x: torch.Tensor, w: torch.Tensor) -> None:
@@ -110,7 +110,7 @@ norm.register_fake(norms.operator_forward_fake)
 
 @torch.library.custom_op("bshmem::norm_backward", mutates_args=())
 def norm_backward(dout: _Optional, dh: _Optional, w1: _Optional, w2: _Optional, gate: _Optional, scale: _Optional, rstd: torch.Tensor, a: _Optional,
-                  b: _Optional, number: float, mode: int, checkpoint: bool, need: Sequence[bool]) -> tuple[
+                  b: _Optional, number: float, mode: int, checkpoint: bool, need: int) -> tuple[
                       torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     return norms.operator_backward(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need)
 
@@ -135,6 +135,46 @@ def _norm_gradients(ctx, dout, dh, *_):
 
 
 norm.register_autograd(_norm_gradients, setup_context=_norm_setup)
+
+
+# ---- activations in 8 bits, the same way -----------------------------------------------------------------------------
+
+@torch.library.custom_op("bshmem::store8", mutates_args=())
+def store8(x: torch.Tensor) -> torch.Tensor:
+    return checkpoint8.store_direct(x)
+
+
+@torch.library.custom_op("bshmem::restore8", mutates_args=())
+def restore8(data: torch.Tensor, cols: int, dtype: torch.dtype) -> torch.Tensor:
+    return checkpoint8.operator_restore(data, cols, dtype)
+
+
+@torch.library.custom_op("bshmem::swiglu8", mutates_args=())
+def swiglu8(gu: torch.Tensor, keep: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return checkpoint8.operator_swiglu(gu, keep)
+
+
+@torch.library.custom_op("bshmem::swiglu8_backward", mutates_args=())
+def swiglu8_backward(data: torch.Tensor, dact: torch.Tensor, act: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return checkpoint8.operator_swiglu_backward(data, dact, act)
+
+
+store8.register_fake(checkpoint8.operator_store_fake)
+restore8.register_fake(checkpoint8.operator_restore_fake)
+swiglu8.register_fake(checkpoint8.operator_swiglu_fake)
+swiglu8_backward.register_fake(checkpoint8.operator_swiglu_backward_fake)
+
+
+def _swiglu_setup(ctx, inputs, output):
+    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(output[1])
+
+
+def _swiglu_gradient(ctx, dact, _):
+    return torch.ops.bshmem.swiglu8_backward(*ctx.saved_tensors, dact, False)[0], None
+
+
+swiglu8.register_autograd(_swiglu_gradient, setup_context=_swiglu_setup)
 
 
 class _LinearFn(torch.autograd.Function):
@@ -164,8 +204,7 @@ class _LinearKeptFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w):
         _check_linear(x, w)
-        kept = store(x) if ctx.needs_input_grad[1] else None
-        ctx.save_for_backward(w, *(() if kept is None else (kept.data,)))
+        ctx.save_for_backward(w, *((checkpoint8.store_direct(x),) if ctx.needs_input_grad[1] else ()))
         ctx.shape = x.shape
         return gemm_bf16(x.contiguous(), w.contiguous())
 
@@ -173,10 +212,17 @@ class _LinearKeptFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         w, *kept = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad
+        if not direct_gradients("linear", dy):
+            ops = torch.ops.bshmem
+            return (ops.linear_dgrad(dy, w) if need_x else None,
+                    ops.linear_wgrad(dy, ops.restore8(*kept, ctx.shape[1], torch.bfloat16)) if need_w else None)
         dy = dy.contiguous()
-        dx = gemm_bf16(dy, w.contiguous(), b_mn=True) if ctx.needs_input_grad[0] else None
-        dw = gemm_bf16(dy, restore(Checkpoint8(*kept, ctx.shape, torch.bfloat16)), a_mn=True, b_mn=True) if ctx.needs_input_grad[1] else None
-        return dx, dw
+        dx = gemm_bf16(dy, w.contiguous(), b_mn=True) if need_x else None
+        if not need_w:
+            return dx, None
+        x = checkpoint8.restore_direct(Checkpoint8(*kept, ctx.shape, torch.bfloat16), torch.bfloat16)
+        return dx, gemm_bf16(dy, x, a_mn=True, b_mn=True)
 
 
 class Linear(torch.nn.Module):

@@ -1,4 +1,4 @@
-"""Norms on anything but plain tensors that nobody watches: fake tensors, tracing, transforms, modes that see operators and
+"""Norms and 8-bit activations on anything but plain tensors that nobody watches: fake tensors, tracing, transforms, modes that see operators and
 forward-mode derivatives, with the formulas in the kernels' place.  Nothing there may reach a native entry, which would read addresses that
 are not there."""
 from types import SimpleNamespace
@@ -8,7 +8,7 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
 
-from roc_shmem_b200.ops import norms, torch_ops  # noqa: F401
+from roc_shmem_b200.ops import checkpoint8, norms, torch_ops  # noqa: F401
 
 BF, F32 = torch.bfloat16, torch.float32
 
@@ -21,6 +21,8 @@ def _native(*_):
 def no_native(monkeypatch):
     for entry in ("_fwd", "_bwd", "_groups", "_finish"):
         monkeypatch.setattr(norms, entry, _native)
+    for entry in ("_store", "_restore", "_swiglu_store", "_swiglu_backward"):
+        monkeypatch.setattr(checkpoint8, entry, _native)
 
 
 def _n(v, eps):
@@ -45,7 +47,7 @@ def formulas(monkeypatch):
         r = torch.rsqrt(b.pow(2).mean(-1, keepdim=True) + rstd[0])
         n, t = b * r, dh * w2
         found = (None, r * (t - n * (t * n).mean(-1, keepdim=True)), None, (dh * n).sum(0), None, None)
-        return tuple(f if n else dh.new_empty(0) for f, n in zip(found, need))
+        return tuple(f if n else dh.new_empty(0) for f, n in zip(found, norms._asked(need)))
     monkeypatch.setattr(norms, "operator_forward", forward)
     monkeypatch.setattr(norms, "operator_backward", backward)
 
@@ -165,7 +167,7 @@ def test_operators_refuse_what_does_not_belong_together():
         x, w = _fakes((4, 8), (8,))
         r, two = torch.empty(1, 4, device="cuda"), torch.empty(2, 4, device="cuda")
         op, back = torch.ops.bshmem.norm, torch.ops.bshmem.norm_backward
-        need = [False, True, False, False, False, False]
+        need = 2
         assert back(None, x, None, w, None, None, r, None, x, 1.0, norms.PRE, False, need)[1].shape == x.shape
         for bad in (lambda: op(None, x, None, w, None, None, 1.0, 1e-6, 3, False), lambda: op(x, x, None, w, None, None, 1.0, 1e-6, norms.PRE, False),
                     lambda: op(None, x, None, w, None, None, 1.0, 1e-6, norms.POST, False), lambda: op(None, x, w, w, None, None, 1.0, 1e-6, norms.PRE, False),
@@ -174,6 +176,70 @@ def test_operators_refuse_what_does_not_belong_together():
                     lambda: back(None, x, None, w, None, None, r, x, None, 1.0, norms.PRE, True, need),
                     lambda: back(x, x, None, w, None, None, r, None, x, 1.0, norms.PRE, False, need),
                     lambda: back(None, None, None, w, None, None, r, None, x, 1.0, norms.PRE, False, need),
-                    lambda: back(None, x, None, None, None, None, r, None, x, 1.0, norms.PRE, False, [False, True, False, True, False, False])):
+                    lambda: back(None, x, None, None, None, None, r, None, x, 1.0, norms.PRE, False, 2 | 8)):
             with pytest.raises(ValueError):
                 bad()
+
+
+def test_fake_eight_bits_launch_nothing():
+    from roc_shmem_b200.ops.checkpoint8 import kept_bytes, restore, store, swiglu, swiglu_backward, swiglu_store
+    with FakeTensorMode():
+        x, gu, d = _fakes((3, 5, 200), (3, 5, 192), (3, 5, 96))
+        kept = store(x)
+        assert kept.data.shape == (kept_bytes(15, 200),) and kept.shape == x.shape and kept.dtype is BF
+        assert restore(kept).shape == x.shape and restore(kept, F32).dtype is F32 and kept.restore().dtype is BF
+        out = torch.empty(15, 300, device="cuda")[:, 4:204]
+        assert restore(kept, out=out) is out
+        act, kept = swiglu_store(gu)
+        assert act.shape == d.shape and kept.data.shape == (kept_bytes(15, 192),)
+        dgu, again = swiglu_backward(kept, d, act=True)
+        assert dgu.shape == gu.shape and again.shape == d.shape and swiglu_backward(kept, d, dgu_out=gu) is gu
+        assert swiglu_backward(kept, d, act_out=d)[1] is d
+        assert swiglu(gu).shape == d.shape and swiglu(gu.requires_grad_(True)).requires_grad
+        for bad in (lambda: store(x.double()), lambda: restore(kept, torch.float64), lambda: restore(store(x), out=x), lambda: swiglu(x),
+                    lambda: swiglu_backward(kept, d[:2]), lambda: swiglu_backward(kept, d, dgu_out=d)):
+            with pytest.raises(ValueError):
+                bad()
+
+
+def test_eight_bits_are_traced(monkeypatch):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from roc_shmem_b200.ops.checkpoint8 import Checkpoint8, restore, store, swiglu
+    monkeypatch.setattr(checkpoint8, "store_direct", lambda x: x.clone().view(torch.uint8).flatten())
+    monkeypatch.setattr(checkpoint8, "operator_restore", lambda data, cols, dtype: data.clone().view(F32).view(-1, cols))
+    monkeypatch.setattr(checkpoint8, "_sized", lambda kept, what: (kept.shape[:-1].numel(), kept.shape[-1]))
+    monkeypatch.setattr(checkpoint8, "operator_swiglu", lambda gu, keep: ((torch.sigmoid(gu) * gu)[:, 32:], gu.new_empty((0,), dtype=torch.uint8)))
+    x, gu = torch.randn(5, 8), torch.randn(5, 64)
+    for f, v, names in ((lambda t: restore(store(t)), x, ("store8", "restore8")), (swiglu, gu, ("swiglu8",))):
+        for traced in (make_fx(f)(torch.zeros_like(v)), torch.jit.trace(f, (torch.zeros_like(v),), check_trace=False)):
+            assert all(n in str(traced.graph) for n in names)
+            _close(traced(v), v if f is not swiglu else (torch.sigmoid(v) * v)[:, 32:])
+    kept = Checkpoint8(x.view(torch.uint8).flatten(), x.shape, F32)
+    with forward_ad.dual_level():
+        d, g = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, gu))
+        for call in (lambda: store(d), lambda: swiglu(g), lambda: checkpoint8.swiglu_store(g), lambda: checkpoint8.swiglu_backward(kept, d), lambda: restore(kept, out=d)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+
+
+def test_watched_backward_of_kept_activations(monkeypatch):
+    """A plain forward pass whose backward pass is batched."""
+    from roc_shmem_b200.ops import torch_ops
+    gu, d = torch.randn(5, 64, dtype=torch.float32).to(BF), torch.randn(3, 5, 32).to(BF)
+    monkeypatch.setattr(checkpoint8, "_swiglu_forward", lambda gu, keep: (gu[:, 32:].clone(), gu.view(torch.uint8).flatten().clone()))
+    monkeypatch.setattr(checkpoint8, "operator_swiglu_backward",
+                        lambda data, dact, act: (data.view(BF).view(-1, 64) * dact.repeat(1, 2), dact.new_empty(0)))
+    leaf = gu.clone().requires_grad_(True)
+    got, = torch.autograd.grad(checkpoint8._SwigluFn.apply(leaf), leaf, d, is_grads_batched=True)
+    assert torch.equal(got, gu * d.repeat(1, 1, 2))
+
+    def product(a, b, out=None, *, a_mn=False, b_mn=False):
+        return ((a.t() if a_mn else a).float() @ (b if b_mn else b.t()).float()).to(BF)
+    monkeypatch.setattr(torch_ops, "gemm_bf16", product)
+    monkeypatch.setattr(checkpoint8, "store_direct", lambda x: x.detach().clone().view(torch.uint8).flatten())
+    monkeypatch.setattr(checkpoint8, "operator_restore", lambda data, cols, dtype: data.clone().view(BF).view(-1, cols))
+    x, w, dy = torch.randn(5, 16).to(BF).requires_grad_(True), torch.randn(8, 16).to(BF).requires_grad_(True), torch.randn(3, 5, 8).to(BF)
+    dx, dw = torch.autograd.grad(torch_ops._LinearKeptFn.apply(x, w), (x, w), dy, is_grads_batched=True)
+    for i in range(3):
+        assert torch.equal(dx[i], product(dy[i], w, b_mn=True)) and torch.equal(dw[i], product(dy[i], x, a_mn=True, b_mn=True))

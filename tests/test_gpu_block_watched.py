@@ -1,6 +1,7 @@
-"""Norms that somebody traces, compiles, transforms or watches give what the plain calls give, and refuse what they do not have."""
+"""Norms and 8-bit activations that somebody traces, compiles, transforms or watches give what the plain calls give, and refuse what they do not have."""
 import pytest
 import torch
+from torch.utils._python_dispatch import TorchDispatchMode
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -27,6 +28,16 @@ def _step(y, x, w, g, checkpoint=False, form="post_pre"):
 FORMS = ["pre", "post", "post_pre"]
 
 
+class Watch(TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.seen.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+
 @pytest.mark.parametrize("form", FORMS)
 def test_traced_norms(form):
     from torch.fx.experimental.proxy_tensor import make_fx
@@ -43,17 +54,9 @@ def test_traced_norms(form):
 @pytest.mark.parametrize("checkpoint", [False, True])
 def test_watched_training_equals_plain_training(form, checkpoint):
     """Under a mode, compiled without a code generator, and a plain forward pass with a watched backward pass."""
-    from torch.utils._python_dispatch import TorchDispatchMode
     leaves = [t.requires_grad_(True) for t in _operands()]
     used = [t for t, unused in zip(leaves, (form == "pre", False, False, form == "pre")) if not unused]
     dys = [_rand(6, 40, 264, seed=20 + i) for i in range(2 if form == "post_pre" else 1)]
-    seen = []
-
-    class Watch(TorchDispatchMode):
-        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
-            seen.append(str(func))
-            return func(*args, **(kwargs or {}))
-
     def forward():
         return _step(*leaves, checkpoint, form)
     outs = forward()
@@ -61,14 +64,14 @@ def test_watched_training_equals_plain_training(form, checkpoint):
 
     def same(outs, grads):
         assert all(torch.equal(a, b) for a, b in zip((*outs, *grads), expect))
-    with Watch():
+    with Watch() as watch:
         outs = forward()
         same(outs, torch.autograd.grad(outs, used, dys))
-    assert "bshmem.norm.default" in seen and "bshmem.norm_backward.default" in seen
+    assert "bshmem.norm.default" in watch.seen and "bshmem.norm_backward.default" in watch.seen
     outs = forward()
-    seen.clear()
-    with Watch():
+    with Watch() as watch:
         same(outs, torch.autograd.grad(outs, used, dys))
+    assert "bshmem.norm_backward.default" in watch.seen
     compiled = torch.compile(lambda *t: _step(*t, checkpoint, form), backend="aot_eager", fullgraph=True)
     outs = compiled(*leaves)
     same(outs, torch.autograd.grad(outs, used, dys))
@@ -111,3 +114,49 @@ def test_batched_and_dual_norms():
     dx, = torch.autograd.grad(torch.ops.bshmem.norm(None, leaf, None, w, None, None, 1.0, 1e-6, 0, False)[1], leaf, y, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(dx.float().sum(), leaf)
+
+
+def test_watched_eight_bits():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from roc_shmem_b200.ops.checkpoint8 import restore, store, swiglu, swiglu_backward, swiglu_store
+    x, gu, d = _rand(40, 200, seed=1), _rand(40, 192, seed=2), _rand(40, 96, seed=3)
+    there = lambda t: restore(store(t))  # noqa: E731
+
+    def both(t, e):
+        act, kept = swiglu_store(t)
+        return (act, *swiglu_backward(kept, e, act=True))
+    expect, pair = there(x), both(gu, d)
+    for traced in (make_fx(there)(torch.zeros_like(x)), torch.jit.trace(there, (torch.zeros_like(x),)),
+                   torch.compile(there, backend="aot_eager", fullgraph=True)):
+        assert torch.equal(traced(x), expect)
+    for traced in (make_fx(both)(torch.zeros_like(gu), d), torch.compile(both, backend="aot_eager", fullgraph=True)):
+        assert all(torch.equal(a, b) for a, b in zip(traced(gu, d), pair))
+    assert torch.equal(torch.func.vmap(there)(x.view(5, 8, 200)).view(40, 200), expect)
+    leaf = gu.clone().requires_grad_(True)
+    grad, = torch.autograd.grad(swiglu(leaf), leaf, d)
+    assert torch.equal(grad, pair[1])
+    compiled = torch.compile(swiglu, backend="aot_eager", fullgraph=True)
+    assert torch.equal(torch.autograd.grad(compiled(leaf), leaf, d)[0], grad)
+    act = swiglu(leaf)
+    with Watch():
+        assert torch.equal(torch.autograd.grad(act, leaf, d, retain_graph=True)[0], grad)
+        assert torch.equal(swiglu(gu), pair[0]) and torch.equal(restore(store(x), out=torch.empty_like(x)), expect)
+    assert torch.equal(torch.autograd.grad(act, leaf, torch.stack([d, d]), is_grads_batched=True)[0][1], grad)
+    with FakeTensorMode() as mode:
+        f = mode.from_tensor(gu).requires_grad_(True)
+        assert torch.autograd.grad(swiglu(f), f, mode.from_tensor(d))[0].shape == gu.shape
+
+
+def test_watched_backward_of_a_linear_layer_with_kept_input():
+    from roc_shmem_b200.ops.torch_ops import Linear
+    layer = Linear(200, 264, device="cuda", checkpoint=True)
+    x, dy = _rand(40, 200, seed=1).requires_grad_(True), _rand(40, 264, seed=2)
+    y = layer(x)
+    expect = torch.autograd.grad(y, (x, layer.weight), dy, retain_graph=True)
+    with Watch():
+        got = torch.autograd.grad(y, (x, layer.weight), dy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, expect))
+    got = torch.autograd.grad(y, (x, layer.weight), torch.stack([dy, dy]), is_grads_batched=True)
+    assert all(torch.equal(a[1], b) for a, b in zip(got, expect))
