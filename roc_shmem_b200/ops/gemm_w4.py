@@ -2,7 +2,9 @@
 point z of 4 bits, per row and group of columns.
 
 Few tokens (a decode step) run on a kernel that streams the 4 bits and multiplies them as they are; with many the weights are
-widened to bf16 once and the bf16 tcgen05 GEMM takes them.  The reference contains no GEMM, so there is no parity citation.
+widened to bf16 once and the bf16 tcgen05 GEMM takes them.  Traced, compiled, fake and watched calls are the registered operators
+``torch.ops.bshmem.linear_w4``, ``widen_w4`` and ``quantize_w4``; there is no derivative of either mode.  The reference contains no GEMM, so there
+is no parity citation.
 """
 from __future__ import annotations
 
@@ -15,6 +17,7 @@ import torch
 from .. import _native
 from .checkpoint8 import block_lib, on_current_device
 from .gemm import current_stream, gemm_bf16
+from .watched import direct
 
 _U8, _BF16 = torch.uint8, torch.bfloat16
 
@@ -73,7 +76,8 @@ class W4Tensor:
         return (q - z) * self.scales.float().repeat_interleave(self.group, dim=1)
 
 
-def _checked(w: W4Tensor, what: str) -> tuple[int, int, int]:
+def _sized(w: W4Tensor, what: str) -> tuple[int, int, int]:
+    """N, K and group of `w`, without a look at addresses."""
     q, s, z = w.q, w.scales, w.zeros
     if not (q.dtype is _U8 and s.dtype is _BF16 and q.is_cuda and (z is None or z.dtype is _U8)):
         raise ValueError(f"{what} needs CUDA tensors q (uint8), scales (bf16) and zeros (uint8 or None)")
@@ -86,22 +90,41 @@ def _checked(w: W4Tensor, what: str) -> tuple[int, int, int]:
         raise ValueError(f"{what} needs whole groups of 32, 64 or a multiple of 128 columns, got K {K} in {ss[1]} groups")
     if s.get_device() != q.get_device() or (z is not None and z.get_device() != q.get_device()):
         raise ValueError(f"{what}: q, scales and zeros must be on one device")
-    if not (q.is_contiguous() and s.is_contiguous() and (z is None or z.is_contiguous())) or q.data_ptr() % 16:
+    if not (q.is_contiguous() and s.is_contiguous() and (z is None or z.is_contiguous())):
         raise ValueError(f"{what} needs contiguous tensors and q on a 16-byte boundary")
     return N, K, group
 
 
-def quantize_w4(w: torch.Tensor, group: int = 128, *, zeros: bool = False) -> W4Tensor:
-    """bf16 [N, K] → 4 bits.  Without zero points a group's scale is (largest magnitude) / 7; with them (largest - smallest) / 15, of a range
-    that holds zero; both rounded to bf16, and every value goes to the nearest that they can say."""
+def _checked(w: W4Tensor, what: str) -> tuple[int, int, int]:
+    found = _sized(w, what)
+    if w.q.data_ptr() % 16:
+        raise ValueError(f"{what} needs contiguous tensors and q on a 16-byte boundary")
+    return found
+
+
+def _check_weight(w: torch.Tensor, group: int) -> None:
     if not w.is_cuda or w.dtype is not torch.bfloat16 or w.dim() != 2 or w.stride(1) != 1:
         raise ValueError("quantize_w4 needs a K-major bf16 CUDA matrix")
     N, K = w.shape
     if N < 1 or not (group in (32, 64) or (group > 0 and group % 128 == 0)) or K < group or K % group:
         raise ValueError(f"quantize_w4 needs rows of whole groups of 32, 64 or a multiple of 128 columns, got K {K}, group {group}")
+
+
+def quantize_w4(w: torch.Tensor, group: int = 128, *, zeros: bool = False) -> W4Tensor:
+    """bf16 [N, K] → 4 bits.  Without zero points a group's scale is (largest magnitude) / 7; with them (largest - smallest) / 15, of a range
+    that holds zero; both rounded to bf16, and every value goes to the nearest that they can say."""
+    if not direct("quantize_w4", w):
+        q, s, z = _operators().quantize_w4(w, group, zeros)
+        return W4Tensor(q, s, z if zeros else None)
+    return quantize_direct(w, group, zeros)
+
+
+def quantize_direct(w: torch.Tensor, group: int, zeros: bool) -> W4Tensor:
+    _check_weight(w, group)
     if not on_current_device(w):
         with torch.cuda.device(w.device):
-            return quantize_w4(w, group, zeros=zeros)
+            return quantize_direct(w, group, zeros)
+    N, K = w.shape
     lib = _lib()
     q = torch.empty((N, K // 2), dtype=torch.uint8, device=w.device)
     s = torch.empty((N, K // group), dtype=torch.bfloat16, device=w.device)
@@ -113,10 +136,16 @@ def quantize_w4(w: torch.Tensor, group: int = 128, *, zeros: bool = False) -> W4
 
 def widen_w4(w: W4Tensor) -> torch.Tensor:
     """The weight in bf16 [N, K], each value rounded once."""
+    if not direct("widen_w4", w.q, w.scales, w.zeros):
+        return _operators().widen_w4(w.q, w.scales, w.zeros)
+    return widen_direct(w)
+
+
+def widen_direct(w: W4Tensor) -> torch.Tensor:
     N, K, group = _checked(w, "widen_w4")
     if not on_current_device(w.q):
         with torch.cuda.device(w.q.device):
-            return widen_w4(w)
+            return widen_direct(w)
     if _widen is None:
         _lib()
     out = torch.empty((N, K), dtype=torch.bfloat16, device=w.q.device)
@@ -127,15 +156,27 @@ def widen_w4(w: W4Tensor) -> torch.Tensor:
 
 def linear_w4(x: torch.Tensor, w: W4Tensor) -> torch.Tensor:
     """x [..., K] bf16 times the weight [N, K] of 4 bits, in bf16 [..., N] (forward only)."""
-    N, K, group = _checked(w, "linear_w4")
+    if direct("linear_w4", x, w.q, w.scales, w.zeros):
+        return linear_direct(x, w)
+    _check_x(x, w, _sized(w, "linear_w4")[1])
+    return _operators().linear_w4(x, w.q, w.scales, w.zeros)
+
+
+def _check_x(x: torch.Tensor, w: W4Tensor, K: int) -> None:
     shape = x.shape
     if x.dtype is not _BF16 or not shape or shape[-1] != K or not x.is_cuda or x.get_device() != w.q.get_device():
         raise ValueError(f"linear_w4 needs bf16 [..., {K}] on {w.q.device}, got {x.dtype} {tuple(shape)} on {x.device}")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("linear_w4 has no gradient: detach x, or call it under torch.no_grad()")
+
+
+def linear_direct(x: torch.Tensor, w: W4Tensor) -> torch.Tensor:
+    N, K, group = _checked(w, "linear_w4")
+    _check_x(x, w, K)
     if not on_current_device(x):
         with torch.cuda.device(x.device):
-            return linear_w4(x, w)
+            return linear_direct(x, w)
+    shape = x.shape
     m = x if len(shape) == 2 else x.reshape(-1, K)
     T = m.shape[0]
     ld, columns = m.stride()
@@ -147,7 +188,7 @@ def linear_w4(x: torch.Tensor, w: W4Tensor) -> torch.Tensor:
             m = m.clone()
         ld = K
     if T > few_tokens(group) and N % 8 == 0:                 # the bf16 GEMM's columns come in eights
-        out = gemm_bf16(m, widen_w4(w))
+        out = gemm_bf16(m, widen_direct(w))
     else:
         if _few is None:
             _lib()
@@ -157,6 +198,37 @@ def linear_w4(x: torch.Tensor, w: W4Tensor) -> torch.Tensor:
         if st != 0:
             _check(st, "linear_w4")
     return out if len(shape) == 2 else out.view(*shape[:-1], N)
+
+
+# ---- registered operators: calls that somebody watches, traces or transforms ------------------------------------------------
+
+def _operators():
+    from . import torch_ops  # noqa: F401
+    return torch.ops.bshmem
+
+
+def operator_quantize(w, group, zeros):
+    t = quantize_direct(w, group, zeros)
+    return t.q, t.scales, t.q.new_empty((0,)) if t.zeros is None else t.zeros
+
+
+def operator_quantize_fake(w, group, zeros):
+    _check_weight(w, group)
+    N, K = w.shape
+    return (w.new_empty((N, K // 2), dtype=torch.uint8), w.new_empty((N, K // group)),
+            w.new_empty((N, K // group) if zeros else (0,), dtype=torch.uint8))
+
+
+def operator_widen_fake(q, scales, zeros):
+    N, K, _ = _sized(W4Tensor(q, scales, zeros), "widen_w4")
+    return scales.new_empty((N, K))
+
+
+def operator_linear_fake(x, q, scales, zeros):
+    w = W4Tensor(q, scales, zeros)
+    N, K, _ = _sized(w, "linear_w4")
+    _check_x(x, w, K)
+    return x.new_empty((*x.shape[:-1], N))
 
 
 def w4_error_site(clear: bool = True) -> int:
@@ -169,7 +241,7 @@ class LinearW4(torch.nn.Module):
 
     def __init__(self, weight: W4Tensor):
         super().__init__()
-        N, K, _ = _checked(weight, "LinearW4")
+        N, K, _ = (_checked if direct("LinearW4", weight.q, weight.scales, weight.zeros) else _sized)(weight, "LinearW4")
         self.in_features, self.out_features = K, N
         self.register_buffer("q", weight.q)
         self.register_buffer("scales", weight.scales)

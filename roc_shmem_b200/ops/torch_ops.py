@@ -12,7 +12,7 @@ from typing import Optional
 
 import torch
 
-from . import checkpoint8, norms
+from . import checkpoint8, gemm_w4, norms
 from .checkpoint8 import Checkpoint8
 from .gemm import gemm_bf16
 from .gemm_fp8 import gemm_fp8, quantize_act, quantize_weight
@@ -175,6 +175,28 @@ def _swiglu_gradient(ctx, dact, _):
 
 
 swiglu8.register_autograd(_swiglu_gradient, setup_context=_swiglu_setup)
+
+
+# ---- 4-bit weights, the same way; forward only -------------------------------------------------------------------------
+
+@torch.library.custom_op("bshmem::quantize_w4", mutates_args=())
+def quantize_w4(w: torch.Tensor, group: int, zeros: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return gemm_w4.operator_quantize(w, group, zeros)
+
+
+@torch.library.custom_op("bshmem::widen_w4", mutates_args=())
+def widen_w4(q: torch.Tensor, scales: torch.Tensor, zeros: _Optional) -> torch.Tensor:
+    return gemm_w4.widen_direct(gemm_w4.W4Tensor(q, scales, zeros))
+
+
+@torch.library.custom_op("bshmem::linear_w4", mutates_args=())
+def linear_w4(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: _Optional) -> torch.Tensor:
+    return gemm_w4.linear_direct(x, gemm_w4.W4Tensor(q, scales, zeros))
+
+
+quantize_w4.register_fake(gemm_w4.operator_quantize_fake)
+widen_w4.register_fake(gemm_w4.operator_widen_fake)
+linear_w4.register_fake(gemm_w4.operator_linear_fake)
 
 
 class _LinearFn(torch.autograd.Function):

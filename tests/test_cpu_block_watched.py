@@ -1,4 +1,4 @@
-"""Norms and 8-bit activations on anything but plain tensors that nobody watches: fake tensors, tracing, transforms, modes that see operators and
+"""Norms, 8-bit activations and 4-bit products on anything but plain tensors that nobody watches: fake tensors, tracing, transforms, modes that see operators and
 forward-mode derivatives, with the formulas in the kernels' place.  Nothing there may reach a native entry, which would read addresses that
 are not there."""
 from types import SimpleNamespace
@@ -8,7 +8,7 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
 
-from roc_shmem_b200.ops import checkpoint8, norms, torch_ops  # noqa: F401
+from roc_shmem_b200.ops import checkpoint8, gemm_w4, norms, torch_ops  # noqa: F401
 
 BF, F32 = torch.bfloat16, torch.float32
 
@@ -23,6 +23,8 @@ def no_native(monkeypatch):
         monkeypatch.setattr(norms, entry, _native)
     for entry in ("_store", "_restore", "_swiglu_store", "_swiglu_backward"):
         monkeypatch.setattr(checkpoint8, entry, _native)
+    for entry in ("_few", "_widen", "_lib", "gemm_bf16"):
+        monkeypatch.setattr(gemm_w4, entry, _native)
 
 
 def _n(v, eps):
@@ -243,3 +245,39 @@ def test_watched_backward_of_kept_activations(monkeypatch):
     dx, dw = torch.autograd.grad(torch_ops._LinearKeptFn.apply(x, w), (x, w), dy, is_grads_batched=True)
     for i in range(3):
         assert torch.equal(dx[i], product(dy[i], w, b_mn=True)) and torch.equal(dw[i], product(dy[i], x, a_mn=True, b_mn=True))
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_fake_four_bits_launch_nothing(zeros):
+    from roc_shmem_b200.ops.gemm_w4 import LinearW4, linear_w4, quantize_w4, widen_w4
+    with FakeTensorMode():
+        w, x = _fakes((24, 256), (3, 5, 256))
+        t = quantize_w4(w, 64, zeros=zeros)
+        assert t.q.shape == (24, 128) and t.scales.shape == (24, 4) and t.scales.dtype is BF and t.group == 64
+        assert t.zeros is None if not zeros else t.zeros.shape == (24, 4) and t.zeros.dtype is torch.uint8
+        assert widen_w4(t).shape == (24, 256) and linear_w4(x, t).shape == (3, 5, 24) and linear_w4(x.new_empty(500, 256), t).shape == (500, 24)
+        assert LinearW4(t)(x).shape == (3, 5, 24)
+        for bad in (lambda: quantize_w4(w, 48), lambda: quantize_w4(w.float()), lambda: linear_w4(x[..., :128], t), lambda: linear_w4(x.float(), t),
+                    lambda: linear_w4(x.clone().requires_grad_(True), t)):
+            with pytest.raises(ValueError):
+                bad()
+
+
+def test_four_bits_are_traced(monkeypatch):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from roc_shmem_b200.ops.gemm_w4 import W4Tensor, linear_w4, quantize_w4, widen_w4
+    t = W4Tensor(torch.zeros(8, 32, dtype=torch.uint8), torch.ones(8, 1, dtype=BF))
+    monkeypatch.setattr(gemm_w4, "linear_direct", lambda x, w: x @ w.dequantize().t())
+    monkeypatch.setattr(gemm_w4, "_check_x", lambda *_: None)
+    monkeypatch.setattr(gemm_w4, "_sized", lambda *_: (8, 64, 64))
+    x = torch.randn(5, 64)
+    for traced in (make_fx(lambda v: linear_w4(v, t))(torch.zeros(5, 64)), torch.jit.trace(lambda v: linear_w4(v, t), (torch.zeros(5, 64),), check_trace=False)):
+        assert "linear_w4" in str(traced.graph)
+        _close(traced(x), x @ t.dequantize().t())
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, x)
+        s = forward_ad.make_dual(t.scales, t.scales)
+        for call in (lambda: linear_w4(d, t), lambda: linear_w4(x, W4Tensor(t.q, s)), lambda: widen_w4(W4Tensor(t.q, s)), lambda: quantize_w4(d)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()

@@ -1,4 +1,4 @@
-"""Norms and 8-bit activations that somebody traces, compiles, transforms or watches give what the plain calls give, and refuse what they do not have."""
+"""Norms, 8-bit activations and 4-bit products that somebody traces, compiles, transforms or watches give what the plain calls give, and refuse what they do not have."""
 import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
@@ -160,3 +160,30 @@ def test_watched_backward_of_a_linear_layer_with_kept_input():
     assert all(torch.equal(a, b) for a, b in zip(got, expect))
     got = torch.autograd.grad(y, (x, layer.weight), torch.stack([dy, dy]), is_grads_batched=True)
     assert all(torch.equal(a[1], b) for a, b in zip(got, expect))
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_watched_four_bits(zeros):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from roc_shmem_b200.ops.gemm_w4 import LinearW4, W4Tensor, linear_w4, quantize_w4, widen_w4
+    w = _rand(264, 512, seed=1)
+    t = quantize_w4(w, 64, zeros=zeros)
+    layer = LinearW4(t)
+    for rows in (5, 200):                                     # the 4-bit kernel and the bf16 GEMM
+        x, other = _rand(rows, 512, seed=2), _rand(rows, 512, seed=3)
+        expect = linear_w4(x, t)
+        for traced in (make_fx(lambda v: linear_w4(v, t))(other), torch.jit.trace(lambda v: linear_w4(v, t), (other,)),
+                       torch.compile(layer, backend="aot_eager", fullgraph=True)):
+            assert torch.equal(traced(x), expect)
+    assert torch.equal(torch.func.vmap(layer)(x.view(5, -1, 512)).view(rows, 264)[:40], linear_w4(x[:40], t))      # of 40 tokens each
+    with Watch() as watch:
+        again = quantize_w4(w, 64, zeros=zeros)
+        wide = widen_w4(again)
+    assert torch.equal(again.q, t.q) and torch.equal(again.scales, t.scales) and (not zeros or torch.equal(again.zeros, t.zeros))
+    assert torch.equal(wide, widen_w4(t)) and {"bshmem.quantize_w4.default", "bshmem.widen_w4.default"} <= set(watch.seen)
+    with FakeTensorMode() as mode:
+        f = W4Tensor(*[None if v is None else mode.from_tensor(v) for v in (t.q, t.scales, t.zeros)])
+        assert linear_w4(mode.from_tensor(x), f).shape == (200, 264) and widen_w4(f).shape == (264, 512)
+        assert LinearW4(quantize_w4(mode.from_tensor(w), 64, zeros=zeros))(mode.from_tensor(x)).shape == (200, 264)
