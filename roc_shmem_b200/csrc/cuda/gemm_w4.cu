@@ -47,7 +47,8 @@ __global__ void __launch_bounds__(256) w4_widen_kernel(const WidenParams p) {
 }
 
 // bf16 weights to 4 bits; a warp has a group.  Without zero points the scale is (largest magnitude) / 7, with them
-// (largest - smallest) / 15 of a range that has zero in it, rounded to bf16; q is the nearest of what that can say.
+// (largest - smallest) / 15 of a range that has zero in it, rounded to bf16; q is the nearest of what that can say.  A group with an
+// infinity or a NaN has no scale: it gets NaN, and so all of its weights are.
 struct QuantParams {
   const __nv_bfloat16* w;
   long long ldw;
@@ -65,18 +66,21 @@ __global__ void __launch_bounds__(256) w4_quant_kernel(const QuantParams p) {
   const int k0 = (int)(i - row * per_row) * p.group;
   const __nv_bfloat16* w = p.w + row * p.ldw + k0;
   float lo = 0.f, hi = 0.f;
+  bool odd = false;                                   // the minimum and the maximum pass over a NaN
   for (int k = lane; k < p.group; k += 32) {
     const float v = __bfloat162float(w[k]);
+    odd |= (__float_as_uint(v) & 0x7fffffffu) >= 0x7f800000u;
     lo = fminf(lo, v);
     hi = fmaxf(hi, v);
   }
+  odd = __any_sync(0xffffffffu, odd);
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  const __nv_bfloat16 sb = __float2bfloat16_rn(p.z ? __fdiv_rn(hi - lo, 15.f) : __fdiv_rn(fmaxf(hi, -lo), 7.f));
-  const float s = __bfloat162float(sb);
+  const __nv_bfloat16 sb = odd ? __ushort_as_bfloat16(0x7fff) : __float2bfloat16_rn(p.z ? __fdiv_rn(hi - lo, 15.f) : __fdiv_rn(fmaxf(hi, -lo), 7.f));
+  const float s = odd ? 0.f : __bfloat162float(sb);
   const float z = !p.z ? 8.f : s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(-lo, s)), 0.f), 15.f) : 0.f;
   if (lane == 0) {
     p.s[i] = sb;

@@ -112,7 +112,7 @@ def _check_weight(w: torch.Tensor, group: int) -> None:
 
 def quantize_w4(w: torch.Tensor, group: int = 128, *, zeros: bool = False) -> W4Tensor:
     """bf16 [N, K] → 4 bits.  Without zero points a group's scale is (largest magnitude) / 7; with them (largest - smallest) / 15, of a range
-    that holds zero; both rounded to bf16, and every value goes to the nearest that they can say."""
+    that holds zero; both rounded to bf16, and every value goes to the nearest that they can say.  A group with an infinity or a NaN becomes NaN."""
     if not direct("quantize_w4", w):
         q, s, z = _operators().quantize_w4(w, group, zeros)
         return W4Tensor(q, s, z if zeros else None)
