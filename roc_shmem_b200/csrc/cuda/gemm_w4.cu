@@ -79,7 +79,9 @@ __global__ void __launch_bounds__(256) w4_quant_kernel(const QuantParams p) {
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  const __nv_bfloat16 sb = odd ? __ushort_as_bfloat16(0x7fff) : __float2bfloat16_rn(p.z ? __fdiv_rn(hi - lo, 15.f) : __fdiv_rn(fmaxf(hi, -lo), 7.f));
+  // a range that fp32 does not hold is fifteen parts all the same
+  const float range = hi - lo, part = range <= 3.4028234e38f ? __fdiv_rn(range, 15.f) : __fdiv_rn(hi, 15.f) + __fdiv_rn(-lo, 15.f);
+  const __nv_bfloat16 sb = odd ? __ushort_as_bfloat16(0x7fff) : __float2bfloat16_rn(p.z ? part : __fdiv_rn(fmaxf(hi, -lo), 7.f));
   const float s = odd ? 0.f : __bfloat162float(sb);
   const float z = !p.z ? 8.f : s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(-lo, s)), 0.f), 15.f) : 0.f;
   if (lane == 0) {

@@ -27,3 +27,19 @@ def test_not_finite(group, zeros):
     x = torch.randn(3, 512, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(BF)
     got, rows = linear_w4(x, t), hit.any(1)
     assert torch.isnan(got[:, rows]).all() and torch.equal(got[:, ~rows], linear_w4(x, ref)[:, ~rows])
+
+
+def test_range_beyond_fp32():
+    """Weights of both signs near the end of their type: the range is twice what fp32 holds, the scale a fifteenth of it.  The scale's own
+    error is half a step of bf16 (2^-8) and three fp32 roundings; a weight is off by half a step, half a step more for the zero point, and
+    by what up to 15 steps lack of the scale."""
+    from roc_shmem_b200.ops.gemm_w4 import quantize_w4
+    w = torch.zeros(4, 64, dtype=BF, device="cuda")
+    for row, (lo, hi) in enumerate(((-3e38, 3e38), (-2e38, 1.9e38), (-1e38, 3.3e38), (-1.6e38, 1.6e38))):
+        w[row] = torch.linspace(lo / 1e38, hi / 1e38, 64, device="cuda", dtype=torch.float64).mul(1e38).to(BF)
+    t = quantize_w4(w, 64, zeros=True)
+    d = w.double()
+    s = (d.amax(1) - d.amin(1)) / 15
+    assert ((t.scales.double()[:, 0] - s).abs() <= s * (2.0 ** -8 + 2.0 ** -22)).all()
+    back = (torch.stack((t.q & 15, t.q >> 4), 2).flatten(1).double() - t.zeros.double()) * t.scales.double()
+    assert ((back - d).abs() <= t.scales.double() * (1 + 15 * 2.0 ** -8)).all()
