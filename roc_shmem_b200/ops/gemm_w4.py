@@ -16,7 +16,7 @@ import torch
 
 from .. import _native
 from .checkpoint8 import block_lib, on_current_device
-from .gemm import current_stream, gemm_bf16
+from .gemm import current_stream, gemm_bf16, gemm_error_site
 from .watched import direct
 
 _U8, _BF16 = torch.uint8, torch.bfloat16
@@ -155,7 +155,10 @@ def widen_direct(w: W4Tensor) -> torch.Tensor:
 
 
 def linear_w4(x: torch.Tensor, w: W4Tensor) -> torch.Tensor:
-    """x [..., K] bf16 times the weight [N, K] of 4 bits, in bf16 [..., N] (forward only)."""
+    """x [..., K] bf16 times the weight [N, K] of 4 bits, in bf16 [..., N] (forward only).
+
+    A kernel whose bounded wait runs out leaves its result unfinished and says so on request: ``w4_error_site``, ``gemm_error_site`` (many
+    tokens), or ``LinearW4.check``, which asks both."""
     if direct("linear_w4", x, w.q, w.scales, w.zeros):
         return linear_direct(x, w)
     _check_x(x, w, _sized(w, "linear_w4")[1])
@@ -256,3 +259,10 @@ class LinearW4(torch.nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return linear_w4(x, W4Tensor(self.q, self.scales, self.zeros))
+
+    def check(self) -> None:
+        """Raises if an in-kernel wait of the products on this device ran out since the last check; synchronises."""
+        with torch.cuda.device(self.q.device):
+            site = w4_error_site() or gemm_error_site()
+        if site:
+            raise RuntimeError(f"a bounded in-kernel wait ran out (site {site})")

@@ -122,3 +122,22 @@ def test_kept_norms_hold_every_word_that_is_read(monkeypatch):
                 count = 2 if mode == norms.POST_PRE else 1
                 last = count * rows * ((n + 15) // 16 * 16 + (n + 127) // 128) - 1
                 assert last // 4 * 4 + 4 <= kept.numel() < last + 5
+
+
+def test_layer_reports_a_wait_that_ran_out(monkeypatch):
+    """Of either kernel that it runs on; a layer whose device no longer answers says so too."""
+    from contextlib import nullcontext
+    from types import SimpleNamespace
+
+    from roc_shmem_b200.ops import gemm_w4
+    monkeypatch.setattr(torch.cuda, "device", lambda d: nullcontext())
+    layer = SimpleNamespace(q=torch.zeros(1))
+    sites = {"w4_error_site": 0, "gemm_error_site": 0}
+    for name in sites:
+        monkeypatch.setattr(gemm_w4, name, lambda name=name: sites[name])
+    gemm_w4.LinearW4.check(layer)
+    for name, site in (("w4_error_site", 403), ("gemm_error_site", 7), ("w4_error_site", -1)):
+        sites[name] = site
+        with pytest.raises(RuntimeError, match=f"site {site}"):
+            gemm_w4.LinearW4.check(layer)
+        sites[name] = 0
