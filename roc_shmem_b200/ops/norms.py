@@ -212,6 +212,10 @@ def _gradients(call, need, saved, dout, dh):
     if dh is not None and not dh.is_contiguous():
         dh = dh.contiguous()
     kept8 = what & KEPT
+    if not rstd.is_contiguous():                        # a hook on saved tensors may have brought them back some other way
+        rstd = rstd.contiguous()
+    if kept8 and (a.data_ptr() % 16 or not a.is_contiguous()):
+        a = a.clone(memory_format=_CONTIGUOUS)
     y = None if kept8 or a is None else _matrix(a, n)
     z = None if kept8 or b is None else _matrix(b, n)
     dz = _new_like(like, memory_format=_CONTIGUOUS) if mode != POST else dout

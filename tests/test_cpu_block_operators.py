@@ -141,3 +141,21 @@ def test_layer_reports_a_wait_that_ran_out(monkeypatch):
         with pytest.raises(RuntimeError, match=f"site {site}"):
             gemm_w4.LinearW4.check(layer)
         sites[name] = 0
+
+
+def test_kept_norms_from_a_hook_are_aligned(monkeypatch):
+    """What a hook on saved tensors brings back may lie anywhere; the kernels get kept bytes on a 16-byte boundary and 1 / sqrt(...) side by side."""
+    from roc_shmem_b200.ops import norms
+    seen = []
+    monkeypatch.setattr(norms, "_bwd", lambda *a: seen.append((a[13], a[14])) or 0)
+    monkeypatch.setattr(norms, "current_stream", lambda: 0)
+    rows, n = 6, 200
+    x = torch.zeros(rows, n, dtype=torch.bfloat16)
+    buffer = torch.zeros(norms.kept_size(1, rows, n) + 16, dtype=torch.uint8)
+    for off in (0, 1, 4, 8):
+        a = buffer[off:off + norms.kept_size(1, rows, n)]
+        for rstd in (torch.zeros(1, rows), torch.zeros(1, 2 * rows)[:, ::2]):
+            seen.clear()
+            norms._gradients((norms.PRE, norms.KEPT, n, rows, norms.NO_GATE, 0), (False, True) + (False,) * 4, (None, None, None, None, rstd, a, None), None, x)
+            (r, k), = seen
+            assert k % 16 == 0 and (k == a.data_ptr()) == (off == 0) and (r == rstd.data_ptr()) == rstd.is_contiguous()
