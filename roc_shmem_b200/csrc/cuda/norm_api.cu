@@ -112,7 +112,6 @@ int groups_of(long long rows, int n, int* groups) {
 extern "C" {
 
 const char* bshmem_norm_last_error() { return host::last_error().c_str(); }
-int bshmem_norm_max_columns() { return kMaxColumns; }
 
 // Number of groups of rows whose column sums a backward pass leaves: part_w2 and part_c are [groups][n rounded up to 8] floats,
 // part_s [groups].  Negative: an error.

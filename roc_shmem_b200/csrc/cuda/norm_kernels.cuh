@@ -652,8 +652,10 @@ template <typename F, typename G> Shape backward_shape(long long rows, int n, bo
 }
 
 template <typename T, int kMode, bool kKeep, int kElement> int forward_ring(const Shape& s, const Params& p, dim3 grid, dim3 block, cudaStream_t stream) {
-  if (s.chunks == 2) return launch(norm_fwd_kernel<T, kMode, 2, kRing, kKeep, kElement>, grid, block, shared_of(s), p, stream);
-  return launch(norm_fwd_kernel<T, kMode, 4, kRing, kKeep, kElement>, grid, block, shared_of(s), p, stream);
+  if constexpr (ring_threads(kMode, 2, kKeep || kElement != kNone) == 512) {               // see forward_shape
+    if (s.chunks == 4) return launch(norm_fwd_kernel<T, kMode, 4, kRing, kKeep, kElement>, grid, block, shared_of(s), p, stream);
+  }
+  return launch(norm_fwd_kernel<T, kMode, 2, kRing, kKeep, kElement>, grid, block, shared_of(s), p, stream);
 }
 template <typename T, int kMode, bool kKeep> int forward_ring(const Shape& s, const Params& p, dim3 grid, dim3 block, cudaStream_t stream) {
   if constexpr (kMode != kPre) {
