@@ -101,32 +101,22 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     return m if m.stride(1) == 1 else m.contiguous()
 
 
-def _sized(kept: Checkpoint8, what: str) -> tuple[int, int]:
-    """Rows and columns of `kept`, whose shape says what the kernels write."""
+def _held(kept: Checkpoint8, what: str, addressed: bool = True) -> tuple[torch.Tensor, int, int]:
+    """(bytes, rows, columns) of `kept`, whose shape says what the kernels write.  Not `addressed`: it is not for a kernel of this call."""
     data, shape = kept.data, kept.shape
     cols = shape[-1] if shape else 0
     rows = shape.numel() // cols if cols else 0
-    if not cols or data.numel() != kept_bytes(rows, cols) or data.dtype is not torch.uint8 or not data.is_contiguous():
+    if (not cols or data.numel() != kept_bytes(rows, cols) or data.dtype is not torch.uint8 or not data.is_contiguous()
+            or (addressed and data.data_ptr() % 16)):
         raise ValueError(f"{what}: the checkpoint does not hold a {tuple(shape)}")
-    return rows, cols
-
-
-def _held(kept: Checkpoint8, what: str) -> tuple[torch.Tensor, int, int]:
-    """(bytes, rows, columns) of `kept`."""
-    rows, cols = _sized(kept, what)
-    data = kept.data
-    if data.data_ptr() % 16:
-        raise ValueError(f"{what}: the checkpoint does not hold a {tuple(kept.shape)}")
-    if not data.is_cuda:
+    if not data.is_cuda and addressed:
         raise ValueError(f"{what} needs a checkpoint of a CUDA tensor, got one on {data.device}")
     return data, rows, cols
 
 
 def store(x: torch.Tensor) -> Checkpoint8:
     """bf16, fp16 or fp32 [..., columns] → 8 bits."""
-    if not direct("store", x):
-        return Checkpoint8(_operators().store8(x), x.shape, x.dtype)
-    return Checkpoint8(store_direct(x), x.shape, x.dtype)
+    return Checkpoint8(store_direct(x) if direct("store", x) else _operators().store8(x), x.shape, x.dtype)
 
 
 def store_direct(x: torch.Tensor) -> torch.Tensor:
@@ -150,7 +140,7 @@ def restore(kept: Checkpoint8, dtype: Optional[torch.dtype] = None, out: Optiona
     if direct("restore", kept.data, out):
         return restore_direct(kept, dtype, out)
     _check_dtype(dtype)
-    rows, cols = _sized(kept, "restore")
+    _, rows, cols = _held(kept, "restore", False)
     if out is not None:
         _check_out(out, rows, cols, dtype, kept.data)
     got = _operators().restore8(kept.data, cols, dtype)
@@ -169,7 +159,8 @@ def _check_out(out: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, data
 
 def restore_direct(kept: Checkpoint8, dtype: torch.dtype, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     data, rows, cols = _held(kept, "restore")
-    _check_dtype(dtype)
+    if dtype not in _TYPES:
+        _check_dtype(dtype)
     if not on_current_device(data):
         with torch.cuda.device(data.device):
             return restore_direct(kept, dtype, out)
@@ -229,7 +220,7 @@ def swiglu_backward(kept: Checkpoint8, dact: torch.Tensor, *, act: bool = False,
     act = act or act_out is not None
     if direct("swiglu_backward", kept.data, dact, dgu_out, act_out):
         return swiglu_backward_direct(kept, dact, act, dgu_out, act_out)
-    _check_dact(kept, _sized(kept, "swiglu_backward")[1], dact)
+    _check_dact(kept, _held(kept, "swiglu_backward", False)[2], dact)
     for given, like in ((dgu_out, kept.shape), (act_out, dact.shape)):
         if given is not None:
             _check_buffer(given, like, dact)
@@ -353,5 +344,5 @@ def operator_swiglu_backward(data, dact, act):
 
 def operator_swiglu_backward_fake(data, dact, act):
     kept = _kept_gu(data, dact)
-    _check_dact(kept, _sized(kept, "swiglu_backward")[1], dact)
+    _check_dact(kept, _held(kept, "swiglu_backward", False)[2], dact)
     return dact.new_empty(kept.shape), dact.new_empty(dact.shape if act else (0,))

@@ -76,8 +76,8 @@ class W4Tensor:
         return (q - z) * self.scales.float().repeat_interleave(self.group, dim=1)
 
 
-def _sized(w: W4Tensor, what: str) -> tuple[int, int, int]:
-    """N, K and group of `w`, without a look at addresses."""
+def _checked(w: W4Tensor, what: str, addressed: bool = True) -> tuple[int, int, int]:
+    """N, K and group of `w`.  Not `addressed`: it is not for a kernel of this call."""
     q, s, z = w.q, w.scales, w.zeros
     if not (q.dtype is _U8 and s.dtype is _BF16 and q.is_cuda and (z is None or z.dtype is _U8)):
         raise ValueError(f"{what} needs CUDA tensors q (uint8), scales (bf16) and zeros (uint8 or None)")
@@ -90,16 +90,9 @@ def _sized(w: W4Tensor, what: str) -> tuple[int, int, int]:
         raise ValueError(f"{what} needs whole groups of 32, 64 or a multiple of 128 columns, got K {K} in {ss[1]} groups")
     if s.get_device() != q.get_device() or (z is not None and z.get_device() != q.get_device()):
         raise ValueError(f"{what}: q, scales and zeros must be on one device")
-    if not (q.is_contiguous() and s.is_contiguous() and (z is None or z.is_contiguous())):
+    if not (q.is_contiguous() and s.is_contiguous() and (z is None or z.is_contiguous())) or (addressed and q.data_ptr() % 16):
         raise ValueError(f"{what} needs contiguous tensors and q on a 16-byte boundary")
     return N, K, group
-
-
-def _checked(w: W4Tensor, what: str) -> tuple[int, int, int]:
-    found = _sized(w, what)
-    if w.q.data_ptr() % 16:
-        raise ValueError(f"{what} needs contiguous tensors and q on a 16-byte boundary")
-    return found
 
 
 def _check_weight(w: torch.Tensor, group: int) -> None:
@@ -161,7 +154,7 @@ def linear_w4(x: torch.Tensor, w: W4Tensor) -> torch.Tensor:
     tokens), or ``LinearW4.check``, which asks both."""
     if direct("linear_w4", x, w.q, w.scales, w.zeros):
         return linear_direct(x, w)
-    _check_x(x, w, _sized(w, "linear_w4")[1])
+    _check_x(x, w, _checked(w, "linear_w4", False)[1])
     return _operators().linear_w4(x, w.q, w.scales, w.zeros)
 
 
@@ -175,11 +168,12 @@ def _check_x(x: torch.Tensor, w: W4Tensor, K: int) -> None:
 
 def linear_direct(x: torch.Tensor, w: W4Tensor) -> torch.Tensor:
     N, K, group = _checked(w, "linear_w4")
-    _check_x(x, w, K)
+    shape = x.shape
+    if x.dtype is not _BF16 or not shape or shape[-1] != K or x.get_device() != w.q.get_device() or x.requires_grad:
+        _check_x(x, w, K)
     if not on_current_device(x):
         with torch.cuda.device(x.device):
             return linear_direct(x, w)
-    shape = x.shape
     m = x if len(shape) == 2 else x.reshape(-1, K)
     T = m.shape[0]
     ld, columns = m.stride()
@@ -223,13 +217,13 @@ def operator_quantize_fake(w, group, zeros):
 
 
 def operator_widen_fake(q, scales, zeros):
-    N, K, _ = _sized(W4Tensor(q, scales, zeros), "widen_w4")
+    N, K, _ = _checked(W4Tensor(q, scales, zeros), "widen_w4", False)
     return scales.new_empty((N, K))
 
 
 def operator_linear_fake(x, q, scales, zeros):
     w = W4Tensor(q, scales, zeros)
-    N, K, _ = _sized(w, "linear_w4")
+    N, K, _ = _checked(w, "linear_w4", False)
     _check_x(x, w, K)
     return x.new_empty((*x.shape[:-1], N))
 
@@ -244,7 +238,7 @@ class LinearW4(torch.nn.Module):
 
     def __init__(self, weight: W4Tensor):
         super().__init__()
-        N, K, _ = (_checked if direct("LinearW4", weight.q, weight.scales, weight.zeros) else _sized)(weight, "LinearW4")
+        N, K, _ = _checked(weight, "LinearW4", direct("LinearW4", weight.q, weight.scales, weight.zeros))
         self.in_features, self.out_features = K, N
         self.register_buffer("q", weight.q)
         self.register_buffer("scales", weight.scales)

@@ -193,7 +193,7 @@ def _forward(c: _Call, mode: int, train: bool):
 def _gradients(call, need, saved, dout, dh):
     """Gradients of y, x, w1, w2, gate and scale, as far as `need` asks for them, from what _NormFn keeps."""
     w1, w2, gate, scale, rstd, a, b = saved
-    need_y, need_x, need_w1, need_w2, need_gate, need_scale = need
+    need_y, need_x, need_w1, need_w2, need_gate, need_scale = need[:6]
     mode, what, n, rows, kind, number = call
     if dout is None and dh is None:
         return (None,) * 6
@@ -259,15 +259,9 @@ def _gradients(call, need, saved, dout, dh):
     return dy, dz if need_x else None, dw1, dw2 if dw_next is None else dw_next, dgate, dscale
 
 
-def _given(mode, grads):
-    return grads[0] if mode != PRE else None, grads[-1] if mode != POST else None
-
-
-def _backward(ctx, *grads):
-    return *_gradients(ctx.call, ctx.needs_input_grad[:6], ctx.saved_tensors, *_given(ctx.call[0], grads)), None, None
-
-
-_backward_once = torch.autograd.function.once_differentiable(_backward)
+@torch.autograd.function.once_differentiable
+def _backward_once(ctx, dout, dh):
+    return *_gradients(ctx.call, ctx.needs_input_grad, ctx.saved_tensors, dout, dh), None, None
 
 
 class _NormFn(torch.autograd.Function):
@@ -284,11 +278,15 @@ class _NormFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        mode, what = ctx.call[:2]
-        if not direct_gradients(_NAMES[mode], *grads):
-            number = struct.unpack("<f", struct.pack("<I", ctx.call[5]))[0]
-            return *_registered_gradients(mode, bool(what & KEPT), number, ctx.needs_input_grad[:6], ctx.saved_tensors, *_given(mode, grads)), None, None
-        return _backward_once(ctx, *grads) if torch.is_grad_enabled() else _backward(ctx, *grads)
+        call = ctx.call
+        mode = call[0]
+        dout, dh = grads[0] if mode != PRE else None, grads[-1] if mode != POST else None
+        if not direct_gradients(_NAMES[mode], dout, dh):
+            number = struct.unpack("<f", struct.pack("<I", call[5]))[0]
+            return *_registered_gradients(mode, bool(call[1] & KEPT), number, ctx.needs_input_grad[:6], ctx.saved_tensors, dout, dh), None, None
+        if torch.is_grad_enabled():
+            return _backward_once(ctx, dout, dh)
+        return *_gradients(call, ctx.needs_input_grad, ctx.saved_tensors, dout, dh), None, None
 
 
 # ---- registered operators: calls that somebody watches, traces or transforms ------------------------------------------------

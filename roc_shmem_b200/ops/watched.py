@@ -9,34 +9,57 @@ import torch
 from torch.autograd import forward_ad
 from torch.utils._device import DeviceContext
 
+from .. import _native
+
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
-_DIRECT = frozenset((*_PLAIN, type(None), float, int))
+_direct_types = frozenset((*_PLAIN, type(None), float, int)).issuperset
+_compiling = torch.compiler.is_dynamo_compiling
+_dispatch_modes, _function_modes, _function_mode = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack, torch._C._get_function_stack_at
+_batch = torch._C._functorch.is_legacy_batchedtensor
+_transformed, _traced = torch._C._are_functorch_transforms_active, torch._C._is_tracing
 
 
 def _unwatched() -> bool:
     """Nobody watches or rewrites operators: no compilation or tracing, no dispatch or function mode (fake tensors, make_fx,
     counters; the one of a default device only adds an argument to factories), no functorch transform (vmap, grad, jvp)."""
-    if torch.compiler.is_compiling():                    # first: nothing of the rest can be compiled
+    if _compiling() or _dispatch_modes() or _transformed() or _traced():     # compilation first: nothing of the rest can be compiled
         return False
-    C = torch._C
-    modes = C._len_torch_function_stack()
-    return (C._len_torch_dispatch_stack() == 0 and C._functorch.peek_interpreter_stack() is None and C._get_tracing_state() is None
-            and (modes == 0 or modes == 1 and type(C._get_function_stack_at(0)) is DeviceContext))
+    modes = _function_modes()
+    return not modes or modes == 1 and type(_function_mode(0)) is DeviceContext
+
+
+def _first_plain(*operands) -> bool:
+    """`plain` until the extension module is there: True if direct() is without looking further (see csrc/host/pycall.cc)."""
+    global plain
+    native = _native._pycall()
+    native.watch((torch.Tensor, type(None), torch.nn.Parameter, float, int), (_dispatch_modes, _function_modes, _transformed, _traced), vars(forward_ad),
+                 "_current_level")
+    plain = native.plain
+    return plain(*operands)
+
+
+plain = _first_plain
 
 
 def direct(what: str, *operands) -> bool:
     """Whether the kernels may read `operands` (tensors, numbers, None) where they lie; False: through the registered operator.
     There is no forward-mode derivative, so an operand with a tangent is refused."""
-    if torch.compiler.is_compiling():
+    if _compiling():
         return False
+    if plain(*operands):
+        return True
     if forward_ad._current_level >= 0:
         for t in operands:
             if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError(f"{what} has no forward-mode derivative")
-    return _DIRECT.issuperset(map(type, operands)) and _unwatched()
+    return _direct_types(map(type, operands)) and _unwatched()
 
 
 def direct_gradients(what: str, *grads) -> bool:
     """The same for the gradients that a backward pass gets, which may also be batches (``is_grads_batched``)."""
-    batched = torch._C._functorch.is_legacy_batchedtensor
-    return direct(what, *grads) and not any([batched(g) for g in grads if g is not None])
+    if not direct(what, *grads):
+        return False
+    for g in grads:
+        if g is not None and _batch(g):
+            return False
+    return True

@@ -143,6 +143,31 @@ def test_no_forward_mode_derivative():
         torch.func.jvp(lambda v: norms.rms_norm(v, w), (x,), (x,))
 
 
+def test_when_a_call_is_direct():
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from roc_shmem_b200.ops.watched import direct
+
+    class Other(torch.Tensor):
+        pass
+    x, p = torch.zeros(3), torch.nn.Parameter(torch.zeros(3))
+    assert direct("it", x, p, None, 0.5, 1) and direct("it")
+    assert not direct("it", x.as_subclass(Other)) and not direct("it", x, None, [1])
+    with torch.device("cpu"):                                # a default device is no observer
+        assert direct("it", x)
+    with forward_ad.dual_level():                            # nor is a level that none of the operands is of
+        assert direct("it", x, None, 0.5)
+    for mode in (TorchFunctionMode, TorchDispatchMode):
+        with mode():
+            assert not direct("it", x)
+    inside = []
+    for f in (torch.func.vmap, torch.func.functionalize):
+        f(lambda v: (inside.append(direct("it", v)), v)[1])(torch.zeros(2))
+    torch.jit.trace(lambda v: (inside.append(direct("it", v)), v)[1], (x,), check_trace=False)
+    assert inside == [False] * 3 and direct("it", x)
+
+
 def _graph(monkeypatch, x, w):
     """A result of the direct call whose backward pass is still to come, with the formula in the kernel's place."""
     def forward(c, mode, train):
@@ -210,7 +235,7 @@ def test_eight_bits_are_traced(monkeypatch):
     from roc_shmem_b200.ops.checkpoint8 import Checkpoint8, restore, store, swiglu
     monkeypatch.setattr(checkpoint8, "store_direct", lambda x: x.clone().view(torch.uint8).flatten())
     monkeypatch.setattr(checkpoint8, "operator_restore", lambda data, cols, dtype: data.clone().view(F32).view(-1, cols))
-    monkeypatch.setattr(checkpoint8, "_sized", lambda kept, what: (kept.shape[:-1].numel(), kept.shape[-1]))
+    monkeypatch.setattr(checkpoint8, "_held", lambda kept, *_: (kept.data, kept.shape[:-1].numel(), kept.shape[-1]))
     monkeypatch.setattr(checkpoint8, "operator_swiglu", lambda gu, keep: ((torch.sigmoid(gu) * gu)[:, 32:], gu.new_empty((0,), dtype=torch.uint8)))
     x, gu = torch.randn(5, 8), torch.randn(5, 64)
     for f, v, names in ((lambda t: restore(store(t)), x, ("store8", "restore8")), (swiglu, gu, ("swiglu8",))):
@@ -270,7 +295,7 @@ def test_four_bits_are_traced(monkeypatch):
     t = W4Tensor(torch.zeros(8, 32, dtype=torch.uint8), torch.ones(8, 1, dtype=BF))
     monkeypatch.setattr(gemm_w4, "linear_direct", lambda x, w: x @ w.dequantize().t())
     monkeypatch.setattr(gemm_w4, "_check_x", lambda *_: None)
-    monkeypatch.setattr(gemm_w4, "_sized", lambda *_: (8, 64, 64))
+    monkeypatch.setattr(gemm_w4, "_checked", lambda *_: (8, 64, 64))
     x = torch.randn(5, 64)
     for traced in (make_fx(lambda v: linear_w4(v, t))(torch.zeros(5, 64)), torch.jit.trace(lambda v: linear_w4(v, t), (torch.zeros(5, 64),), check_trace=False)):
         assert "linear_w4" in str(traced.graph)
