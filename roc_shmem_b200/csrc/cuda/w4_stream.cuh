@@ -12,11 +12,12 @@
 //   warp 0      TMA producer: {128 rows x 128 bytes of weights, tokens x 256 columns} per stage, i.e. two k-blocks (with rows of 64
 //               bytes the TMA unit's requests, one per row, were the limit); plain loads of local memory
 //   warp 1      MMA issuer: tcgen05.mma M128 x N=tokens x K16, A in tensor memory, B in shared memory
-//   then        three to five groups of four warps: each widens every third to fifth k-block and orders its activations
+//   then        two to five groups of four warps: each widens every second to fifth k-block and orders its activations
 //   last 4      add the accumulators up
 //
 // From a k-block's arrival to its sums it takes a warp of each kind some 900 cycles, and HBM brings an SM the 8 KiB of the next in 370: so several
-// are on their way (kDepth of them in tensor memory), in the hands of different warps.  The ALU is behind that: seven shifts and
+// are on their way (kDepth stages in tensor memory, of two each; one stage where its accumulators take most: 64 tokens in groups of 64,
+// 32 in groups of 32), in the hands of different warps.  The ALU is behind that: seven shifts and
 // logical operations for eight weights at half the rate of the other pipes, 230 cycles for a k-block.
 //
 // A cluster of up to 8 CTAs splits the columns of a tile where tiles are few, and adds the parts through distributed shared memory

@@ -7,8 +7,8 @@
 Rows are bf16, fp16 or fp32, sums fp32.  A weight is one value per column, of the rows' type or fp32; the gate one per column
 ``[H]``, per row ``[..., 1]`` or per element (weights and gates may be left out); the scale a number or a tensor with one
 element.  Every tensor has a gradient; sums over rows are added in a fixed order, so a call gives the same bits again.
-``checkpoint=True`` keeps the norms' inputs for the backward pass in 8 bits (``checkpoint8``): the gradients are then those at the
-kept values.  Rows have 1 to 16384 columns and may be apart (any stride of the leading dimension); rows of a multiple of 8 columns on
+``checkpoint=True`` keeps the norms' inputs for the backward pass in 8 bits (``checkpoint8``): n(v) is then the kept v times the true
+row's 1 / sqrt(mean + eps) wherever a gradient has it.  Rows have 1 to 16384 columns and may be apart (any stride of the leading dimension); rows of a multiple of 8 columns on
 16-byte boundaries are the fast ones.  A backward pass that a CUDA graph captures wants every eager graph of the same leaves gone: torch
 keeps their gradients' accumulators as long, and with them the stream that they were made on.  Squares are fp32: rows whose squares leave its range give what that gives.
 Traced, compiled, fake and watched calls are the registered operators ``torch.ops.bshmem.norm`` and ``norm_backward``; there is no forward-mode
