@@ -296,7 +296,8 @@ def _registered(name, mode, y, x, w1, w2, gate, scale, eps, checkpoint):
     number = 1.0
     if scale is not None and not isinstance(scale, torch.Tensor):
         scale, number = None, float(scale)
-    out, h, _, _ = torch.ops.bshmem.norm(y, x, w1, w2, gate, scale, number, float(eps), mode, bool(checkpoint))
+    checkpoint = bool(checkpoint) and torch.is_grad_enabled() and any([t.requires_grad for t in (y, x, w1, w2, gate, scale) if t is not None])
+    out, h, _, _ = torch.ops.bshmem.norm(y, x, w1, w2, gate, scale, number, float(eps), mode, checkpoint)
     return (out, h) if mode == POST_PRE else out if mode == POST else h
 
 

@@ -12,8 +12,7 @@ from torch.utils._device import DeviceContext
 from .. import _native
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
-_direct_types = frozenset((*_PLAIN, type(None), float, int)).issuperset
-_compiling = torch.compiler.is_dynamo_compiling
+_compiling = torch.compiler.is_compiling
 _dispatch_modes, _function_modes, _function_mode = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack, torch._C._get_function_stack_at
 _batch = torch._C._functorch.is_legacy_batchedtensor
 _transformed, _traced = torch._C._are_functorch_transforms_active, torch._C._is_tracing
@@ -42,7 +41,7 @@ plain = _first_plain
 
 
 def direct(what: str, *operands) -> bool:
-    """Whether the kernels may read `operands` (tensors, numbers, None) where they lie; False: through the registered operator.
+    """Whether the kernels may read `operands` (tensors, and whatever else a call has) where they lie; False: through the registered operator.
     There is no forward-mode derivative, so an operand with a tangent is refused."""
     if _compiling():
         return False
@@ -52,7 +51,7 @@ def direct(what: str, *operands) -> bool:
         for t in operands:
             if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError(f"{what} has no forward-mode derivative")
-    return _direct_types(map(type, operands)) and _unwatched()
+    return all([type(t) in _PLAIN for t in operands if isinstance(t, torch.Tensor)]) and _unwatched()
 
 
 def direct_gradients(what: str, *grads) -> bool:

@@ -3,6 +3,7 @@ forward-mode derivatives, with the formulas in the kernels' place.  Nothing ther
 are not there."""
 from types import SimpleNamespace
 
+import numpy
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -109,6 +110,21 @@ def test_norms_with_gradients_are_traced(formulas):
         _close(got, e)
 
 
+def test_nothing_is_kept_without_a_gradient(formulas, monkeypatch):
+    asked, body = [], norms.operator_forward
+    monkeypatch.setattr(norms, "operator_forward", lambda *a: (asked.append(a[-1]), body(*a))[1])
+
+    class Other(torch.Tensor):
+        pass
+    x, w = torch.randn(5, 8).as_subclass(Other), torch.randn(8, requires_grad=True)
+    norms.rms_norm(x, w, checkpoint=True)
+    norms.rms_norm(x, w)
+    norms.rms_norm(x, w.detach(), checkpoint=True)
+    with torch.no_grad():
+        norms.rms_norm(x, w, checkpoint=True)
+    assert asked == [True, False, False, False]
+
+
 def test_transforms_and_modes(formulas):
     from torch.utils._python_dispatch import TorchDispatchMode
     x, w = torch.randn(3, 5, 8), torch.randn(8)
@@ -153,7 +169,8 @@ def test_when_a_call_is_direct():
         pass
     x, p = torch.zeros(3), torch.nn.Parameter(torch.zeros(3))
     assert direct("it", x, p, None, 0.5, 1) and direct("it")
-    assert not direct("it", x.as_subclass(Other)) and not direct("it", x, None, [1])
+    assert not direct("it", x.as_subclass(Other)) and not direct("it", x, None, torch.empty(3, device="meta").as_subclass(Other))
+    assert direct("it", x, True, numpy.float64(0.5))         # numbers of any kind
     with torch.device("cpu"):                                # a default device is no observer
         assert direct("it", x)
     with forward_ad.dual_level():                            # nor is a level that none of the operands is of
