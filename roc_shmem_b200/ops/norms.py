@@ -306,8 +306,9 @@ def _registered_gradients(mode, checkpoint, number, need, saved, dout, dh):
     need = list(need)
     if dout is None and dh is None:
         return (None,) * 6
-    dx = dout if mode == POST and need[1] else None      # an operator may not return what it was given
-    need[1] = need[1] and mode != POST
+    alone = mode == POST or (mode == POST_PRE and dh is None)
+    dx = dout if alone and need[1] else None             # an operator may not return what it was given
+    need[1] = need[1] and not alone
     found = torch.ops.bshmem.norm_backward(dout, dh, *saved, number, mode, checkpoint, sum(1 << i for i, wanted in enumerate(need) if wanted))
     found = [g if wanted else None for g, wanted in zip(found, need)]
     return found[0], found[1] if dx is None else dx, *found[2:]
@@ -374,7 +375,7 @@ def operator_backward(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, c
     c = _whole_gradients(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need)
     with torch.cuda.device(rstd.device):
         found = _gradients((mode, c.what, c.n, c.rows, c.kind, _bits(number)), _asked(need), (w1, w2, gate, scale, rstd, a, b), dout, dh)
-    return tuple(g if wanted else rstd.new_empty(0) for g, wanted in zip(found, _asked(need)))
+    return tuple(rstd.new_empty(0) if not wanted else g.clone() if g is dout else g for g, wanted in zip(found, _asked(need)))
 
 
 def operator_backward_fake(dout, dh, w1, w2, gate, scale, rstd, a, b, number, mode, checkpoint, need):

@@ -80,6 +80,32 @@ def test_watched_training_equals_plain_training(form, checkpoint):
     same(outs, [b[0] for b in batched])
 
 
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("used", [0, 1])
+def test_one_result_of_a_watched_call_unused(checkpoint, used):
+    leaves = [t.requires_grad_(True) for t in _operands()]
+    dy = _rand(6, 40, 264, seed=20)
+
+    def gradients(f):
+        return torch.autograd.grad(f(*leaves)[used], leaves, dy)
+    f = lambda *t: _step(*t, checkpoint)  # noqa: E731
+    expect = gradients(f)
+    with Watch():
+        got = gradients(f)
+    assert all(torch.equal(a, b) for a, b in zip(got, expect)) and dy.data_ptr() != got[0].data_ptr()
+    out = f(*leaves)[used]
+    with Watch():
+        got = torch.autograd.grad(out, leaves, dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, expect))
+    got = gradients(torch.compile(f, backend="aot_eager", fullgraph=True))
+    assert all(torch.equal(a, b) for a, b in zip(got, expect))
+    y, x, w, g = [t.detach() for t in leaves]
+    _, _, rstd, kept = torch.ops.bshmem.norm(y, x, w, w, g, None, 0.75, 1e-6, 2, True)
+    before = dy.clone()
+    found = torch.ops.bshmem.norm_backward(dy, None, w, w, g, None, rstd, kept, None, 0.75, 2, True, 0b11111)      # the operator itself
+    assert found[1].data_ptr() != dy.data_ptr() and torch.equal(found[1], dy) and torch.equal(dy, before) and not found[3].any()
+
+
 def test_compiled_for_any_number_of_rows():
     from roc_shmem_b200.ops.norms import RMSNorm
     norm = RMSNorm(264, device="cuda")
