@@ -60,7 +60,7 @@ template <typename T, int kAccess> __global__ void __launch_bounds__(kThreads) s
     encode<T, 2>({unpack(r[j][0]), unpack(r[j][1])}, q, e);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
-      if (col[j] + 64 * k < n[j]) *reinterpret_cast<uint2*>(p.q + row[j] * p.ldq + col[j] + 64 * k) = q[k];
+      if (col[j] + 64 * k < byte_columns(n[j])) *reinterpret_cast<uint2*>(p.q + row[j] * p.ldq + col[j] + 64 * k) = q[k];
     if (col[j] % 128 == 0 && col[j] < n[j]) p.e[row[j] * p.lde + col[j] / 128] = (uint8_t)e;
   }
 }
@@ -202,7 +202,7 @@ extern "C" {
 const char* bshmem_ckpt8_last_error() { return host::last_error().c_str(); }
 
 // x: [rows, n] of type 0 bf16, 1 fp16, 2 fp32 with row pitch ldx -> kept: q [rows][n rounded up to 16], then e [rows][blocks of 128
-// columns].  Bytes of q behind the last eight columns are not written.
+// columns].  The columns that q has beyond n are zeros.
 int bshmem_ckpt8_store(int type, const void* x, long long ldx, void* kept, long long rows, int n, void* stream) {
   if (type < 0 || type > 2 || n < 1) { host::last_error() = "checkpoint: unknown type or no columns"; return 1; }
   if (rows <= 0) return 0;

@@ -144,7 +144,7 @@ static int refuse_size() {
 }
 
 // out and h are contiguous; rstd: [rows], in kPostPre [2][rows] (y's, then out's), or null.  kept: q [norms][rows][n rounded up to 16],
-// then e [norms][rows][blocks of 128 columns], in the same order, 16-byte aligned and in whole 4-byte words.  numbers: the bits of eps,
+// then e [norms][rows][blocks of 128 columns], in the same order, 16-byte aligned and in whole 4-byte words; what has no value is zero.  numbers: the bits of eps,
 // and of a scale that is not in memory above them.
 int bshmem_norm_fwd(int what, const void* y, long long ldy, const void* x, long long ldx, void* out, void* h, const void* w1,
                     const void* w2, const void* gate, long long ldg, const void* scale, uint64_t numbers, void* rstd, void* kept,
@@ -175,6 +175,9 @@ int bshmem_norm_fwd(int what, const void* y, long long ldy, const void* x, long 
     p.ldq = (n + 15) / 16 * 16;
     p.lde = (n + 127) / 128;
     uint8_t *qb = static_cast<uint8_t*>(kept), *eb = qb + (c.mode == kPostPre ? 2 : 1) * rows * p.ldq;
+    const long long exponents = (c.mode == kPostPre ? 2 : 1) * rows * p.lde;
+    p.end = eb + exponents;
+    p.tail = (int)(-exponents & 3);                     // q is whole words
     if (c.mode != kPre) { p.q1 = qb; p.e1 = eb; }
     if (c.mode != kPost) { p.q2 = qb + (c.mode == kPre ? 0 : rows * p.ldq); p.e2 = eb + (c.mode == kPre ? 0 : rows * p.lde); }
   }

@@ -36,6 +36,7 @@ struct Params {
   float eps;
   float *rstd1, *rstd2;                 // [rows], kept for the backward pass (null in inference)
   uint8_t *q1, *e1, *q2, *e2;           // y and z in 8 bits (null: not kept)
+  uint8_t* end; int tail;               // bytes behind the last exponent, up to a whole word: zeros
   long long ldq, lde;
   long long rows;
   int n;                                // columns
@@ -144,6 +145,7 @@ __global__ void __launch_bounds__(kForm == kRing ? ring_threads(kMode, kChunks, 
   }
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
+  if (keep && blockIdx.x == 0 && threadIdx.y == 0 && threadIdx.x < p.tail) p.end[threadIdx.x] = 0;
   const float inv_n = 1.f / (float)p.n;
   const long long step = (long long)gridDim.x * blockDim.y;
   auto column = [&](int i) { return (int)(threadIdx.x + i * blockDim.x) * 8; };

@@ -238,16 +238,16 @@ __device__ __forceinline__ Vals decode8(uint2 q, uint32_t e) {
   return v;
 }
 
+// Columns of a row of bytes: those behind the n that have values are zeros.
+__device__ __forceinline__ int byte_columns(int n) { return (n + 15) & ~15; }
 // A lane's eight values into a row of bytes and exponents, and back.  kStrided: the warp's 256 columns are two blocks, of the lanes'
 // first four and last four values.
 template <int kAccess, typename T> __device__ __forceinline__ void keep8(uint8_t* q, uint8_t* e, int col, int n, const Vals& v) {
   if constexpr (kAccess == kVector) {
     uint32_t x;
     const uint2 b = encode8<T>(v, x);
-    if (col < n) {
-      *reinterpret_cast<uint2*>(q + col) = b;
-      if (col % 128 == 0) e[col / 128] = (uint8_t)x;
-    }
+    if (col < byte_columns(n)) *reinterpret_cast<uint2*>(q + col) = b;
+    if (col < n && col % 128 == 0) e[col / 128] = (uint8_t)x;
   } else {
     uint32_t x[2] = {0, 0};
 #pragma unroll
@@ -260,7 +260,7 @@ template <int kAccess, typename T> __device__ __forceinline__ void keep8(uint8_t
     const uint32_t e0 = exponent_byte(x[0]), e1 = exponent_byte(x[1]), low = bytes8<T, true>(v, e0).x, high = bytes8<T, true>(v, e1).y;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (column_of<kAccess>(col, j) < n) q[column_of<kAccess>(col, j)] = (uint8_t)((j < 4 ? low : high) >> (8 * (j & 3)));
+      if (column_of<kAccess>(col, j) < byte_columns(n)) q[column_of<kAccess>(col, j)] = (uint8_t)((j < 4 ? low : high) >> (8 * (j & 3)));
     if (col % 256 == 0) {
       if (col < n) e[col / 128] = (uint8_t)e0;
       if (col + 128 < n) e[col / 128 + 1] = (uint8_t)e1;

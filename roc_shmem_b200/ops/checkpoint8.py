@@ -64,7 +64,7 @@ def kept_bytes(rows: int, cols: int) -> int:
 
 @dataclass
 class Checkpoint8:
-    """An activation in 8 bits.  ``data`` holds ``q`` [rows, columns rounded up to 16], e4m3 bytes, and behind it ``e`` [rows, blocks of 128
+    """An activation in 8 bits.  ``data`` holds ``q`` [rows, columns rounded up to 16], e4m3 bytes (zeros in the columns more), and behind it ``e`` [rows, blocks of 128
     columns], biased exponents: the value of a byte is e4m3 * 2^(e - 127).  ``shape`` and ``dtype`` are those of the tensor that was stored."""
     data: torch.Tensor
     shape: torch.Size

@@ -161,7 +161,8 @@ class _Call:
 
 
 def kept_size(norms: int, rows: int, n: int) -> int:
-    """Bytes that a call of `norms` norms keeps in 8 bits: values, then exponents, which the backward pass reads in whole words."""
+    """Bytes that a call of `norms` norms keeps in 8 bits: values, then exponents, which the backward pass
+    reads in whole words; what has no value is zero."""
     return (norms * kept_bytes(rows, n) + 3) // 4 * 4
 
 
