@@ -3,6 +3,8 @@ import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
 
+from roc_shmem_b200.ops import torch_ops  # noqa: F401
+
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
 
@@ -213,3 +215,37 @@ def test_watched_four_bits(zeros):
         f = W4Tensor(*[None if v is None else mode.from_tensor(v) for v in (t.q, t.scales, t.zeros)])
         assert linear_w4(mode.from_tensor(x), f).shape == (200, 264) and widen_w4(f).shape == (264, 512)
         assert LinearW4(quantize_w4(mode.from_tensor(w), 64, zeros=zeros))(mode.from_tensor(x)).shape == (200, 264)
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("mode", [0, 1, 2])
+def test_norm_operators_keep_torchs_rules(mode, checkpoint):
+    """Schema, fake results and gradients, with fixed and with any sizes."""
+    y, x, w, g = _operands()
+    op, back = torch.ops.bshmem.norm, torch.ops.bshmem.norm_backward
+    for grad in (False, True):
+        leaf = [t.clone().requires_grad_(grad) for t in (y, x, w, w, g)]
+        operands = (leaf[0] if mode else None, leaf[1], leaf[2] if mode else None, leaf[3] if mode != 1 else None, leaf[4] if mode else None, None)
+        torch.library.opcheck(op, (*operands, 0.75, 1e-6, mode, checkpoint))
+    plain = [None if t is None else t.detach() for t in operands]
+    out, _, rstd, kept = op(*plain, 0.75, 1e-6, mode, checkpoint)
+    saved = (kept, None) if checkpoint else (plain[0], (x, None, out)[mode])
+    need = (0b001010, 0b010101, 0b011111)[mode]
+    torch.library.opcheck(back, (y if mode else None, x if mode != 1 else None, *plain[2:], rstd, *saved, 0.75, mode, checkpoint, need))
+
+
+def test_other_operators_keep_torchs_rules():
+    ops = torch.ops.bshmem
+    x, gu, d, w = _rand(40, 200, seed=1), _rand(40, 192, seed=2), _rand(40, 96, seed=3), _rand(264, 512, seed=4)
+    torch.library.opcheck(ops.store8, (x,))
+    torch.library.opcheck(ops.restore8, (ops.store8(x), 200, torch.float32))
+    torch.library.opcheck(ops.swiglu8, (gu, False))
+    torch.library.opcheck(ops.swiglu8, (gu.clone().requires_grad_(True), True))
+    for act in (False, True):
+        torch.library.opcheck(ops.swiglu8_backward, (ops.swiglu8(gu, True)[1], d, act))
+    for zeros in (False, True):
+        torch.library.opcheck(ops.quantize_w4, (w, 64, zeros))
+        q, s, z = ops.quantize_w4(w, 64, zeros)
+        torch.library.opcheck(ops.widen_w4, (q, s, z if zeros else None))
+        for tokens in (5, 200):
+            torch.library.opcheck(ops.linear_w4, (_rand(tokens, 512, seed=5), q, s, z if zeros else None))
